@@ -26,6 +26,9 @@ extern "C" {
 /* element type of an input tensor (outputs are always BF16) */
 #define SE12_STEP_BF16 0
 #define SE12_STEP_F32 1
+/* element type of a paged cache besides SE12_STEP_BF16: 8 bits (OCP E4M3, no
+ * infinities), one FP32 scale per page and KV head */
+#define SE12_STEP_E4M3 2
 
 const char* se12_step_last_error(void);
 
@@ -119,6 +122,100 @@ int se12_step_prefill_attention(uint16_t* qkv, int64_t stride, const uint16_t* c
                                 uint16_t* k_cache_t, uint16_t* v_cache, uint16_t* out, int32_t batch, int32_t tokens,
                                 int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t max_len, float scaling,
                                 float softcap, int32_t window, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* A key/value cache in pages of page_size tokens (16, 32, 64 or 128), any page
+ * of the pool for any part of any sequence:
+ *   k [pages, kv_heads, page_size, head_dim]
+ *   v [pages, kv_heads, head_dim, page_size]
+ *   k_scale, v_scale [pages, kv_heads] FP32 (SE12_STEP_E4M3; else ignored): a
+ *   held value stands for itself times the scale of its page and head
+ * head_dim 64, 128 or 256; k and v 16-byte aligned. */
+typedef struct se12_step_pages {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    int32_t dtype;
+    int32_t pages, page_size, kv_heads, head_dim;
+} se12_step_pages;
+
+/* The new tokens of a call. Sequence s holds lengths[s] tokens before it, and
+ * rows starts[s] .. starts[s + 1] - 1 of q, k, v and out are its next ones, at
+ * positions lengths[s], lengths[s] + 1, ..; token j of a sequence lies in slot
+ * j % page_size of page page_table[s * table_stride + j / page_size]. starts
+ * [sequences + 1] ascends from 0; `tokens` is the number of rows of q, k, v and
+ * out (rows from starts[sequences] on are neither read nor written), max_new at
+ * least the most new tokens of a sequence (of more, the first max_new count).
+ * All device memory, read when the kernels run, so a captured call follows what
+ * they hold then. No entry can lead outside the memory given: a page outside
+ * [0, pages), or a position outside the table, holds nothing and takes nothing.
+ * sequences * table_width and so on are up to the caller; table_width *
+ * page_size <= 2^30, sequences <= 65536. */
+typedef struct se12_step_batch {
+    const int32_t* page_table;
+    int64_t table_stride;
+    const int32_t* lengths;
+    const int32_t* starts;
+    int32_t table_width, sequences, tokens, max_new;
+} se12_step_batch;
+
+/* Appends k and v [tokens, kv_heads, head_dim] to the cache, k rotated to its
+ * position, and writes the rotated q [tokens, heads, head_dim] to q_out (BF16,
+ * contiguous); q may be NULL, then nothing is. Rows `q_stride`, `k_stride`,
+ * `v_stride` elements apart (multiples of 4), heads of a row side by side; dtype
+ * SE12_STEP_BF16 or SE12_STEP_F32 for all three, aligned to four elements. The
+ * rotation takes the pair (x[i], x[i + rotary / 2]) by position * inv_freq[i],
+ * i < rotary / 2 (the angle in 64 bits, the rest in FP32); elements from
+ * `rotary` on stay (a multiple of 8 up to head_dim, 0 for none).
+ *
+ * SE12_STEP_BF16: values are rounded once. SE12_STEP_E4M3: a page and head's
+ * scale is the least power of two, 2^-100 or more, that holds the new finite
+ * values (largest / scale <= 448); where older tokens share the page it is at
+ * least the scale they have, and if it grows they are rounded again to the new
+ * one (powers of two: exact but for values that become subnormal). NaN and
+ * infinities are held as NaN. Slots behind the new tokens keep their bytes. A
+ * page that two sequences of a call write, or that a concurrent call reads or
+ * writes, has undefined contents. */
+int se12_step_paged_append(const se12_step_pages* pages, const se12_step_batch* batch, const void* q, const void* k,
+                           const void* v, int32_t dtype, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                           int32_t heads, const float* inv_freq, int32_t rotary, uint16_t* q_out, void* stream);
+
+/* Attention of the new tokens over their sequences' pages, those of the call
+ * itself included (appended before): the query at position p sees keys
+ * max(0, p - window + 1) .. p (window 0 = all). s = q . k * scaling, soft-capped
+ * tanh(s / softcap) * softcap when softcap > 0; softmax and sums in FP32,
+ * weights rounded to BF16 for the product with v. q BF16 [tokens, heads,
+ * head_dim], rows q_stride apart (a multiple of 8), 16-byte aligned, already
+ * rotated; out BF16 [tokens, heads, head_dim] contiguous, 8-byte aligned. heads
+ * a multiple of kv_heads. What a query may not see has no part in its row,
+ * whatever it holds (NaN too); a query that sees nothing gives zeros.
+ *
+ * `workspace`: se12_step_paged_attention_workspace() bytes for the shape,
+ * 256-byte aligned, contents indifferent; calls sharing it must not run
+ * concurrently. Up to two launches; results do not depend on timing. */
+int64_t se12_step_paged_attention_workspace(const se12_step_pages* pages, const se12_step_batch* batch, int32_t heads);
+
+int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batch* batch, const uint16_t* q,
+                              int64_t q_stride, uint16_t* out, int32_t heads, float scaling, float softcap,
+                              int32_t window, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* What a serving program reports of logits [rows, stride] (BF16 or FP32, vocab
+ * of a row used), with z = softcap tanh(logit / softcap) when softcap > 0, else
+ * the logit, and p = softmax(z) in FP32:
+ *   logprobs[r]  log p of tokens[r] (-inf for a token outside [0, vocab))
+ *   entropy[r]   -sum p log p
+ *   top_logprobs, top_ids [rows, top]  the `top` (0 .. 32) most likely tokens,
+ *                by logit from the highest, equal ones by the lower index
+ * A logit of -inf without a cap has no part in the sums; a row of nothing else
+ * has log probabilities of -inf and entropy 0. A row with a NaN, or +inf without
+ * a cap, has NaN for all but its ids, in whose order a NaN comes last.
+ * `workspace`: se12_step_logprobs_workspace() bytes (may be 0), 16-byte aligned,
+ * contents indifferent; calls sharing it must not run concurrently. */
+int64_t se12_step_logprobs_workspace(int32_t rows, int32_t vocab, int32_t top);
+
+int se12_step_logprobs(const void* logits, int32_t dtype, int64_t stride, int32_t rows, int32_t vocab, float softcap,
+                       const int64_t* tokens, int32_t top, float* logprobs, float* entropy, float* top_logprobs,
+                       int64_t* top_ids, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -97,6 +97,33 @@ class DeviceInfo(ctypes.Structure):
     ]
 
 
+class StepPages(ctypes.Structure):
+    _fields_ = [
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("k_scale", c_void_p),
+        ("v_scale", c_void_p),
+        ("dtype", c_i32),
+        ("pages", c_i32),
+        ("page_size", c_i32),
+        ("kv_heads", c_i32),
+        ("head_dim", c_i32),
+    ]
+
+
+class StepBatch(ctypes.Structure):
+    _fields_ = [
+        ("page_table", c_void_p),
+        ("table_stride", c_i64),
+        ("lengths", c_void_p),
+        ("starts", c_void_p),
+        ("table_width", c_i32),
+        ("sequences", c_i32),
+        ("tokens", c_i32),
+        ("max_new", c_i32),
+    ]
+
+
 # name -> (restype, argtypes): every symbol include/se12_gfx950.h and
 # include/se12_step.h declare
 SIGNATURES = {
@@ -198,10 +225,25 @@ SIGNATURES = {
         [c_void_p, c_i32, c_i64, c_i32, c_i32, ctypes.c_float, c_void_p, c_void_p, c_void_p, c_i64, c_void_p, c_void_p,
          c_void_p, c_i64, c_void_p],
     ),
+    "se12_step_paged_append": (
+        c_i32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_i32, c_i64, c_i64, c_i64, c_i32, c_void_p, c_i32, c_void_p,
+                c_void_p],
+    ),
+    "se12_step_paged_attention_workspace": (c_i64, [c_void_p, c_void_p, c_i32]),
+    "se12_step_paged_attention": (
+        c_i32, [c_void_p, c_void_p, c_void_p, c_i64, c_void_p, c_i32, ctypes.c_float, ctypes.c_float, c_i32, c_void_p, c_i64,
+                c_void_p],
+    ),
+    "se12_step_logprobs_workspace": (c_i64, [c_i32, c_i32, c_i32]),
+    "se12_step_logprobs": (
+        c_i32, [c_void_p, c_i32, c_i64, c_i32, c_i32, ctypes.c_float, c_void_p, c_i32, c_void_p, c_void_p, c_void_p, c_void_p,
+                c_void_p, c_i64, c_void_p],
+    ),
 }
 
 STEP_BF16 = 0
 STEP_F32 = 1
+STEP_E4M3 = 2
 
 _lib: ctypes.CDLL | None = None
 

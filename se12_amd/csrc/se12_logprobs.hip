@@ -1,0 +1,410 @@
+// Log probabilities of given tokens, entropy and the most likely alternatives of
+// rows of logits. Mathematics: z = cap tanh(x / cap) or x; with a reference m,
+// S = sum e^(z - m) and W = sum e^(z - m) (m - z), both of one sign, log p_i =
+// z_i - m - log S and the entropy is log S + W / S. m is a maximum met so far, or
+// up to kSlack below it.
+//
+// One pass over the logits. A wave takes kChunk of them at a time, 16 to a lane,
+// the next chunk's loads in flight. Alternatives: a key per logit, its bits in an
+// order that compares as the logits do, then the index from the highest, so no two
+// are equal and equal logits go by the lower index. A wave keeps candidates in LDS,
+// keys above the top-th best so far; when 128 are full each counts the keys above
+// it, which is its place, and the best stay. The first chunk's bar is the top-th
+// best of the lanes' own best: what passes it lies in `top` lanes. After that a
+// chunk costs a comparison of its largest logit with the bar, and about
+// top ln(length / chunk) logits of a row pass.
+// The waves of a block and the blocks of a row merge the same way, the latter in a
+// second launch, where rows are too few to fill the card with a block each.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "se12_step.h"
+#include "se12_step_math.hpp"
+
+namespace se12step {
+
+constexpr int kLpThreads = 256;
+constexpr int kLpWaves = kLpThreads / 64;
+constexpr int kLpPer = 16;                     // logits of a lane and chunk
+constexpr int kChunk = 64 * kLpPer;
+constexpr int kMaxTop = 32;
+constexpr int kKeys = 128;                     // of a wave's buffer: 32 best and a ballot's 64 fit
+constexpr int kBlocksWanted = 1024;            // four to a CU
+constexpr float kLpSlack = 8.0f;
+
+struct Stats {
+    float m, s, w;
+};
+
+struct LogprobArgs {
+    const void* logits;
+    int64_t stride;
+    int vocab, top, slices, slice;             // slice: logits of a block, a multiple of kLpWaves * kChunk
+    float cap, inv_cap2;                       // inv_cap2: 2 log2(e) / cap
+    const int64_t* tokens;
+    float* logprobs;
+    float* entropy;
+    float* top_logprobs;
+    int64_t* top_ids;
+    Stats* stats;                              // [rows][slices]
+    uint64_t* keys;                            // [rows][slices][top]
+};
+
+// bits that compare as the numbers do (0 for nothing, 1 for a NaN)
+__device__ __forceinline__ uint32_t order_of(float x) {
+    const uint32_t u = __float_as_uint(x + 0.0f);   // -0 ties with 0
+    return x != x ? 1u : (u >> 31 ? ~u : u | 0x80000000u);
+}
+
+__device__ __forceinline__ float number_of(uint32_t order) {
+    return order <= 1u ? __builtin_nanf("") : __uint_as_float(order >> 31 ? order & 0x7FFFFFFFu : ~order);
+}
+
+__device__ __forceinline__ uint64_t key_of(float x, int i) { return ((uint64_t)order_of(x) << 32) | (uint32_t)~i; }
+
+__device__ __forceinline__ uint64_t read_lane64(uint64_t v, int l) {
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)v, l);
+}
+
+// LDS is written and read by lanes of one wave, in order
+__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
+// A wave's best keys. buf: kKeys of LDS; the first n are candidates.
+struct Best {
+    uint64_t* buf;
+    uint64_t bar;      // keys above it count
+    int n, top;
+
+    __device__ __forceinline__ void reset(uint64_t* b, int k) {
+        buf = b;
+        bar = 0;
+        n = 0;
+        top = k;
+    }
+
+    // The best `top` to the front, in order.
+    __device__ __forceinline__ void settle() {
+        const int lane = threadIdx.x & 63;
+        wave_fence();
+        const uint64_t a = lane < n ? buf[lane] : 0, b = lane + 64 < n ? buf[lane + 64] : 0;
+        int above_a = 0, above_b = 0;
+        for (int i = 0; i < n; ++i) {
+            const uint64_t k = buf[i];
+            above_a += k > a;
+            above_b += k > b;
+        }
+        wave_fence();
+        if (lane < n && above_a < top) buf[above_a] = a;
+        if (lane + 64 < n && above_b < top) buf[above_b] = b;
+        wave_fence();
+        n = min(n, top);
+        if (n == top) bar = buf[top - 1];
+        bar = read_lane64(bar, 0);
+    }
+
+    __device__ __forceinline__ void offer(uint64_t key) {
+        uint64_t in = __builtin_amdgcn_ballot_w64(key > bar);
+        if (!in) return;
+        if (n + __builtin_popcountll(in) > kKeys) {
+            settle();
+            in = __builtin_amdgcn_ballot_w64(key > bar);
+        }
+        if (key > bar) buf[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0))] = key;
+        n += __builtin_popcountll(in);
+    }
+
+    // the bar below which no key of the lanes' best can be among the best: the
+    // top-th of them (keys differ, so one less lets it pass itself)
+    __device__ __forceinline__ void bar_of_lanes(uint64_t best) {
+        int above = 0;
+        for (int i = 0; i < 64; ++i) above += read_lane64(best, i) > best;
+        const uint64_t at = __builtin_amdgcn_ballot_w64(above == top - 1 && best > 0);
+        bar = at ? read_lane64(best, __builtin_ctzll(at)) - 1 : 0;
+    }
+};
+
+__device__ __forceinline__ Stats join(Stats a, Stats b) {
+    const float m = fmaxf(a.m, b.m);
+    if (m == -INFINITY) return {m, a.s + b.s, a.w + b.w};
+    // (of m = -inf there is no sum; a NaN stays one)
+    const float da = a.m == -INFINITY ? 0.0f : m - a.m, db = b.m == -INFINITY ? 0.0f : m - b.m;
+    const float fa = __expf(-da), fb = __expf(-db);
+    return {m, a.s * fa + b.s * fb, (a.w + a.s * fminf(da, 1e30f)) * fa + (b.w + b.s * fminf(db, 1e30f)) * fb};
+}
+
+__device__ __forceinline__ Stats shfl_xor(Stats v, int o) { return {__shfl_xor(v.m, o, 64), __shfl_xor(v.s, o, 64), __shfl_xor(v.w, o, 64)}; }
+
+// the row's results, by one wave, from its sums and its best keys in order
+template <int DT>
+__device__ __forceinline__ void finish_row(const LogprobArgs& a, int row, Stats v, const Best& best) {
+    const int lane = threadIdx.x & 63;
+    const float log_s = logf(v.s);
+    auto capped = [&](float x) { return a.cap > 0.0f ? a.cap * tanhf(x / a.cap) : x; };
+    auto logprob = [&](float x) { return v.m == -INFINITY && v.s == 0.0f ? -INFINITY : (capped(x) - v.m) - log_s; };
+    if (lane == 0) {
+        const int64_t t = a.tokens[row];
+        float lp = -INFINITY;
+        if (t >= 0 && t < a.vocab) {
+            const int64_t at = (int64_t)row * a.stride + t;
+            lp = logprob(DT == SE12_STEP_F32 ? static_cast<const float*>(a.logits)[at] : bf16_to_f(static_cast<const uint16_t*>(a.logits)[at]));
+        } else if (v.s != v.s) {
+            lp = v.s;
+        }
+        a.logprobs[row] = lp;
+        a.entropy[row] = v.m == -INFINITY && v.s == 0.0f ? 0.0f : log_s + v.w / v.s;
+    }
+    if (lane < a.top) {
+        const uint64_t k = best.buf[lane];
+        a.top_ids[(int64_t)row * a.top + lane] = (int64_t)(uint32_t)~(uint32_t)k;
+        a.top_logprobs[(int64_t)row * a.top + lane] = logprob(number_of((uint32_t)(k >> 32)));
+    }
+}
+
+// the block's waves to wave 0; true there
+__device__ __forceinline__ bool join_waves(Stats& v, Best& best, uint64_t (*lists)[kMaxTop], Stats* sums) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, top = best.top;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v = join(v, shfl_xor(v, o));
+    if (top > 0) {
+        best.settle();
+        if (lane < top) lists[wave][lane] = lane < best.n ? best.buf[lane] : 0;
+    }
+    if (lane == 0) sums[wave] = v;
+    __syncthreads();
+    if (wave > 0) return false;
+    v = sums[0];
+    for (int k = 1; k < kLpWaves; ++k) v = join(v, sums[k]);
+    if (top > 0) {
+        best.n = 0;
+        best.bar = 0;
+        for (int k = 0; k < kLpWaves * top; k += 64) {
+            const int i = k + lane;
+            best.offer(i < kLpWaves * top ? lists[i / top][i % top] : 0);
+        }
+        best.settle();
+    }
+    return true;
+}
+
+template <int DT>
+__global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs a) {
+    constexpr int kVec = DT == SE12_STEP_F32 ? 4 : 8, kVecs = kLpPer / kVec, kSize = 16 / kVec;
+    __shared__ uint64_t bufs[kLpWaves][kKeys];
+    __shared__ uint64_t lists[kLpWaves][kMaxTop];
+    __shared__ Stats sums[kLpWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
+    const char* base = static_cast<const char*>(a.logits) + (int64_t)row * a.stride * kSize;
+    // whole 16-byte pieces of the row: logit i is value i + skew of them
+    const int skew = (int)((reinterpret_cast<uintptr_t>(base) & 15) / kSize);
+    const char* pieces = base - skew * kSize;
+    const int first = skew, last = skew + a.vocab;      // values of the pieces that are the row's
+    const int per_wave = a.slice / kLpWaves;
+    const int begin = slice * a.slice + wave * per_wave, end = min(begin + per_wave, last);
+    Best best;
+    best.reset(bufs[wave], a.top);
+    Stats v{-INFINITY, 0.0f, 0.0f};
+    uint4 next[kVecs];
+    // a piece that is not wholly the row's is read value by value
+    auto load = [&](int at) {
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) {
+            const int i = at + (j * 64 + lane) * kVec;
+            if (i >= first && i + kVec <= last) {
+                next[j] = *reinterpret_cast<const uint4*>(pieces + (int64_t)i * kSize);
+            } else {
+                uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) {
+                    if (i + e < first || i + e >= last) continue;
+                    if constexpr (DT == SE12_STEP_F32)
+                        w[e] = reinterpret_cast<const uint32_t*>(pieces)[i + e];
+                    else
+                        w[e / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(pieces)[i + e] << (16 * (e & 1));
+                }
+                next[j] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+    };
+    if (begin < end) load(begin);
+    for (int at = begin; at < end; at += kChunk) {
+        float x[kLpPer];
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) {
+            const uint32_t w[4] = {next[j].x, next[j].y, next[j].z, next[j].w};
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) {
+                if constexpr (DT == SE12_STEP_F32)
+                    x[j * kVec + e] = __uint_as_float(w[e]);
+                else
+                    x[j * kVec + e] = __uint_as_float(e & 1 ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16);
+            }
+        }
+        const bool edge = at < first || at + kChunk > last;
+        if (at + kChunk < end) load(at + kChunk);
+        auto index = [&](int k) { return at + (k / kVec * 64 + lane) * kVec + k % kVec; };
+        if (edge) {
+#pragma unroll
+            for (int k = 0; k < kLpPer; ++k) x[k] = index(k) < first || index(k) >= last ? -INFINITY : x[k];
+        }
+        float most = x[0];
+#pragma unroll
+        for (int k = 1; k < kLpPer; ++k) most = fmaxf(most, x[k]);
+        if (a.top > 0) {
+            if (at == begin) {
+                uint64_t mine = 0;
+#pragma unroll
+                for (int k = 0; k < kLpPer; ++k) {
+                    const bool valid = index(k) >= first && index(k) < last;
+                    const uint64_t key = valid ? key_of(x[k], index(k) - skew) : 0;
+                    mine = key > mine ? key : mine;
+                }
+                best.bar_of_lanes(mine);
+            }
+            // (a bar or a logit that is a NaN goes the long way as well)
+            const float bar = number_of((uint32_t)(best.bar >> 32));
+            if (at == begin || __builtin_amdgcn_ballot_w64(!(most <= bar)) != 0) {
+#pragma unroll
+                for (int k = 0; k < kLpPer; ++k) {
+                    const bool valid = index(k) >= first && index(k) < last;
+                    best.offer(valid ? key_of(x[k], index(k) - skew) : 0);
+                }
+            }
+        }
+        if (a.cap > 0.0f) {
+            // cap tanh(x / cap) = cap - 2 cap / (1 + e^(2 x / cap))
+#pragma unroll
+            for (int k = 0; k < kLpPer; ++k)
+                x[k] = a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[k] * a.inv_cap2));
+            most = a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(most * a.inv_cap2));
+            if (edge) {
+#pragma unroll
+                for (int k = 0; k < kLpPer; ++k) x[k] = index(k) < first || index(k) >= last ? -INFINITY : x[k];
+            }
+        }
+        if (__builtin_amdgcn_ballot_w64(most > v.m + kLpSlack) != 0) {
+            const float to = fmaxf(v.m, wave_max(most));
+            const float d = v.m == -INFINITY ? 0.0f : to - v.m, f = __expf(-d);
+            v.w = (v.w + v.s * fminf(d, 1e30f)) * f;
+            v.s *= f;
+            v.m = to;
+        }
+        if (v.m != -INFINITY) {
+#pragma unroll
+            for (int k = 0; k < kLpPer; ++k) {
+                const float d = v.m - x[k], e = __expf(-d);
+                v.s += e;
+                v.w += e * fminf(d, 1e30f);
+            }
+        } else {
+            // nothing but -inf so far, unless there is a NaN
+#pragma unroll
+            for (int k = 0; k < kLpPer; ++k) v.s = x[k] != x[k] ? x[k] : v.s;
+        }
+    }
+    if (!join_waves(v, best, lists, sums)) return;
+    if (a.slices == 1) {
+        finish_row<DT>(a, row, v, best);
+        return;
+    }
+    if (lane == 0) a.stats[blockIdx.x] = v;
+    if (lane < a.top) a.keys[(int64_t)blockIdx.x * a.top + lane] = lane < best.n ? best.buf[lane] : 0;
+}
+
+// the slices of a row
+template <int DT>
+__global__ __launch_bounds__(kLpThreads) void logprobs_join_kernel(LogprobArgs a) {
+    __shared__ uint64_t bufs[kLpWaves][kKeys];
+    __shared__ uint64_t lists[kLpWaves][kMaxTop];
+    __shared__ Stats sums[kLpWaves];
+    const int row = blockIdx.x;
+    Best best;
+    best.reset(bufs[threadIdx.x >> 6], a.top);
+    Stats v{-INFINITY, 0.0f, 0.0f};
+    for (int i = threadIdx.x; i < a.slices; i += kLpThreads) v = join(v, a.stats[(int64_t)row * a.slices + i]);
+    const int count = a.slices * a.top;
+    for (int k = 0; k < count; k += kLpThreads) {
+        const int i = k + threadIdx.x;
+        best.offer(i < count ? a.keys[(int64_t)row * count + i] : 0);
+    }
+    if (join_waves(v, best, lists, sums)) finish_row<DT>(a, row, v, best);
+}
+
+}  // namespace se12step
+
+using namespace se12step;
+
+namespace {
+
+struct LpLayout {
+    int slices, slice;
+    int64_t stats_bytes, total;
+};
+
+// Slices of a row: as many blocks as fill the card, none smaller than a chunk a
+// wave. (+ 7: a row that begins inside a 16-byte piece)
+LpLayout logprobs_layout(int32_t rows, int32_t vocab, int32_t top) {
+    constexpr int64_t unit = (int64_t)kLpWaves * kChunk;
+    const int64_t units = ((int64_t)vocab + 7 + unit - 1) / unit;
+    const int64_t want = std::min<int64_t>(units, std::max(1, kBlocksWanted / rows));
+    const int64_t slice = (units + want - 1) / want * unit;
+    LpLayout l;
+    l.slice = (int)slice;
+    l.slices = (int)(((int64_t)vocab + 7 + slice - 1) / slice);
+    l.stats_bytes = ((int64_t)rows * l.slices * (int64_t)sizeof(Stats) + 15) / 16 * 16;
+    l.total = l.slices == 1 ? 0 : l.stats_bytes + (int64_t)rows * l.slices * top * (int64_t)sizeof(uint64_t);
+    return l;
+}
+
+const char* logprobs_shape_error(int32_t rows, int32_t vocab, int32_t top) {
+    if (rows < 0 || vocab < 1 || vocab > (1 << 30)) return "bad shape";
+    if (top < 0 || top > kMaxTop || top > vocab) return "top must be 0 to 32 and at most vocab";
+    return nullptr;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t se12_step_logprobs_workspace(int32_t rows, int32_t vocab, int32_t top) {
+    if (const char* e = logprobs_shape_error(rows, vocab, top)) return step_fail("se12_step_logprobs_workspace", e);
+    return rows == 0 ? 0 : logprobs_layout(rows, vocab, top).total;
+}
+
+int se12_step_logprobs(const void* logits, int32_t dtype, int64_t stride, int32_t rows, int32_t vocab, float softcap,
+                       const int64_t* tokens, int32_t top, float* logprobs, float* entropy, float* top_logprobs,
+                       int64_t* top_ids, void* workspace, int64_t workspace_bytes, void* stream) {
+    const char* fn = "se12_step_logprobs";
+    if (const char* e = logprobs_shape_error(rows, vocab, top)) return step_fail(fn, e);
+    if (rows == 0) return SE12_STEP_OK;
+    if (!logits || !tokens || !logprobs || !entropy || (top > 0 && (!top_logprobs || !top_ids))) return step_fail(fn, "NULL argument");
+    if (dtype != SE12_STEP_BF16 && dtype != SE12_STEP_F32) return step_fail(fn, "logits must be BF16 or FP32");
+    if (stride < vocab) return step_fail(fn, "rows overlap");
+    if (!(softcap >= 0.0f) || !(softcap < 1e30f)) return step_fail(fn, "softcap must be 0 or more");
+    if (reinterpret_cast<uintptr_t>(logits) % (dtype == SE12_STEP_F32 ? 4 : 2) || reinterpret_cast<uintptr_t>(tokens) % 8 ||
+        reinterpret_cast<uintptr_t>(logprobs) % 4 || reinterpret_cast<uintptr_t>(entropy) % 4 ||
+        reinterpret_cast<uintptr_t>(top_logprobs) % 4 || reinterpret_cast<uintptr_t>(top_ids) % 8)
+        return step_fail(fn, "misaligned tensor");
+    const LpLayout l = logprobs_layout(rows, vocab, top);
+    if ((int64_t)rows * l.slices > INT32_MAX) return step_fail(fn, "too many rows");
+    if (l.total > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < l.total))
+        return step_fail(fn, "workspace missing, misaligned or too small");
+    constexpr float kLog2E = 1.4426950408889634f;
+    const LogprobArgs a{logits, stride, vocab, top, l.slices, l.slice, softcap, softcap > 0.0f ? 2.0f * kLog2E / softcap : 0.0f,
+                        tokens, logprobs, entropy, top_logprobs, top_ids, static_cast<Stats*>(workspace),
+                        reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + (l.slices > 1 ? l.stats_bytes : 0))};
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const dim3 grid((uint32_t)((int64_t)rows * l.slices));
+    if (dtype == SE12_STEP_F32) {
+        hipLaunchKernelGGL(logprobs_kernel<SE12_STEP_F32>, grid, dim3(kLpThreads), 0, st, a);
+        if (l.slices > 1) hipLaunchKernelGGL(logprobs_join_kernel<SE12_STEP_F32>, dim3(rows), dim3(kLpThreads), 0, st, a);
+    } else {
+        hipLaunchKernelGGL(logprobs_kernel<SE12_STEP_BF16>, grid, dim3(kLpThreads), 0, st, a);
+        if (l.slices > 1) hipLaunchKernelGGL(logprobs_join_kernel<SE12_STEP_BF16>, dim3(rows), dim3(kLpThreads), 0, st, a);
+    }
+    return step_launched();
+}
+
+}  // extern "C"

@@ -1,0 +1,150 @@
+"""token_logprobs on the GPU against float64.
+
+Tolerance of a log probability and of the entropy, from the FP32 arithmetic: a lane
+sums vocab / 256 + 64 terms one after the other (2^-24 of the sum each), a term's
+exponent is off by 2^-23 of |m - z| < 32 in the terms that matter (2^-18), the cap's
+reciprocal form by 2^-21 cap in z; the log and the difference by 2^-23 of their
+size."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _tol(vocab: int, cap: float, size: torch.Tensor) -> torch.Tensor:
+    return (vocab / 256 + 64) * 2.0 ** -24 + 2.0 ** -18 + cap * 2.0 ** -20 + 2.0 ** -22 * size.abs()
+
+
+def _check(logits, tokens, top, cap):
+    from se12_amd.logprobs import token_logprobs
+
+    r = token_logprobs(logits, tokens, top=top, softcap=cap)
+    x, t = logits.cpu().double(), tokens.cpu()
+    z = cap * torch.tanh(x / cap) if cap else x
+    z = z - z.amax(1, keepdim=True)      # (64 bits hold no log of a sum beside 3e38 either)
+    lp = z - torch.logsumexp(z, 1, keepdim=True)
+    vocab = x.shape[1]
+    want = lp[torch.arange(x.shape[0]), t]
+    assert ((r.logprobs.cpu().double() - want).abs() <= _tol(vocab, cap, want)).all()
+    ent = torch.special.entr(lp.exp()).sum(1)
+    # W / S is a weighted mean of m - z: the relative errors of a sum apply to it, up to log(vocab)
+    assert ((r.entropy.cpu().double() - ent).abs() <= 2 * (1 + math.log(vocab)) * _tol(vocab, cap, ent)).all()
+    assert r.top_ids.shape == (x.shape[0], top) and r.top_ids.dtype == torch.int64
+    ids = torch.stack([torch.tensor(sorted(range(vocab), key=lambda i: (-row[i], i))[:top], dtype=torch.int64) for row in x.tolist()]) \
+        if vocab * x.shape[0] < 40_000 else torch.sort(x, dim=1, descending=True, stable=True).indices[:, :top]
+    assert torch.equal(r.top_ids.cpu(), ids)
+    want = lp.gather(1, ids)
+    got = r.top_logprobs.cpu().double()
+    fine = want.isfinite()
+    assert torch.equal(fine, got.isfinite()) and ((got - want).abs()[fine] <= _tol(vocab, cap, want[fine])).all()
+
+
+def _logits(gpu, rows, vocab, dtype, seed, scale=4.0):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    x = (torch.randn((rows, vocab), generator=g) * scale).to(dtype)
+    t = torch.randint(0, vocab, (rows,), generator=g)
+    return x.to(gpu), t.to(gpu)
+
+
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (3, 2, 2), (5, 31, 0), (2, 33, 32), (1, 255, 7), (4, 1023, 20), (3, 1025, 32),
+                                            (2, 4097, 5), (7, 9001, 20), (1, 256000, 20), (300, 5003, 1)])
+def test_logprobs(gpu, rows, vocab, top, dtype, cap):
+    x, t = _logits(gpu, rows, vocab, dtype, rows * 1000 + vocab)
+    _check(x, t, top, cap)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_that_begin_anywhere(gpu, dtype):
+    """Strided rows, of an odd length, from an odd offset: 16-byte pieces cross both ends of a row."""
+    big, _ = _logits(gpu, 6, 5000, dtype, 1)
+    for first, vocab in ((1, 4001), (3, 4093), (7, 999), (5, 8)):
+        _check(big[:, first:first + vocab], torch.tensor([0, vocab - 1, vocab // 2, 1, 2, 3], device=gpu) % vocab, 8, 0.0)
+
+
+def test_more_rows_than_blocks_fill_the_card(gpu):
+    x, t = _logits(gpu, 1500, 2100, torch.bfloat16, 2)
+    _check(x, t, 3, 0.0)
+
+
+def test_equal_logits_go_by_the_lower_index(gpu):
+    for vocab in (64, 5000, 70000):
+        x = torch.zeros((2, vocab), device=gpu)
+        x[1, ::3] = 1.0
+        x[0, 1::2] = -0.0
+        _check(x, torch.tensor([0, 1], device=gpu), 32, 0.0)
+        _check(x.to(torch.bfloat16), torch.tensor([0, 1], device=gpu), 32, 5.0)
+    # ascending and descending: every chunk, or only the first, passes the bar
+    x = torch.arange(30000, device=gpu).float()[None] / 1000
+    _check(torch.cat([x, x.flip(1)]), torch.tensor([29999, 0], device=gpu), 20, 0.0)
+
+
+def test_masked_logits(gpu):
+    x, t = _logits(gpu, 8, 20000, torch.float32, 3)
+    allowed = torch.rand((8, 20000), device=gpu) < 0.01
+    allowed[3] = False
+    allowed[3, 17] = True                       # one token is certain
+    allowed[4] = False
+    allowed[4, :2] = True
+    t[3], t[4] = 17, 1
+    allowed.scatter_(1, t[:, None], True)
+    _check(x.masked_fill(~allowed, float("-inf")), t, 20, 0.0)
+    # the type's lowest value is a logit like others: a row of it alone is uniform
+    low = torch.full((2, 3000), torch.finfo(torch.float32).min, device=gpu)
+    low[1, 5] = 3.0
+    _check(low, torch.tensor([7, 5], device=gpu), 4, 0.0)
+    low = torch.full((1, 3000), torch.finfo(torch.bfloat16).min, device=gpu, dtype=torch.bfloat16)
+    _check(low, torch.tensor([7], device=gpu), 4, 0.0)
+
+
+def test_rows_without_a_distribution(gpu):
+    from se12_amd.logprobs import token_logprobs
+
+    for vocab in (40, 9000):
+        x, _ = _logits(gpu, 6, vocab, torch.float32, 4)
+        x[0] = float("-inf")
+        x[1, 33] = float("nan")
+        x[2, 7] = float("inf")
+        x[3] = float("nan")
+        x[4] = float("-inf")
+        x[4, 9] = float("nan")
+        t = torch.tensor([3, 2, 1, 0, 0, vocab], device=gpu)
+        r = token_logprobs(x, t, top=5)
+        assert r.logprobs[0] == float("-inf") and r.entropy[0] == 0 and (r.top_logprobs[0] == float("-inf")).all()
+        assert r.top_ids[0].tolist() == [0, 1, 2, 3, 4] and r.top_ids[3].tolist() == [0, 1, 2, 3, 4]
+        assert r.top_ids[4].tolist() == [0, 1, 2, 3, 4]
+        for i in (1, 2, 3, 4):
+            assert r.logprobs[i].isnan() and r.entropy[i].isnan() and r.top_logprobs[i].isnan().all()
+        row = x[1].clone()
+        row[33] = float("-inf")
+        assert r.top_ids[1].tolist() == torch.sort(row, descending=True, stable=True).indices[:5].tolist()
+        assert r.top_ids[2][0] == 7
+        # a token that there is not
+        assert r.logprobs[5] == float("-inf") and r.entropy[5].isfinite()
+        assert token_logprobs(x[5:], torch.tensor([-100], device=gpu)).logprobs[0] == float("-inf")
+
+
+def test_no_rows_and_a_graph(gpu):
+    from se12_amd.logprobs import token_logprobs
+
+    r = token_logprobs(torch.empty((0, 50), device=gpu), torch.empty(0, dtype=torch.int64, device=gpu), top=3)
+    assert r.logprobs.shape == (0,) and r.top_ids.shape == (0, 3)
+    x, t = _logits(gpu, 2, 30000, torch.float32, 5)
+    token_logprobs(x, t, top=4)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        r = token_logprobs(x, t, top=4, softcap=20.0)
+    for i in range(4):
+        x.copy_(_logits(gpu, 2, 30000, torch.float32, 6 + i)[0])
+        graph.replay()
+        e = token_logprobs(x, t, top=4, softcap=20.0)
+        assert torch.equal(r.logprobs, e.logprobs) and torch.equal(r.top_ids, e.top_ids) and torch.equal(r.entropy, e.entropy)
+        assert torch.equal(r.top_logprobs, e.top_logprobs)

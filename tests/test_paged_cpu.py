@@ -1,0 +1,135 @@
+"""What the paged cache, its attention and the log probabilities refuse before any
+launch: the C entries with made-up pointers (never followed: each call has something
+wrong with it), and the Python wrappers with tensors on the CPU."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+import paged_oracle as o
+from se12_amd import _native as nat
+
+P = 4096      # a pointer no call reads
+
+
+def _pages(**kw):
+    f = dict(k=P, v=P, k_scale=P, v_scale=P, dtype=nat.STEP_E4M3, pages=10, page_size=64, kv_heads=4, head_dim=128)
+    f.update(kw)
+    return nat.StepPages(*f.values())
+
+
+def _batch(**kw):
+    f = dict(page_table=P, table_stride=8, lengths=P, starts=P, table_width=8, sequences=3, tokens=3, max_new=1)
+    f.update(kw)
+    return nat.StepBatch(*f.values())
+
+
+BAD_SHARED = [
+    (dict(k=None), {}, "NULL cache"), (dict(dtype=1), {}, "BF16 or E4M3"), (dict(k_scale=None), {}, "needs scales"),
+    (dict(page_size=48), {}, "page_size"), (dict(page_size=8), {}, "page_size"), (dict(head_dim=96), {}, "head_dim"),
+    (dict(pages=0), {}, "cache shape"), (dict(kv_heads=0), {}, "cache shape"), (dict(kv_heads=3), {}, "multiple of kv_heads"),
+    (dict(k=P + 8), {}, "16-byte aligned"), (dict(v_scale=P + 2), {}, "misaligned"),
+    ({}, dict(page_table=None), "NULL batch"), ({}, dict(lengths=None), "NULL batch"), ({}, dict(starts=None), "NULL batch"),
+    ({}, dict(sequences=0), "batch shape"), ({}, dict(sequences=65537), "batch shape"), ({}, dict(tokens=-1), "batch shape"),
+    ({}, dict(max_new=0), "batch shape"), ({}, dict(table_stride=7), "batch shape"), ({}, dict(starts=P + 1), "misaligned"),
+    ({}, dict(table_width=2 ** 25, table_stride=2 ** 25), "2^30"),
+]
+
+
+@pytest.mark.parametrize("pages,batch,message", BAD_SHARED)
+def test_both_calls_refuse_bad_caches_and_batches(pages, batch, message):
+    lib, p, b = nat.lib(), _pages(**pages), _batch(**batch)
+    for call in (lambda: lib.se12_step_paged_append(ctypes.byref(p), ctypes.byref(b), P, P, P, nat.STEP_F32, 1024, 512, 512, 8, P, 128, P,
+                                                    None),
+                 lambda: lib.se12_step_paged_attention(ctypes.byref(p), ctypes.byref(b), P, 1024, P, 8, 0.1, 0.0, 0, P, 1 << 30, None),
+                 lambda: lib.se12_step_paged_attention_workspace(ctypes.byref(p), ctypes.byref(b), 8)):
+        with pytest.raises(nat.Se12Error, match=message.replace("^", r"\^")):
+            nat.step_check(call())
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(k=None), "NULL"), (dict(v=None), "NULL"), (dict(q_out=None), "NULL"), (dict(inv=None), "NULL"), (dict(dtype=2), "BF16 or FP32"),
+    (dict(rotary=12), "rotary"), (dict(rotary=136), "rotary"), (dict(rotary=-8), "rotary"), (dict(ks=510), "multiple of 4"),
+    (dict(vs=508), "hold all heads"), (dict(qs=1020), "hold all heads"), (dict(heads=6), "kv_heads"), (dict(k=P + 8), "misaligned"),
+    (dict(q_out=P + 4), "misaligned"), (dict(inv=P + 4), "misaligned"),
+])
+def test_append_refuses(change, message):
+    f = dict(q=P, k=P, v=P, dtype=nat.STEP_F32, qs=1024, ks=512, vs=512, heads=8, inv=P, rotary=128, q_out=P)
+    f.update(change)
+    with pytest.raises(nat.Se12Error, match=message):
+        nat.step_check(nat.lib().se12_step_paged_append(ctypes.byref(_pages()), ctypes.byref(_batch()), *f.values(), None))
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(q=None), "NULL"), (dict(out=None), "NULL"), (dict(qs=1016), "hold all heads"), (dict(qs=1028), "multiple of 8"),
+    (dict(cap=-1.0), "softcap"), (dict(cap=float("nan")), "softcap"), (dict(window=-1), "window"), (dict(q=P + 8), "misaligned"),
+    (dict(out=P + 4), "misaligned"), (dict(ws=None), "workspace"), (dict(ws=P + 128), "workspace"), (dict(size=100), "workspace"),
+    (dict(heads=7), "kv_heads"),
+])
+def test_attention_refuses(change, message):
+    f = dict(q=P, qs=1024, out=P, heads=8, scaling=0.1, cap=0.0, window=0, ws=P, size=1 << 30)
+    f.update(change)
+    with pytest.raises(nat.Se12Error, match=message):
+        nat.step_check(nat.lib().se12_step_paged_attention(ctypes.byref(_pages()), ctypes.byref(_batch()), *f.values(), None))
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(vocab=0), "bad shape"), (dict(rows=-1), "bad shape"), (dict(top=33), "top"), (dict(top=-1), "top"), (dict(vocab=4, top=5), "top"),
+    (dict(logits=None), "NULL"), (dict(tokens=None), "NULL"), (dict(tl=None), "NULL"), (dict(dtype=2), "BF16 or FP32"),
+    (dict(stride=999), "overlap"), (dict(cap=-1.0), "softcap"), (dict(logits=P + 2), "misaligned"), (dict(tokens=P + 4), "misaligned"),
+    (dict(vocab=50000, stride=50000, ws=None), "workspace"), (dict(vocab=50000, stride=50000, size=8), "workspace"),
+])
+def test_logprobs_refuse(change, message):
+    f = dict(logits=P, dtype=nat.STEP_F32, stride=1000, rows=2, vocab=1000, cap=0.0, tokens=P, top=5, lp=P, ent=P, tl=P, ti=P, ws=P,
+             size=1 << 30)
+    f.update(change)
+    with pytest.raises(nat.Se12Error, match=message):
+        nat.step_check(nat.lib().se12_step_logprobs(*f.values(), None))
+
+
+def test_calls_without_tokens_or_rows_do_nothing():
+    lib, p, b = nat.lib(), _pages(), _batch(tokens=0)
+    assert lib.se12_step_paged_append(ctypes.byref(p), ctypes.byref(b), P, P, P, nat.STEP_F32, 1024, 512, 512, 8, P, 128, P, None) == 0
+    assert lib.se12_step_paged_attention(ctypes.byref(p), ctypes.byref(b), P, 1024, P, 8, 0.1, 0.0, 0, None, 0, None) == 0
+    assert lib.se12_step_paged_attention_workspace(ctypes.byref(p), ctypes.byref(b), 8) == 0
+    assert lib.se12_step_logprobs(None, 0, 10, 0, 10, 0.0, None, 0, None, None, None, None, None, 0, None) == 0
+
+
+def test_wrappers_refuse_tensors_on_the_cpu_and_bad_shapes():
+    from se12_amd.logprobs import token_logprobs
+    from se12_amd.paged import PagedBatch, PagedKvCache
+
+    i32 = torch.zeros((2, 3), dtype=torch.int32)
+    with pytest.raises(ValueError, match="HIP device"):
+        PagedBatch(i32, i32[0, :2], i32[0])
+    with pytest.raises(ValueError, match="int32"):
+        PagedBatch(i32.long(), i32[0, :2], i32[0])
+    k = torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="HIP device"):
+        PagedKvCache.from_tensors(k, torch.zeros((4, 2, 64, 16), dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="v must be"):
+        PagedKvCache.from_tensors(k, k)
+    with pytest.raises(ValueError, match="needs k_scale"):
+        PagedKvCache.from_tensors(k.to(torch.float8_e4m3fn), torch.zeros((4, 2, 64, 16), dtype=torch.float8_e4m3fn))
+    with pytest.raises(ValueError, match="page_size"):
+        PagedKvCache.from_tensors(k[:, :, :8], k)
+    with pytest.raises(ValueError, match="goes with"):
+        PagedKvCache.from_tensors(k, torch.zeros((4, 2, 64, 16), dtype=torch.bfloat16), torch.ones((4, 2)), torch.ones((4, 2)))
+    with pytest.raises(ValueError, match="HIP device"):
+        token_logprobs(torch.zeros((2, 5)), torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(ValueError, match="bfloat16 or float32"):
+        token_logprobs(torch.zeros((2, 5), dtype=torch.float16), torch.zeros(2, dtype=torch.int64))
+
+
+def test_the_oracle_rounds_as_the_type_does():
+    """Every E4M3 value, every midpoint between two of them and its neighbours, against torch's conversion on the CPU."""
+    values = torch.arange(0, 127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    mid = (values[1:] + values[:-1]) / 2
+    x = torch.cat([values, mid, mid * (1 + 1e-6), mid * (1 - 1e-6)])
+    x = torch.cat([x, -x])
+    assert torch.equal(o.e4m3(x), x.float().to(torch.float8_e4m3fn).double())
+    assert o.scale_for(torch.tensor([448.0])) == 1.0 and o.scale_for(torch.tensor([448.1])) == 2.0
+    assert o.scale_for(torch.tensor([0.0, float("nan")])) == 2.0 ** -100 and o.scale_for(torch.tensor([1e30, float("inf")])) == 2.0 ** 91
