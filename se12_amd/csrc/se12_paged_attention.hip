@@ -23,101 +23,10 @@
 
 namespace se12step {
 
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-typedef float floatx4_t __attribute__((ext_vector_type(4)));
-
 constexpr int kColumns = 16;          // columns of a unit
+constexpr int kFewColumns = 64;       // of a sequence and KV head; with more it is se12_paged_prompt.hip's
 constexpr int kAttendThreads = 256;   // four waves, each with tiles of its own
 constexpr int kWorkers = 256 * 4;     // waves of a launch: one per SIMD
-constexpr float kSlack = 8.0f;        // base 2
-
-struct AttendArgs {
-    const uint16_t* q;
-    int64_t q_stride;
-    uint16_t* out;
-    const void* kc;
-    const void* vc;
-    const float* k_scale;
-    const float* v_scale;
-    Batch b;
-    int heads, kvh, group, pages, page_log2, window;
-    float c1, cap;       // scores: c1 x (no cap), or cap - 2 cap / (1 + 2^(c1 x)), base 2
-    float* part;         // [workers][2][columns][d] sums, then [workers][2][columns][2]: m, l
-    int workers, columns;
-};
-
-// What a lane holds of a tile, by the cache's type: 16 bytes of each key row's
-// 64-byte part, and the lane's keys of a value column, 16 bytes as well.
-template <int CT>
-struct Form {
-    static constexpr int kPer = CT == SE12_STEP_E4M3 ? 16 : 8;   // values of 16 bytes, and keys of a lane
-    static constexpr int kTile = 4 * kPer;                        // keys of a tile
-    static constexpr int kHalves = kPer / 8;                      // matrix operands of a piece
-    static constexpr int kWord = kPer / 4;                        // values of a 32-bit word
-};
-
-template <int CT>
-__device__ __forceinline__ uint4 load_piece(const void* p, int64_t i) {
-    return *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + i * (16 / Form<CT>::kPer));
-}
-
-// values 8 h .. 8 h + 7 of a piece in BF16 (every E4M3 value is one)
-template <int CT>
-__device__ __forceinline__ bf16x8_t operand(const uint4 v, int h) {
-    if constexpr (CT == SE12_STEP_E4M3) {
-        const uint32_t a = h ? v.z : v.x, b = h ? v.w : v.y;
-        const bf16x2_t w0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false);
-        const bf16x2_t w1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true);
-        const bf16x2_t w2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false);
-        const bf16x2_t w3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true);
-        return bf16x8_t{w0.x, w0.y, w1.x, w1.y, w2.x, w2.y, w3.x, w3.y};
-    } else {
-        return __builtin_bit_cast(bf16x8_t, v);
-    }
-}
-
-// the bits of values from .. to - 1 of the kWord values of a word
-template <int CT>
-__device__ __forceinline__ uint32_t word_mask(int from, int to) {
-    constexpr int per = Form<CT>::kWord, bits = 32 / per;
-    const uint32_t below_to = to <= 0 ? 0u : to >= per ? ~0u : (1u << (bits * to)) - 1u;
-    const uint32_t below_from = from <= 0 ? 0u : from >= per ? ~0u : (1u << (bits * from)) - 1u;
-    return below_to & ~below_from;
-}
-
-template <int CT>
-__device__ __forceinline__ uint4 piece_mask(int from, int to) {
-    constexpr int per = Form<CT>::kWord;
-    return make_uint4(word_mask<CT>(from, to), word_mask<CT>(from - per, to - per), word_mask<CT>(from - 2 * per, to - 2 * per),
-                      word_mask<CT>(from - 3 * per, to - 3 * per));
-}
-
-__device__ __forceinline__ uint4 masked(const uint4 v, const uint4 m) { return make_uint4(v.x & m.x, v.y & m.y, v.z & m.z, v.w & m.w); }
-
-// bit 7 of every value (bit 15 of a BF16 one) that is a NaN or an infinity:
-// exponent all ones; E4M3: all ones but the sign
-template <int CT>
-__device__ __forceinline__ uint32_t no_numbers(uint32_t w) {
-    return CT == SE12_STEP_E4M3 ? ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u : ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
-}
-
-template <int CT>
-__device__ __forceinline__ bool has_no_number(const uint4 v) {
-    return (no_numbers<CT>(v.x) | no_numbers<CT>(v.y) | no_numbers<CT>(v.z) | no_numbers<CT>(v.w)) != 0;
-}
-
-template <int CT>
-__device__ __forceinline__ uint32_t numbers_only(uint32_t w) {
-    return CT == SE12_STEP_E4M3 ? w & ~((no_numbers<CT>(w) >> 7) * 0xFFu) : w & ~((no_numbers<CT>(w) >> 15) * 0xFFFFu);
-}
-
-// BF16 values: 1 where a value is a NaN (kind 0), +inf (1) or -inf (2), else 0
-__device__ __forceinline__ uint32_t where_no_number(uint32_t w, int kind) {
-    const uint32_t all = no_numbers<SE12_STEP_BF16>(w) >> 8, fraction = ((w & 0x007F007Fu) + 0x007F007Fu) & 0x00800080u;
-    const uint32_t is = kind == 0 ? all & fraction : kind == 1 ? all & ~fraction & ~(w >> 8) : all & ~fraction & (w >> 8);
-    return is * 0x7Fu;
-}
 
 // The work: units of up to 16 columns of one sequence and KV head, each a run of
 // key tiles; all units' tiles in one line (sequence, head, column unit, tile),
@@ -138,7 +47,8 @@ __device__ __forceinline__ SeqWork seq_work(const AttendArgs& a, int s) {
     w.keys = min(w.seq.len + w.seq.n, capacity);
     const int low = a.window > 0 ? max(0, w.seq.len - a.window + 1) : 0;
     w.tile0 = low / kTile;
-    w.units = (int)(((int64_t)w.seq.n * a.group + kColumns - 1) / kColumns);
+    const int columns = w.seq.n * a.group;
+    w.units = columns > a.few ? 0 : (columns + kColumns - 1) / kColumns;
     w.tiles = w.units > 0 ? max((w.keys + kTile - 1) / kTile - w.tile0, 1) : 0;
     return w;
 }
@@ -364,10 +274,6 @@ struct Attend {
     }
 };
 
-__device__ __forceinline__ void store4(uint16_t* p, float a, float b, float c, float d) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(f_to_bf16x2(a, b), f_to_bf16x2(c, d));
-}
-
 // a worker's sums of a run that is not a whole unit: slot 0 where the unit began
 // before its run, slot 1 where it goes on after it
 __device__ __forceinline__ int64_t part_at(const AttendArgs& a, int worker, int slot) { return ((int64_t)worker * 2 + slot) * a.columns; }
@@ -432,7 +338,7 @@ __global__ __launch_bounds__(kAttendThreads) void paged_join_kernel(AttendArgs a
     const int unit = (int)(blockIdx.x % max_units), kh = (int)(blockIdx.x / max_units % a.kvh), s = (int)(blockIdx.x / max_units / a.kvh);
     const int col = blockIdx.y, c = unit * kColumns + col;
     const SeqWork w = seq_work<kTile>(a, s);
-    if (c >= w.seq.n * a.group) return;
+    if (unit >= w.units || c >= w.seq.n * a.group) return;
     int64_t base = 0, total = 0;
     for (int s0 = 0; s0 < a.b.seqs; s0 += 64) {
         const int64_t mine = seq_tiles<kTile>(a, s0 + lane), upto = scan64(mine, lane);
@@ -490,20 +396,26 @@ int column_count(const Batch& b, int group) {
 int worker_count(const se12_step_pages* p, const Batch& b, int group) {
     // no more than there can be tiles
     const int64_t tiles = ((int64_t)b.width * p->page_size + 31) / 32;
-    const int64_t units = ((int64_t)b.max_new * group + kColumns - 1) / kColumns;
+    const int64_t units = (std::min<int64_t>((int64_t)b.max_new * group, kFewColumns) + kColumns - 1) / kColumns;
     int64_t all = tiles;
     for (const int64_t f : {(int64_t)b.seqs, (int64_t)p->kv_heads, units}) all = std::min<int64_t>(all * f, kWorkers);
     return (int)((all + 3) / 4 * 4);
 }
 
+int64_t few_bytes(const se12_step_pages* p, const Batch& b, int group) {
+    return ((int64_t)worker_count(p, b, group) * 2 * column_count(b, group) * (p->head_dim + 2) * (int64_t)sizeof(float) + 255) / 256 * 256;
+}
+
+bool any_many(const Batch& b, int group) { return (int64_t)b.max_new * group > kFewColumns; }
+
 int64_t part_bytes(const se12_step_pages* p, const Batch& b, int group) {
-    return (int64_t)worker_count(p, b, group) * 2 * column_count(b, group) * (p->head_dim + 2) * (int64_t)sizeof(float);
+    return few_bytes(p, b, group) + (any_many(b, group) ? prompt_part_bytes(b, p->kv_heads, group, p->page_size, p->head_dim) : 0);
 }
 
 template <int CT, int D>
 void launch_attend(const AttendArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((paged_attention_kernel<CT, D>), dim3(a.workers / (kAttendThreads / 64)), dim3(kAttendThreads), 0, st, a);
-    const int max_units = (int)(((int64_t)a.b.max_new * a.group + kColumns - 1) / kColumns);
+    const int max_units = (int)((std::min<int64_t>((int64_t)a.b.max_new * a.group, kFewColumns) + kColumns - 1) / kColumns);
     hipLaunchKernelGGL((paged_join_kernel<CT, D>), dim3((uint32_t)((int64_t)a.b.seqs * a.kvh * max_units), a.columns), dim3(kAttendThreads), 0,
                        st, a, max_units);
 }
@@ -532,12 +444,13 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
     const int group = heads / pages->kv_heads;
     if (reinterpret_cast<uintptr_t>(workspace) % 256 || !workspace || workspace_bytes < part_bytes(pages, b, group))
         return step_fail(fn, "workspace missing, misaligned or too small");
-    if ((int64_t)b.seqs * pages->kv_heads * (((int64_t)b.max_new * group + kColumns - 1) / kColumns) > INT32_MAX)
-        return step_fail(fn, "too many units");
+    if ((int64_t)b.seqs * pages->kv_heads * (kFewColumns / kColumns) > INT32_MAX || !prompt_fits(b, pages->kv_heads, group, pages->page_size))
+        return step_fail(fn, "too many sequences, tokens and heads for one launch");
     constexpr float kLog2E = 1.4426950408889634f;
     AttendArgs a{q, q_stride, out, pages->k, pages->v, pages->k_scale, pages->v_scale, b, heads, pages->kv_heads, group, pages->pages,
                  log2_of(pages->page_size), window, softcap > 0.0f ? 2.0f * scaling / softcap * kLog2E : scaling * kLog2E,
-                 softcap * kLog2E, static_cast<float*>(workspace), worker_count(pages, b, group), column_count(b, group)};
+                 softcap * kLog2E, static_cast<float*>(workspace), worker_count(pages, b, group), column_count(b, group), kFewColumns,
+                 prompt_splits(b, pages->kv_heads, group, pages->page_size)};
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const bool e4m3 = pages->dtype == SE12_STEP_E4M3;
     switch (pages->head_dim) {
@@ -549,6 +462,10 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
             break;
         default:
             e4m3 ? launch_attend<SE12_STEP_E4M3, 256>(a, st) : launch_attend<SE12_STEP_BF16, 256>(a, st);
+    }
+    if (any_many(b, group)) {
+        a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + few_bytes(pages, b, group));
+        launch_prompt(a, e4m3, pages->head_dim, st);
     }
     return step_launched();
 }

@@ -39,6 +39,105 @@ __device__ __forceinline__ int page_of(const Batch& b, int s, int c, int pages) 
     return (uint32_t)id < (uint32_t)pages ? id : -1;
 }
 
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef float floatx4_t __attribute__((ext_vector_type(4)));
+
+constexpr float kSlack = 8.0f;        // how far a score may pass the maximum it is taken from, base 2
+
+struct AttendArgs {
+    const uint16_t* q;
+    int64_t q_stride;
+    uint16_t* out;
+    const void* kc;
+    const void* vc;
+    const float* k_scale;
+    const float* v_scale;
+    Batch b;
+    int heads, kvh, group, pages, page_log2, window;
+    float c1, cap;       // scores: c1 x (no cap), or cap - 2 cap / (1 + 2^(c1 x)), base 2
+    float* part;         // sums of a part of a unit's keys, then their (m, l)
+    int workers, columns;
+    int few;             // sequences of more columns are se12_paged_prompt.hip's
+    int splits;          // there: blocks that may share a unit's keys
+};
+
+// What a lane holds of a tile, by the cache's type: 16 bytes of each key row's
+// 64-byte part, and the lane's keys of a value column, 16 bytes as well.
+template <int CT>
+struct Form {
+    static constexpr int kPer = CT == SE12_STEP_E4M3 ? 16 : 8;   // values of 16 bytes, and keys of a lane
+    static constexpr int kTile = 4 * kPer;                        // keys of a tile
+    static constexpr int kHalves = kPer / 8;                      // matrix operands of a piece
+    static constexpr int kWord = kPer / 4;                        // values of a 32-bit word
+};
+
+template <int CT>
+__device__ __forceinline__ uint4 load_piece(const void* p, int64_t i) {
+    return *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + i * (16 / Form<CT>::kPer));
+}
+
+// values 8 h .. 8 h + 7 of a piece in BF16 (every E4M3 value is one)
+template <int CT>
+__device__ __forceinline__ bf16x8_t operand(const uint4 v, int h) {
+    if constexpr (CT == SE12_STEP_E4M3) {
+        const uint32_t a = h ? v.z : v.x, b = h ? v.w : v.y;
+        const bf16x2_t w0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false);
+        const bf16x2_t w1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true);
+        const bf16x2_t w2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false);
+        const bf16x2_t w3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true);
+        return bf16x8_t{w0.x, w0.y, w1.x, w1.y, w2.x, w2.y, w3.x, w3.y};
+    } else {
+        return __builtin_bit_cast(bf16x8_t, v);
+    }
+}
+
+// the bits of values from .. to - 1 of the kWord values of a word
+template <int CT>
+__device__ __forceinline__ uint32_t word_mask(int from, int to) {
+    constexpr int per = Form<CT>::kWord, bits = 32 / per;
+    const uint32_t below_to = to <= 0 ? 0u : to >= per ? ~0u : (1u << (bits * to)) - 1u;
+    const uint32_t below_from = from <= 0 ? 0u : from >= per ? ~0u : (1u << (bits * from)) - 1u;
+    return below_to & ~below_from;
+}
+
+template <int CT>
+__device__ __forceinline__ uint4 piece_mask(int from, int to) {
+    constexpr int per = Form<CT>::kWord;
+    return make_uint4(word_mask<CT>(from, to), word_mask<CT>(from - per, to - per), word_mask<CT>(from - 2 * per, to - 2 * per),
+                      word_mask<CT>(from - 3 * per, to - 3 * per));
+}
+
+__device__ __forceinline__ uint4 masked(const uint4 v, const uint4 m) { return make_uint4(v.x & m.x, v.y & m.y, v.z & m.z, v.w & m.w); }
+
+// bit 7 of every value (bit 15 of a BF16 one) that is a NaN or an infinity:
+// exponent all ones; E4M3: all ones but the sign
+template <int CT>
+__device__ __forceinline__ uint32_t no_numbers(uint32_t w) {
+    return CT == SE12_STEP_E4M3 ? ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u : ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
+}
+
+template <int CT>
+__device__ __forceinline__ bool has_no_number(const uint4 v) {
+    return (no_numbers<CT>(v.x) | no_numbers<CT>(v.y) | no_numbers<CT>(v.z) | no_numbers<CT>(v.w)) != 0;
+}
+
+template <int CT>
+__device__ __forceinline__ uint32_t numbers_only(uint32_t w) {
+    return CT == SE12_STEP_E4M3 ? w & ~((no_numbers<CT>(w) >> 7) * 0xFFu) : w & ~((no_numbers<CT>(w) >> 15) * 0xFFFFu);
+}
+
+// BF16 values: 1 where a value is a NaN (kind 0), +inf (1) or -inf (2), else 0
+__device__ __forceinline__ uint32_t where_no_number(uint32_t w, int kind) {
+    const uint32_t all = no_numbers<SE12_STEP_BF16>(w) >> 8, fraction = ((w & 0x007F007Fu) + 0x007F007Fu) & 0x00800080u;
+    const uint32_t is = kind == 0 ? all & fraction : kind == 1 ? all & ~fraction & ~(w >> 8) : all & ~fraction & (w >> 8);
+    return is * 0x7Fu;
+}
+
+__device__ __forceinline__ void store4(uint16_t* p, float a, float b, float c, float d) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(f_to_bf16x2(a, b), f_to_bf16x2(c, d));
+}
+
 // host: the first thing wrong with a cache and the new tokens of a call, or NULL
 inline const char* paged_error(const se12_step_pages* p, const se12_step_batch* b, int32_t heads) {
     if (!p || !b) return "NULL argument";
@@ -67,6 +166,12 @@ inline Batch device_batch(const se12_step_batch* b) {
     return {b->page_table, b->table_stride, b->lengths,  b->starts,
             b->table_width, b->sequences,   b->tokens, b->max_new < b->tokens ? b->max_new : b->tokens};
 }
+
+// se12_paged_prompt.hip
+bool prompt_fits(const Batch& b, int kvh, int group, int page_size);
+int prompt_splits(const Batch& b, int kvh, int group, int page_size);
+int64_t prompt_part_bytes(const Batch& b, int kvh, int group, int page_size, int d);
+void launch_prompt(const AttendArgs& a, bool e4m3, int d, hipStream_t st);
 
 inline int log2_of(int n) { return 31 - __builtin_clz((unsigned)n); }
 

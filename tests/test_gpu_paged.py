@@ -237,6 +237,20 @@ def _poison(c, table, keys, page):
         c.k_scale[empty], c.v_scale[empty] = float("nan"), float("nan")
 
 
+def test_pages_behind_the_window_may_be_anything(gpu):
+    """Pages no query sees any more went to others: their values and scales are NaN, or the table names no page."""
+    for new in (1, 40):
+        c, batch, q, before = _attend_case(gpu, E4M3, 128, 16, 4, 1, [200], [new], 0.0, 60, seed=7, extra=0)
+        gone = (200 - 60 + 1) // 16
+        ids = batch.page_table[0, :gone].long()
+        c.k.view(torch.uint8)[ids] = 127
+        c.v.view(torch.uint8)[ids] = 127
+        c.k_scale[ids], c.v_scale[ids] = float("nan"), float("inf")
+        assert torch.equal(c.attend(batch, q, 128 ** -0.5, window=60), before)
+        batch.page_table[0, :gone] = torch.tensor([-1, 1 << 30] * 8, dtype=torch.int32, device=gpu)[:gone]
+        assert torch.equal(c.attend(batch, q, 128 ** -0.5, window=60), before)
+
+
 def _attend_case(gpu, dtype, d, page, heads, kvh, lengths, new, softcap, window, seed=0, max_new=None, extra=2, scales=(-7, -4)):
     columns = max((a + b + page - 1) // page for a, b in zip(lengths, new)) + 1
     pages = len(new) * columns + 1
@@ -265,6 +279,10 @@ def _attend_case(gpu, dtype, d, page, heads, kvh, lengths, new, softcap, window,
     (128, 32, 6, 2, [0, 33, 200, 8], [5, 1, 9, 0], 0.0, 0),              # drafted tokens; 27 columns; a sequence with none
     (256, 16, 4, 4, [3, 0, 90], [40, 65, 33], 50.0, 17),                 # prompts under a window shorter than they are
     (64, 64, 24, 1, [50, 0], [3, 130], 0.0, 64),                         # more heads than a unit's columns
+    (256, 64, 8, 4, [700, 1500, 0, 33], [70, 1, 129, 40], 50.0, 0),       # prompts beside a decode step
+    (128, 32, 8, 1, [2100], [60], 0.0, 0),                               # few columns, many keys: a unit's keys in parts
+    (128, 16, 6, 2, [500, 3], [200, 64], 30.0, 100),                     # a window over columns that share a block
+    (64, 16, 8, 8, [0, 2000], [65, 129], 0.0, 0),                        # one column into the second, third block
 ])
 def test_attend(gpu, dtype, d, page, heads, kvh, lengths, new, softcap, window):
     _attend_case(gpu, dtype, d, page, heads, kvh, lengths, new, softcap, window)
@@ -286,11 +304,12 @@ def test_attend_scales_that_are_no_powers_of_two(gpu):
     _close(c.attend(batch, q, 128 ** -0.5, softcap=30.0), ref, size, mine)
 
 
+@pytest.mark.parametrize("many", [20, 70])
 @pytest.mark.parametrize("dtype,bad", [(E4M3, float("nan")), (BF16, float("nan")), (BF16, float("inf")), (BF16, float("-inf"))])
-def test_what_a_query_may_not_see_has_no_part_in_its_row(gpu, dtype, bad):
+def test_what_a_query_may_not_see_has_no_part_in_its_row(gpu, dtype, bad, many):
     """A later token of the call, and one behind the window, hold values that are no numbers: rows that do not see them
     stay as they are, the others have them in exactly the columns they are in."""
-    d, page, lengths, new, window = 128, 16, [40, 9], [12, 20], 24
+    d, page, lengths, new, window = 128, 16, [40, 9], [12, many], 24
     c, batch, q, before = _attend_case(gpu, dtype, d, page, 4, 2, lengths, new, 0.0, window, seed=5, extra=0)
     table = batch.page_table.tolist()
     bad_keys = {0: (47, 20), 1: (17, 0)}
@@ -314,8 +333,9 @@ def test_what_a_query_may_not_see_has_no_part_in_its_row(gpu, dtype, bad):
             r += 1
 
 
-def test_infinities_of_both_signs_meet_in_a_nan(gpu):
-    c, batch, q, _ = _attend_case(gpu, BF16, 64, 16, 2, 1, [10], [8], 0.0, 0, seed=6, extra=0)
+@pytest.mark.parametrize("new", [8, 50])
+def test_infinities_of_both_signs_meet_in_a_nan(gpu, new):
+    c, batch, q, _ = _attend_case(gpu, BF16, 64, 16, 2, 1, [10], [new], 0.0, 0, seed=6, extra=0)
     page = batch.page_table[0, 0].item()
     c.v[page, 0, 9, 12], c.v[page, 0, 9, 14] = float("inf"), float("-inf")
     got = c.attend(batch, q, 0.125).cpu()[:, 0, 9]
