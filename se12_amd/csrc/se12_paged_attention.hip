@@ -40,65 +40,45 @@ struct SeqWork {
 };
 
 template <int kTile>
-__device__ __forceinline__ SeqWork seq_work(const AttendArgs& a, int s) {
+__device__ __forceinline__ SeqWork seq_work(const AttendArgs& a, Seq seq) {
     SeqWork w;
-    const int capacity = a.b.width << a.page_log2;
-    w.seq = load_seq(a.b, s, capacity);
-    w.keys = min(w.seq.len + w.seq.n, capacity);
-    const int low = a.window > 0 ? max(0, w.seq.len - a.window + 1) : 0;
+    w.seq = seq;
+    w.keys = min(seq.len + seq.n, a.b.width << a.page_log2);
+    const int low = a.window > 0 ? max(0, seq.len - a.window + 1) : 0;
     w.tile0 = low / kTile;
-    const int columns = w.seq.n * a.group;
+    const int columns = seq.n * a.group;
     w.units = columns > a.few ? 0 : (columns + kColumns - 1) / kColumns;
     w.tiles = w.units > 0 ? max((w.keys + kTile - 1) / kTile - w.tile0, 1) : 0;
     return w;
 }
 
-__device__ __forceinline__ int64_t shfl64(int64_t v, int from) {
-    const int lo = __shfl((int)v, from, 64), hi = __shfl((int)(v >> 32), from, 64);
-    return ((int64_t)hi << 32) | (uint32_t)lo;
-}
+// 64 sequences' work, one to a lane: the tiles of all heads and units, those of the
+// lanes up to it, and of all (the C entry sees to it that 32 bits hold them)
+struct Chunk {
+    Seq seq;
+    int tiles, upto, all;
+};
 
-// inclusive prefix sums of a wave's values
-__device__ __forceinline__ int64_t scan64(int64_t v, int lane) {
+template <int kTile>
+__device__ __forceinline__ Chunk load_chunk(const AttendArgs& a, int s0, int lane) {
+    Chunk c;
+    const int s = s0 + lane;
+    c.seq = load_seq(a.b, min(s, a.b.seqs - 1), a.b.width << a.page_log2);
+    if (s >= a.b.seqs) c.seq.n = 0;
+    const SeqWork w = seq_work<kTile>(a, c.seq);
+    c.tiles = w.tiles * w.units * a.kvh;
+    c.upto = c.tiles;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const int64_t u = shfl64(v, lane - o);
-        v += lane >= o ? u : 0;
+        const int u = __shfl_up(c.upto, o, 64);
+        c.upto += lane >= o ? u : 0;
     }
-    return v;
+    c.all = __builtin_amdgcn_readlane(c.upto, 63);
+    return c;
 }
 
-// tiles of sequence s over all heads and units
-template <int kTile>
-__device__ __forceinline__ int64_t seq_tiles(const AttendArgs& a, int s) {
-    if (s >= a.b.seqs) return 0;
-    const SeqWork w = seq_work<kTile>(a, s);
-    return (int64_t)w.tiles * w.units * a.kvh;
-}
-
-template <int kTile>
-__device__ __forceinline__ int64_t all_tiles(const AttendArgs& a, int lane) {
-    int64_t total = 0;
-    for (int s0 = 0; s0 < a.b.seqs; s0 += 64) total += shfl64(scan64(seq_tiles<kTile>(a, s0 + lane), lane), 63);
-    return total;
-}
-
-// the sequence that holds tile `at` of the line, and the tile its part begins at
-template <int kTile>
-__device__ __forceinline__ int seq_of_tile(const AttendArgs& a, int64_t at, int lane, int64_t& base) {
-    int64_t before = 0;
-    for (int s0 = 0; s0 < a.b.seqs; s0 += 64) {
-        const int64_t mine = seq_tiles<kTile>(a, s0 + lane), upto = scan64(mine, lane);
-        const uint64_t past = __builtin_amdgcn_ballot_w64(before + upto > at);
-        if (past) {
-            const int l = __builtin_ctzll(past);
-            base = before + shfl64(upto - mine, l);
-            return s0 + l;
-        }
-        before += shfl64(upto, 63);
-    }
-    base = before;
-    return a.b.seqs;
+__device__ __forceinline__ Seq seq_of(const Chunk& c, int l) {
+    return {__builtin_amdgcn_readlane(c.seq.start, l), __builtin_amdgcn_readlane(c.seq.n, l), __builtin_amdgcn_readlane(c.seq.len, l)};
 }
 
 template <int CT, int D>
@@ -154,77 +134,11 @@ struct Attend {
         int vpage = entry(t0 * kTile + vkey), vpage_next = entry(min(t0 + 1, t1 - 1) * kTile + vkey);
         int kpage_next = entry(min(t0 + 1, t1 - 1) * kTile + kgroup);
         load_k(t0, entry(t0 * kTile + kgroup));
-        for (int t = t0; t < t1; ++t) {
-            const int k0 = t * kTile, key0 = k0 + vkey;
-            const int64_t head_page = (int64_t)held_page(vpage) * a.kvh + kh;
-            const int next = min(t + 1, t1 - 1), after = min(t + 2, t1 - 1);
-            const int kpage_after = entry(after * kTile + kgroup), vpage_after = entry(after * kTile + vkey);
-            uint4 vf[kRows];
-            {
-                const int64_t at = head_page * page_elems + (int64_t)col * P + (key0 & (P - 1));
-#pragma unroll
-                for (int i = 0; i < kRows; ++i) vf[i] = load_piece<CT>(a.vc, at + 16 * i * P);
-            }
-            // (what the page of unseen keys holds, its scales too, may be anything)
-            const bool held = (uint32_t)vpage < (uint32_t)a.pages && key0 < high && key0 + kPer > low;
-            float ks = 1.0f, vs = 1.0f;
-            if constexpr (CT == SE12_STEP_E4M3) {
-                ks = a.k_scale[head_page];
-                vs = held ? a.v_scale[head_page] : 0.0f;
-            }
-            float sc[kPer];
-#pragma unroll
-            for (int g = 0; g < kSteps; ++g) {
-                floatx4_t d = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int i = 0; i < kChunks; ++i)
-#pragma unroll
-                    for (int h = 0; h < kHalves; ++h)
-                        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand<CT>(kf[g][i], h), qf[i][h], d, 0, 0, 0);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sc[4 * g + e] = d[e];
-            }
-            load_k(next, kpage_next);
-            const float by = a.c1 * ks;
-            if (a.cap > 0.0f) {
-#pragma unroll
-                for (int e = 0; e < kPer; ++e)
-                    sc[e] = a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(sc[e] * by));
-            } else {
-#pragma unroll
-                for (int e = 0; e < kPer; ++e) sc[e] *= by;
-            }
-            const bool inside = k0 + kTile - 1 <= pos_min && k0 + kTile <= w.keys && pos_max - k0 < reach &&
-                                __builtin_amdgcn_ballot_w64(!held) == 0;
-            bool apart = false;     // a value that is no number may be hidden from some of the columns
-            if (!inside) {
-                const int from = max(pos - reach + 1, 0) - key0, to = held ? min(pos + 1, w.keys) - key0 : 0;
-#pragma unroll
-                for (int e = 0; e < kPer; ++e) sc[e] = (e < from || e >= to) ? -INFINITY : sc[e];
-                const uint4 mask = piece_mask<CT>(low - key0, held ? high - key0 : 0);
-                bool bad = false;
-#pragma unroll
-                for (int i = 0; i < kRows; ++i) {
-                    vf[i] = masked(vf[i], mask);
-                    bad |= has_no_number<CT>(vf[i]);
-                }
-                apart = __builtin_amdgcn_ballot_w64(bad) != 0;
-            }
-            float top = sc[0];
-#pragma unroll
-            for (int e = 1; e < kPer; ++e) top = fmaxf(top, sc[e]);
-            if (__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0) {
-                top = fmaxf(top, __shfl_xor(top, 16, 64));
-                top = fmaxf(top, __shfl_xor(top, 32, 64));
-                const float to = fmaxf(m, top);
-                const float scale = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
-                m = to;
-                l *= scale;
-#pragma unroll
-                for (int i = 0; i < kRows; ++i) o[i] *= scale;
-            }
+        uint4 vf[kRows];
+        float sc[kPer], top = 0.0f, vs = 1.0f;
+        bf16x8_t pf[kHalves];
+        auto weights = [&]() {
             const float base = m == -INFINITY ? 0.0f : m;
-            bf16x8_t pf[kHalves];
 #pragma unroll
             for (int h = 0; h < kHalves; ++h) {
                 uint32_t u[4];
@@ -237,9 +151,103 @@ struct Attend {
                 }
                 pf[h] = __builtin_bit_cast(bf16x8_t, make_uint4(u[0], u[1], u[2], u[3]));
             }
+        };
+        auto add_values = [&]() {
+#pragma unroll
+            for (int i = 0; i < kRows; ++i)
+#pragma unroll
+                for (int h = 0; h < kHalves; ++h)
+                    o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand<CT>(vf[i], h), pf[h], o[i], 0, 0, 0);
+        };
+        auto column_max = [&](float v) {
+            v = fmaxf(v, __shfl_xor(v, 16, 64));
+            return fmaxf(v, __shfl_xor(v, 32, 64));
+        };
+        for (int t = t0;; ++t) {
+            bool apart = false;     // a value that is no number may be hidden from some of the columns
+            bool higher = false;    // a score passes the maximum by more than kSlack
+            for (; t < t1; ++t) {
+                const int k0 = t * kTile, key0 = k0 + vkey;
+                const int64_t head_page = (int64_t)held_page(vpage) * a.kvh + kh;
+                // (what the page of unseen keys holds, its scales too, may be anything)
+                const bool held = (uint32_t)vpage < (uint32_t)a.pages && key0 < high && key0 + kPer > low;
+                const int next = min(t + 1, t1 - 1), after = min(t + 2, t1 - 1);
+                const int kpage_after = entry(after * kTile + kgroup), vpage_after = entry(after * kTile + vkey);
+                float ks = 1.0f;
+                if constexpr (CT == SE12_STEP_E4M3) {
+                    ks = a.k_scale[head_page];
+                    vs = a.v_scale[head_page];
+                }
+                {
+                    const int64_t at = head_page * page_elems + (int64_t)col * P + (key0 & (P - 1));
+#pragma unroll
+                    for (int i = 0; i < kRows; ++i) vf[i] = load_piece<CT>(a.vc, at + 16 * i * P);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int g = 0; g < kSteps; ++g) {
+                    floatx4_t d = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+                        for (int h = 0; h < kHalves; ++h)
+                            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand<CT>(kf[g][i], h), qf[i][h], d, 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sc[4 * g + e] = d[e];
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                load_k(next, kpage_next);
+                __builtin_amdgcn_sched_barrier(0);
+                const float by = a.c1 * ks;
+                if (a.cap > 0.0f) {
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e)
+                        sc[e] = a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(sc[e] * by));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) sc[e] *= by;
+                }
+                const bool inside = k0 + kTile - 1 <= pos_min && k0 + kTile <= w.keys && pos_max - k0 < reach &&
+                                    __builtin_amdgcn_ballot_w64(!held) == 0;
+                if (!inside) {
+                    vs = held ? vs : 0.0f;
+                    const int from = max(pos - reach + 1, 0) - key0, to = held ? min(pos + 1, w.keys) - key0 : 0;
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) sc[e] = (e < from || e >= to) ? -INFINITY : sc[e];
+                    const uint4 mask = piece_mask<CT>(low - key0, held ? high - key0 : 0);
+                    bool bad = false;
+#pragma unroll
+                    for (int i = 0; i < kRows; ++i) {
+                        vf[i] = masked(vf[i], mask);
+                        bad |= has_no_number<CT>(vf[i]);
+                    }
+                    apart = __builtin_amdgcn_ballot_w64(bad) != 0;
+                }
+                top = sc[0];
+#pragma unroll
+                for (int e = 1; e < kPer; ++e) top = fmaxf(top, sc[e]);
+                if (t == t0) m = column_max(top);
+                higher = __builtin_amdgcn_ballot_w64(top > m + kSlack) != 0;
+                vpage = vpage_next;
+                vpage_next = vpage_after;
+                kpage_next = kpage_after;
+                if (higher || apart) break;
+                weights();
+                add_values();
+            }
+            if (t >= t1) break;
+            // The rare tile, outside the loop, where the sums may stay in accumulation
+            // registers: the maximum moves, and what is summed with it; 0 x NaN is
+            // NaN, so a value that is no number leaves the product and comes back in
+            // the columns that give it a weight.
+            const float to = fmaxf(m, column_max(top));
+            const float scale = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            l *= scale;
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) o[i] *= scale;
+            weights();
             if (apart) {
-                // 0 x NaN is NaN, so what is no number leaves the product, and comes
-                // back in the columns that give it a weight
 #pragma unroll
                 for (int i = 0; i < kRows; ++i) {
 #pragma unroll
@@ -260,14 +268,15 @@ struct Attend {
                                        numbers_only<CT>(vf[i].w));
                 }
             }
+            // (a row at a time, for the registers' sake)
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < kRows; ++i)
+            for (int i = 0; i < kRows; ++i) {
 #pragma unroll
                 for (int h = 0; h < kHalves; ++h)
                     o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand<CT>(vf[i], h), pf[h], o[i], 0, 0, 0);
-            vpage = vpage_next;
-            vpage_next = vpage_after;
-            kpage_next = kpage_after;
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
@@ -283,26 +292,28 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : 2) void paged_attent
     constexpr int kTile = Form<CT>::kTile;
     const int lane = threadIdx.x & 63;
     const int worker = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * (kAttendThreads / 64) + (threadIdx.x >> 6)));
-    const int64_t total = all_tiles<kTile>(a, lane);
+    Chunk chunk = load_chunk<kTile>(a, 0, lane);
+    int64_t total = chunk.all;
+    for (int s0 = 64; s0 < a.b.seqs; s0 += 64) total += load_chunk<kTile>(a, s0, lane).all;
     const int64_t per = (total + a.workers - 1) / a.workers;
     int64_t at = worker * per;
     const int64_t end = min(at + per, total);
-    if (at >= end) return;
-    int64_t base;
-    int s = __builtin_amdgcn_readfirstlane(seq_of_tile<kTile>(a, at, lane, base));
-    while (at < end && s < a.b.seqs) {
-        const SeqWork w = seq_work<kTile>(a, s);
-        const int64_t size = (int64_t)w.tiles * w.units * a.kvh;
-        if (at >= base + size) {
-            base += size;
-            ++s;
+    int64_t before = 0;      // tiles of the sequences before the chunk
+    for (int s0 = 0; at < end;) {
+        const uint64_t past = __builtin_amdgcn_ballot_w64(before + chunk.upto > at);
+        if (!past) {
+            before += chunk.all;
+            s0 += 64;
+            chunk = load_chunk<kTile>(a, s0, lane);
             continue;
         }
-        const int64_t in = at - base;
-        const int tile = (int)(in % w.tiles), unit = (int)(in / w.tiles % w.units), kh = (int)(in / w.tiles / w.units);
+        const int of = __builtin_ctzll(past);
+        const SeqWork w = seq_work<kTile>(a, seq_of(chunk, of));
+        const int in = (int)(at - before) - (__builtin_amdgcn_readlane(chunk.upto, of) - __builtin_amdgcn_readlane(chunk.tiles, of));
+        const int line = in / w.tiles, tile = in - line * w.tiles, kh = line / w.units, unit = line - kh * w.units;
         const int tiles = (int)min((int64_t)(w.tiles - tile), end - at);
         Attend<CT, D> x;
-        x.run(a, s, w, kh, unit, tile, tiles);
+        x.run(a, s0 + of, w, kh, unit, tile, tiles);
         const int col = lane & 15, quarter = lane >> 4, c = unit * kColumns + col;
         if (c < w.seq.n * a.group) {
             if (tiles == w.tiles) {
@@ -328,55 +339,82 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : 2) void paged_attent
 }
 
 // The units that several workers share, from their parts in order: one block per
-// (sequence, KV head, column unit) and column, D / 4 lanes a part.
+// (sequence, KV head, column unit) and column. A wave takes every kParts-th part, D /
+// 4 lanes to one, all its loads at once up to kBatch of them; a part's maximum may lie
+// above those before it, so what is summed moves with it.
 template <int CT, int D>
 __global__ __launch_bounds__(kAttendThreads) void paged_join_kernel(AttendArgs a, int max_units) {
     constexpr int kTile = Form<CT>::kTile;
+    constexpr int kLanes = D / 4, kParts = kAttendThreads / kLanes, kBatch = 4;
     __shared__ float4 sums[kAttendThreads];
-    __shared__ float ls[kAttendThreads];
-    const int tid = threadIdx.x, lane = tid & 63;
+    __shared__ float2 mls[kParts];
+    const int tid = threadIdx.x, lane = tid & 63, part = tid / kLanes, at = tid % kLanes;
     const int unit = (int)(blockIdx.x % max_units), kh = (int)(blockIdx.x / max_units % a.kvh), s = (int)(blockIdx.x / max_units / a.kvh);
     const int col = blockIdx.y, c = unit * kColumns + col;
-    const SeqWork w = seq_work<kTile>(a, s);
+    Chunk chunk = load_chunk<kTile>(a, s & ~63, lane);
+    const SeqWork w = seq_work<kTile>(a, seq_of(chunk, s & 63));
     if (unit >= w.units || c >= w.seq.n * a.group) return;
-    int64_t base = 0, total = 0;
+    int64_t base = __builtin_amdgcn_readlane(chunk.upto, s & 63) - __builtin_amdgcn_readlane(chunk.tiles, s & 63), total = chunk.all;
     for (int s0 = 0; s0 < a.b.seqs; s0 += 64) {
-        const int64_t mine = seq_tiles<kTile>(a, s0 + lane), upto = scan64(mine, lane);
-        if (s >= s0 && s < s0 + 64) base = total + shfl64(upto - mine, s - s0);
-        total += shfl64(upto, 63);
+        if (s0 == (s & ~63)) continue;
+        const int all = load_chunk<kTile>(a, s0, lane).all;
+        total += all;
+        base += s0 < s ? all : 0;
     }
     const int64_t per = (total + a.workers - 1) / a.workers;
     const int64_t first = base + ((int64_t)kh * w.units + unit) * w.tiles, last = first + w.tiles - 1;
     const int w0 = (int)(first / per), w1 = (int)(last / per);
     if (w0 == w1) return;      // one worker had it all
-    constexpr int kLanes = D / 4, kParts = kAttendThreads / kLanes;
-    const float* ml = a.part + (int64_t)a.workers * 2 * a.columns * D;
-    float m = -INFINITY;
-    for (int k = w0; k <= w1; ++k) m = fmaxf(m, ml[2 * (part_at(a, k, k == w0 ? 1 : 0) + col)]);
-    const float top = m == -INFINITY ? 0.0f : m;
+    const float2* mlp = reinterpret_cast<const float2*>(a.part + (int64_t)a.workers * 2 * a.columns * D);
+    float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float l = 0.0f;
-    for (int k = w0 + tid / kLanes; k <= w1; k += kParts) {
-        const int64_t p = part_at(a, k, k == w0 ? 1 : 0) + col;
-        const float by = __builtin_amdgcn_exp2f(ml[2 * p] - top);
-        const float4 v = *reinterpret_cast<const float4*>(a.part + p * D + 4 * (tid % kLanes));
-        l += by * ml[2 * p + 1];
+    for (int k0 = w0 + part; k0 <= w1; k0 += kParts * kBatch) {
+        float2 ml[kBatch];
+        float4 v[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int k = k0 + i * kParts;
+            const int64_t p = part_at(a, min(k, w1), k == w0 ? 1 : 0) + col;
+            ml[i] = mlp[p];
+            v[i] = *reinterpret_cast<const float4*>(a.part + p * D + 4 * at);
+        }
+        float to = m;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) to = k0 + i * kParts <= w1 ? fmaxf(to, ml[i].x) : to;
+        const float top = to == -INFINITY ? 0.0f : to, keep = __builtin_amdgcn_exp2f(m - top);
+        m = to;
+        l *= keep;
+        o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (k0 + i * kParts > w1) continue;
+            const float by = __builtin_amdgcn_exp2f(ml[i].x - top);
+            l += by * ml[i].y;
+            o.x += by * v[i].x;
+            o.y += by * v[i].y;
+            o.z += by * v[i].z;
+            o.w += by * v[i].w;
+        }
+    }
+    sums[tid] = o;
+    if (at == 0) mls[part] = make_float2(m, l);
+    __syncthreads();
+    if (tid >= kLanes) return;
+    float to = mls[0].x;
+#pragma unroll
+    for (int k = 1; k < kParts; ++k) to = fmaxf(to, mls[k].x);
+    to = to == -INFINITY ? 0.0f : to;
+    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kParts; ++k) {
+        const float4 v = sums[k * kLanes + tid];
+        const float by = __builtin_amdgcn_exp2f(mls[k].x - to);
+        l += by * mls[k].y;
         o.x += by * v.x;
         o.y += by * v.y;
         o.z += by * v.z;
         o.w += by * v.w;
-    }
-    sums[tid] = o;
-    ls[tid] = l;
-    __syncthreads();
-    if (tid >= kLanes) return;
-    for (int k = 1; k < kParts; ++k) {
-        const float4 v = sums[k * kLanes + tid];
-        o.x += v.x;
-        o.y += v.y;
-        o.z += v.z;
-        o.w += v.w;
-        l += ls[k * kLanes + tid];
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     store4(a.out + ((int64_t)(w.seq.start + c / a.group) * a.heads + kh * a.group + c % a.group) * D + 4 * tid, o.x * inv, o.y * inv,
@@ -446,6 +484,8 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
         return step_fail(fn, "workspace missing, misaligned or too small");
     if ((int64_t)b.seqs * pages->kv_heads * (kFewColumns / kColumns) > INT32_MAX || !prompt_fits(b, pages->kv_heads, group, pages->page_size))
         return step_fail(fn, "too many sequences, tokens and heads for one launch");
+    if (std::min<int64_t>(b.seqs, 64) * (((int64_t)b.width * pages->page_size + 31) / 32) * (kFewColumns / kColumns) * pages->kv_heads > INT32_MAX)
+        return step_fail(fn, "too long a table for so many sequences and heads");
     constexpr float kLog2E = 1.4426950408889634f;
     AttendArgs a{q, q_stride, out, pages->k, pages->v, pages->k_scale, pages->v_scale, b, heads, pages->kv_heads, group, pages->pages,
                  log2_of(pages->page_size), window, softcap > 0.0f ? 2.0f * scaling / softcap * kLog2E : scaling * kLog2E,

@@ -43,7 +43,7 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef float floatx4_t __attribute__((ext_vector_type(4)));
 
-constexpr float kSlack = 8.0f;        // how far a score may pass the maximum it is taken from, base 2
+constexpr float kSlack = 16.0f;       // how far a score may pass the maximum it is taken from, base 2
 
 struct AttendArgs {
     const uint16_t* q;
