@@ -25,8 +25,10 @@ namespace se12step {
 
 constexpr int kColumns = 16;          // columns of a unit
 constexpr int kFewColumns = 64;       // of a sequence and KV head; with more it is se12_paged_prompt.hip's
+// waves of a launch: one per SIMD of 256 CUs (3 x 65,000 keys, 28 / 4 heads of 128: 31.5
+// us, 36 with two, which have two starts and twice the parts to join)
+constexpr int kWorkersLog2 = 10, kWorkers = 1 << kWorkersLog2;
 constexpr int kAttendThreads = 256;   // four waves, each with tiles of its own
-constexpr int kWorkers = 256 * 4;     // waves of a launch: one per SIMD
 
 // The work: units of up to 16 columns of one sequence and KV head, each a run of
 // key tiles; all units' tiles in one line (sequence, head, column unit, tile),
@@ -75,6 +77,15 @@ __device__ __forceinline__ Chunk load_chunk(const AttendArgs& a, int s0, int lan
     }
     c.all = __builtin_amdgcn_readlane(c.upto, 63);
     return c;
+}
+
+// tiles of a worker (workers that are not launched, where there can be no more
+// tiles than are, would have none)
+__device__ __forceinline__ int64_t tiles_each(int64_t total) { return (total + kWorkers - 1) >> kWorkersLog2; }
+
+// (at / each is below kWorkers; 64-bit division only where it takes one)
+__device__ __forceinline__ int worker_of(int64_t at, int64_t each) {
+    return ((at | each) >> 32) == 0 ? (int)((uint32_t)at / (uint32_t)each) : (int)(at / each);
 }
 
 __device__ __forceinline__ Seq seq_of(const Chunk& c, int l) {
@@ -295,7 +306,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : 2) void paged_attent
     Chunk chunk = load_chunk<kTile>(a, 0, lane);
     int64_t total = chunk.all;
     for (int s0 = 64; s0 < a.b.seqs; s0 += 64) total += load_chunk<kTile>(a, s0, lane).all;
-    const int64_t per = (total + a.workers - 1) / a.workers;
+    const int64_t per = tiles_each(total);
     int64_t at = worker * per;
     const int64_t end = min(at + per, total);
     int64_t before = 0;      // tiles of the sequences before the chunk
@@ -361,9 +372,9 @@ __global__ __launch_bounds__(kAttendThreads) void paged_join_kernel(AttendArgs a
         total += all;
         base += s0 < s ? all : 0;
     }
-    const int64_t per = (total + a.workers - 1) / a.workers;
+    const int64_t per = tiles_each(total);
     const int64_t first = base + ((int64_t)kh * w.units + unit) * w.tiles, last = first + w.tiles - 1;
-    const int w0 = (int)(first / per), w1 = (int)(last / per);
+    const int w0 = worker_of(first, per), w1 = worker_of(last, per);
     if (w0 == w1) return;      // one worker had it all
     const float2* mlp = reinterpret_cast<const float2*>(a.part + (int64_t)a.workers * 2 * a.columns * D);
     float m = -INFINITY, l = 0.0f;

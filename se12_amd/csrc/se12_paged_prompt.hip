@@ -55,12 +55,15 @@ __device__ __forceinline__ bool find_unit(const AttendArgs& a, int slot, Unit& u
         else
             hi = mid;
     }
+    // (the same for all lanes, and kept in scalar registers)
+    lo = __builtin_amdgcn_readfirstlane(lo);
     u.s = lo;
     const int capacity = a.b.width << a.page_log2;
-    u.seq = load_seq(a.b, lo, capacity);
+    const Seq seq = load_seq(a.b, lo, capacity);
+    u.seq = {__builtin_amdgcn_readfirstlane(seq.start), __builtin_amdgcn_readfirstlane(seq.n), __builtin_amdgcn_readfirstlane(seq.len)};
     u.keys = min(u.seq.len + u.seq.n, capacity);
     u.columns = u.seq.n * a.group;
-    const int64_t first = (int64_t)(slot - base(lo)) * kBlockColumns;
+    const int64_t first = (int64_t)(slot - __builtin_amdgcn_readfirstlane(base(lo))) * kBlockColumns;
     u.first = (int)first;
     return first >= 0 && first < u.columns && u.columns > a.few;
 }
@@ -74,7 +77,7 @@ __device__ __forceinline__ void unit_tiles(const AttendArgs& a, const Unit& u, i
     t1 = max((min(u.keys, pos1 + 1) + kTile - 1) / kTile, t0 + 1);
 }
 
-template <int CT, int D>
+template <int CT, int D, bool kCapped>
 __global__ __launch_bounds__(kPromptThreads, 1) void paged_prompt_kernel(AttendArgs a) {
     using F = Form<CT>;
     constexpr int kTile = F::kTile, kSubs = kTile / kSubTile;
@@ -84,7 +87,7 @@ __global__ __launch_bounds__(kPromptThreads, 1) void paged_prompt_kernel(AttendA
     constexpr int kLoads = kHalfTile / 1024 / kPromptWaves;   // of a wave, 64 pieces each
     constexpr int kRows = D / 32;
     static_assert(kValuePieces == 4 && kLoads >= 1, "");
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];     // [2][keys, values], a wave's own values each
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];     // [2][keys, values]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int kh = blockIdx.x % a.kvh, rest = blockIdx.x / a.kvh, split = rest % a.splits;
     const int slot = (int)(gridDim.x / a.kvh / a.splits) - 1 - rest / a.splits;   // the last columns, with the most keys, first
@@ -139,7 +142,7 @@ __global__ __launch_bounds__(kPromptThreads, 1) void paged_prompt_kernel(AttendA
     const uint32_t lds0 = se12::lds_address(lds);
     auto load_tile = [&](int t, int buffer, int key_entry, int value_entry) {
         const int k0 = t * kTile;
-        const uint32_t to = lds0 + buffer * 2 * kHalfTile;
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + buffer * 2 * kHalfTile);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int n = wave * kLoads + i;
@@ -179,143 +182,190 @@ __global__ __launch_bounds__(kPromptThreads, 1) void paged_prompt_kernel(AttendA
         }
         return x;
     };
+    // What the wave holds of a sub-tile of 32 keys: keys' pieces, value columns' pieces.
+    constexpr int kKeyReads = kKeyPieces / 2, kValueReads = 2 / F::kHalves;
+    // (of a key no more than 8 pieces at once)
+    constexpr int kAhead = kKeyReads < 8 ? kKeyReads : 8;
+    uint4 kf[kAhead], vf[kRows][kValueReads];
+    auto key_piece = [&](int t, int j, int i) {
+        const int row = j * kSubTile + key_of_row(col), twist = key_twist(row);
+        const uint8_t* p = lds + ((t - t0) & 1) * 2 * kHalfTile + row * (kKeyPieces * 16);
+        return *reinterpret_cast<const uint4*>(p + 16 * ((2 * i + half) ^ twist));
+    };
+    auto read_keys = [&](int t, int j) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) kf[i] = key_piece(t, j, i);
+    };
+    auto read_values = [&](int t, int j) {
+        const uint8_t* p = lds + (((t - t0) & 1) * 2 + 1) * kHalfTile;
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+#pragma unroll
+            for (int n = 0; n < kValueReads; ++n) {
+                const int r = 32 * i + col, piece = CT == SE12_STEP_E4M3 ? 2 * j + half : 2 * half + n;
+                vf[i][n] = *reinterpret_cast<const uint4*>(p + r * 64 + 16 * (piece ^ ((r >> 2) & 3)));
+            }
+    };
+    float sc[16], top = 0.0f, vs = 1.0f;    // sc: scores, or r of cap - 2 cap r
+    bf16x8_t pf[2];
+    auto weights = [&]() {
+        const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float p0, p1;
+                if constexpr (kCapped) {
+                    p0 = __builtin_amdgcn_exp2f((a.cap - base) - 2.0f * a.cap * sc[8 * h + 2 * k]);
+                    p1 = __builtin_amdgcn_exp2f((a.cap - base) - 2.0f * a.cap * sc[8 * h + 2 * k + 1]);
+                } else {
+                    p0 = __builtin_amdgcn_exp2f(sc[8 * h + 2 * k] - base);
+                    p1 = __builtin_amdgcn_exp2f(sc[8 * h + 2 * k + 1] - base);
+                }
+                l += p0 + p1;
+                if constexpr (CT == SE12_STEP_E4M3)
+                    w[k] = f_to_bf16x2(p0 * vs, p1 * vs);
+                else
+                    w[k] = f_to_bf16x2(p0, p1);
+            }
+            pf[h] = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+        }
+    };
+
     int ke = key_entry_of(t0), ve = value_entry_of(t0);
-    Lane next = lane_of(ke);
+    Lane now, next = lane_of(ke);
     load_tile(t0, 0, ke, ve);
     ke = key_entry_of(min(t0 + 1, t1 - 1));
     ve = value_entry_of(min(t0 + 1, t1 - 1));
-
-    for (int t = t0; t < t1; ++t) {
-        const int buffer = (t - t0) & 1;
+    // Tile t + 1 (its loads were sent a tile ago) takes over: after the barrier it is
+    // whole, and every wave is done with tile t, whose place tile t + 2 may take.
+    auto next_tile = [&](int t) {
         se12::wait_vector_loads();
-        Lane now = next;
+        now = next;
 #pragma unroll
         for (int j = 0; j < kSubs; ++j) asm volatile("" : "+v"(now.ks[j]), "+v"(now.vs[j]), "+v"(now.held[j]));
         asm volatile("" : "+v"(ke), "+v"(ve));
-        __syncthreads();     // tile t is whole, and every wave is done with the other buffer
-        if (t + 1 < t1) {
+        __syncthreads();
+        if (t + 2 < t1) {
             next = lane_of(ke);
-            load_tile(t + 1, buffer ^ 1, ke, ve);
-            ke = key_entry_of(min(t + 2, t1 - 1));
-            ve = value_entry_of(min(t + 2, t1 - 1));
+            load_tile(t + 2, (t - t0) & 1, ke, ve);
+            ke = key_entry_of(min(t + 3, t1 - 1));
+            ve = value_entry_of(min(t + 3, t1 - 1));
         }
-        const uint8_t* keys = lds + buffer * 2 * kHalfTile;
-        const uint8_t* values = keys + kHalfTile;
-#pragma unroll
-        for (int j = 0; j < kSubs; ++j) {
-            const int k0 = t * kTile + j * kSubTile, key0 = k0 + 16 * half;
-            if (k0 >= high || k0 + kSubTile <= low) continue;
-            const int row = j * kSubTile + key_of_row(col);
-            const uint8_t* kp = keys + row * (kKeyPieces * 16);
-            const int twist = key_twist(row);
+    };
+    next_tile(t0 - 1);
+    read_keys(t0, 0);
+    bool known = false;      // what is no number in the sub-tile's values has been dealt with
+    for (int n32 = t0 * kSubs; n32 < t1 * kSubs;) {
+        bool apart = false;
+        for (; n32 < t1 * kSubs; ++n32) {
+            const int t = n32 / kSubs, j = n32 % kSubs, k0 = n32 * kSubTile, key0 = k0 + 16 * half;
             floatx16_t d;
 #pragma unroll
             for (int e = 0; e < 16; ++e) d[e] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kKeyPieces / 2; ++i) {
-                const uint4 v = *reinterpret_cast<const uint4*>(kp + 16 * ((2 * i + half) ^ twist));
+            for (int i = 0; i < kKeyReads; ++i) {
 #pragma unroll
                 for (int h = 0; h < F::kHalves; ++h)
-                    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand<CT>(v, h), qf[i * F::kHalves + h], d, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand<CT>(kf[i % kAhead], h), qf[i * F::kHalves + h], d, 0, 0, 0);
+                if (i + kAhead < kKeyReads) kf[i % kAhead] = key_piece(t, j, i + kAhead);
             }
-            float sc[16];
-            const float by = a.c1 * now.ks[j];
-            if (a.cap > 0.0f) {
+            __builtin_amdgcn_sched_barrier(0);
+            read_values(t, j);
+            __builtin_amdgcn_sched_barrier(0);
+            const float by = a.c1 * (j ? now.ks[kSubs - 1] : now.ks[0]);
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    sc[e] = a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(d[e] * by));
-            } else {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) sc[e] = d[e] * by;
-            }
-            const bool held = now.held[j] != 0 && key0 < high && key0 + 16 > low;
+            for (int e = 0; e < 16; ++e)
+                sc[e] = kCapped ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(d[e] * by)) : d[e] * by;
+            const bool held = (j ? now.held[kSubs - 1] : now.held[0]) != 0 && key0 < high && key0 + 16 > low;
             const bool inside = k0 + kSubTile - 1 <= pos_min && k0 + kSubTile <= u.keys && pos_max - k0 < reach &&
                                 __builtin_amdgcn_ballot_w64(!held) == 0;
-            const float vs = held ? now.vs[j] : 0.0f;
+            vs = j ? now.vs[kSubs - 1] : now.vs[0];
             if (!inside) {
+                vs = held ? vs : 0.0f;
                 const int since = max(pos - reach + 1, 0) - key0, to = held ? min(pos + 1, u.keys) - key0 : 0;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) sc[e] = (e < since || e >= to) ? -INFINITY : sc[e];
-            }
-            float top = sc[0];
+                for (int e = 0; e < 16; ++e) sc[e] = (e < since || e >= to) ? (kCapped ? INFINITY : -INFINITY) : sc[e];
+                bool bad = false;
 #pragma unroll
-            for (int e = 1; e < 16; ++e) top = fmaxf(top, sc[e]);
-            if (__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0) {
-                const float to = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
-                const float scale = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
-                m = to;
-                l *= scale;
+                for (int n = 0; n < kValueReads; ++n) {
+                    const uint4 mask = piece_mask<CT>(low - key0 - n * F::kPer, held ? high - key0 - n * F::kPer : 0);
 #pragma unroll
-                for (int i = 0; i < kRows; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) o[i][e] *= scale;
-            }
-            const float base = m == -INFINITY ? 0.0f : m;
-            bf16x8_t pf[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t w[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float p0 = __builtin_amdgcn_exp2f(sc[8 * h + 2 * k] - base);
-                    const float p1 = __builtin_amdgcn_exp2f(sc[8 * h + 2 * k + 1] - base);
-                    l += p0 + p1;
-                    w[k] = f_to_bf16x2(p0 * vs, p1 * vs);
-                }
-                pf[h] = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
-            }
-            // values: pieces of column 32 i + lane % 32 with the lane's 16 keys
-            constexpr int kPieces = 2 / F::kHalves;
-            auto place = [&](int i, int p) {
-                const int r = 32 * i + col, piece = CT == SE12_STEP_E4M3 ? 2 * j + half : 2 * half + p;
-                return r * 64 + 16 * (piece ^ ((r >> 2) & 3));
-            };
-            const uint8_t* from = values;
-            if (!inside) {
-                // Through the wave's own copy: keys no column sees zeroed; a value that
-                // is no number would make 0 x NaN of a hidden key, so it leaves the copy
-                // and comes back in the columns that give it a weight.
-                uint8_t* own = lds + 4 * kHalfTile + wave * kHalfTile;
-#pragma unroll
-                for (int i = 0; i < kRows; ++i)
-#pragma unroll
-                    for (int p = 0; p < kPieces; ++p) {
-                        const int first = key0 + p * F::kPer;
-                        uint4 v = masked(*reinterpret_cast<const uint4*>(values + place(i, p)),
-                                         piece_mask<CT>(low - first, held ? high - first : 0));
-                        if (__builtin_amdgcn_ballot_w64(has_no_number<CT>(v)) != 0) {
-#pragma unroll
-                            for (int kind = 0; kind < (CT == SE12_STEP_E4M3 ? 1 : 3); ++kind) {
-                                floatx16_t x;
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) x[e] = 0.0f;
-#pragma unroll
-                                for (int h = 0; h < F::kHalves; ++h) {
-                                    const uint4 w = __builtin_bit_cast(uint4, operand<CT>(v, h));
-                                    const uint4 is = make_uint4(where_no_number(w.x, kind), where_no_number(w.y, kind),
-                                                                where_no_number(w.z, kind), where_no_number(w.w, kind));
-                                    x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, is), pf[p + h], x, 0, 0, 0);
-                                }
-#pragma unroll
-                                for (int e = 0; e < 16; ++e)
-                                    o[i][e] += x[e] == 0.0f ? 0.0f : kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY;
-                            }
-                            v = make_uint4(numbers_only<CT>(v.x), numbers_only<CT>(v.y), numbers_only<CT>(v.z), numbers_only<CT>(v.w));
-                        }
-                        *reinterpret_cast<uint4*>(own + place(i, p)) = v;
+                    for (int i = 0; i < kRows; ++i) {
+                        vf[i][n] = masked(vf[i][n], mask);
+                        bad |= has_no_number<CT>(vf[i][n]);
+                        if (known)
+                            vf[i][n] = make_uint4(numbers_only<CT>(vf[i][n].x), numbers_only<CT>(vf[i][n].y),
+                                                  numbers_only<CT>(vf[i][n].z), numbers_only<CT>(vf[i][n].w));
                     }
-                from = own;
+                }
+                apart = !known && __builtin_amdgcn_ballot_w64(bad) != 0;
             }
+            top = sc[0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) top = kCapped ? fminf(top, sc[e]) : fmaxf(top, sc[e]);
+            if constexpr (kCapped) top = a.cap - 2.0f * a.cap * top;
+            if (n32 == t0 * kSubs) m = fmaxf(top, __shfl_xor(top, 32, 64));
+            if (__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0 || apart) break;
+            weights();
+            known = false;
+            // (after the last sub-tile its own keys again: on every path as many reads,
+            // so that the waits below count exactly)
+            if (j == kSubs - 1 && t + 1 < t1) next_tile(t);
+            const int n = min(n32 + 1, t1 * kSubs - 1);
+            read_keys(n / kSubs, n % kSubs);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < kRows; ++i)
 #pragma unroll
-                for (int p = 0; p < kPieces; ++p) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(from + place(i, p));
+                for (int n = 0; n < kValueReads; ++n)
 #pragma unroll
                     for (int h = 0; h < F::kHalves; ++h)
-                        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand<CT>(v, h), pf[p + h], o[i], 0, 0, 0);
-                }
+                        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand<CT>(vf[i][n], h), pf[n + h], o[i], 0, 0, 0);
         }
+        if (n32 >= t1 * kSubs) break;
+        // The rare sub-tile, outside the loop, where the sums may stay in accumulation
+        // registers: the maximum moves, and what is summed with it; 0 x NaN is NaN, so
+        // a value that is no number comes in the columns that give it a weight, and
+        // leaves the product. Then the sub-tile starts again.
+        const float to = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
+        const float scale = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+        m = to;
+        l *= scale;
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[i][e] *= scale;
+        if (apart) {
+            const float sum = l;
+            weights();
+            l = sum;
+#pragma unroll
+            for (int i = 0; i < kRows; ++i)
+#pragma unroll
+                for (int n = 0; n < kValueReads; ++n) {
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int kind = 0; kind < (CT == SE12_STEP_E4M3 ? 1 : 3); ++kind) {
+                        floatx16_t x;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) x[e] = 0.0f;
+#pragma unroll
+                        for (int h = 0; h < F::kHalves; ++h) {
+                            const uint4 w = __builtin_bit_cast(uint4, operand<CT>(vf[i][n], h));
+                            const uint4 is = make_uint4(where_no_number(w.x, kind), where_no_number(w.y, kind),
+                                                        where_no_number(w.z, kind), where_no_number(w.w, kind));
+                            x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, is), pf[n + h], x, 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            o[i][e] += x[e] == 0.0f ? 0.0f : kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY;
+                    }
+                }
+            known = true;
+        }
+        read_keys(n32 / kSubs, n32 % kSubs);
     }
     l += __shfl_xor(l, 32, 64);
     if (!live) return;
@@ -382,7 +432,10 @@ namespace {
 template <int CT, int D>
 void launch(const AttendArgs& a, int slots, hipStream_t st) {
     const int grid = slots * a.splits * a.kvh;
-    hipLaunchKernelGGL((paged_prompt_kernel<CT, D>), dim3(grid), dim3(kPromptThreads), (4 + kPromptWaves) * 64 * D, st, a);
+    if (a.cap > 0.0f)
+        hipLaunchKernelGGL((paged_prompt_kernel<CT, D, true>), dim3(grid), dim3(kPromptThreads), 4 * 64 * D, st, a);
+    else
+        hipLaunchKernelGGL((paged_prompt_kernel<CT, D, false>), dim3(grid), dim3(kPromptThreads), 4 * 64 * D, st, a);
     if (a.splits > 1)
         hipLaunchKernelGGL((paged_prompt_join_kernel<CT, D>), dim3(slots * a.kvh, kBlockColumns / kPromptWaves), dim3(kPromptThreads), 0,
                            st, a, (int64_t)grid);
