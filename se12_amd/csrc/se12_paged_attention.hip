@@ -350,7 +350,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : 2) void paged_attent
 }
 
 // The units that several workers share, from their parts in order: one block per
-// (sequence, KV head, column unit) and column. A wave takes every kParts-th part, D /
+// (sequence, KV head, column unit) and column (or every fourth). A wave takes every kParts-th part, D /
 // 4 lanes to one, all its loads at once up to kBatch of them; a part's maximum may lie
 // above those before it, so what is summed moves with it.
 template <int CT, int D>
@@ -361,10 +361,9 @@ __global__ __launch_bounds__(kAttendThreads) void paged_join_kernel(AttendArgs a
     __shared__ float2 mls[kParts];
     const int tid = threadIdx.x, lane = tid & 63, part = tid / kLanes, at = tid % kLanes;
     const int unit = (int)(blockIdx.x % max_units), kh = (int)(blockIdx.x / max_units % a.kvh), s = (int)(blockIdx.x / max_units / a.kvh);
-    const int col = blockIdx.y, c = unit * kColumns + col;
     Chunk chunk = load_chunk<kTile>(a, s & ~63, lane);
     const SeqWork w = seq_work<kTile>(a, seq_of(chunk, s & 63));
-    if (unit >= w.units || c >= w.seq.n * a.group) return;
+    if (unit >= w.units) return;
     int64_t base = __builtin_amdgcn_readlane(chunk.upto, s & 63) - __builtin_amdgcn_readlane(chunk.tiles, s & 63), total = chunk.all;
     for (int s0 = 0; s0 < a.b.seqs; s0 += 64) {
         if (s0 == (s & ~63)) continue;
@@ -377,59 +376,65 @@ __global__ __launch_bounds__(kAttendThreads) void paged_join_kernel(AttendArgs a
     const int w0 = worker_of(first, per), w1 = worker_of(last, per);
     if (w0 == w1) return;      // one worker had it all
     const float2* mlp = reinterpret_cast<const float2*>(a.part + (int64_t)a.workers * 2 * a.columns * D);
-    float m = -INFINITY, l = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int k0 = w0 + part; k0 <= w1; k0 += kParts * kBatch) {
-        float2 ml[kBatch];
-        float4 v[kBatch];
+    for (int col = blockIdx.y; col < kColumns; col += gridDim.y) {
+        const int c = unit * kColumns + col;
+        if (c >= w.seq.n * a.group) break;
+        float m = -INFINITY, l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int k0 = w0 + part; k0 <= w1; k0 += kParts * kBatch) {
+            float2 ml[kBatch];
+            float4 v[kBatch];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const int k = k0 + i * kParts;
-            const int64_t p = part_at(a, min(k, w1), k == w0 ? 1 : 0) + col;
-            ml[i] = mlp[p];
-            v[i] = *reinterpret_cast<const float4*>(a.part + p * D + 4 * at);
+            for (int i = 0; i < kBatch; ++i) {
+                const int k = k0 + i * kParts;
+                const int64_t p = part_at(a, min(k, w1), k == w0 ? 1 : 0) + col;
+                ml[i] = mlp[p];
+                v[i] = *reinterpret_cast<const float4*>(a.part + p * D + 4 * at);
+            }
+            float to = m;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) to = k0 + i * kParts <= w1 ? fmaxf(to, ml[i].x) : to;
+            const float top = to == -INFINITY ? 0.0f : to, keep = __builtin_amdgcn_exp2f(m - top);
+            m = to;
+            l *= keep;
+            o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                if (k0 + i * kParts > w1) continue;
+                const float by = __builtin_amdgcn_exp2f(ml[i].x - top);
+                l += by * ml[i].y;
+                o.x += by * v[i].x;
+                o.y += by * v[i].y;
+                o.z += by * v[i].z;
+                o.w += by * v[i].w;
+            }
         }
-        float to = m;
+        sums[tid] = o;
+        if (at == 0) mls[part] = make_float2(m, l);
+        __syncthreads();
+        if (tid < kLanes) {
+            float to = mls[0].x;
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) to = k0 + i * kParts <= w1 ? fmaxf(to, ml[i].x) : to;
-        const float top = to == -INFINITY ? 0.0f : to, keep = __builtin_amdgcn_exp2f(m - top);
-        m = to;
-        l *= keep;
-        o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+            for (int k = 1; k < kParts; ++k) to = fmaxf(to, mls[k].x);
+            to = to == -INFINITY ? 0.0f : to;
+            o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            l = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            if (k0 + i * kParts > w1) continue;
-            const float by = __builtin_amdgcn_exp2f(ml[i].x - top);
-            l += by * ml[i].y;
-            o.x += by * v[i].x;
-            o.y += by * v[i].y;
-            o.z += by * v[i].z;
-            o.w += by * v[i].w;
+            for (int k = 0; k < kParts; ++k) {
+                const float4 v = sums[k * kLanes + tid];
+                const float by = __builtin_amdgcn_exp2f(mls[k].x - to);
+                l += by * mls[k].y;
+                o.x += by * v.x;
+                o.y += by * v.y;
+                o.z += by * v.z;
+                o.w += by * v.w;
+            }
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            store4(a.out + ((int64_t)(w.seq.start + c / a.group) * a.heads + kh * a.group + c % a.group) * D + 4 * tid, o.x * inv, o.y * inv,
+                   o.z * inv, o.w * inv);
         }
+        __syncthreads();      // sums and mls are free again
     }
-    sums[tid] = o;
-    if (at == 0) mls[part] = make_float2(m, l);
-    __syncthreads();
-    if (tid >= kLanes) return;
-    float to = mls[0].x;
-#pragma unroll
-    for (int k = 1; k < kParts; ++k) to = fmaxf(to, mls[k].x);
-    to = to == -INFINITY ? 0.0f : to;
-    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    l = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kParts; ++k) {
-        const float4 v = sums[k * kLanes + tid];
-        const float by = __builtin_amdgcn_exp2f(mls[k].x - to);
-        l += by * mls[k].y;
-        o.x += by * v.x;
-        o.y += by * v.y;
-        o.z += by * v.z;
-        o.w += by * v.w;
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    store4(a.out + ((int64_t)(w.seq.start + c / a.group) * a.heads + kh * a.group + c % a.group) * D + 4 * tid, o.x * inv, o.y * inv,
-           o.z * inv, o.w * inv);
 }
 
 }  // namespace se12step
@@ -465,7 +470,7 @@ template <int CT, int D>
 void launch_attend(const AttendArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((paged_attention_kernel<CT, D>), dim3(a.workers / (kAttendThreads / 64)), dim3(kAttendThreads), 0, st, a);
     const int max_units = (int)((std::min<int64_t>((int64_t)a.b.max_new * a.group, kFewColumns) + kColumns - 1) / kColumns);
-    hipLaunchKernelGGL((paged_join_kernel<CT, D>), dim3((uint32_t)((int64_t)a.b.seqs * a.kvh * max_units), a.columns), dim3(kAttendThreads), 0,
+    hipLaunchKernelGGL((paged_join_kernel<CT, D>), dim3((uint32_t)((int64_t)a.b.seqs * a.kvh * max_units), max_units > 1 ? 4 : a.columns), dim3(kAttendThreads), 0,
                        st, a, max_units);
 }
 

@@ -43,29 +43,70 @@ struct Unit {
     int keys, columns;     // of the sequence
 };
 
-// Unit slots: sequence s has slots starts[s] * group / 128 + s onwards, enough for
-// its ceil(n group / 128) units.
-__device__ __forceinline__ bool find_unit(const AttendArgs& a, int slot, Unit& u) {
-    auto base = [&](int s) { return (int)((int64_t)min(max(a.b.starts[s], 0), a.b.tokens) * a.group / kBlockColumns) + s; };
-    int lo = 0, hi = a.b.seqs;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (base(mid) <= slot)
-            lo = mid;
-        else
-            hi = mid;
+// The units in the order they are started: 64 sequences after the other, and among
+// those by the last key they see, the most first, so that what is left for the last
+// blocks is short. One lane holds one sequence: how many of its units see a key past
+// 64 x is in closed form, so the x of a rank is found by halving.
+struct UnitCounts {
+    Seq seq;
+    int keys, columns, units;
+    // units that see past key x
+    __device__ __forceinline__ int past(int x, int group) const {
+        const int64_t c = (int64_t)max(x - seq.len, 0) * group;     // the first column that does
+        return keys > x && c < columns ? units - (int)(c / kBlockColumns) : 0;
     }
-    // (the same for all lanes, and kept in scalar registers)
-    lo = __builtin_amdgcn_readfirstlane(lo);
-    u.s = lo;
-    const int capacity = a.b.width << a.page_log2;
-    const Seq seq = load_seq(a.b, lo, capacity);
-    u.seq = {__builtin_amdgcn_readfirstlane(seq.start), __builtin_amdgcn_readfirstlane(seq.n), __builtin_amdgcn_readfirstlane(seq.len)};
-    u.keys = min(u.seq.len + u.seq.n, capacity);
-    u.columns = u.seq.n * a.group;
-    const int64_t first = (int64_t)(slot - __builtin_amdgcn_readfirstlane(base(lo))) * kBlockColumns;
-    u.first = (int)first;
-    return first >= 0 && first < u.columns && u.columns > a.few;
+};
+
+__device__ __forceinline__ int wave_total(int v) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+    return __builtin_amdgcn_readfirstlane(v);
+}
+
+__device__ __forceinline__ bool find_unit(const AttendArgs& a, int rank, Unit& u) {
+    const int lane = threadIdx.x & 63, capacity = a.b.width << a.page_log2;
+    for (int s0 = 0; s0 < a.b.seqs; s0 += 64) {
+        UnitCounts c;
+        c.seq = load_seq(a.b, min(s0 + lane, a.b.seqs - 1), capacity);
+        c.keys = min(c.seq.len + c.seq.n, capacity);
+        c.columns = s0 + lane < a.b.seqs ? c.seq.n * a.group : 0;
+        c.units = c.columns > a.few ? (c.columns + kBlockColumns - 1) / kBlockColumns : 0;
+        c.columns = c.units > 0 ? c.columns : 0;
+        const int all = wave_total(c.units);
+        if (rank >= all) {
+            rank -= all;
+            continue;
+        }
+        int most = c.units > 0 ? c.keys : 0;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o, 64));
+        // the largest x with more than `rank` units past 64 x (every unit is past -1)
+        int lo = -1, hi = (__builtin_amdgcn_readfirstlane(most) + 63) / 64;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (wave_total(c.past(64 * mid, a.group)) > rank)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        const int here = lo < 0 ? c.units : c.past(64 * lo, a.group), beyond = c.past(64 * (lo + 1), a.group);
+        rank -= wave_total(beyond);
+        int upto = here - beyond;      // of this x: a sequence's are units - here .. units - beyond - 1
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(upto, o, 64);
+            upto += lane >= o ? v : 0;
+        }
+        const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > rank));
+        auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+        u.s = s0 + l;
+        u.seq = {of(c.seq.start), of(c.seq.n), of(c.seq.len)};
+        u.keys = of(c.keys);
+        u.columns = of(c.columns);
+        u.first = kBlockColumns * (of(c.units) - of(here) + rank - (of(upto) - (of(here) - of(beyond))));
+        return true;
+    }
+    return false;
 }
 
 // the key tiles the unit's columns see
@@ -76,6 +117,30 @@ __device__ __forceinline__ void unit_tiles(const AttendArgs& a, const Unit& u, i
     t0 = (a.window > 0 ? max(0, pos0 - a.window + 1) : 0) / kTile;
     t1 = max((min(u.keys, pos1 + 1) + kTile - 1) / kTile, t0 + 1);
 }
+
+// se12::lds_load16 from a uniform address and the lane's offset
+__device__ __forceinline__ void lds_load16(const void* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds) : "memory", "m0");
+}
+
+// A sum where it is kept, in an accumulation register. (Written with the register's
+// class: as ordinary arithmetic it makes the compiler keep all sums in vector registers
+// as well, over the whole walk, and spill.) The compiler's wait states between matrix
+// instructions and others do not see into these, so settle_products() stands on both
+// sides: no matrix instruction is in flight for longer.
+__device__ __forceinline__ float times(float x, float by) {
+    float t;
+    asm volatile("v_accvgpr_read_b32 %1, %0\n\ts_nop 1\n\tv_mul_f32 %1, %1, %2\n\ts_nop 1\n\tv_accvgpr_write_b32 %0, %1"
+                 : "+a"(x), "=&v"(t) : "v"(by));
+    return x;
+}
+__device__ __forceinline__ float plus(float x, float y) {
+    float t;
+    asm volatile("v_accvgpr_read_b32 %1, %0\n\ts_nop 1\n\tv_add_f32 %1, %1, %2\n\ts_nop 1\n\tv_accvgpr_write_b32 %0, %1"
+                 : "+a"(x), "=&v"(t) : "v"(y));
+    return x;
+}
+__device__ __forceinline__ void settle_products() { asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15"); }
 
 template <int CT, int D, bool kCapped>
 __global__ __launch_bounds__(kPromptThreads, 1) void paged_prompt_kernel(AttendArgs a) {
@@ -89,10 +154,9 @@ __global__ __launch_bounds__(kPromptThreads, 1) void paged_prompt_kernel(AttendA
     static_assert(kValuePieces == 4 && kLoads >= 1, "");
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];     // [2][keys, values]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int kh = blockIdx.x % a.kvh, rest = blockIdx.x / a.kvh, split = rest % a.splits;
-    const int slot = (int)(gridDim.x / a.kvh / a.splits) - 1 - rest / a.splits;   // the last columns, with the most keys, first
+    const int kh = blockIdx.x % a.kvh, rest = blockIdx.x / a.kvh, split = rest % a.splits, rank = rest / a.splits;
     Unit u;
-    if (!find_unit(a, slot, u)) return;
+    if (!find_unit(a, rank, u)) return;
     int t0, t1;
     unit_tiles<kTile>(a, u, t0, t1);
     const int length = max((t1 - t0 + a.splits - 1) / a.splits, kLeastTiles);
@@ -119,6 +183,11 @@ __global__ __launch_bounds__(kPromptThreads, 1) void paged_prompt_kernel(AttendA
         for (int i = 0; i < kQSteps; ++i)
             qf[i] = *reinterpret_cast<const bf16x8_t*>(qp + (i / F::kHalves) * 2 * F::kPer + half * F::kPer + 8 * (i % F::kHalves));
     }
+    // (in accumulation registers, which the products read as well)
+    if constexpr (D == 256) {
+#pragma unroll
+        for (int i = 0; i < kQSteps; ++i) asm volatile("" : "+a"(qf[i]));
+    }
     floatx16_t o[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
@@ -127,7 +196,9 @@ __global__ __launch_bounds__(kPromptThreads, 1) void paged_prompt_kernel(AttendA
     float m = -INFINITY, l = 0.0f;
 
     // Loads of a tile. Piece p of a row lies at place p ^ f(row): f of a key from the
-    // four bits that tell the rows of 16 lanes apart, of a value column from two.
+    // four bits that tell the rows of 16 lanes apart, of a value column from two. A
+    // wave's keys lie in one page (16 of a tile, or 8); a lane's values in the page of
+    // its piece.
     const int P = 1 << a.page_log2;
     constexpr int kElem = 16 / F::kPer;
     const int32_t* table = a.b.table + u.s * a.b.table_stride;
@@ -137,74 +208,93 @@ __global__ __launch_bounds__(kPromptThreads, 1) void paged_prompt_kernel(AttendA
         const int b = (r & 7) | ((r & 16) >> 1);
         return kKeyPieces >= 16 ? b : b >> (kKeyPieces == 8 ? 1 : 2);
     };
-    constexpr int kRowsPerLoad = 64 / kKeyPieces;     // keys of one load, of one group of 16
+    constexpr int kWaveKeys = kTile / kPromptWaves, kRowsPerLoad = 64 / kKeyPieces;
+    static_assert(kLoads * kRowsPerLoad == kWaveKeys, "");
     const int vpiece = (lane & 3) ^ ((lane >> 4) & 3);
     const uint32_t lds0 = se12::lds_address(lds);
-    auto load_tile = [&](int t, int buffer, int key_entry, int value_entry) {
-        const int k0 = t * kTile;
-        const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + buffer * 2 * kHalfTile);
+    uint32_t key_at[kLoads];      // the lane's bytes of a load, from the wave's first key
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int n = wave * kLoads + i;
-            const int r = n * kRowsPerLoad + lane / kKeyPieces, g = n * kRowsPerLoad / 16;
-            const int page = in_pool(__builtin_amdgcn_readlane(key_entry, g));
-            const int piece = (lane % kKeyPieces) ^ key_twist(r);
-            const int64_t at = (((int64_t)page * a.kvh + kh) * P + ((k0 + r) & (P - 1))) * (D * kElem) + 16 * piece;
-            se12::lds_load16(static_cast<const uint8_t*>(a.kc) + at, to + n * 1024);
-        }
-        const int64_t vbase = (((int64_t)in_pool(value_entry) * a.kvh + kh) * D + (lane >> 2)) * (int64_t)(P * kElem) +
-                              ((k0 + vpiece * F::kPer) & (P - 1)) * kElem;
+    for (int i = 0; i < kLoads; ++i) {
+        const int r = i * kRowsPerLoad + lane / kKeyPieces;
+        key_at[i] = r * (D * kElem) + 16 * ((lane % kKeyPieces) ^ key_twist(wave * kWaveKeys + r));
+    }
+    auto load_keys = [&](int t, int buffer, int key_entry) {
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + buffer * 2 * kHalfTile) + wave * kLoads * 1024;
+        const int page = in_pool(__builtin_amdgcn_readfirstlane(key_entry)), first = (t * kTile + wave * kWaveKeys) & (P - 1);
+        const uint8_t* from = static_cast<const uint8_t*>(a.kc) + (((int64_t)page * a.kvh + kh) * P + first) * (D * kElem);
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int n = wave * kLoads + i;
-            se12::lds_load16(static_cast<const uint8_t*>(a.vc) + vbase + (int64_t)n * 16 * P * kElem, to + kHalfTile + n * 1024);
-        }
+        for (int i = 0; i < kLoads; ++i) lds_load16(from, key_at[i], to + i * 1024);
     };
-    auto key_entry_of = [&](int t) { return entry(t * kTile + 16 * (lane & (kTile / 16 - 1))); };
+    auto load_values = [&](int t, int buffer, int value_entry) {
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + buffer * 2 * kHalfTile) + kHalfTile + wave * kLoads * 1024;
+        const uint8_t* from = static_cast<const uint8_t*>(a.vc) +
+                              (((int64_t)in_pool(value_entry) * a.kvh + kh) * D + wave * kLoads * 16 + (lane >> 2)) * (int64_t)(P * kElem) +
+                              ((t * kTile + vpiece * F::kPer) & (P - 1)) * kElem;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) se12::lds_load16(from + i * 16 * P * kElem, to + i * 1024);
+    };
+    auto key_entry_of = [&](int t) { return entry(t * kTile + wave * kWaveKeys); };
     auto value_entry_of = [&](int t) { return entry(t * kTile + vpiece * F::kPer); };
     // scales of the lane's 16 keys of each sub-tile, and whether a page holds them
     struct Lane {
-        float ks[kSubs], vs[kSubs];
-        int held[kSubs];
+        float ks0 = 1.0f, vs0 = 1.0f, ks1 = 1.0f, vs1 = 1.0f;
+        int held0 = 0, held1 = 0;
     };
-    auto lane_of = [&](int key_entry) {
+    auto lane_of = [&](int2 e) {
         Lane x;
-#pragma unroll
-        for (int j = 0; j < kSubs; ++j) {
-            const int e = __shfl(key_entry, 2 * j + half, 64);
-            x.held[j] = (uint32_t)e < (uint32_t)a.pages;
-            x.ks[j] = x.vs[j] = 1.0f;
-            if constexpr (CT == SE12_STEP_E4M3) {
-                const int64_t at = (int64_t)in_pool(e) * a.kvh + kh;
-                x.ks[j] = a.k_scale[at];
-                x.vs[j] = a.v_scale[at];
-            }
+        x.held0 = (uint32_t)e.x < (uint32_t)a.pages;
+        x.held1 = (uint32_t)e.y < (uint32_t)a.pages;
+        if constexpr (CT == SE12_STEP_E4M3) {
+            const int64_t at0 = (int64_t)in_pool(e.x) * a.kvh + kh, at1 = (int64_t)in_pool(e.y) * a.kvh + kh;
+            x.ks0 = a.k_scale[at0];
+            x.vs0 = a.v_scale[at0];
+            x.ks1 = a.k_scale[at1];
+            x.vs1 = a.v_scale[at1];
         }
         return x;
     };
+    auto lane_entries_of = [&](int t) {
+        return make_int2(entry(t * kTile + 16 * half), entry(t * kTile + (kSubs - 1) * kSubTile + 16 * half));
+    };
+    auto arrived = [](Lane& x) {     // (loaded with what is waited for here)
+        asm volatile("" : "+v"(x.ks0), "+v"(x.vs0), "+v"(x.ks1), "+v"(x.vs1), "+v"(x.held0), "+v"(x.held1));
+    };
     // What the wave holds of a sub-tile of 32 keys: keys' pieces, value columns' pieces.
     constexpr int kKeyReads = kKeyPieces / 2, kValueReads = 2 / F::kHalves;
-    // (of a key no more than 8 pieces at once)
-    constexpr int kAhead = kKeyReads < 8 ? kKeyReads : 8;
-    uint4 kf[kAhead], vf[kRows][kValueReads];
-    auto key_piece = [&](int t, int j, int i) {
-        const int row = j * kSubTile + key_of_row(col), twist = key_twist(row);
-        const uint8_t* p = lds + ((t - t0) & 1) * 2 * kHalfTile + row * (kKeyPieces * 16);
-        return *reinterpret_cast<const uint4*>(p + 16 * ((2 * i + half) ^ twist));
-    };
-    auto read_keys = [&](int t, int j) {
+    uint4 kf[kKeyReads], vf[kRows];
+    // (pieces 2 i + half of the lane's row: the place's bits and those of i meet in an
+    // exclusive or, so one address gives all of them)
+    const int key_row0 = key_of_row(col), key_off0 = key_row0 * (kKeyPieces * 16) + 16 * (half ^ key_twist(key_row0));
+    auto read_keys = [&](int u) {
+        const int t = u / kSubs, j = u % kSubs;
+        const int at = key_off0 + ((t - t0) & 1) * 2 * kHalfTile + j * kSubTile * kKeyPieces * 16;
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) kf[i] = key_piece(t, j, i);
+        for (int i = 0; i < kKeyReads; ++i) kf[i] = *reinterpret_cast<const uint4*>(lds + (at ^ (32 * (i & 7))) + 256 * (i >> 3));
     };
-    auto read_values = [&](int t, int j) {
+    // (the n-th of the lane's pieces of each row)
+    auto read_values = [&](int t, int j, int n) {
         const uint8_t* p = lds + (((t - t0) & 1) * 2 + 1) * kHalfTile;
 #pragma unroll
-        for (int i = 0; i < kRows; ++i)
+        for (int i = 0; i < kRows; ++i) {
+            const int r = 32 * i + col, piece = CT == SE12_STEP_E4M3 ? 2 * j + half : 2 * half + n;
+            vf[i] = *reinterpret_cast<const uint4*>(p + r * 64 + 16 * (piece ^ ((r >> 2) & 3)));
+        }
+    };
+    auto mask_values = [&](int key0, bool held, int n) {
+        const uint4 mask = piece_mask<CT>(low - key0 - n * F::kPer, held ? high - key0 - n * F::kPer : 0);
 #pragma unroll
-            for (int n = 0; n < kValueReads; ++n) {
-                const int r = 32 * i + col, piece = CT == SE12_STEP_E4M3 ? 2 * j + half : 2 * half + n;
-                vf[i][n] = *reinterpret_cast<const uint4*>(p + r * 64 + 16 * (piece ^ ((r >> 2) & 3)));
-            }
+        for (int i = 0; i < kRows; ++i) vf[i] = masked(vf[i], mask);
+    };
+    auto numbers_of_values = [&]() {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+            vf[i] = make_uint4(numbers_only<CT>(vf[i].x), numbers_only<CT>(vf[i].y), numbers_only<CT>(vf[i].z), numbers_only<CT>(vf[i].w));
+    };
+    auto any_no_number = [&]() {
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) bad |= has_no_number<CT>(vf[i]);
+        return __builtin_amdgcn_ballot_w64(bad) != 0;
     };
     float sc[16], top = 0.0f, vs = 1.0f;    // sc: scores, or r of cap - 2 cap r
     bf16x8_t pf[2];
@@ -233,139 +323,178 @@ __global__ __launch_bounds__(kPromptThreads, 1) void paged_prompt_kernel(AttendA
         }
     };
 
-    int ke = key_entry_of(t0), ve = value_entry_of(t0);
-    Lane now, next = lane_of(ke);
-    load_tile(t0, 0, ke, ve);
-    ke = key_entry_of(min(t0 + 1, t1 - 1));
-    ve = value_entry_of(min(t0 + 1, t1 - 1));
-    // Tile t + 1 (its loads were sent a tile ago) takes over: after the barrier it is
-    // whole, and every wave is done with tile t, whose place tile t + 2 may take.
-    auto next_tile = [&](int t) {
-        se12::wait_vector_loads();
-        now = next;
-#pragma unroll
-        for (int j = 0; j < kSubs; ++j) asm volatile("" : "+v"(now.ks[j]), "+v"(now.vs[j]), "+v"(now.held[j]));
-        asm volatile("" : "+v"(ke), "+v"(ve));
-        __syncthreads();
-        if (t + 2 < t1) {
-            next = lane_of(ke);
-            load_tile(t + 2, (t - t0) & 1, ke, ve);
-            ke = key_entry_of(min(t + 3, t1 - 1));
-            ve = value_entry_of(min(t + 3, t1 - 1));
-        }
+    // The walk, sub-tile by sub-tile (u of u0 .. u1 - 1): scores of u + 1 while the
+    // weights of u are worked out, then the product of u's weights and values while the
+    // scores of u + 1 are capped; keys are in registers two sub-tiles ahead of the
+    // values. At the start of a tile a barrier: its values and the keys kLead tiles on
+    // have come (their loads were sent a tile ago), and every wave is done with what
+    // the next loads overwrite.
+    constexpr int kLead = 2 / kSubs;
+    const int u0 = t0 * kSubs, u1 = t1 * kSubs;
+    auto key_tile = [&](int t, int entry) {
+        if (t < t1) load_keys(t, (t - t0) & 1, entry);
     };
-    next_tile(t0 - 1);
-    read_keys(t0, 0);
-    bool known = false;      // what is no number in the sub-tile's values has been dealt with
-    for (int n32 = t0 * kSubs; n32 < t1 * kSubs;) {
-        bool apart = false;
-        for (; n32 < t1 * kSubs; ++n32) {
-            const int t = n32 / kSubs, j = n32 % kSubs, k0 = n32 * kSubTile, key0 = k0 + 16 * half;
-            floatx16_t d;
+    // `ke`, `ve`: table entries of the tiles whose keys and values are loaded next; `se`:
+    // of the lane's keys in the next tile, for their scales
+    int ke = key_entry_of(t0);
+    key_tile(t0, ke);
+    Lane now = lane_of(lane_entries_of(t0)), next = now;
+    if constexpr (kLead == 2) {
+        ke = key_entry_of(min(t0 + 1, t1 - 1));
+        asm volatile("" : "+v"(ke));
+        key_tile(t0 + 1, ke);
+    }
+    se12::wait_vector_loads();
+    arrived(now);
+    __syncthreads();
+    floatx16_t d;
+    auto scores = [&]() {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) d[e] = 0.0f;
+        for (int e = 0; e < 16; ++e) d[e] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kKeyReads; ++i) {
+        for (int i = 0; i < kKeyReads; ++i)
 #pragma unroll
-                for (int h = 0; h < F::kHalves; ++h)
-                    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand<CT>(kf[i % kAhead], h), qf[i * F::kHalves + h], d, 0, 0, 0);
-                if (i + kAhead < kKeyReads) kf[i % kAhead] = key_piece(t, j, i + kAhead);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            read_values(t, j);
-            __builtin_amdgcn_sched_barrier(0);
-            const float by = a.c1 * (j ? now.ks[kSubs - 1] : now.ks[0]);
+            for (int h = 0; h < F::kHalves; ++h)
+                d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand<CT>(kf[i], h), qf[i * F::kHalves + h], d, 0, 0, 0);
+    };
+    auto cap_scores = [&](float ks) {
+        const float by = a.c1 * ks;
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                sc[e] = kCapped ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(d[e] * by)) : d[e] * by;
-            const bool held = (j ? now.held[kSubs - 1] : now.held[0]) != 0 && key0 < high && key0 + 16 > low;
-            const bool inside = k0 + kSubTile - 1 <= pos_min && k0 + kSubTile <= u.keys && pos_max - k0 < reach &&
-                                __builtin_amdgcn_ballot_w64(!held) == 0;
-            vs = j ? now.vs[kSubs - 1] : now.vs[0];
-            if (!inside) {
-                vs = held ? vs : 0.0f;
-                const int since = max(pos - reach + 1, 0) - key0, to = held ? min(pos + 1, u.keys) - key0 : 0;
+        for (int e = 0; e < 16; ++e)
+            sc[e] = kCapped ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(d[e] * by)) : d[e] * by;
+    };
+    auto find_top = [&]() {
+        top = sc[0];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) sc[e] = (e < since || e >= to) ? (kCapped ? INFINITY : -INFINITY) : sc[e];
-                bool bad = false;
-#pragma unroll
-                for (int n = 0; n < kValueReads; ++n) {
-                    const uint4 mask = piece_mask<CT>(low - key0 - n * F::kPer, held ? high - key0 - n * F::kPer : 0);
-#pragma unroll
-                    for (int i = 0; i < kRows; ++i) {
-                        vf[i][n] = masked(vf[i][n], mask);
-                        bad |= has_no_number<CT>(vf[i][n]);
-                        if (known)
-                            vf[i][n] = make_uint4(numbers_only<CT>(vf[i][n].x), numbers_only<CT>(vf[i][n].y),
-                                                  numbers_only<CT>(vf[i][n].z), numbers_only<CT>(vf[i][n].w));
-                    }
-                }
-                apart = !known && __builtin_amdgcn_ballot_w64(bad) != 0;
-            }
-            top = sc[0];
-#pragma unroll
-            for (int e = 1; e < 16; ++e) top = kCapped ? fminf(top, sc[e]) : fmaxf(top, sc[e]);
-            if constexpr (kCapped) top = a.cap - 2.0f * a.cap * top;
-            if (n32 == t0 * kSubs) m = fmaxf(top, __shfl_xor(top, 32, 64));
-            if (__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0 || apart) break;
-            weights();
-            known = false;
-            // (after the last sub-tile its own keys again: on every path as many reads,
-            // so that the waits below count exactly)
-            if (j == kSubs - 1 && t + 1 < t1) next_tile(t);
-            const int n = min(n32 + 1, t1 * kSubs - 1);
-            read_keys(n / kSubs, n % kSubs);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int i = 0; i < kRows; ++i)
-#pragma unroll
-                for (int n = 0; n < kValueReads; ++n)
-#pragma unroll
-                    for (int h = 0; h < F::kHalves; ++h)
-                        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand<CT>(vf[i][n], h), pf[n + h], o[i], 0, 0, 0);
-        }
-        if (n32 >= t1 * kSubs) break;
-        // The rare sub-tile, outside the loop, where the sums may stay in accumulation
-        // registers: the maximum moves, and what is summed with it; 0 x NaN is NaN, so
-        // a value that is no number comes in the columns that give it a weight, and
-        // leaves the product. Then the sub-tile starts again.
+        for (int e = 1; e < 16; ++e) top = kCapped ? fminf(top, sc[e]) : fmaxf(top, sc[e]);
+        if constexpr (kCapped) top = a.cap - 2.0f * a.cap * top;
+    };
+    read_keys(u0);
+    scores();
+    read_keys(min(u0 + 1, u1 - 1));
+    cap_scores(now.ks0);
+    find_top();
+    ke = key_entry_of(min(t0 + kLead, t1 - 1));
+    int ve = value_entry_of(t0);
+    asm volatile("" : "+v"(ke), "+v"(ve));
+    key_tile(t0 + kLead, ke);
+    load_values(t0, 0, ve);
+    ke = key_entry_of(min(t0 + kLead + 1, t1 - 1));
+    ve = value_entry_of(min(t0 + 1, t1 - 1));
+    int2 se = lane_entries_of(min(t0 + 1, t1 - 1));
+
+    auto move_maximum = [&]() {
         const float to = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
         const float scale = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
         m = to;
         l *= scale;
+        settle_products();
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[i][e] *= scale;
-        if (apart) {
-            const float sum = l;
-            weights();
-            l = sum;
+            for (int e = 0; e < 16; ++e) o[i][e] = times(o[i][e], scale);
+        settle_products();
+    };
+    // 0 x NaN is NaN: what is no number comes in the columns that give it a weight (and
+    // leaves the product)
+    auto bring_no_numbers = [&](int t, int j, int key0, bool held) {
+#pragma unroll
+        for (int n = 0; n < kValueReads; ++n) {
+            read_values(t, j, n);
+            mask_values(key0, held, n);
 #pragma unroll
             for (int i = 0; i < kRows; ++i)
 #pragma unroll
-                for (int n = 0; n < kValueReads; ++n) {
+                for (int kind = 0; kind < (CT == SE12_STEP_E4M3 ? 1 : 3); ++kind) {
                     __builtin_amdgcn_sched_barrier(0);
+                    settle_products();
+                    floatx16_t x;
 #pragma unroll
-                    for (int kind = 0; kind < (CT == SE12_STEP_E4M3 ? 1 : 3); ++kind) {
-                        floatx16_t x;
+                    for (int e = 0; e < 16; ++e) x[e] = 0.0f;
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) x[e] = 0.0f;
-#pragma unroll
-                        for (int h = 0; h < F::kHalves; ++h) {
-                            const uint4 w = __builtin_bit_cast(uint4, operand<CT>(vf[i][n], h));
-                            const uint4 is = make_uint4(where_no_number(w.x, kind), where_no_number(w.y, kind),
-                                                        where_no_number(w.z, kind), where_no_number(w.w, kind));
-                            x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, is), pf[n + h], x, 0, 0, 0);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            o[i][e] += x[e] == 0.0f ? 0.0f : kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY;
+                    for (int h = 0; h < F::kHalves; ++h) {
+                        const uint4 w = __builtin_bit_cast(uint4, operand<CT>(vf[i], h));
+                        const uint4 is = make_uint4(where_no_number(w.x, kind), where_no_number(w.y, kind),
+                                                    where_no_number(w.z, kind), where_no_number(w.w, kind));
+                        x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, is), pf[n + h], x, 0, 0, 0);
                     }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        o[i][e] = plus(o[i][e], x[e] == 0.0f ? 0.0f : kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY);
                 }
-            known = true;
         }
-        read_keys(n32 / kSubs, n32 % kSubs);
+        settle_products();
+    };
+    for (int u32 = u0; u32 < u1; ++u32) {
+        bool apart = false;      // a value that is no number may be hidden from some of the columns
+        const int t = u32 / kSubs, j = u32 % kSubs, k0 = u32 * kSubTile, key0 = k0 + 16 * half;
+        if (j == 0) {
+            se12::wait_vector_loads();
+            if (t > t0) now = next;
+            arrived(now);
+            asm volatile("" : "+v"(ke), "+v"(ve), "+v"(se.x), "+v"(se.y));
+            __syncthreads();
+            if (t + 1 < t1) {
+                next = lane_of(se);
+                key_tile(t + kLead + 1, ke);
+                load_values(t + 1, (t + 1 - t0) & 1, ve);
+                ke = key_entry_of(min(t + kLead + 2, t1 - 1));
+                ve = value_entry_of(min(t + 2, t1 - 1));
+                se = lane_entries_of(min(t + 2, t1 - 1));
+            }
+        }
+        const bool held = (j ? now.held1 : now.held0) != 0 && key0 < high && key0 + 16 > low;
+        const bool inside = k0 + kSubTile - 1 <= pos_min && k0 + kSubTile <= u.keys && pos_max - k0 < reach &&
+                            __builtin_amdgcn_ballot_w64(!held) == 0;
+        vs = j ? now.vs1 : now.vs0;
+        if (!inside) {
+            vs = held ? vs : 0.0f;
+            const int since = max(pos - reach + 1, 0) - key0, to = held ? min(pos + 1, u.keys) - key0 : 0;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[e] = (e < since || e >= to) ? (kCapped ? INFINITY : -INFINITY) : sc[e];
+            find_top();
+#pragma unroll
+            for (int n = 1; n < kValueReads; ++n) {
+                read_values(t, j, n);
+                mask_values(key0, held, n);
+                apart |= any_no_number();
+            }
+        }
+        read_values(t, j, 0);
+        if (!inside) {
+            mask_values(key0, held, 0);
+            apart |= any_no_number();
+        }
+        if (u32 == u0) m = fmaxf(top, __shfl_xor(top, 32, 64));
+        if (__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0) move_maximum();
+        scores();
+        weights();
+        if (apart) {
+            bring_no_numbers(t, j, key0, held);
+            read_values(t, j, 0);
+            mask_values(key0, held, 0);
+            numbers_of_values();
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        read_keys(min(u32 + 2, u1 - 1));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < kValueReads; ++n) {
+            if (n > 0) {
+                read_values(t, j, n);
+                if (!inside) {
+                    mask_values(key0, held, n);
+                    if (apart) numbers_of_values();
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kRows; ++i)
+#pragma unroll
+                for (int h = 0; h < F::kHalves; ++h)
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand<CT>(vf[i], h), pf[n + h], o[i], 0, 0, 0);
+        }
+        cap_scores(j + 1 < kSubs ? now.ks1 : next.ks0);
+        find_top();
     }
     l += __shfl_xor(l, 32, 64);
     if (!live) return;
@@ -379,8 +508,8 @@ __global__ __launch_bounds__(kPromptThreads, 1) void paged_prompt_kernel(AttendA
                 store4(out + 32 * i + 8 * g, o[i][4 * g] * inv, o[i][4 * g + 1] * inv, o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv);
         return;
     }
-    // the part of (slot, head, split)
-    const int64_t p = (((int64_t)slot * a.kvh + kh) * a.splits + split) * kBlockColumns + wave * kWaveColumns + col;
+    // the part of (unit, head, split)
+    const int64_t p = (((int64_t)rank * a.kvh + kh) * a.splits + split) * kBlockColumns + wave * kWaveColumns + col;
     float* to = a.part + p * D + 4 * half;
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
@@ -394,37 +523,42 @@ __global__ __launch_bounds__(kPromptThreads, 1) void paged_prompt_kernel(AttendA
     }
 }
 
-// Units whose keys were split, from their parts in order: a wave per column.
+// Units whose keys were split, from their parts in order: a wave per column, and then
+// the next.
+constexpr int kJoinBlocks = 4;      // of a unit
+
 template <int CT, int D>
 __global__ __launch_bounds__(kPromptThreads) void paged_prompt_join_kernel(AttendArgs a, int64_t parts) {
     constexpr int kTile = Form<CT>::kTile, kPerLane = D / 64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int kh = blockIdx.x % a.kvh, slot = blockIdx.x / a.kvh;
+    const int kh = blockIdx.x % a.kvh, rank = blockIdx.x / a.kvh;
     Unit u;
-    if (!find_unit(a, slot, u)) return;
+    if (!find_unit(a, rank, u)) return;
     int t0, t1;
     unit_tiles<kTile>(a, u, t0, t1);
     const int length = max((t1 - t0 + a.splits - 1) / a.splits, kLeastTiles), count = (t1 - t0 + length - 1) / length;
-    const int c = blockIdx.y * kPromptWaves + wave;
-    if (count <= 1 || u.first + c >= u.columns) return;
-    const int64_t p0 = ((int64_t)slot * a.kvh + kh) * a.splits * kBlockColumns + c;
+    if (count <= 1) return;
     const float* ml = a.part + parts * kBlockColumns * D;
-    float m = -INFINITY;
-    for (int k = 0; k < count; ++k) m = fmaxf(m, ml[2 * (p0 + (int64_t)k * kBlockColumns)]);
-    const float top = m == -INFINITY ? 0.0f : m;
-    float o[kPerLane] = {}, l = 0.0f;
-    for (int k = 0; k < count; ++k) {
-        const int64_t p = p0 + (int64_t)k * kBlockColumns;
-        const float by = __builtin_amdgcn_exp2f(ml[2 * p] - top);
-        l += by * ml[2 * p + 1];
+    for (int c = blockIdx.y * kPromptWaves + wave; c < kBlockColumns && u.first + c < u.columns; c += kJoinBlocks * kPromptWaves) {
+        const int64_t p0 = ((int64_t)rank * a.kvh + kh) * a.splits * kBlockColumns + c;
+        float m = -INFINITY;
+        for (int k = 0; k < count; ++k) m = fmaxf(m, ml[2 * (p0 + (int64_t)k * kBlockColumns)]);
+        const float top = m == -INFINITY ? 0.0f : m;
+        float o[kPerLane] = {}, l = 0.0f;
+#pragma unroll 4
+        for (int k = 0; k < count; ++k) {
+            const int64_t p = p0 + (int64_t)k * kBlockColumns;
+            const float by = __builtin_amdgcn_exp2f(ml[2 * p] - top);
+            l += by * ml[2 * p + 1];
 #pragma unroll
-        for (int e = 0; e < kPerLane; ++e) o[e] += by * a.part[p * D + 64 * e + lane];
+            for (int e = 0; e < kPerLane; ++e) o[e] += by * a.part[p * D + 64 * e + lane];
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const int col = u.first + c;
+        uint16_t* out = a.out + ((int64_t)(u.seq.start + col / a.group) * a.heads + kh * a.group + col % a.group) * D + lane;
+#pragma unroll
+        for (int e = 0; e < kPerLane; ++e) out[64 * e] = f_to_bf16(o[e] * inv);
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int col = u.first + c;
-    uint16_t* out = a.out + ((int64_t)(u.seq.start + col / a.group) * a.heads + kh * a.group + col % a.group) * D + lane;
-#pragma unroll
-    for (int e = 0; e < kPerLane; ++e) out[64 * e] = f_to_bf16(o[e] * inv);
 }
 
 namespace {
@@ -437,11 +571,12 @@ void launch(const AttendArgs& a, int slots, hipStream_t st) {
     else
         hipLaunchKernelGGL((paged_prompt_kernel<CT, D, false>), dim3(grid), dim3(kPromptThreads), 4 * 64 * D, st, a);
     if (a.splits > 1)
-        hipLaunchKernelGGL((paged_prompt_join_kernel<CT, D>), dim3(slots * a.kvh, kBlockColumns / kPromptWaves), dim3(kPromptThreads), 0,
+        hipLaunchKernelGGL((paged_prompt_join_kernel<CT, D>), dim3(slots * a.kvh, kJoinBlocks), dim3(kPromptThreads), 0,
                            st, a, (int64_t)grid);
 }
 
-int unit_slots(const Batch& b, int group) { return (int)((int64_t)b.tokens * group / kBlockColumns) + b.seqs; }
+// at most: a sequence has n group / 128 units, rounded up
+int unit_slots(const Batch& b, int group) { return (int)((int64_t)b.tokens * group / kBlockColumns) + std::min(b.seqs, b.tokens); }
 
 }  // namespace
 
@@ -449,7 +584,7 @@ int unit_slots(const Batch& b, int group) { return (int)((int64_t)b.tokens * gro
 int prompt_splits(const Batch& b, int kvh, int group, int page_size) {
     const int64_t units = std::max<int64_t>((int64_t)b.tokens * group / kBlockColumns, 1) * kvh;
     const int64_t most = ((int64_t)b.width * page_size + 32 * kLeastTiles - 1) / (32 * kLeastTiles);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(512 / units, most));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(256 / units, most));
 }
 
 bool prompt_fits(const Batch& b, int kvh, int group, int page_size) {
