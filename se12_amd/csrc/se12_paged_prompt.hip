@@ -123,27 +123,34 @@ __device__ __forceinline__ void lds_load16(const void* base, uint32_t offset, ui
     asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds) : "memory", "m0");
 }
 
-// A sum where it is kept, in an accumulation register. (Written with the register's
-// class: as ordinary arithmetic it makes the compiler keep all sums in vector registers
-// as well, over the whole walk, and spill.) The compiler's wait states between matrix
-// instructions and others do not see into these, so settle_products() stands on both
-// sides: no matrix instruction is in flight for longer.
+// x by and x + y of a sum. At D = 256 in an accumulation register, where it is kept,
+// written with the register's class: as ordinary arithmetic it makes the compiler keep
+// all sums in vector registers as well, over the whole walk, and spill. The wait states
+// it puts between matrix instructions and others do not cover these, so
+// settle_products() stands on both sides: no matrix instruction is in flight for longer.
+template <int D>
 __device__ __forceinline__ float times(float x, float by) {
+    if constexpr (D < 256) return x * by;
     float t;
     asm volatile("v_accvgpr_read_b32 %1, %0\n\ts_nop 1\n\tv_mul_f32 %1, %1, %2\n\ts_nop 1\n\tv_accvgpr_write_b32 %0, %1"
                  : "+a"(x), "=&v"(t) : "v"(by));
     return x;
 }
+template <int D>
 __device__ __forceinline__ float plus(float x, float y) {
+    if constexpr (D < 256) return x + y;
     float t;
     asm volatile("v_accvgpr_read_b32 %1, %0\n\ts_nop 1\n\tv_add_f32 %1, %1, %2\n\ts_nop 1\n\tv_accvgpr_write_b32 %0, %1"
                  : "+a"(x), "=&v"(t) : "v"(y));
     return x;
 }
-__device__ __forceinline__ void settle_products() { asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15"); }
+template <int D>
+__device__ __forceinline__ void settle_products() {
+    if constexpr (D == 256) asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15");
+}
 
 template <int CT, int D, bool kCapped>
-__global__ __launch_bounds__(kPromptThreads, 1) void paged_prompt_kernel(AttendArgs a) {
+__global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_STEP_E4M3) ? 2 : 1) void paged_prompt_kernel(AttendArgs a) {
     using F = Form<CT>;
     constexpr int kTile = F::kTile, kSubs = kTile / kSubTile;
     constexpr int kKeyPieces = D / F::kPer;           // 16-byte pieces of a key
@@ -265,8 +272,7 @@ __global__ __launch_bounds__(kPromptThreads, 1) void paged_prompt_kernel(AttendA
     // (pieces 2 i + half of the lane's row: the place's bits and those of i meet in an
     // exclusive or, so one address gives all of them)
     const int key_row0 = key_of_row(col), key_off0 = key_row0 * (kKeyPieces * 16) + 16 * (half ^ key_twist(key_row0));
-    auto read_keys = [&](int u) {
-        const int t = u / kSubs, j = u % kSubs;
+    auto read_keys = [&](int t, int j) {
         const int at = key_off0 + ((t - t0) & 1) * 2 * kHalfTile + j * kSubTile * kKeyPieces * 16;
 #pragma unroll
         for (int i = 0; i < kKeyReads; ++i) kf[i] = *reinterpret_cast<const uint4*>(lds + (at ^ (32 * (i & 7))) + 256 * (i >> 3));
@@ -296,10 +302,12 @@ __global__ __launch_bounds__(kPromptThreads, 1) void paged_prompt_kernel(AttendA
         for (int i = 0; i < kRows; ++i) bad |= has_no_number<CT>(vf[i]);
         return __builtin_amdgcn_ballot_w64(bad) != 0;
     };
-    float sc[16], top = 0.0f, vs = 1.0f;    // sc: scores, or r of cap - 2 cap r
+    float sc[16], top = 0.0f;      // scores, or r of cap - 2 cap r
+    float lv = 0.0f, iv = 1.0f;    // the values' scale, in the weights' exponent: log2, and its inverse
     bf16x8_t pf[2];
     auto weights = [&]() {
-        const float base = m == -INFINITY ? 0.0f : m;
+        const float base = (m == -INFINITY ? 0.0f : m) - lv;
+        float sum = 0.0f;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             uint32_t w[4];
@@ -313,39 +321,37 @@ __global__ __launch_bounds__(kPromptThreads, 1) void paged_prompt_kernel(AttendA
                     p0 = __builtin_amdgcn_exp2f(sc[8 * h + 2 * k] - base);
                     p1 = __builtin_amdgcn_exp2f(sc[8 * h + 2 * k + 1] - base);
                 }
-                l += p0 + p1;
-                if constexpr (CT == SE12_STEP_E4M3)
-                    w[k] = f_to_bf16x2(p0 * vs, p1 * vs);
-                else
-                    w[k] = f_to_bf16x2(p0, p1);
+                w[k] = f_to_bf16x2(p0, p1);
+                // (the sum of what the product takes: two at once, times 1)
+                sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w[k]), __builtin_bit_cast(bf16x2_t, 0x3F803F80u), sum, false);
             }
             pf[h] = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
         }
+        l += sum * iv;
     };
 
-    // The walk, sub-tile by sub-tile (u of u0 .. u1 - 1): scores of u + 1 while the
-    // weights of u are worked out, then the product of u's weights and values while the
-    // scores of u + 1 are capped; keys are in registers two sub-tiles ahead of the
+    // The walk, sub-tile by sub-tile: scores of the next while the weights of this one are
+    // worked out, then the product of its weights and values while the scores of the
+    // next are capped; keys are in registers two sub-tiles ahead of the
     // values. At the start of a tile a barrier: its values and the keys kLead tiles on
     // have come (their loads were sent a tile ago), and every wave is done with what
     // the next loads overwrite.
     constexpr int kLead = 2 / kSubs;
-    const int u0 = t0 * kSubs, u1 = t1 * kSubs;
-    auto key_tile = [&](int t, int entry) {
-        if (t < t1) load_keys(t, (t - t0) & 1, entry);
-    };
     // `ke`, `ve`: table entries of the tiles whose keys and values are loaded next; `se`:
-    // of the lane's keys in the next tile, for their scales
+    // of the lane's keys two tiles on, for their scales. Behind the last tile it is loaded
+    // again: nothing reads those places.
+    auto to_last = [&](int t) { return min(t, t1 - 1); };
     int ke = key_entry_of(t0);
-    key_tile(t0, ke);
-    Lane now = lane_of(lane_entries_of(t0)), next = now;
+    load_keys(t0, 0, ke);
+    Lane now = lane_of(lane_entries_of(t0)), next = lane_of(lane_entries_of(to_last(t0 + 1))), after = next;
     if constexpr (kLead == 2) {
-        ke = key_entry_of(min(t0 + 1, t1 - 1));
+        ke = key_entry_of(to_last(t0 + 1));
         asm volatile("" : "+v"(ke));
-        key_tile(t0 + 1, ke);
+        load_keys(to_last(t0 + 1), 1, ke);
     }
     se12::wait_vector_loads();
     arrived(now);
+    arrived(next);
     __syncthreads();
     floatx16_t d;
     auto scores = [&]() {
@@ -369,31 +375,31 @@ __global__ __launch_bounds__(kPromptThreads, 1) void paged_prompt_kernel(AttendA
         for (int e = 1; e < 16; ++e) top = kCapped ? fminf(top, sc[e]) : fmaxf(top, sc[e]);
         if constexpr (kCapped) top = a.cap - 2.0f * a.cap * top;
     };
-    read_keys(u0);
+    read_keys(t0, 0);
     scores();
-    read_keys(min(u0 + 1, u1 - 1));
+    read_keys(t0 + 1 / kSubs, 1 % kSubs);
     cap_scores(now.ks0);
     find_top();
-    ke = key_entry_of(min(t0 + kLead, t1 - 1));
+    ke = key_entry_of(to_last(t0 + kLead));
     int ve = value_entry_of(t0);
     asm volatile("" : "+v"(ke), "+v"(ve));
-    key_tile(t0 + kLead, ke);
+    load_keys(to_last(t0 + kLead), kLead & 1, ke);
     load_values(t0, 0, ve);
-    ke = key_entry_of(min(t0 + kLead + 1, t1 - 1));
-    ve = value_entry_of(min(t0 + 1, t1 - 1));
-    int2 se = lane_entries_of(min(t0 + 1, t1 - 1));
+    ke = key_entry_of(to_last(t0 + kLead + 1));
+    ve = value_entry_of(to_last(t0 + 1));
+    int2 se = lane_entries_of(to_last(t0 + 2));
 
     auto move_maximum = [&]() {
         const float to = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
         const float scale = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
         m = to;
         l *= scale;
-        settle_products();
+        settle_products<D>();
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[i][e] = times(o[i][e], scale);
-        settle_products();
+            for (int e = 0; e < 16; ++e) o[i][e] = times<D>(o[i][e], scale);
+        settle_products<D>();
     };
     // 0 x NaN is NaN: what is no number comes in the columns that give it a weight (and
     // leaves the product)
@@ -407,7 +413,7 @@ __global__ __launch_bounds__(kPromptThreads, 1) void paged_prompt_kernel(AttendA
 #pragma unroll
                 for (int kind = 0; kind < (CT == SE12_STEP_E4M3 ? 1 : 3); ++kind) {
                     __builtin_amdgcn_sched_barrier(0);
-                    settle_products();
+                    settle_products<D>();
                     floatx16_t x;
 #pragma unroll
                     for (int e = 0; e < 16; ++e) x[e] = 0.0f;
@@ -420,82 +426,104 @@ __global__ __launch_bounds__(kPromptThreads, 1) void paged_prompt_kernel(AttendA
                     }
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        o[i][e] = plus(o[i][e], x[e] == 0.0f ? 0.0f : kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY);
+                        o[i][e] = plus<D>(o[i][e], x[e] == 0.0f ? 0.0f : kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY);
                 }
         }
-        settle_products();
+        settle_products<D>();
     };
-    for (int u32 = u0; u32 < u1; ++u32) {
-        bool apart = false;      // a value that is no number may be hidden from some of the columns
-        const int t = u32 / kSubs, j = u32 % kSubs, k0 = u32 * kSubTile, key0 = k0 + 16 * half;
-        if (j == 0) {
-            se12::wait_vector_loads();
-            if (t > t0) now = next;
-            arrived(now);
-            asm volatile("" : "+v"(ke), "+v"(ve), "+v"(se.x), "+v"(se.y));
-            __syncthreads();
-            if (t + 1 < t1) {
-                next = lane_of(se);
-                key_tile(t + kLead + 1, ke);
-                load_values(t + 1, (t + 1 - t0) & 1, ve);
-                ke = key_entry_of(min(t + kLead + 2, t1 - 1));
-                ve = value_entry_of(min(t + 2, t1 - 1));
-                se = lane_entries_of(min(t + 2, t1 - 1));
-            }
+    auto edge = []() { asm volatile(""); };
+    for (int t = t0; t < t1; ++t) {
+        se12::wait_vector_loads();
+        if (t > t0) {
+            now = next;
+            next = after;
         }
-        const bool held = (j ? now.held1 : now.held0) != 0 && key0 < high && key0 + 16 > low;
-        const bool inside = k0 + kSubTile - 1 <= pos_min && k0 + kSubTile <= u.keys && pos_max - k0 < reach &&
-                            __builtin_amdgcn_ballot_w64(!held) == 0;
-        vs = j ? now.vs1 : now.vs0;
-        if (!inside) {
-            vs = held ? vs : 0.0f;
-            const int since = max(pos - reach + 1, 0) - key0, to = held ? min(pos + 1, u.keys) - key0 : 0;
+        arrived(next);
+        asm volatile("" : "+v"(ke), "+v"(ve), "+v"(se.x), "+v"(se.y));
+        __syncthreads();
+        after = lane_of(se);
+        se = lane_entries_of(to_last(t + 3));
 #pragma unroll
-            for (int e = 0; e < 16; ++e) sc[e] = (e < since || e >= to) ? (kCapped ? INFINITY : -INFINITY) : sc[e];
-            find_top();
+        for (int j = 0; j < kSubs; ++j) {
+            const int k0 = (t * kSubs + j) * kSubTile, key0 = k0 + 16 * half;
+            const bool held = ((j ? now.held1 : now.held0) != 0) & (key0 < high) & (key0 + 16 > low);
+            const bool inside = (k0 + kSubTile - 1 <= pos_min) & (k0 + kSubTile <= u.keys) & (pos_max - k0 < reach) &
+                                (__builtin_amdgcn_ballot_w64(!held) == 0);
+            if constexpr (CT == SE12_STEP_E4M3) {
+                const float vs = j ? now.vs1 : now.vs0;
+                lv = __builtin_amdgcn_logf(vs);
+                iv = __builtin_amdgcn_rcpf(vs);
+            }
+            bool apart = false;      // a value that is no number may be hidden from some of the columns
+            // (edge(): what follows is left to the sub-tiles that need it, not worked out for
+            // all and chosen from)
+            if (!inside) {
+                edge();
+                if constexpr (CT == SE12_STEP_E4M3) {
+                    // (what no page holds, or nobody sees, has any scale; its weights are 0)
+                    lv = held ? lv : 0.0f;
+                    iv = held ? iv : 0.0f;
+                }
+                const int since = max(pos - reach + 1, 0) - key0, to = held ? min(pos + 1, u.keys) - key0 : 0;
 #pragma unroll
-            for (int n = 1; n < kValueReads; ++n) {
-                read_values(t, j, n);
-                mask_values(key0, held, n);
+                for (int e = 0; e < 16; ++e) sc[e] = (e < since || e >= to) ? (kCapped ? INFINITY : -INFINITY) : sc[e];
+                find_top();
+#pragma unroll
+                for (int n = 1; n < kValueReads; ++n) {
+                    read_values(t, j, n);
+                    mask_values(key0, held, n);
+                    apart |= any_no_number();
+                }
+            }
+            read_values(t, j, 0);
+            if (!inside) {
+                edge();
+                mask_values(key0, held, 0);
                 apart |= any_no_number();
             }
-        }
-        read_values(t, j, 0);
-        if (!inside) {
-            mask_values(key0, held, 0);
-            apart |= any_no_number();
-        }
-        if (u32 == u0) m = fmaxf(top, __shfl_xor(top, 32, 64));
-        if (__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0) move_maximum();
-        scores();
-        weights();
-        if (apart) {
-            bring_no_numbers(t, j, key0, held);
-            read_values(t, j, 0);
-            mask_values(key0, held, 0);
-            numbers_of_values();
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        read_keys(min(u32 + 2, u1 - 1));
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int n = 0; n < kValueReads; ++n) {
-            if (n > 0) {
-                read_values(t, j, n);
-                if (!inside) {
-                    mask_values(key0, held, n);
-                    if (apart) numbers_of_values();
-                }
+            if (__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0) move_maximum();
+            scores();
+            weights();
+            if (apart) {
+                bring_no_numbers(t, j, key0, held);
+                read_values(t, j, 0);
+                mask_values(key0, held, 0);
+                numbers_of_values();
             }
+            // (the loads of the tiles to come, apart from each other: a wave waits for as
+            // long as its loads are not taken)
+            if (j == 0) {
+                load_keys(to_last(t + kLead + 1), (t + kLead + 1 - t0) & 1, ke);
+                ke = key_entry_of(to_last(t + kLead + 2));
+            }
+            if (j == kSubs - 1) {
+                load_values(to_last(t + 1), (t + 1 - t0) & 1, ve);
+                ve = value_entry_of(to_last(t + 2));
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            read_keys(t + (j + 2) / kSubs, (j + 2) % kSubs);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < kRows; ++i)
+            for (int n = 0; n < kValueReads; ++n) {
+                if (n > 0) {
+                    read_values(t, j, n);
+                    if (!inside) {
+                        edge();
+                        mask_values(key0, held, n);
+                        if (apart) numbers_of_values();
+                    }
+                }
 #pragma unroll
-                for (int h = 0; h < F::kHalves; ++h)
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand<CT>(vf[i], h), pf[n + h], o[i], 0, 0, 0);
+                for (int i = 0; i < kRows; ++i)
+#pragma unroll
+                    for (int h = 0; h < F::kHalves; ++h)
+                        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand<CT>(vf[i], h), pf[n + h], o[i], 0, 0, 0);
+            }
+            cap_scores(j + 1 < kSubs ? now.ks1 : next.ks0);
+            find_top();
         }
-        cap_scores(j + 1 < kSubs ? now.ks1 : next.ks0);
-        find_top();
     }
+    se12::wait_vector_loads();      // (before this block's LDS is another's)
     l += __shfl_xor(l, 32, 64);
     if (!live) return;
     if (whole) {
