@@ -30,6 +30,7 @@ constexpr int kPromptWaves = kPromptThreads / 64;
 constexpr int kWaveColumns = 32;
 constexpr int kBlockColumns = kPromptWaves * kWaveColumns;
 constexpr int kSubTile = 32;              // keys of a first product
+constexpr int kSharedUnits = 1024;        // with more, blocks end close enough to each other as they are
 constexpr int kLeastTiles = 8;            // of a block, where a unit's keys are split
 
 // the key (of 32) of row m of the first product's A operand: lane half h = bit 2 of
@@ -57,31 +58,61 @@ struct UnitCounts {
     }
 };
 
+// (within rows of 16 lanes by DPP, as the float sums of se12_step_math.hpp)
+template <typename Op>
+__device__ __forceinline__ int wave_all(int v, Op op) {
+    v = op(v, __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, true));
+    v = op(v, __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, true));
+    v = op(v, __builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, true));
+    v = op(v, __builtin_amdgcn_mov_dpp(v, 0x140, 0xF, 0xF, true));
+    return op(op(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+              op(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
 __device__ __forceinline__ int wave_total(int v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
-    return __builtin_amdgcn_readfirstlane(v);
+    return wave_all(v, [](int a, int b) { return a + b; });
+}
+__device__ __forceinline__ int wave_most(int v) {
+    return wave_all(v, [](int a, int b) { return a > b ? a : b; });
+}
+
+__device__ __forceinline__ UnitCounts load_counts(const AttendArgs& a, int s0, int lane, int capacity) {
+    UnitCounts c;
+    c.seq = load_seq(a.b, min(s0 + lane, a.b.seqs - 1), capacity);
+    c.keys = min(c.seq.len + c.seq.n, capacity);
+    c.columns = s0 + lane < a.b.seqs ? c.seq.n * a.group : 0;
+    c.units = c.columns > a.few ? (c.columns + kBlockColumns - 1) / kBlockColumns : 0;
+    c.columns = c.units > 0 ? c.columns : 0;
+    return c;
+}
+
+// Keys of a block where units are shared (splits > 1): about as many as make all units'
+// keys one round of blocks, those of a sequence's units taken as a run from the first
+// to the last.
+template <int kTile>
+__device__ __forceinline__ int shared_tiles(const AttendArgs& a, int lane, int resident) {
+    const int capacity = a.b.width << a.page_log2;
+    int64_t all = 0;
+    for (int s0 = 0; s0 < a.b.seqs; s0 += 64) {
+        const UnitCounts c = load_counts(a, s0, lane, capacity);
+        const int last = c.keys, first = min(c.seq.len + kBlockColumns / a.group, last), reach = a.window > 0 ? a.window + kTile : INT32_MAX;
+        // (a float holds it closely enough, and is the same for every block)
+        all += wave_total((int)fminf((float)c.units * (float)(min(first, reach) / 2 + min(last, reach) / 2) / kTile, 1e7f));
+    }
+    return (int)min(all * a.kvh / resident + 1, (int64_t)INT32_MAX);
 }
 
 __device__ __forceinline__ bool find_unit(const AttendArgs& a, int rank, Unit& u) {
     const int lane = threadIdx.x & 63, capacity = a.b.width << a.page_log2;
     for (int s0 = 0; s0 < a.b.seqs; s0 += 64) {
-        UnitCounts c;
-        c.seq = load_seq(a.b, min(s0 + lane, a.b.seqs - 1), capacity);
-        c.keys = min(c.seq.len + c.seq.n, capacity);
-        c.columns = s0 + lane < a.b.seqs ? c.seq.n * a.group : 0;
-        c.units = c.columns > a.few ? (c.columns + kBlockColumns - 1) / kBlockColumns : 0;
-        c.columns = c.units > 0 ? c.columns : 0;
+        const UnitCounts c = load_counts(a, s0, lane, capacity);
         const int all = wave_total(c.units);
         if (rank >= all) {
             rank -= all;
             continue;
         }
-        int most = c.units > 0 ? c.keys : 0;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o, 64));
+        const int most = wave_most(c.units > 0 ? c.keys : 0);
         // the largest x with more than `rank` units past 64 x (every unit is past -1)
-        int lo = -1, hi = (__builtin_amdgcn_readfirstlane(most) + 63) / 64;
+        int lo = -1, hi = (most + 63) / 64;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             if (wave_total(c.past(64 * mid, a.group)) > rank)
@@ -149,6 +180,33 @@ __device__ __forceinline__ void settle_products() {
     if constexpr (D == 256) asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15");
 }
 
+// blocks the card holds at once
+template <int CT, int D>
+constexpr int kResidentBlocks = 256 * (D == 256 || (D == 128 && CT == SE12_STEP_BF16) ? 1 : 2);
+
+// Which units are shared: the first `units` of the order, in parts of about `tiles`
+// tiles. Their parts come first, and then the others, the most keys first.
+struct Sharing {
+    int units, tiles;
+};
+
+template <int CT, int D>
+__device__ __forceinline__ Sharing sharing_of(const AttendArgs& a, int lane) {
+    constexpr int kTile = Form<CT>::kTile;
+    if (a.splits == 1) return {0, INT32_MAX};
+    const int tiles = max(shared_tiles<kTile>(a, lane, kResidentBlocks<CT, D>), kLeastTiles);
+    // (all of them where their order is not that of their keys)
+    if (a.b.seqs > 64 || a.window > 0) return {INT32_MAX / a.splits, tiles};
+    return {wave_total(load_counts(a, 0, lane, a.b.width << a.page_log2).past((int)min((int64_t)tiles * kTile, (int64_t)INT32_MAX), a.group)), tiles};
+}
+
+// tiles of a block of a unit that has `tiles`
+__device__ __forceinline__ int part_tiles(const AttendArgs& a, const Sharing& x, int rank, int tiles) {
+    if (rank >= x.units) return tiles;
+    const int parts = min((tiles + x.tiles - 1) / x.tiles, a.splits);
+    return (tiles + parts - 1) / parts;
+}
+
 template <int CT, int D, bool kCapped>
 __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_STEP_E4M3) ? 2 : 1) void paged_prompt_kernel(AttendArgs a) {
     using F = Form<CT>;
@@ -161,12 +219,20 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
     static_assert(kValuePieces == 4 && kLoads >= 1, "");
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];     // [2][keys, values]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int kh = blockIdx.x % a.kvh, rest = blockIdx.x / a.kvh, split = rest % a.splits, rank = rest / a.splits;
+    const int kh = blockIdx.x % a.kvh;
+    int rank = blockIdx.x / a.kvh, split = 0;
+    const Sharing sharing = sharing_of<CT, D>(a, lane);
+    if (rank < sharing.units * a.splits) {
+        split = rank % a.splits;
+        rank /= a.splits;
+    } else {
+        rank -= sharing.units * (a.splits - 1);
+    }
     Unit u;
     if (!find_unit(a, rank, u)) return;
     int t0, t1;
     unit_tiles<kTile>(a, u, t0, t1);
-    const int length = max((t1 - t0 + a.splits - 1) / a.splits, kLeastTiles);
+    const int length = part_tiles(a, sharing, rank, t1 - t0);
     const bool whole = t1 - t0 <= length;
     t0 += split * length;
     t1 = min(t1, t0 + length);
@@ -184,17 +250,6 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
     // Q: inner positions as the pieces of a key bring them
     constexpr int kQSteps = D / 16;
     bf16x8_t qf[kQSteps];
-    {
-        const uint16_t* qp = a.q + (u.seq.start + token) * a.q_stride + (int64_t)(kh * a.group + c % a.group) * D;
-#pragma unroll
-        for (int i = 0; i < kQSteps; ++i)
-            qf[i] = *reinterpret_cast<const bf16x8_t*>(qp + (i / F::kHalves) * 2 * F::kPer + half * F::kPer + 8 * (i % F::kHalves));
-    }
-    // (in accumulation registers, which the products read as well)
-    if constexpr (D == 256) {
-#pragma unroll
-        for (int i = 0; i < kQSteps; ++i) asm volatile("" : "+a"(qf[i]));
-    }
     floatx16_t o[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
@@ -225,20 +280,32 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
         const int r = i * kRowsPerLoad + lane / kKeyPieces;
         key_at[i] = r * (D * kElem) + 16 * ((lane % kKeyPieces) ^ key_twist(wave * kWaveKeys + r));
     }
-    auto load_keys = [&](int t, int buffer, int key_entry) {
-        const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + buffer * 2 * kHalfTile) + wave * kLoads * 1024;
+    struct Source {
+        const uint8_t* from;
+        uint32_t to;
+    };
+    auto keys_of = [&](int t, int buffer, int key_entry) {
         const int page = in_pool(__builtin_amdgcn_readfirstlane(key_entry)), first = (t * kTile + wave * kWaveKeys) & (P - 1);
-        const uint8_t* from = static_cast<const uint8_t*>(a.kc) + (((int64_t)page * a.kvh + kh) * P + first) * (D * kElem);
+        return Source{static_cast<const uint8_t*>(a.kc) + (((int64_t)page * a.kvh + kh) * P + first) * (D * kElem),
+                      (uint32_t)(__builtin_amdgcn_readfirstlane(lds0 + buffer * 2 * kHalfTile) + wave * kLoads * 1024)};
+    };
+    auto values_of = [&](int t, int buffer, int value_entry) {
+        return Source{static_cast<const uint8_t*>(a.vc) +
+                          (((int64_t)in_pool(value_entry) * a.kvh + kh) * D + wave * kLoads * 16 + (lane >> 2)) * (int64_t)(P * kElem) +
+                          ((t * kTile + vpiece * F::kPer) & (P - 1)) * kElem,
+                      (uint32_t)(__builtin_amdgcn_readfirstlane(lds0 + buffer * 2 * kHalfTile) + kHalfTile + wave * kLoads * 1024)};
+    };
+    auto load_key = [&](const Source& x, int i) { lds_load16(x.from, key_at[i], x.to + i * 1024); };
+    auto load_value = [&](const Source& x, int i) { se12::lds_load16(x.from + i * 16 * P * kElem, x.to + i * 1024); };
+    auto load_keys = [&](int t, int buffer, int key_entry) {
+        const Source x = keys_of(t, buffer, key_entry);
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) lds_load16(from, key_at[i], to + i * 1024);
+        for (int i = 0; i < kLoads; ++i) load_key(x, i);
     };
     auto load_values = [&](int t, int buffer, int value_entry) {
-        const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + buffer * 2 * kHalfTile) + kHalfTile + wave * kLoads * 1024;
-        const uint8_t* from = static_cast<const uint8_t*>(a.vc) +
-                              (((int64_t)in_pool(value_entry) * a.kvh + kh) * D + wave * kLoads * 16 + (lane >> 2)) * (int64_t)(P * kElem) +
-                              ((t * kTile + vpiece * F::kPer) & (P - 1)) * kElem;
+        const Source x = values_of(t, buffer, value_entry);
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) se12::lds_load16(from + i * 16 * P * kElem, to + i * 1024);
+        for (int i = 0; i < kLoads; ++i) load_value(x, i);
     };
     auto key_entry_of = [&](int t) { return entry(t * kTile + wave * kWaveKeys); };
     auto value_entry_of = [&](int t) { return entry(t * kTile + vpiece * F::kPer); };
@@ -348,6 +415,17 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
         ke = key_entry_of(to_last(t0 + 1));
         asm volatile("" : "+v"(ke));
         load_keys(to_last(t0 + 1), 1, ke);
+    }
+    {
+        const uint16_t* qp = a.q + (u.seq.start + token) * a.q_stride + (int64_t)(kh * a.group + c % a.group) * D;
+#pragma unroll
+        for (int i = 0; i < kQSteps; ++i)
+            qf[i] = *reinterpret_cast<const bf16x8_t*>(qp + (i / F::kHalves) * 2 * F::kPer + half * F::kPer + 8 * (i % F::kHalves));
+    }
+    // (in accumulation registers, which the products read as well)
+    if constexpr (D == 256) {
+#pragma unroll
+        for (int i = 0; i < kQSteps; ++i) asm volatile("" : "+a"(qf[i]));
     }
     se12::wait_vector_loads();
     arrived(now);
@@ -490,16 +568,13 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
                 mask_values(key0, held, 0);
                 numbers_of_values();
             }
-            // (the loads of the tiles to come, apart from each other: a wave waits for as
-            // long as its loads are not taken)
-            if (j == 0) {
-                load_keys(to_last(t + kLead + 1), (t + kLead + 1 - t0) & 1, ke);
-                ke = key_entry_of(to_last(t + kLead + 2));
-            }
-            if (j == kSubs - 1) {
-                load_values(to_last(t + 1), (t + 1 - t0) & 1, ve);
-                ve = value_entry_of(to_last(t + 2));
-            }
+            // The loads of the tiles to come, one beside every other row's products: a wave
+            // waits for as long as a load is not taken.
+            static_assert(kRows == 2 * kLoads, "");
+            const Source ks = keys_of(to_last(t + kLead + 1), (t + kLead + 1 - t0) & 1, ke);
+            const Source vs = values_of(to_last(t + 1), (t + 1 - t0) & 1, ve);
+            if (j == 0) ke = key_entry_of(to_last(t + kLead + 2));
+            if (j == kSubs - 1) ve = value_entry_of(to_last(t + 2));
             __builtin_amdgcn_sched_barrier(0);
             read_keys(t + (j + 2) / kSubs, (j + 2) % kSubs);
             __builtin_amdgcn_sched_barrier(0);
@@ -514,10 +589,13 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < kRows; ++i)
+                for (int i = 0; i < kRows; ++i) {
+                    if (n == 0 && j == 0 && i % 2 == 0) load_key(ks, i / 2);
+                    if (n == kValueReads - 1 && j == kSubs - 1 && i % 2 == 0) load_value(vs, i / 2);
 #pragma unroll
                     for (int h = 0; h < F::kHalves; ++h)
                         o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand<CT>(vf[i], h), pf[n + h], o[i], 0, 0, 0);
+                }
             }
             cap_scores(j + 1 < kSubs ? now.ks1 : next.ks0);
             find_top();
@@ -525,68 +603,94 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
     }
     se12::wait_vector_loads();      // (before this block's LDS is another's)
     l += __shfl_xor(l, 32, 64);
-    if (!live) return;
-    if (whole) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        uint16_t* out = a.out + ((int64_t)(u.seq.start + token) * a.heads + kh * a.group + c % a.group) * D + 4 * half;
+    if (!whole) {
+        // the part of (unit, head, split), as the lanes hold it
+        const int64_t p = ((int64_t)rank * a.kvh + kh) * a.splits + split;
+        float4* to = reinterpret_cast<float4*>(a.part + p * kBlockColumns * D) + wave * (D / 8) * 64 + lane;
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                store4(out + 32 * i + 8 * g, o[i][4 * g] * inv, o[i][4 * g + 1] * inv, o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv);
+                to[(4 * i + g) * 64] = make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
+        if (half == 0)
+            reinterpret_cast<float2*>(a.part + (int64_t)gridDim.x * kBlockColumns * D)[p * kBlockColumns + wave * kWaveColumns + col] =
+                make_float2(m, l);
         return;
     }
-    // the part of (unit, head, split)
-    const int64_t p = (((int64_t)rank * a.kvh + kh) * a.splits + split) * kBlockColumns + wave * kWaveColumns + col;
-    float* to = a.part + p * D + 4 * half;
+    // Through LDS to whole rows (a lane holds four values of a row in a row; written from
+    // there, 8 bytes of 64 rows at once, they took 11,000 cycles of a block). The 16-byte
+    // pieces of a row in an order of its own, as those of the keys.
+    __syncthreads();
+    constexpr int kOutPieces = D / 8, kTwist = kOutPieces < 16 ? kOutPieces - 1 : 15, kRowsAtOnce = 64 / kOutPieces;
+    uint8_t* own = lds + wave * kWaveColumns * 2 * D;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<float4*>(to + 32 * i + 8 * g) = make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
-    if (half == 0) {
-        float* ml = a.part + (int64_t)(gridDim.x) * kBlockColumns * D + 2 * p;
-        ml[0] = m;
-        ml[1] = l;
+            store4(reinterpret_cast<uint16_t*>(own + col * 2 * D + 16 * ((4 * i + g) ^ (col & kTwist)) + 8 * half), o[i][4 * g] * inv,
+                   o[i][4 * g + 1] * inv, o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int k = 0; k < kWaveColumns / kRowsAtOnce; ++k) {
+        const int r = k * kRowsAtOnce + lane / kOutPieces, piece = lane % kOutPieces, x = c0 + r;
+        if (r >= mine) continue;
+        const uint4 v = *reinterpret_cast<const uint4*>(own + r * 2 * D + 16 * (piece ^ (r & kTwist)));
+        *reinterpret_cast<uint2*>(a.out + ((int64_t)(u.seq.start + x / a.group) * a.heads + kh * a.group + x % a.group) * D + 8 * piece) =
+            make_uint2(v.x, v.y);
+        *reinterpret_cast<uint2*>(a.out + ((int64_t)(u.seq.start + x / a.group) * a.heads + kh * a.group + x % a.group) * D + 8 * piece + 4) =
+            make_uint2(v.z, v.w);
     }
 }
 
-// Units whose keys were split, from their parts in order: a wave per column, and then
-// the next.
-constexpr int kJoinBlocks = 4;      // of a unit
+// Units whose keys were split, from their parts in order: a wave has the columns of one
+// of the unit's waves, and every kJoinBlocks-th of its lanes' pieces.
+// (Of each unit 2 pieces at D = 256: 16 units of 16 parts, 34 MB, 45 us with 4 blocks a unit.)
+template <int D>
+constexpr int kJoinBlocks = D / 16;
 
 template <int CT, int D>
 __global__ __launch_bounds__(kPromptThreads) void paged_prompt_join_kernel(AttendArgs a, int64_t parts) {
-    constexpr int kTile = Form<CT>::kTile, kPerLane = D / 64;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int kTile = Form<CT>::kTile, kPieces = D / 8 / kJoinBlocks<D>;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31;
     const int kh = blockIdx.x % a.kvh, rank = blockIdx.x / a.kvh;
+    const Sharing sharing = sharing_of<CT, D>(a, lane);
     Unit u;
-    if (!find_unit(a, rank, u)) return;
+    if (rank >= sharing.units || !find_unit(a, rank, u)) return;
     int t0, t1;
     unit_tiles<kTile>(a, u, t0, t1);
-    const int length = max((t1 - t0 + a.splits - 1) / a.splits, kLeastTiles), count = (t1 - t0 + length - 1) / length;
-    if (count <= 1) return;
-    const float* ml = a.part + parts * kBlockColumns * D;
-    for (int c = blockIdx.y * kPromptWaves + wave; c < kBlockColumns && u.first + c < u.columns; c += kJoinBlocks * kPromptWaves) {
-        const int64_t p0 = ((int64_t)rank * a.kvh + kh) * a.splits * kBlockColumns + c;
-        float m = -INFINITY;
-        for (int k = 0; k < count; ++k) m = fmaxf(m, ml[2 * (p0 + (int64_t)k * kBlockColumns)]);
-        const float top = m == -INFINITY ? 0.0f : m;
-        float o[kPerLane] = {}, l = 0.0f;
+    const int length = part_tiles(a, sharing, rank, t1 - t0), count = (t1 - t0 + length - 1) / length;
+    const int c = u.first + wave * kWaveColumns + col;
+    if (count <= 1 || c >= u.columns) return;
+    const int64_t p0 = ((int64_t)rank * a.kvh + kh) * a.splits;
+    const float2* ml = reinterpret_cast<const float2*>(a.part + parts * kBlockColumns * D) + p0 * kBlockColumns + wave * kWaveColumns + col;
+    const float4* from = reinterpret_cast<const float4*>(a.part + p0 * kBlockColumns * D) + wave * (D / 8) * 64 + lane;
+    float m = -INFINITY;
+    for (int k = 0; k < count; ++k) m = fmaxf(m, ml[k * kBlockColumns].x);
+    const float top = m == -INFINITY ? 0.0f : m;
+    float4 o[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float l = 0.0f;
 #pragma unroll 4
-        for (int k = 0; k < count; ++k) {
-            const int64_t p = p0 + (int64_t)k * kBlockColumns;
-            const float by = __builtin_amdgcn_exp2f(ml[2 * p] - top);
-            l += by * ml[2 * p + 1];
+    for (int k = 0; k < count; ++k) {
+        const float2 x = ml[k * kBlockColumns];
+        const float by = __builtin_amdgcn_exp2f(x.x - top);
+        l += by * x.y;
 #pragma unroll
-            for (int e = 0; e < kPerLane; ++e) o[e] += by * a.part[p * D + 64 * e + lane];
+        for (int i = 0; i < kPieces; ++i) {
+            const float4 v = from[(int64_t)k * (kBlockColumns * D / 4) + (i * kJoinBlocks<D> + blockIdx.y) * 64];
+            o[i].x += by * v.x;
+            o[i].y += by * v.y;
+            o[i].z += by * v.z;
+            o[i].w += by * v.w;
         }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const int col = u.first + c;
-        uint16_t* out = a.out + ((int64_t)(u.seq.start + col / a.group) * a.heads + kh * a.group + col % a.group) * D + lane;
-#pragma unroll
-        for (int e = 0; e < kPerLane; ++e) out[64 * e] = f_to_bf16(o[e] * inv);
     }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* out = a.out + ((int64_t)(u.seq.start + c / a.group) * a.heads + kh * a.group + c % a.group) * D + 4 * (lane >> 5);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+        store4(out + 8 * (i * kJoinBlocks<D> + blockIdx.y), o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv);
 }
 
 namespace {
@@ -599,7 +703,7 @@ void launch(const AttendArgs& a, int slots, hipStream_t st) {
     else
         hipLaunchKernelGGL((paged_prompt_kernel<CT, D, false>), dim3(grid), dim3(kPromptThreads), 4 * 64 * D, st, a);
     if (a.splits > 1)
-        hipLaunchKernelGGL((paged_prompt_join_kernel<CT, D>), dim3(slots * a.kvh, kJoinBlocks), dim3(kPromptThreads), 0,
+        hipLaunchKernelGGL((paged_prompt_join_kernel<CT, D>), dim3(slots * a.kvh, kJoinBlocks<D>), dim3(kPromptThreads), 0,
                            st, a, (int64_t)grid);
 }
 
@@ -612,7 +716,8 @@ int unit_slots(const Batch& b, int group) { return (int)((int64_t)b.tokens * gro
 int prompt_splits(const Batch& b, int kvh, int group, int page_size) {
     const int64_t units = std::max<int64_t>((int64_t)b.tokens * group / kBlockColumns, 1) * kvh;
     const int64_t most = ((int64_t)b.width * page_size + 32 * kLeastTiles - 1) / (32 * kLeastTiles);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(256 / units, most));
+    if (units > kSharedUnits) return 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::max<int64_t>(256 / units, 2), most));
 }
 
 bool prompt_fits(const Batch& b, int kvh, int group, int page_size) {
