@@ -32,6 +32,7 @@ constexpr int kChunk = 64 * kLpPer;
 constexpr int kMaxTop = 32;
 constexpr int kKeys = 128;                     // of a wave's buffer: 32 best and a ballot's 64 fit
 constexpr int kBlocksWanted = 1024;            // four to a CU
+constexpr int kJoinKeys = 8;                   // that a thread of the second launch loads at once
 constexpr float kLpSlack = 8.0f;
 
 struct Stats {
@@ -84,14 +85,22 @@ struct Best {
         top = k;
     }
 
-    // The best `top` to the front, in order.
+    // The best `top` to the front, in order: a key's place is the number of keys above it,
+    // compared from registers, each as a scalar in turn. (From LDS, a read at a time,
+    // the 80 keys of a block's waves took 5 us.)
     __device__ __forceinline__ void settle() {
         const int lane = threadIdx.x & 63;
         wave_fence();
         const uint64_t a = lane < n ? buf[lane] : 0, b = lane + 64 < n ? buf[lane + 64] : 0;
         int above_a = 0, above_b = 0;
-        for (int i = 0; i < n; ++i) {
-            const uint64_t k = buf[i];
+        const int first = min(n, 64);
+        for (int i = 0; i < first; ++i) {
+            const uint64_t k = read_lane64(a, i);
+            above_a += k > a;
+            above_b += k > b;
+        }
+        for (int i = 64; i < n; ++i) {
+            const uint64_t k = read_lane64(b, i - 64);
             above_a += k > a;
             above_b += k > b;
         }
@@ -100,8 +109,7 @@ struct Best {
         if (lane + 64 < n && above_b < top) buf[above_b] = b;
         wave_fence();
         n = min(n, top);
-        if (n == top) bar = buf[top - 1];
-        bar = read_lane64(bar, 0);
+        if (n == top) bar = read_lane64(buf[top - 1], 0);
     }
 
     __device__ __forceinline__ void offer(uint64_t key) {
@@ -115,43 +123,48 @@ struct Best {
         n += __builtin_popcountll(in);
     }
 
-    // the bar below which no key of the lanes' best can be among the best: the
-    // top-th of them (keys differ, so one less lets it pass itself)
-    __device__ __forceinline__ void bar_of_lanes(uint64_t best) {
-        int above = 0;
-        for (int i = 0; i < 64; ++i) above += read_lane64(best, i) > best;
-        const uint64_t at = __builtin_amdgcn_ballot_w64(above == top - 1 && best > 0);
-        bar = at ? read_lane64(best, __builtin_ctzll(at)) - 1 : 0;
+    // A bar that at least `top` of the lanes' best reach, in the upper 16 bits of the
+    // logits' order: the largest that so many do, less one in the last place.
+    __device__ __forceinline__ void bar_of_lanes(uint32_t order) {
+        const uint32_t mine = order >> 16;
+        uint32_t at = 0;
+#pragma unroll
+        for (int bit = 15; bit >= 0; --bit) {
+            const uint32_t next = at | (1u << bit);
+            at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(mine >= next)) >= top ? next : at;
+        }
+        bar = at ? ((uint64_t)at << 48) - 1 : 0;
     }
 };
 
-__device__ __forceinline__ Stats join(Stats a, Stats b) {
-    const float m = fmaxf(a.m, b.m);
-    if (m == -INFINITY) return {m, a.s + b.s, a.w + b.w};
+// the sums of a wave's lanes, on the largest of their references
+__device__ __forceinline__ Stats wave_join(Stats v) {
+    const float m = wave_max(v.m);
     // (of m = -inf there is no sum; a NaN stays one)
-    const float da = a.m == -INFINITY ? 0.0f : m - a.m, db = b.m == -INFINITY ? 0.0f : m - b.m;
-    const float fa = __expf(-da), fb = __expf(-db);
-    return {m, a.s * fa + b.s * fb, (a.w + a.s * fminf(da, 1e30f)) * fa + (b.w + b.s * fminf(db, 1e30f)) * fb};
+    const float d = v.m == -INFINITY ? 0.0f : m - v.m, f = __expf(-d);
+    return {m, wave_sum(v.s * f), wave_sum((v.w + v.s * fminf(d, 1e30f)) * f)};
 }
 
-__device__ __forceinline__ Stats shfl_xor(Stats v, int o) { return {__shfl_xor(v.m, o, 64), __shfl_xor(v.s, o, 64), __shfl_xor(v.w, o, 64)}; }
+// the logit of the row's given token (false where there is none): two loads, one
+// after the other, sent before the row's
+template <int DT>
+__device__ __forceinline__ bool token_logit(const LogprobArgs& a, int row, float& x) {
+    const int64_t t = a.tokens[row];
+    const bool valid = t >= 0 && t < a.vocab;
+    const int64_t at = (int64_t)row * a.stride + (valid ? t : 0);
+    x = DT == SE12_STEP_F32 ? static_cast<const float*>(a.logits)[at] : bf16_to_f(static_cast<const uint16_t*>(a.logits)[at]);
+    return valid;
+}
 
 // the row's results, by one wave, from its sums and its best keys in order
-template <int DT>
-__device__ __forceinline__ void finish_row(const LogprobArgs& a, int row, Stats v, const Best& best) {
+__device__ __forceinline__ void finish_row(const LogprobArgs& a, int row, Stats v, const Best& best, bool valid, float x) {
     const int lane = threadIdx.x & 63;
     const float log_s = logf(v.s);
     auto capped = [&](float x) { return a.cap > 0.0f ? a.cap * tanhf(x / a.cap) : x; };
     auto logprob = [&](float x) { return v.m == -INFINITY && v.s == 0.0f ? -INFINITY : (capped(x) - v.m) - log_s; };
     if (lane == 0) {
-        const int64_t t = a.tokens[row];
-        float lp = -INFINITY;
-        if (t >= 0 && t < a.vocab) {
-            const int64_t at = (int64_t)row * a.stride + t;
-            lp = logprob(DT == SE12_STEP_F32 ? static_cast<const float*>(a.logits)[at] : bf16_to_f(static_cast<const uint16_t*>(a.logits)[at]));
-        } else if (v.s != v.s) {
-            lp = v.s;
-        }
+        // (a token that there is not: -inf, in a row of numbers)
+        const float lp = valid ? logprob(x) : v.s != v.s ? v.s : -INFINITY;
         a.logprobs[row] = lp;
         a.entropy[row] = v.m == -INFINITY && v.s == 0.0f ? 0.0f : log_s + v.w / v.s;
     }
@@ -165,8 +178,7 @@ __device__ __forceinline__ void finish_row(const LogprobArgs& a, int row, Stats 
 // the block's waves to wave 0; true there
 __device__ __forceinline__ bool join_waves(Stats& v, Best& best, uint64_t (*lists)[kMaxTop], Stats* sums) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, top = best.top;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v = join(v, shfl_xor(v, o));
+    v = wave_join(v);
     if (top > 0) {
         best.settle();
         if (lane < top) lists[wave][lane] = lane < best.n ? best.buf[lane] : 0;
@@ -174,15 +186,17 @@ __device__ __forceinline__ bool join_waves(Stats& v, Best& best, uint64_t (*list
     if (lane == 0) sums[wave] = v;
     __syncthreads();
     if (wave > 0) return false;
-    v = sums[0];
-    for (int k = 1; k < kLpWaves; ++k) v = join(v, sums[k]);
+    v = lane < kLpWaves ? sums[lane] : Stats{-INFINITY, 0.0f, 0.0f};
+    v = wave_join(v);
     if (top > 0) {
+        // (what the last of a wave's list is above needs no look)
+        static_assert(kLpWaves * kMaxTop <= kKeys, "");
+        uint64_t least = 0;
+#pragma unroll
+        for (int k = 0; k < kLpWaves; ++k) least = max(least, lists[k][top - 1]);
         best.n = 0;
-        best.bar = 0;
-        for (int k = 0; k < kLpWaves * top; k += 64) {
-            const int i = k + lane;
-            best.offer(i < kLpWaves * top ? lists[i / top][i % top] : 0);
-        }
+        best.bar = least ? read_lane64(least, 0) - 1 : 0;
+        for (int i = lane; i - lane < kLpWaves * top; i += 64) best.offer(i < kLpWaves * top ? lists[i / top][i % top] : 0);
         best.settle();
     }
     return true;
@@ -194,6 +208,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs a) {
     __shared__ uint64_t bufs[kLpWaves][kKeys];
     __shared__ uint64_t lists[kLpWaves][kMaxTop];
     __shared__ Stats sums[kLpWaves];
+    __shared__ float held[kLpWaves][kChunk];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
     const char* base = static_cast<const char*>(a.logits) + (int64_t)row * a.stride * kSize;
@@ -203,6 +218,9 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs a) {
     const int first = skew, last = skew + a.vocab;      // values of the pieces that are the row's
     const int per_wave = a.slice / kLpWaves;
     const int begin = slice * a.slice + wave * per_wave, end = min(begin + per_wave, last);
+    float token_x = 0.0f;
+    bool valid = false;
+    if (a.slices == 1) valid = token_logit<DT>(a, row, token_x);
     Best best;
     best.reset(bufs[wave], a.top);
     Stats v{-INFINITY, 0.0f, 0.0f};
@@ -253,23 +271,24 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs a) {
 #pragma unroll
         for (int k = 1; k < kLpPer; ++k) most = fmaxf(most, x[k]);
         if (a.top > 0) {
-            if (at == begin) {
-                uint64_t mine = 0;
-#pragma unroll
-                for (int k = 0; k < kLpPer; ++k) {
-                    const bool valid = index(k) >= first && index(k) < last;
-                    const uint64_t key = valid ? key_of(x[k], index(k) - skew) : 0;
-                    mine = key > mine ? key : mine;
-                }
-                best.bar_of_lanes(mine);
-            }
+            // (-inf may stand for no logit of the row beside one that is a NaN)
+            if (at == begin) best.bar_of_lanes(most > -INFINITY ? order_of(most) : 0);
             // (a bar or a logit that is a NaN goes the long way as well)
             const float bar = number_of((uint32_t)(best.bar >> 32));
             if (at == begin || __builtin_amdgcn_ballot_w64(!(most <= bar)) != 0) {
+                // what passes, a lane's logits one after the other, by way of LDS
+                float* mine = held[wave] + lane;
+                uint32_t hits = 0;
 #pragma unroll
                 for (int k = 0; k < kLpPer; ++k) {
+                    mine[64 * k] = x[k];
                     const bool valid = index(k) >= first && index(k) < last;
-                    best.offer(valid ? key_of(x[k], index(k) - skew) : 0);
+                    hits |= (valid && key_of(x[k], index(k) - skew) > best.bar ? 1u : 0u) << k;
+                }
+                while (__builtin_amdgcn_ballot_w64(hits != 0)) {
+                    const int k = hits ? __builtin_ctz(hits) : 0;
+                    best.offer(hits ? key_of(mine[64 * k], index(k) - skew) : 0);
+                    hits &= hits - 1;
                 }
             }
         }
@@ -306,7 +325,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs a) {
     }
     if (!join_waves(v, best, lists, sums)) return;
     if (a.slices == 1) {
-        finish_row<DT>(a, row, v, best);
+        finish_row(a, row, v, best, valid, token_x);
         return;
     }
     if (lane == 0) a.stats[blockIdx.x] = v;
@@ -319,17 +338,50 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_join_kernel(LogprobArgs a
     __shared__ uint64_t bufs[kLpWaves][kKeys];
     __shared__ uint64_t lists[kLpWaves][kMaxTop];
     __shared__ Stats sums[kLpWaves];
+    __shared__ uint64_t held[kLpWaves][kJoinKeys * 64];
     const int row = blockIdx.x;
+    float token_x;
+    const bool valid = token_logit<DT>(a, row, token_x);
     Best best;
     best.reset(bufs[threadIdx.x >> 6], a.top);
     Stats v{-INFINITY, 0.0f, 0.0f};
-    for (int i = threadIdx.x; i < a.slices; i += kLpThreads) v = join(v, a.stats[(int64_t)row * a.slices + i]);
     const int count = a.slices * a.top;
-    for (int k = 0; k < count; k += kLpThreads) {
-        const int i = k + threadIdx.x;
-        best.offer(i < count ? a.keys[(int64_t)row * count + i] : 0);
+    const uint64_t* keys = a.keys + (int64_t)row * count;
+    uint64_t key[kJoinKeys];
+#pragma unroll
+    for (int k = 0; k < kJoinKeys; ++k) {
+        const int i = k * kLpThreads + threadIdx.x;
+        key[k] = i < count ? keys[i] : 0;
     }
-    if (join_waves(v, best, lists, sums)) finish_row<DT>(a, row, v, best);
+    // (a block's slices, 1,024 at most, on a reference of their own)
+    for (int i = threadIdx.x; i < a.slices; i += kLpThreads) {
+        const Stats x = a.stats[(int64_t)row * a.slices + i];
+        const float to = fmaxf(v.m, x.m);
+        const float d0 = v.m == -INFINITY ? 0.0f : to - v.m, d1 = x.m == -INFINITY ? 0.0f : to - x.m;
+        const float f0 = __expf(-d0), f1 = __expf(-d1);
+        v = {to, v.s * f0 + x.s * f1, (v.w + v.s * fminf(d0, 1e30f)) * f0 + (x.w + x.s * fminf(d1, 1e30f)) * f1};
+    }
+    if (a.top > 0) {
+        uint32_t mine = 0, hits = 0;
+#pragma unroll
+        for (int k = 0; k < kJoinKeys; ++k) mine = max(mine, (uint32_t)(key[k] >> 32));
+        best.bar_of_lanes(mine);
+        uint64_t* mine64 = held[threadIdx.x >> 6] + (threadIdx.x & 63);
+#pragma unroll
+        for (int k = 0; k < kJoinKeys; ++k) {
+            mine64[64 * k] = key[k];
+            hits |= (key[k] > best.bar ? 1u : 0u) << k;
+        }
+        while (__builtin_amdgcn_ballot_w64(hits != 0)) {
+            best.offer(hits ? mine64[64 * __builtin_ctz(hits)] : 0);
+            hits &= hits - 1;
+        }
+        for (int k = kJoinKeys * kLpThreads; k < count; k += kLpThreads) {
+            const int i = k + threadIdx.x;
+            best.offer(i < count ? keys[i] : 0);
+        }
+    }
+    if (join_waves(v, best, lists, sums)) finish_row(a, row, v, best, valid, token_x);
 }
 
 }  // namespace se12step
