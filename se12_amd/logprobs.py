@@ -6,18 +6,17 @@ runtime leaves sampling to the framework."""
 
 from __future__ import annotations
 
-import dataclasses
+from typing import NamedTuple
 
 import torch
 
 from . import _native as nat
-from .paged import _on
+from .paged import _on, _stream
 
 MAX_TOP = 32
 
 
-@dataclasses.dataclass(frozen=True)
-class TokenLogprobs:
+class TokenLogprobs(NamedTuple):
     logprobs: torch.Tensor      # FP32 [rows]
     entropy: torch.Tensor       # FP32 [rows], in nats
     top_logprobs: torch.Tensor  # FP32 [rows, top], from the most likely
@@ -50,9 +49,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, sof
     if (logits.stride(1) != 1 and vocab > 1) or (logits.stride(0) < vocab and rows > 1):
         logits = logits.contiguous()
     tokens = tokens.contiguous()
+    stride = max(logits.stride(0), vocab)
     with _on(dev):
-        out = torch.empty((2 + top, rows), dtype=torch.float32, device=dev)
-        top_logprobs = out[2:].view(rows, top)
+        logprobs, entropy = torch.empty((2, rows), dtype=torch.float32, device=dev).unbind()
+        top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=dev)
         top_ids = torch.empty((rows, top), dtype=torch.int64, device=dev)
         if rows:
             lib = nat.lib()
@@ -61,7 +61,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, sof
                 nat.step_check(n)
             ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
             nat.step_check(lib.se12_step_logprobs(
-                nat.ptr(logits), nat.STEP_F32 if logits.dtype == torch.float32 else nat.STEP_BF16, max(logits.stride(0), vocab),
-                rows, vocab, float(softcap), nat.ptr(tokens), top, nat.ptr(out[0]), nat.ptr(out[1]), nat.ptr(top_logprobs),
-                nat.ptr(top_ids), nat.ptr(ws), n, nat.stream_ptr()))
-    return TokenLogprobs(out[0], out[1], top_logprobs, top_ids)
+                logits.data_ptr(), nat.STEP_F32 if logits.dtype == torch.float32 else nat.STEP_BF16, stride, rows, vocab, float(softcap),
+                tokens.data_ptr(), int(top), logprobs.data_ptr(), entropy.data_ptr(), top_logprobs.data_ptr(), top_ids.data_ptr(),
+                ws.data_ptr() if n else None, n, _stream(dev)))
+    return TokenLogprobs(logprobs, entropy, top_logprobs, top_ids)

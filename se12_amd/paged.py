@@ -36,6 +36,11 @@ def _on(device: torch.device):
     return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
+def _stream(device: torch.device) -> int:
+    """The handle of the device's current stream."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def _int32(t: torch.Tensor, name: str, shape: tuple, device: torch.device) -> torch.Tensor:
     if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device:
         raise ValueError(f"{name} must be an int32 tensor on {device}")
@@ -77,9 +82,14 @@ class PagedBatch:
             raise ValueError("lengths and starts must be contiguous")
         self.sequences, self.max_new = n, int(max_new)
         self._fields = (page_table.data_ptr(), max(page_table.stride(0), width), lengths.data_ptr(), starts.data_ptr(), width, n)
+        self._last = (-1, None)
 
-    def _struct(self, tokens: int) -> nat.StepBatch:
-        return nat.StepBatch(*self._fields, tokens, self.max_new)
+    def _struct(self, tokens: int):
+        """The C struct of a call with so many rows, by reference; the layers of a step share it."""
+        last = self._last
+        if last[0] != tokens:
+            last = self._last = (tokens, ctypes.byref(nat.StepBatch(*self._fields, tokens, self.max_new)))
+        return last[1]
 
 
 class PagedKvCache:
@@ -127,26 +137,27 @@ class PagedKvCache:
         if any(not t.is_cuda or t.device != k.device for t in tensors):
             raise ValueError("a cache's tensors must be on one HIP device")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.device, self.dtype = k.device, k.dtype
+        self.device, self.dtype, self._index = k.device, k.dtype, k.get_device()
         self.pages, self.kv_heads, self.page_size, self.head_dim = pages, kv_heads, page_size, head_dim
-        self._struct = nat.StepPages(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if e4m3 else None,
+        self._struct = ctypes.byref(nat.StepPages(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if e4m3 else None,
                                      v_scale.data_ptr() if e4m3 else None, nat.STEP_E4M3 if e4m3 else nat.STEP_BF16, pages,
-                                     page_size, kv_heads, head_dim)
+                                     page_size, kv_heads, head_dim))
 
     def _rows(self, t: torch.Tensor, name: str, heads: int | None, tokens: int | None, dtype: torch.dtype | None,
               multiple: int) -> torch.Tensor:
         """t [tokens, heads, head_dim] with heads side by side and rows `multiple` elements apart: itself, or a copy."""
-        if not isinstance(t, torch.Tensor) or t.dim() != 3 or t.shape[2] != self.head_dim or (heads is not None and t.shape[1] != heads):
+        shape = t.shape if isinstance(t, torch.Tensor) else ()
+        if len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
             raise ValueError(f"{name} must be [tokens, {'heads' if heads is None else heads}, {self.head_dim}]")
-        if tokens is not None and t.shape[0] != tokens:
-            raise ValueError(f"{name} has {t.shape[0]} rows, k has {tokens}")
-        if t.device != self.device:
+        if tokens is not None and shape[0] != tokens:
+            raise ValueError(f"{name} has {shape[0]} rows, k has {tokens}")
+        if t.get_device() != self._index:
             raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
         if dtype is not None and t.dtype != dtype:
             raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
         row, head, one = t.stride()
-        if (one != 1 or (head != self.head_dim and t.shape[1] > 1) or row % multiple or t.data_ptr() % (multiple * t.element_size())
-                or row < t.shape[1] * self.head_dim):
+        if (one != 1 or (head != self.head_dim and shape[1] > 1) or row % multiple or row < shape[1] * self.head_dim
+                or t.data_ptr() % (multiple * t.element_size())):
             t = t.contiguous()
             if t.data_ptr() % (multiple * t.element_size()):
                 t = t.clone()
@@ -195,9 +206,10 @@ class PagedKvCache:
             raise ValueError("out goes with q")
         with _on(self.device):
             nat.step_check(nat.lib().se12_step_paged_append(
-                ctypes.byref(self._struct), ctypes.byref(batch._struct(tokens)), nat.ptr(q), nat.ptr(k), nat.ptr(v),
+                self._struct, batch._struct(tokens), None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(),
                 nat.STEP_F32 if k.dtype == torch.float32 else nat.STEP_BF16, q_stride, k.stride(0), v.stride(0), heads,
-                nat.ptr(inv_freq), rotary, nat.ptr(out), nat.stream_ptr()))
+                None if inv_freq is None else inv_freq.data_ptr(), rotary, None if q is None else out.data_ptr(),
+                _stream(self.device)))
         return out
 
     def attend(self, batch: PagedBatch, q: torch.Tensor, scaling: float, softcap: float = 0.0, window: int = 0,
@@ -220,7 +232,7 @@ class PagedKvCache:
         if tokens == 0:
             return out
         lib = nat.lib()
-        pages, new = ctypes.byref(self._struct), ctypes.byref(batch._struct(tokens))
+        pages, new = self._struct, batch._struct(tokens)
         with _on(self.device):
             if workspace is None:
                 n = lib.se12_step_paged_attention_workspace(pages, new, heads)
@@ -230,14 +242,14 @@ class PagedKvCache:
             elif workspace.dtype != torch.uint8 or workspace.device != self.device or not workspace.is_contiguous():
                 raise ValueError(f"workspace must be a contiguous uint8 tensor on {self.device}")
             nat.step_check(lib.se12_step_paged_attention(
-                pages, new, nat.ptr(q), q.stride(0), nat.ptr(out), heads, float(scaling), float(softcap), int(window),
-                nat.ptr(workspace), workspace.numel(), nat.stream_ptr()))
+                pages, new, q.data_ptr(), q.stride(0), out.data_ptr(), heads, float(scaling), float(softcap), int(window),
+                workspace.data_ptr(), workspace.numel(), _stream(self.device)))
         return out
 
     def attend_workspace(self, batch: PagedBatch, tokens: int, heads: int) -> int:
         """Bytes of `attend`'s workspace."""
         self._check(batch)
-        n = nat.lib().se12_step_paged_attention_workspace(ctypes.byref(self._struct), ctypes.byref(batch._struct(tokens)), heads)
+        n = nat.lib().se12_step_paged_attention_workspace(self._struct, batch._struct(tokens), heads)
         if n < 0:
             nat.step_check(n)
         return int(n)
