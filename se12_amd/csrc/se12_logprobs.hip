@@ -19,6 +19,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "se12_step.h"
 #include "se12_step_math.hpp"
@@ -34,6 +35,7 @@ constexpr int kKeys = 128;                     // of a wave's buffer: 32 best an
 constexpr int kBlocksWanted = 1024;            // four to a CU
 constexpr int kJoinKeys = 8;                   // that a thread of the second launch loads at once
 constexpr float kLpSlack = 8.0f;
+constexpr float kLog2E = 1.4426950408889634f;
 
 struct Stats {
     float m, s, w;
@@ -209,7 +211,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs a) {
     __shared__ uint64_t lists[kLpWaves][kMaxTop];
     __shared__ Stats sums[kLpWaves];
     __shared__ float held[kLpWaves][kChunk];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
     const char* base = static_cast<const char*>(a.logits) + (int64_t)row * a.stride * kSize;
     // whole 16-byte pieces of the row: logit i is value i + skew of them
@@ -223,10 +225,17 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs a) {
     if (a.slices == 1) valid = token_logit<DT>(a, row, token_x);
     Best best;
     best.reset(bufs[wave], a.top);
-    Stats v{-INFINITY, 0.0f, 0.0f};
+    float bar = -INFINITY;                              // no logit up to it counts
+    float m = -INFINITY, sum = 0.0f, mean = 0.0f;       // the reference, S, and W in units of log 2
     uint4 next[kVecs];
-    // a piece that is not wholly the row's is read value by value
     auto load = [&](int at) {
+        if (at >= first && at + kChunk <= last) {
+            const uint4* p = reinterpret_cast<const uint4*>(pieces + (int64_t)at * kSize) + lane;
+#pragma unroll
+            for (int j = 0; j < kVecs; ++j) next[j] = p[j * 64];
+            return;
+        }
+        // a piece that is not wholly the row's is read value by value
 #pragma unroll
         for (int j = 0; j < kVecs; ++j) {
             const int i = at + (j * 64 + lane) * kVec;
@@ -263,9 +272,10 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs a) {
         const bool edge = at < first || at + kChunk > last;
         if (at + kChunk < end) load(at + kChunk);
         auto index = [&](int k) { return at + (k / kVec * 64 + lane) * kVec + k % kVec; };
+        auto outside = [&](int k) { return index(k) < first || index(k) >= last; };
         if (edge) {
 #pragma unroll
-            for (int k = 0; k < kLpPer; ++k) x[k] = index(k) < first || index(k) >= last ? -INFINITY : x[k];
+            for (int k = 0; k < kLpPer; ++k) x[k] = outside(k) ? -INFINITY : x[k];
         }
         float most = x[0];
 #pragma unroll
@@ -274,7 +284,6 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs a) {
             // (-inf may stand for no logit of the row beside one that is a NaN)
             if (at == begin) best.bar_of_lanes(most > -INFINITY ? order_of(most) : 0);
             // (a bar or a logit that is a NaN goes the long way as well)
-            const float bar = number_of((uint32_t)(best.bar >> 32));
             if (at == begin || __builtin_amdgcn_ballot_w64(!(most <= bar)) != 0) {
                 // what passes, a lane's logits one after the other, by way of LDS
                 float* mine = held[wave] + lane;
@@ -282,47 +291,56 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs a) {
 #pragma unroll
                 for (int k = 0; k < kLpPer; ++k) {
                     mine[64 * k] = x[k];
-                    const bool valid = index(k) >= first && index(k) < last;
-                    hits |= (valid && key_of(x[k], index(k) - skew) > best.bar ? 1u : 0u) << k;
+                    hits |= (!outside(k) && key_of(x[k], index(k) - skew) > best.bar ? 1u : 0u) << k;
                 }
                 while (__builtin_amdgcn_ballot_w64(hits != 0)) {
                     const int k = hits ? __builtin_ctz(hits) : 0;
                     best.offer(hits ? key_of(mine[64 * k], index(k) - skew) : 0);
                     hits &= hits - 1;
                 }
+                bar = number_of((uint32_t)(best.bar >> 32));
             }
         }
-        if (a.cap > 0.0f) {
-            // cap tanh(x / cap) = cap - 2 cap / (1 + e^(2 x / cap))
-#pragma unroll
-            for (int k = 0; k < kLpPer; ++k)
-                x[k] = a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[k] * a.inv_cap2));
-            most = a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(most * a.inv_cap2));
-            if (edge) {
-#pragma unroll
-                for (int k = 0; k < kLpPer; ++k) x[k] = index(k) < first || index(k) >= last ? -INFINITY : x[k];
-            }
+        if (a.cap > 0.0f) most = a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(most * a.inv_cap2));
+        if (__builtin_amdgcn_ballot_w64(most > m + kLpSlack) != 0) {
+            const float to = fmaxf(m, wave_max(most));
+            const float d = m == -INFINITY ? 0.0f : (to - m) * kLog2E, f = __builtin_amdgcn_exp2f(-d);
+            mean = (mean + sum * fminf(d, 1e30f)) * f;
+            sum *= f;
+            m = to;
         }
-        if (__builtin_amdgcn_ballot_w64(most > v.m + kLpSlack) != 0) {
-            const float to = fmaxf(v.m, wave_max(most));
-            const float d = v.m == -INFINITY ? 0.0f : to - v.m, f = __expf(-d);
-            v.w = (v.w + v.s * fminf(d, 1e30f)) * f;
-            v.s *= f;
-            v.m = to;
-        }
-        if (v.m != -INFINITY) {
-#pragma unroll
-            for (int k = 0; k < kLpPer; ++k) {
-                const float d = v.m - x[k], e = __expf(-d);
-                v.s += e;
-                v.w += e * fminf(d, 1e30f);
-            }
-        } else {
+        if (m == -INFINITY) {
             // nothing but -inf so far, unless there is a NaN
 #pragma unroll
-            for (int k = 0; k < kLpPer; ++k) v.s = x[k] != x[k] ? x[k] : v.s;
+            for (int k = 0; k < kLpPer; ++k) sum = x[k] != x[k] ? x[k] : sum;
+        } else if (a.cap > 0.0f) {
+            // m - cap tanh(x / cap) = m - cap + 2 cap / (1 + e^(2 x / cap)): three instructions of
+            // a quarter of the rate and six others to a logit
+            const float scale = 2.0f * a.cap * kLog2E, from = (m - a.cap) * kLog2E;
+            auto add = [&](auto at_edge) {
+#pragma unroll
+                for (int k = 0; k < kLpPer; ++k) {
+                    float d = fmaf(scale, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[k] * a.inv_cap2)), from);
+                    if (at_edge.value && outside(k)) d = 1e30f;
+                    const float e = __builtin_amdgcn_exp2f(-d);
+                    sum += e;
+                    mean = fmaf(e, d, mean);
+                }
+            };
+            if (edge)
+                add(std::true_type{});
+            else
+                add(std::false_type{});
+        } else {
+#pragma unroll
+            for (int k = 0; k < kLpPer; ++k) {
+                const float d = (m - x[k]) * kLog2E, e = __builtin_amdgcn_exp2f(-d);
+                sum += e;
+                mean = fmaf(e, fminf(d, 1e30f), mean);
+            }
         }
     }
+    Stats v{m, sum, mean * (1.0f / kLog2E)};
     if (!join_waves(v, best, lists, sums)) return;
     if (a.slices == 1) {
         finish_row(a, row, v, best, valid, token_x);
@@ -443,7 +461,6 @@ int se12_step_logprobs(const void* logits, int32_t dtype, int64_t stride, int32_
     if ((int64_t)rows * l.slices > INT32_MAX) return step_fail(fn, "too many rows");
     if (l.total > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < l.total))
         return step_fail(fn, "workspace missing, misaligned or too small");
-    constexpr float kLog2E = 1.4426950408889634f;
     const LogprobArgs a{logits, stride, vocab, top, l.slices, l.slice, softcap, softcap > 0.0f ? 2.0f * kLog2E / softcap : 0.0f,
                         tokens, logprobs, entropy, top_logprobs, top_ids, static_cast<Stats*>(workspace),
                         reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + (l.slices > 1 ? l.stats_bytes : 0))};
