@@ -88,23 +88,25 @@ struct Best {
     }
 
     // The best `top` to the front, in order: a key's place is the number of keys above it,
-    // compared from registers, each as a scalar in turn. (From LDS, a read at a time,
-    // the 80 keys of a block's waves took 5 us.)
+    // read from LDS, up to eight at a time, by all lanes alike. (A key a time, from registers by
+    // readlane, the keys of a block's four waves took 14,000 cycles.)
+    template <int kAtOnce>
     __device__ __forceinline__ void settle() {
         const int lane = threadIdx.x & 63;
+        if (lane < 8) buf[n + lane] = 0;
         wave_fence();
         const uint64_t a = lane < n ? buf[lane] : 0, b = lane + 64 < n ? buf[lane + 64] : 0;
         int above_a = 0, above_b = 0;
-        const int first = min(n, 64);
-        for (int i = 0; i < first; ++i) {
-            const uint64_t k = read_lane64(a, i);
-            above_a += k > a;
-            above_b += k > b;
-        }
-        for (int i = 64; i < n; ++i) {
-            const uint64_t k = read_lane64(b, i - 64);
-            above_a += k > a;
-            above_b += k > b;
+        for (int i = 0; i < n; i += kAtOnce) {
+            uint64_t k[kAtOnce];
+#pragma unroll
+            for (int e = 0; e < kAtOnce; ++e) k[e] = buf[i + e];
+#pragma unroll
+            for (int e = 0; e < kAtOnce; ++e) above_a += k[e] > a;
+            if (n > 64) {
+#pragma unroll
+                for (int e = 0; e < kAtOnce; ++e) above_b += k[e] > b;
+            }
         }
         wave_fence();
         if (lane < n && above_a < top) buf[above_a] = a;
@@ -118,11 +120,18 @@ struct Best {
         uint64_t in = __builtin_amdgcn_ballot_w64(key > bar);
         if (!in) return;
         if (n + __builtin_popcountll(in) > kKeys) {
-            settle();
+            settle<2>();
             in = __builtin_amdgcn_ballot_w64(key > bar);
         }
         if (key > bar) buf[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0))] = key;
         n += __builtin_popcountll(in);
+    }
+
+    // Logits up to it are below the bar. (Zero is above a bar just below it; as numbers,
+    // -0 and 0 are equal.)
+    __device__ __forceinline__ float bar_number() const {
+        const uint32_t order = (uint32_t)(bar >> 32);
+        return order == 0x7FFFFFFFu ? -1.17549435e-38f : number_of(order);
     }
 
     // A bar that at least `top` of the lanes' best reach, in the upper 16 bits of the
@@ -177,39 +186,52 @@ __device__ __forceinline__ void finish_row(const LogprobArgs& a, int row, Stats 
     }
 }
 
-// the block's waves to wave 0; true there
-__device__ __forceinline__ bool join_waves(Stats& v, Best& best, uint64_t (*lists)[kMaxTop], Stats* sums) {
+// What the waves of a block hand to the first of them.
+struct Waves {
+    uint64_t keys[kLpWaves][kKeys + 8];
+    uint64_t bar[kLpWaves];
+    int n[kLpWaves];
+    Stats sums[kLpWaves];
+};
+
+// the block's waves to wave 0; true there, with the best keys in order
+__device__ __forceinline__ bool join_waves(Stats& v, Best& best, Waves& of) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, top = best.top;
     v = wave_join(v);
-    if (top > 0) {
-        best.settle();
-        if (lane < top) lists[wave][lane] = lane < best.n ? best.buf[lane] : 0;
+    if (best.n > 64) best.settle<2>();
+    if (lane == 0) {
+        of.sums[wave] = v;
+        of.n[wave] = best.n;
+        of.bar[wave] = best.bar;
     }
-    if (lane == 0) sums[wave] = v;
     __syncthreads();
     if (wave > 0) return false;
-    v = lane < kLpWaves ? sums[lane] : Stats{-INFINITY, 0.0f, 0.0f};
+    v = lane < kLpWaves ? of.sums[lane] : Stats{-INFINITY, 0.0f, 0.0f};
     v = wave_join(v);
     if (top > 0) {
-        // (what the last of a wave's list is above needs no look)
-        static_assert(kLpWaves * kMaxTop <= kKeys, "");
-        uint64_t least = 0;
+        // as in a chunk: a bar from the lanes' best, and what passes all bars
+        uint64_t key[kLpWaves], most = 0, least = 0;
 #pragma unroll
-        for (int k = 0; k < kLpWaves; ++k) least = max(least, lists[k][top - 1]);
+        for (int k = 0; k < kLpWaves; ++k) {
+            key[k] = lane < of.n[k] ? of.keys[k][lane] : 0;
+            most = max(most, key[k]);
+            least = max(least, of.bar[k]);
+        }
+        wave_fence();
         best.n = 0;
-        best.bar = least ? read_lane64(least, 0) - 1 : 0;
-        for (int i = lane; i - lane < kLpWaves * top; i += 64) best.offer(i < kLpWaves * top ? lists[i / top][i % top] : 0);
-        best.settle();
+        best.bar_of_lanes((uint32_t)(most >> 32));
+        best.bar = max(best.bar, (least ? read_lane64(least, 0) : 1) - 1);
+#pragma unroll
+        for (int k = 0; k < kLpWaves; ++k) best.offer(key[k]);
+        best.settle<8>();
     }
     return true;
 }
 
 template <int DT>
-__global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs a) {
+__global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(LogprobArgs a) {
     constexpr int kVec = DT == SE12_STEP_F32 ? 4 : 8, kVecs = kLpPer / kVec, kSize = 16 / kVec;
-    __shared__ uint64_t bufs[kLpWaves][kKeys];
-    __shared__ uint64_t lists[kLpWaves][kMaxTop];
-    __shared__ Stats sums[kLpWaves];
+    __shared__ Waves waves;
     __shared__ float held[kLpWaves][kChunk];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
@@ -224,7 +246,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs a) {
     bool valid = false;
     if (a.slices == 1) valid = token_logit<DT>(a, row, token_x);
     Best best;
-    best.reset(bufs[wave], a.top);
+    best.reset(waves.keys[wave], a.top);
     float bar = -INFINITY;                              // no logit up to it counts
     float m = -INFINITY, sum = 0.0f, mean = 0.0f;       // the reference, S, and W in units of log 2
     uint4 next[kVecs];
@@ -282,7 +304,10 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs a) {
         for (int k = 1; k < kLpPer; ++k) most = fmaxf(most, x[k]);
         if (a.top > 0) {
             // (-inf may stand for no logit of the row beside one that is a NaN)
-            if (at == begin) best.bar_of_lanes(most > -INFINITY ? order_of(most) : 0);
+            if (at == begin) {
+                best.bar_of_lanes(most > -INFINITY ? order_of(most) : 0);
+                bar = best.bar_number();
+            }
             // (a bar or a logit that is a NaN goes the long way as well)
             if (at == begin || __builtin_amdgcn_ballot_w64(!(most <= bar)) != 0) {
                 // what passes, a lane's logits one after the other, by way of LDS
@@ -291,14 +316,14 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs a) {
 #pragma unroll
                 for (int k = 0; k < kLpPer; ++k) {
                     mine[64 * k] = x[k];
-                    hits |= (!outside(k) && key_of(x[k], index(k) - skew) > best.bar ? 1u : 0u) << k;
+                    hits |= (x[k] <= bar ? 0u : 1u) << k;
                 }
                 while (__builtin_amdgcn_ballot_w64(hits != 0)) {
                     const int k = hits ? __builtin_ctz(hits) : 0;
-                    best.offer(hits ? key_of(mine[64 * k], index(k) - skew) : 0);
+                    best.offer(hits && !outside(k) ? key_of(mine[64 * k], index(k) - skew) : 0);
                     hits &= hits - 1;
                 }
-                bar = number_of((uint32_t)(best.bar >> 32));
+                bar = best.bar_number();
             }
         }
         if (a.cap > 0.0f) most = a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(most * a.inv_cap2));
@@ -341,7 +366,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs a) {
         }
     }
     Stats v{m, sum, mean * (1.0f / kLog2E)};
-    if (!join_waves(v, best, lists, sums)) return;
+    if (!join_waves(v, best, waves)) return;
     if (a.slices == 1) {
         finish_row(a, row, v, best, valid, token_x);
         return;
@@ -353,15 +378,13 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs a) {
 // the slices of a row
 template <int DT>
 __global__ __launch_bounds__(kLpThreads) void logprobs_join_kernel(LogprobArgs a) {
-    __shared__ uint64_t bufs[kLpWaves][kKeys];
-    __shared__ uint64_t lists[kLpWaves][kMaxTop];
-    __shared__ Stats sums[kLpWaves];
+    __shared__ Waves waves;
     __shared__ uint64_t held[kLpWaves][kJoinKeys * 64];
     const int row = blockIdx.x;
     float token_x;
     const bool valid = token_logit<DT>(a, row, token_x);
     Best best;
-    best.reset(bufs[threadIdx.x >> 6], a.top);
+    best.reset(waves.keys[threadIdx.x >> 6], a.top);
     Stats v{-INFINITY, 0.0f, 0.0f};
     const int count = a.slices * a.top;
     const uint64_t* keys = a.keys + (int64_t)row * count;
@@ -399,7 +422,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_join_kernel(LogprobArgs a
             best.offer(i < count ? keys[i] : 0);
         }
     }
-    if (join_waves(v, best, lists, sums)) finish_row(a, row, v, best, valid, token_x);
+    if (join_waves(v, best, waves)) finish_row(a, row, v, best, valid, token_x);
 }
 
 }  // namespace se12step

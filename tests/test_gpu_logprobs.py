@@ -104,6 +104,19 @@ def test_masked_logits(gpu):
     _check(low, torch.tensor([7], device=gpu), 4, 0.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_best_are_zeros(gpu, dtype):
+    """0 and -0 tie; they are above every number below, the smallest ones too."""
+    x, t = _logits(gpu, 3, 20_000, dtype, 6)
+    x = -x.relu()
+    x[1] = torch.where(x[1] == 0, -1e-38, x[1])
+    x[1, ::37] = torch.where(x[1, ::37] > -1, 0.0, x[1, ::37])
+    x[2, :9_000] = -1.0
+    x[2, 9_003] = -0.0
+    x[2, 15_000] = 0.0
+    _check(x, t, 7, 0.0)
+
+
 def test_rows_without_a_distribution(gpu):
     from se12_amd.logprobs import token_logprobs
 
