@@ -10,8 +10,11 @@
 // its bytes have one writer and no order to depend on; further blocks rotate q,
 // a wave per token. Angles: position * inv_freq / 2 pi in 64 bits (positions
 // beyond 2^17 would lose a radian's third digit in FP32), its fraction of a turn
-// in FP32. Bound by the bytes of q, k and v at prompt sizes, by the launch at
-// decode sizes.
+// in FP32, sine and cosine by the instructions that take turns: within 1.3e-7 at
+// every multiple of 2^-24, as near as FP32 routines in the rounding that follows.
+// Bound by the bytes of q, k and v at prompt sizes: 9,001 BF16 tokens of 16 and 8
+// heads of 256 (258 MB) take 62 us, 4.2 TB/s (72 with a routine of 40 instructions
+// for each sine and cosine); at decode sizes by the launch: 48 tokens, 7 us.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -73,7 +76,9 @@ __device__ __forceinline__ Turn turn_of(const float* inv_freq, int lo, int pos) 
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const double turns = (double)pos * (double)w[i] * 0.15915494309189535;
-        sincospif(2.0f * (float)(turns - rint(turns)), &t.s[i], &t.c[i]);
+        const float f = (float)(turns - rint(turns));
+        t.s[i] = __builtin_amdgcn_sinf(f);
+        t.c[i] = __builtin_amdgcn_cosf(f);
     }
     return t;
 }
