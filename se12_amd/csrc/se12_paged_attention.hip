@@ -221,7 +221,7 @@ struct Attend {
                 const bool inside = k0 + kTile - 1 <= pos_min && k0 + kTile <= w.keys && pos_max - k0 < reach &&
                                     __builtin_amdgcn_ballot_w64(!held) == 0;
                 if (!inside) {
-                    vs = held ? vs : 0.0f;
+                    if constexpr (CT == SE12_STEP_E4M3) vs = held ? vs : 0.0f;   // (of this tile's page)
                     const int from = max(pos - reach + 1, 0) - key0, to = held ? min(pos + 1, w.keys) - key0 : 0;
 #pragma unroll
                     for (int e = 0; e < kPer; ++e) sc[e] = (e < from || e >= to) ? -INFINITY : sc[e];

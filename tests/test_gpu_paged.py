@@ -294,6 +294,43 @@ def test_attend_many_sequences(gpu):
     _attend_case(gpu, E4M3, 64, 16, 2, 1, lengths, [1 if i % 7 else 0 for i in range(150)], 0.0, 0)
 
 
+def _again(c, batch, q, d, softcap, window, bound=2.0 ** -10):
+    """The call once more, on what the cache and the batch hold now; `bound`: of the weights' exponents."""
+    kp, vp, ks, vs = _state(c)
+    table, lengths, starts = batch.page_table.tolist(), batch.lengths.tolist(), batch.starts.tolist()
+    ref, size, mine = o.attend(kp, vp, ks, vs, table, lengths, starts, q.cpu(), d ** -0.5, softcap, window, batch.max_new)
+    err = (c.attend(batch, q, d ** -0.5, softcap=softcap, window=window).cpu().double() - ref).abs()[mine]
+    assert (err <= (2.0 ** -8 * ref.abs() + (2.0 ** -8 + bound) * size + 1e-30)[mine]).all()
+
+
+@pytest.mark.parametrize("dtype", [E4M3, BF16])
+@pytest.mark.parametrize("d,page,heads,kvh,softcap,window", [(64, 32, 16, 8, 0.0, 0), (64, 16, 8, 8, 30.0, 333), (128, 64, 28, 4, 0.0, 500),
+                                                             (256, 32, 8, 4, 50.0, 490)])
+def test_many_tiles_to_a_wave(gpu, dtype, d, page, heads, kvh, softcap, window):
+    """More key tiles than the card has waves: a wave's run goes from tile to tile and over the ends of sequences, from
+    tiles that a window or a missing page cuts into whole ones."""
+    lengths = [(i * 271) % 1100 for i in range(48)]
+    c, batch, q, _ = _attend_case(gpu, dtype, d, page, heads, kvh, lengths, [1] * 48, softcap, window, seed=30, extra=0)
+    gone = torch.rand(batch.page_table.shape, generator=_gen(31)) < 0.3
+    batch.page_table[gone.to(gpu)] = -1
+    _again(c, batch, q, d, softcap, window)
+
+
+@pytest.mark.parametrize("dtype", [E4M3, BF16])
+@pytest.mark.parametrize("d,heads,kvh", [(128, 4, 4), (256, 8, 4)])
+def test_the_maximum_moves_within_a_waves_run(gpu, dtype, d, heads, kvh):
+    """Keys grow along the sequences; scores reach 2^7, so the bound on the weights' exponents is 2^-24 d 2^7 or less."""
+    lengths = [(i * 271) % 1100 for i in range(48)]
+    c, batch, q, _ = _attend_case(gpu, dtype, d, 64, heads, kvh, lengths, [1] * 48, 0.0, 0, seed=40, extra=0)
+    for row in batch.page_table.tolist():
+        for j, pid in enumerate(row):
+            if dtype == E4M3:
+                c.k_scale[pid] = 2.0 ** (-9 + j // 3)
+            else:
+                c.k[pid] = (c.k[pid].float() * 2.0 ** (-3 + j // 3)).to(BF16)
+    _again(c, batch, q, d, 0.0, 0, bound=2.0 ** -6)
+
+
 def test_attend_scales_that_are_no_powers_of_two(gpu):
     c, batch, q, _ = _attend_case(gpu, E4M3, 128, 32, 8, 4, [100, 7], [2, 1], 30.0, 0)
     for t in (c.k_scale, c.v_scale):
