@@ -8,13 +8,13 @@
 //
 // One launch. A block owns one (sequence, page, head, K or V), so its scale and
 // its bytes have one writer and no order to depend on; further blocks rotate q,
-// a wave per token. Angles: position * inv_freq / 2 pi in 64 bits (positions
-// beyond 2^17 would lose a radian's third digit in FP32), its fraction of a turn
-// in FP32, sine and cosine by the instructions that take turns: within 1.3e-7 at
-// every multiple of 2^-24, as near as FP32 routines in the rounding that follows.
-// Bound by the bytes of q, k and v at prompt sizes: 9,001 BF16 tokens of 16 and 8
-// heads of 256 (258 MB) take 62 us, 4.2 TB/s (72 with a routine of 40 instructions
-// for each sine and cosine); at decode sizes by the launch: 48 tokens, 7 us.
+// a wave per token. Angles: position * inv_freq in quarter turns, in 64 bits
+// (positions beyond 2^17 would lose a radian's third digit in FP32); sine and cosine
+// of what is beyond a whole quarter, up to pi / 4, by their series, a unit or two of
+// 2^-24 off. Bound by the bytes of q, k and v at prompt sizes: 9,001 BF16 tokens of 16
+// and 8 heads of 256 (258 MB) take 66 us (70 with a library's sine and cosine;
+// 64 with the card's instructions, whose 2^-23 change an E4M3 digit ten times as
+// often); at decode sizes by the launch: 48 tokens, 7 us.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -75,10 +75,15 @@ __device__ __forceinline__ Turn turn_of(const float* inv_freq, int lo, int pos) 
     Turn t;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const double turns = (double)pos * (double)w[i] * 0.15915494309189535;
-        const float f = (float)(turns - rint(turns));
-        t.s[i] = __builtin_amdgcn_sinf(f);
-        t.c[i] = __builtin_amdgcn_cosf(f);
+        // (to a whole number in the last places of a double's 53 bits)
+        const double quarters = (double)pos * (double)w[i] * 0.63661977236758134, whole = quarters + 0x1.8p52;
+        const int turn = __double2loint(whole);
+        const float x = (float)(quarters - (whole - 0x1.8p52)) * 1.57079632679489662f, x2 = x * x;
+        const float s = fmaf(x * x2, fmaf(x2, fmaf(x2, fmaf(x2, 1.0f / 362880, -1.0f / 5040), 1.0f / 120), -1.0f / 6), x);
+        const float c = fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, -1.0f / 3628800, 1.0f / 40320), -1.0f / 720), 1.0f / 24), -0.5f), 1.0f);
+        const uint32_t sn = __float_as_uint(turn & 1 ? c : s), cs = __float_as_uint(turn & 1 ? s : c);
+        t.s[i] = __uint_as_float(sn ^ ((uint32_t)(turn & 2) << 30));
+        t.c[i] = __uint_as_float(cs ^ ((uint32_t)((turn + 1) & 2) << 30));
     }
     return t;
 }
