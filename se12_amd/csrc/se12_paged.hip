@@ -12,8 +12,8 @@
 // (positions beyond 2^17 would lose a radian's third digit in FP32); sine and cosine
 // of what is beyond a whole quarter, up to pi / 4, by their series, a unit or two of
 // 2^-24 off. Bound by the bytes of q, k and v at prompt sizes: 9,001 BF16 tokens of 16
-// and 8 heads of 256 (258 MB) take 66 us (70 with a library's sine and cosine;
-// 64 with the card's instructions, whose 2^-23 change an E4M3 digit ten times as
+// and 8 heads of 256 (258 MB) take 64 us (68 with a library's sine and cosine;
+// 62 with the card's instructions, whose 2^-23 change an E4M3 digit ten times as
 // often); at decode sizes by the launch: 48 tokens, 7 us.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -22,8 +22,8 @@
 
 namespace se12step {
 
-constexpr int kAppendMaxThreads = 512;
-constexpr int kAppendUnits = 8;          // units of 8 values a thread of a prompt's block holds
+constexpr int kAppendMaxThreads = 1024;
+constexpr int kAppendUnits = 4;          // units of 8 values a thread of a prompt's block holds
 constexpr int kDirectTokens = 16;        // V of fewer tokens is written value by value
 
 struct AppendArgs {
@@ -373,7 +373,7 @@ int se12_step_paged_append(const se12_step_pages* pages, const se12_step_batch* 
                  log2_of(pages->page_size), pages->head_dim, rotary / 2};
     const int per_token = pages->head_dim / 8;
     const int units = (pages->page_size < a.b.max_new ? pages->page_size : a.b.max_new) * per_token;   // of a block, at most
-    const int threads = units <= 64 ? 64 : units <= 256 * kAppendUnits ? 256 : kAppendMaxThreads;
+    const int threads = units <= 64 ? 64 : units <= 256 * kAppendUnits ? 256 : units <= 512 * kAppendUnits ? 512 : kAppendMaxThreads;
     const int64_t slots = a.b.max_new == 1 ? a.b.seqs : (int64_t)(a.b.tokens >> a.page_log2) + 2 * (int64_t)a.b.seqs;
     const int64_t kv_blocks = slots * 2 * pages->kv_heads;
     const int64_t q_blocks = q ? ((int64_t)a.b.tokens + threads / 64 - 1) / (threads / 64) : 0;
