@@ -128,7 +128,8 @@ int se12_step_prefill_attention(uint16_t* qkv, int64_t stride, const uint16_t* c
  *   k [pages, kv_heads, page_size, head_dim]
  *   v [pages, kv_heads, head_dim, page_size]
  *   k_scale, v_scale [pages, kv_heads] FP32 (SE12_STEP_E4M3; else ignored): a
- *   held value stands for itself times the scale of its page and head
+ *   held value stands for itself times the scale of its page and head, a positive
+ *   number (se12_step_paged_append writes powers of two)
  * head_dim 64, 128 or 256; k and v 16-byte aligned. */
 typedef struct se12_step_pages {
     void* k;
@@ -183,16 +184,18 @@ int se12_step_paged_append(const se12_step_pages* pages, const se12_step_batch* 
 /* Attention of the new tokens over their sequences' pages, those of the call
  * itself included (appended before): the query at position p sees keys
  * max(0, p - window + 1) .. p (window 0 = all). s = q . k * scaling, soft-capped
- * tanh(s / softcap) * softcap when softcap > 0; softmax and sums in FP32,
- * weights rounded to BF16 for the product with v. q BF16 [tokens, heads,
+ * tanh(s / softcap) * softcap when softcap > 0 (up to 1024; held to 2^-22 of
+ * it); softmax and sums in FP32, weights rounded to BF16 for the product with v. q BF16 [tokens, heads,
  * head_dim], rows q_stride apart (a multiple of 8), 16-byte aligned, already
  * rotated; out BF16 [tokens, heads, head_dim] contiguous, 8-byte aligned. heads
  * a multiple of kv_heads. What a query may not see has no part in its row,
  * whatever it holds (NaN too); a query that sees nothing gives zeros.
  *
  * `workspace`: se12_step_paged_attention_workspace() bytes for the shape,
- * 256-byte aligned, contents indifferent; calls sharing it must not run
- * concurrently. Up to two launches; results do not depend on timing. */
+ * 256-byte aligned, contents indifferent; calls sharing it (two captured graphs
+ * too) must not run concurrently. Two launches, four where max_new allows a
+ * sequence more than 64 (token, query head) pairs to a KV head; results do not
+ * depend on timing. */
 int64_t se12_step_paged_attention_workspace(const se12_step_pages* pages, const se12_step_batch* batch, int32_t heads);
 
 int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batch* batch, const uint16_t* q,
@@ -200,8 +203,8 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
                               int32_t window, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* What a serving program reports of logits [rows, stride] (BF16 or FP32, vocab
- * of a row used), with z = softcap tanh(logit / softcap) when softcap > 0, else
- * the logit, and p = softmax(z) in FP32:
+ * of a row used), with z = softcap tanh(logit / softcap) when softcap > 0 (up to
+ * 1024; held to 2^-22 of it), else the logit, and p = softmax(z) in FP32:
  *   logprobs[r]  log p of tokens[r] (-inf for a token outside [0, vocab))
  *   entropy[r]   -sum p log p
  *   top_logprobs, top_ids [rows, top]  the `top` (0 .. 32) most likely tokens,

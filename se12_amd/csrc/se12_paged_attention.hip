@@ -491,7 +491,8 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
     if (const char* e = paged_error(pages, batch, heads)) return step_fail(fn, e);
     if (!q || !out) return step_fail(fn, "NULL argument");
     if (q_stride < (int64_t)heads * pages->head_dim || q_stride % 8) return step_fail(fn, "q rows must be a multiple of 8 elements apart and hold all heads");
-    if (!(softcap >= 0.0f) || !(softcap < 1e30f) || window < 0) return step_fail(fn, "softcap and window must be 0 or more");
+    // (the cap's form holds a score to 2^-22 of the cap)
+    if (!(softcap >= 0.0f) || !(softcap <= 1024.0f) || window < 0) return step_fail(fn, "softcap must be 0 to 1024 and window 0 or more");
     if (reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(out) % 8) return step_fail(fn, "misaligned tensor");
     if (batch->tokens == 0) return SE12_STEP_OK;
     const Batch b = device_batch(batch);

@@ -96,8 +96,8 @@ class PagedKvCache:
     """One layer's cache: `k` [pages, kv_heads, page_size, head_dim] and `v` [pages,
     kv_heads, head_dim, page_size] (a value column's tokens side by side, as the
     attention's matrix operands take them), dtype float8_e4m3fn or bfloat16; with
-    float8_e4m3fn `k_scale` and `v_scale` FP32 [pages, kv_heads], by which a held
-    value is multiplied. page_size 16, 32, 64 or 128, head_dim 64, 128 or 256."""
+    float8_e4m3fn `k_scale` and `v_scale` FP32 [pages, kv_heads], positive numbers by
+    which a held value is multiplied. page_size 16, 32, 64 or 128, head_dim 64, 128 or 256."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.float8_e4m3fn,
                  device=None) -> None:
@@ -216,8 +216,8 @@ class PagedKvCache:
                out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of the new tokens' q [tokens, heads, head_dim] (BF16, rotated; rows may be strided) over their
         sequences' pages, the tokens of this call appended before: softmax(cap(q . k scaling)) . v over the keys max(0,
-        p - window + 1) .. p of the query's position p, cap(s) = softcap tanh(s / softcap) where softcap > 0, window 0 =
-        all. Returns BF16 [tokens, heads, head_dim] (`out` if given; rows of no sequence are not written).
+        p - window + 1) .. p of the query's position p, cap(s) = softcap tanh(s / softcap) where softcap > 0 (to 1024),
+        window 0 = all. Returns BF16 [tokens, heads, head_dim] (`out` if given; rows of no sequence are not written).
 
         FP32 scores and sums; weights rounded to BF16. A query that sees nothing gives zeros. `workspace`: uint8 of at
         least `attend_workspace()` bytes for callers that must not allocate; calls that share one must not overlap."""
@@ -226,8 +226,8 @@ class PagedKvCache:
         tokens, heads = q.shape[0], q.shape[1]
         if heads % self.kv_heads or heads == 0:
             raise ValueError(f"q's {heads} heads are no multiple of the cache's {self.kv_heads}")
-        if not softcap >= 0.0 or int(window) != window or not 0 <= window < 2 ** 31:
-            raise ValueError("softcap and window must be 0 or more")
+        if not 0.0 <= softcap <= 1024.0 or int(window) != window or not 0 <= window < 2 ** 31:
+            raise ValueError("softcap must be 0 to 1024 and window 0 or more")
         out = self._out(out, tokens, heads)
         if tokens == 0:
             return out

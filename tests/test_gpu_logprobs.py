@@ -69,6 +69,11 @@ def test_rows_that_begin_anywhere(gpu, dtype):
         _check(big[:, first:first + vocab], torch.tensor([0, vocab - 1, vocab // 2, 1, 2, 3], device=gpu) % vocab, 8, 0.0)
 
 
+def test_the_largest_cap(gpu):
+    x, t = _logits(gpu, 3, 5000, torch.float32, 7)
+    _check(x, t, 6, 1024.0)
+
+
 def test_more_rows_than_blocks_fill_the_card(gpu):
     x, t = _logits(gpu, 1500, 2100, torch.bfloat16, 2)
     _check(x, t, 3, 0.0)

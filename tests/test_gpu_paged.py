@@ -316,6 +316,13 @@ def test_many_tiles_to_a_wave(gpu, dtype, d, page, heads, kvh, softcap, window):
     _again(c, batch, q, d, softcap, window)
 
 
+@pytest.mark.parametrize("new", [1, 50])
+def test_the_largest_cap(gpu, new):
+    """A score is held to 2^-22 of the cap, here 2^-12, twice in a quotient of sums."""
+    c, batch, q, _ = _attend_case(gpu, E4M3, 128, 32, 4, 2, [600, 3], [new, 1], 0.0, 0, seed=50, extra=0)
+    _again(c, batch, q, 128, 1024.0, 0, bound=2.0 ** -10 + 2.0 ** -11)
+
+
 @pytest.mark.parametrize("dtype", [E4M3, BF16])
 @pytest.mark.parametrize("d,heads,kvh", [(128, 4, 4), (256, 8, 4)])
 def test_the_maximum_moves_within_a_waves_run(gpu, dtype, d, heads, kvh):
