@@ -13,6 +13,11 @@
 // are the second product's operand where they are. The 16-byte pieces of a row lie in
 // LDS in an order of its own, row by row, so that the 16 lanes that read the same
 // piece of 16 rows take all banks once.
+//
+// Bound by the instructions of the one wave a SIMD has room for at head dim 256 (128
+// sums, 64 registers of Q): per 32 keys 388 vector instructions, a third of them
+// conversions of 8 bits, in 1,750 cycles, beside 1,030 of the matrix unit. 6,194 tokens of
+// 5 prompts behind up to 1,500 keys, 8 / 4 heads of 256, E4M3, cap: 170 us, 0.50 PFLOP/s.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
