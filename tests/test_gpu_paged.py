@@ -316,6 +316,43 @@ def test_many_tiles_to_a_wave(gpu, dtype, d, page, heads, kvh, softcap, window):
     _again(c, batch, q, d, softcap, window)
 
 
+@pytest.mark.parametrize("dtype", [E4M3, BF16])
+@pytest.mark.parametrize("window", [0, 90])
+def test_prompts_among_more_sequences_than_a_wave_scans(gpu, dtype, window):
+    """Units of prompts in the second 64 sequences too, decode steps and sequences with nothing between them."""
+    new = [(0, 1, 1, 1, 5)[i % 5] for i in range(100)]
+    new[3], new[70], new[71], new[99] = 40, 33, 90, 70
+    lengths = [(i * 53) % 150 for i in range(100)]
+    _attend_case(gpu, dtype, 64, 16, 4, 2, lengths, new, 0.0, window, seed=60)
+
+
+@pytest.mark.parametrize("dtype", [E4M3, BF16])
+@pytest.mark.parametrize("d,window", [(64, 1000), (256, 700)])
+def test_parts_of_a_units_keys_under_a_window(gpu, dtype, d, window):
+    _attend_case(gpu, dtype, d, 32, 4, 1, [2600, 900], [70, 35], 0.0, window, seed=61)
+
+
+@pytest.mark.parametrize("dtype", [E4M3, BF16])
+def test_more_query_heads_to_one_than_columns_of_a_block(gpu, dtype):
+    _attend_case(gpu, dtype, 64, 16, 160, 1, [100, 5, 0], [1, 3, 1], 0.0, 0, seed=62)
+    _attend_case(gpu, dtype, 64, 16, 80, 1, [300, 5], [1, 2], 0.0, 70, seed=63)
+
+
+def test_more_allowed_new_tokens_than_there_are(gpu):
+    """max_new is a bound: decode steps beside kernels for prompts that find nothing to do."""
+    _attend_case(gpu, E4M3, 128, 32, 8, 2, [100, 33, 0], [1, 1, 1], 0.0, 0, seed=64, max_new=500)
+    _attend_case(gpu, BF16, 64, 16, 2, 2, [100] * 80, [1] * 80, 0.0, 20, seed=65, max_new=100)
+
+
+def test_sequences_that_share_pages(gpu):
+    """The same pages under two sequences, and one page twice in a row, are read like others."""
+    for dtype in (E4M3, BF16):
+        c, batch, q, _ = _attend_case(gpu, dtype, 128, 32, 4, 2, [200, 170, 90], [1, 3, 40], 0.0, 0, seed=66, extra=0)
+        batch.page_table[1, :5] = batch.page_table[0, :5]
+        batch.page_table[2, 1] = batch.page_table[2, 0]
+        _again(c, batch, q, 128, 0.0, 0)
+
+
 @pytest.mark.parametrize("new", [1, 50])
 def test_the_largest_cap(gpu, new):
     """A score is held to 2^-22 of the cap, here 2^-12, twice in a quotient of sums."""
