@@ -24,7 +24,7 @@
 
 #include <algorithm>
 
-#include "se12_paged_device.hpp"
+#include "se12_paged_units.hpp"
 
 namespace se12step {
 
@@ -308,6 +308,11 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : 2) void paged_attent
     constexpr int kTile = Form<CT>::kTile;
     const int lane = threadIdx.x & 63;
     const int worker = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * (kAttendThreads / 64) + (threadIdx.x >> 6)));
+    // (workers come four to a block; behind them waves for the units of se12_paged_prompt.hip)
+    if (worker >= a.workers) {
+        if (worker - a.workers < a.unit_count) write_unit<CT, D>(a, worker - a.workers);
+        return;
+    }
     Chunk chunk = load_chunk<kTile>(a, 0, lane);
     int64_t total = chunk.all;
     for (int s0 = 64; s0 < a.b.seqs; s0 += 64) total += load_chunk<kTile>(a, s0, lane).all;
@@ -468,12 +473,14 @@ int64_t few_bytes(const se12_step_pages* p, const Batch& b, int group) {
 bool any_many(const Batch& b, int group) { return (int64_t)b.max_new * group > kFewColumns; }
 
 int64_t part_bytes(const se12_step_pages* p, const Batch& b, int group) {
-    return few_bytes(p, b, group) + (any_many(b, group) ? prompt_part_bytes(b, p->kv_heads, group, p->page_size, p->head_dim) : 0);
+    if (!any_many(b, group)) return few_bytes(p, b, group);
+    return few_bytes(p, b, group) + prompt_unit_bytes(b, p->kv_heads, group, p->page_size) +
+           prompt_part_bytes(b, p->kv_heads, group, p->page_size, p->head_dim);
 }
 
 template <int CT, int D>
 void launch_attend(const AttendArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((paged_attention_kernel<CT, D>), dim3(a.workers / (kAttendThreads / 64)), dim3(kAttendThreads), 0, st, a);
+    hipLaunchKernelGGL((paged_attention_kernel<CT, D>), dim3((uint32_t)(((int64_t)a.workers + a.unit_count + 3) / (kAttendThreads / 64))), dim3(kAttendThreads), 0, st, a);
     const int max_units = (int)((std::min<int64_t>((int64_t)a.b.max_new * a.group, kFewColumns) + kColumns - 1) / kColumns);
     hipLaunchKernelGGL((paged_join_kernel<CT, D>), dim3((uint32_t)((int64_t)a.b.seqs * a.kvh * max_units), max_units > 1 ? 4 : a.columns), dim3(kAttendThreads), 0,
                        st, a, max_units);
@@ -512,7 +519,9 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
     AttendArgs a{q, q_stride, out, pages->k, pages->v, pages->k_scale, pages->v_scale, b, heads, pages->kv_heads, group, pages->pages,
                  log2_of(pages->page_size), window, softcap > 0.0f ? 2.0f * scaling / softcap * kLog2E : scaling * kLog2E,
                  softcap * kLog2E, static_cast<float*>(workspace), worker_count(pages, b, group), column_count(b, group), kFewColumns,
-                 prompt_splits(b, pages->kv_heads, group, pages->page_size)};
+                 prompt_splits(b, pages->kv_heads, group, pages->page_size),
+                 reinterpret_cast<UnitWork*>(static_cast<char*>(workspace) + few_bytes(pages, b, group)),
+                 any_many(b, group) ? prompt_units(b, pages->kv_heads, group, pages->page_size) : 0};
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const bool e4m3 = pages->dtype == SE12_STEP_E4M3;
     switch (pages->head_dim) {
@@ -526,7 +535,8 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
             e4m3 ? launch_attend<SE12_STEP_E4M3, 256>(a, st) : launch_attend<SE12_STEP_BF16, 256>(a, st);
     }
     if (any_many(b, group)) {
-        a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + few_bytes(pages, b, group));
+        a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + few_bytes(pages, b, group) +
+                                          prompt_unit_bytes(b, pages->kv_heads, group, pages->page_size));
         launch_prompt(a, e4m3, pages->head_dim, st);
     }
     return step_launched();

@@ -60,6 +60,8 @@ struct AttendArgs {
     int workers, columns;
     int few;             // sequences of more columns are se12_paged_prompt.hip's
     int splits;          // there: blocks that may share a unit's keys
+    struct UnitWork* units;   // and what its blocks are to do, `unit_count` of them
+    int unit_count;
 };
 
 // What a lane holds of a tile, by the cache's type: 16 bytes of each key row's
@@ -170,6 +172,8 @@ inline Batch device_batch(const se12_step_batch* b) {
 // se12_paged_prompt.hip
 bool prompt_fits(const Batch& b, int kvh, int group, int page_size);
 int prompt_splits(const Batch& b, int kvh, int group, int page_size);
+int prompt_units(const Batch& b, int kvh, int group, int page_size);
+int64_t prompt_unit_bytes(const Batch& b, int kvh, int group, int page_size);
 int64_t prompt_part_bytes(const Batch& b, int kvh, int group, int page_size, int d);
 void launch_prompt(const AttendArgs& a, bool e4m3, int d, hipStream_t st);
 

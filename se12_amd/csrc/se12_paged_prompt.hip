@@ -17,14 +17,14 @@
 // Bound by the instructions of the one wave a SIMD has room for at head dim 256 (128
 // sums, 64 registers of Q): per 32 keys 388 vector instructions, a third of them
 // conversions of 8 bits, in 1,750 cycles, beside 1,030 of the matrix unit. 6,194 tokens of
-// 5 prompts behind up to 1,500 keys, 8 / 4 heads of 256, E4M3, cap: 170 us, 0.50 PFLOP/s.
+// 5 prompts behind up to 1,500 keys, 8 / 4 heads of 256, E4M3, cap: 164 us, 0.52 PFLOP/s.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include <algorithm>
 
 #include "se12_device.hpp"
-#include "se12_paged_device.hpp"
+#include "se12_paged_units.hpp"
 
 namespace se12step {
 
@@ -33,126 +33,13 @@ typedef float floatx16_t __attribute__((ext_vector_type(16)));
 constexpr int kPromptThreads = 256;
 constexpr int kPromptWaves = kPromptThreads / 64;
 constexpr int kWaveColumns = 32;
-constexpr int kBlockColumns = kPromptWaves * kWaveColumns;
+static_assert(kBlockColumns == kPromptWaves * kWaveColumns, "");
 constexpr int kSubTile = 32;              // keys of a first product
 constexpr int kSharedUnits = 1024;        // with more, blocks end close enough to each other as they are
-constexpr int kLeastTiles = 8;            // of a block, where a unit's keys are split
 
 // the key (of 32) of row m of the first product's A operand: lane half h = bit 2 of
 // m takes keys 16 h ..
 __device__ __forceinline__ int key_of_row(int m) { return (m & 3) | ((m & 8) >> 1) | ((m & 16) >> 1) | ((m & 4) << 2); }
-
-// one unit: 128 columns of a sequence and KV head
-struct Unit {
-    int s, first;          // sequence, its first column of the unit
-    Seq seq;
-    int keys, columns;     // of the sequence
-};
-
-// The units in the order they are started: 64 sequences after the other, and among
-// those by the last key they see, the most first, so that what is left for the last
-// blocks is short. One lane holds one sequence: how many of its units see a key past
-// 64 x is in closed form, so the x of a rank is found by halving.
-struct UnitCounts {
-    Seq seq;
-    int keys, columns, units;
-    // units that see past key x
-    __device__ __forceinline__ int past(int x, int group) const {
-        const int64_t c = (int64_t)max(x - seq.len, 0) * group;     // the first column that does
-        return keys > x && c < columns ? units - (int)(c / kBlockColumns) : 0;
-    }
-};
-
-// (within rows of 16 lanes by DPP, as the float sums of se12_step_math.hpp)
-template <typename Op>
-__device__ __forceinline__ int wave_all(int v, Op op) {
-    v = op(v, __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, true));
-    v = op(v, __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, true));
-    v = op(v, __builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, true));
-    v = op(v, __builtin_amdgcn_mov_dpp(v, 0x140, 0xF, 0xF, true));
-    return op(op(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
-              op(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
-}
-__device__ __forceinline__ int wave_total(int v) {
-    return wave_all(v, [](int a, int b) { return a + b; });
-}
-__device__ __forceinline__ int wave_most(int v) {
-    return wave_all(v, [](int a, int b) { return a > b ? a : b; });
-}
-
-__device__ __forceinline__ UnitCounts load_counts(const AttendArgs& a, int s0, int lane, int capacity) {
-    UnitCounts c;
-    c.seq = load_seq(a.b, min(s0 + lane, a.b.seqs - 1), capacity);
-    c.keys = min(c.seq.len + c.seq.n, capacity);
-    c.columns = s0 + lane < a.b.seqs ? c.seq.n * a.group : 0;
-    c.units = c.columns > a.few ? (c.columns + kBlockColumns - 1) / kBlockColumns : 0;
-    c.columns = c.units > 0 ? c.columns : 0;
-    return c;
-}
-
-// Keys of a block where units are shared (splits > 1): about as many as make all units'
-// keys one round of blocks, those of a sequence's units taken as a run from the first
-// to the last.
-template <int kTile>
-__device__ __forceinline__ int shared_tiles(const AttendArgs& a, int lane, int resident) {
-    const int capacity = a.b.width << a.page_log2;
-    int64_t all = 0;
-    for (int s0 = 0; s0 < a.b.seqs; s0 += 64) {
-        const UnitCounts c = load_counts(a, s0, lane, capacity);
-        const int last = c.keys, first = min(c.seq.len + kBlockColumns / a.group, last), reach = a.window > 0 ? a.window + kTile : INT32_MAX;
-        // (a float holds it closely enough, and is the same for every block)
-        all += wave_total((int)fminf((float)c.units * (float)(min(first, reach) / 2 + min(last, reach) / 2) / kTile, 1e7f));
-    }
-    return (int)min(all * a.kvh / resident + 1, (int64_t)INT32_MAX);
-}
-
-__device__ __forceinline__ bool find_unit(const AttendArgs& a, int rank, Unit& u) {
-    const int lane = threadIdx.x & 63, capacity = a.b.width << a.page_log2;
-    for (int s0 = 0; s0 < a.b.seqs; s0 += 64) {
-        const UnitCounts c = load_counts(a, s0, lane, capacity);
-        const int all = wave_total(c.units);
-        if (rank >= all) {
-            rank -= all;
-            continue;
-        }
-        const int most = wave_most(c.units > 0 ? c.keys : 0);
-        // the largest x with more than `rank` units past 64 x (every unit is past -1)
-        int lo = -1, hi = (most + 63) / 64;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (wave_total(c.past(64 * mid, a.group)) > rank)
-                lo = mid;
-            else
-                hi = mid;
-        }
-        const int here = lo < 0 ? c.units : c.past(64 * lo, a.group), beyond = c.past(64 * (lo + 1), a.group);
-        rank -= wave_total(beyond);
-        int upto = here - beyond;      // of this x: a sequence's are units - here .. units - beyond - 1
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(upto, o, 64);
-            upto += lane >= o ? v : 0;
-        }
-        const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > rank));
-        auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-        u.s = s0 + l;
-        u.seq = {of(c.seq.start), of(c.seq.n), of(c.seq.len)};
-        u.keys = of(c.keys);
-        u.columns = of(c.columns);
-        u.first = kBlockColumns * (of(c.units) - of(here) + rank - (of(upto) - (of(here) - of(beyond))));
-        return true;
-    }
-    return false;
-}
-
-// the key tiles the unit's columns see
-template <int kTile>
-__device__ __forceinline__ void unit_tiles(const AttendArgs& a, const Unit& u, int& t0, int& t1) {
-    const int pos0 = u.seq.len + u.first / a.group;
-    const int pos1 = u.seq.len + (min(u.first + kBlockColumns, u.columns) - 1) / a.group;
-    t0 = (a.window > 0 ? max(0, pos0 - a.window + 1) : 0) / kTile;
-    t1 = max((min(u.keys, pos1 + 1) + kTile - 1) / kTile, t0 + 1);
-}
 
 // se12::lds_load16 from a uniform address and the lane's offset
 __device__ __forceinline__ void lds_load16(const void* base, uint32_t offset, uint32_t lds) {
@@ -185,33 +72,6 @@ __device__ __forceinline__ void settle_products() {
     if constexpr (D == 256) asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15");
 }
 
-// blocks the card holds at once
-template <int CT, int D>
-constexpr int kResidentBlocks = 256 * (D == 256 || (D == 128 && CT == SE12_STEP_BF16) ? 1 : 2);
-
-// Which units are shared: the first `units` of the order, in parts of about `tiles`
-// tiles. Their parts come first, and then the others, the most keys first.
-struct Sharing {
-    int units, tiles;
-};
-
-template <int CT, int D>
-__device__ __forceinline__ Sharing sharing_of(const AttendArgs& a, int lane) {
-    constexpr int kTile = Form<CT>::kTile;
-    if (a.splits == 1) return {0, INT32_MAX};
-    const int tiles = max(shared_tiles<kTile>(a, lane, kResidentBlocks<CT, D>), kLeastTiles);
-    // (all of them where their order is not that of their keys)
-    if (a.b.seqs > 64 || a.window > 0) return {INT32_MAX / a.splits, tiles};
-    return {wave_total(load_counts(a, 0, lane, a.b.width << a.page_log2).past((int)min((int64_t)tiles * kTile, (int64_t)INT32_MAX), a.group)), tiles};
-}
-
-// tiles of a block of a unit that has `tiles`
-__device__ __forceinline__ int part_tiles(const AttendArgs& a, const Sharing& x, int rank, int tiles) {
-    if (rank >= x.units) return tiles;
-    const int parts = min((tiles + x.tiles - 1) / x.tiles, a.splits);
-    return (tiles + parts - 1) / parts;
-}
-
 template <int CT, int D, bool kCapped>
 __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_STEP_E4M3) ? 2 : 1) void paged_prompt_kernel(AttendArgs a) {
     using F = Form<CT>;
@@ -225,30 +85,16 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];     // [2][keys, values]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int kh = blockIdx.x % a.kvh;
-    int rank = blockIdx.x / a.kvh, split = 0;
-    const Sharing sharing = sharing_of<CT, D>(a, lane);
-    if (rank < sharing.units * a.splits) {
-        split = rank % a.splits;
-        rank /= a.splits;
-    } else {
-        rank -= sharing.units * (a.splits - 1);
-    }
-    Unit u;
-    if (!find_unit(a, rank, u)) return;
-    int t0, t1;
-    unit_tiles<kTile>(a, u, t0, t1);
-    const int length = part_tiles(a, sharing, rank, t1 - t0);
-    const bool whole = t1 - t0 <= length;
-    t0 += split * length;
-    t1 = min(t1, t0 + length);
-    if (t0 >= t1) return;
+    const UnitWork u = unit_work(a, blockIdx.x / a.kvh);
+    if (u.s < 0) return;
+    const int t0 = u.t0, t1 = u.t1;
 
     const int col = lane & 31, half = lane >> 5;
     const int c0 = u.first + wave * kWaveColumns, mine = min(kWaveColumns, u.columns - c0);   // (may be none)
     const bool live = col < mine;
     const int c = live ? c0 + col : u.first, token = c / a.group;
-    const int pos = live ? u.seq.len + token : -1;
-    const int pos_min = u.seq.len + c0 / a.group, pos_max = mine > 0 ? u.seq.len + (c0 + mine - 1) / a.group : -1;
+    const int pos = live ? u.len + token : -1;
+    const int pos_min = u.len + c0 / a.group, pos_max = mine > 0 ? u.len + (c0 + mine - 1) / a.group : -1;
     const int reach = a.window > 0 ? a.window : INT32_MAX;
     const int low = max(0, pos_min - reach + 1), high = min(u.keys, pos_max + 1);      // keys some column of the wave sees
 
@@ -422,7 +268,7 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
         load_keys(to_last(t0 + 1), 1, ke);
     }
     {
-        const uint16_t* qp = a.q + (u.seq.start + token) * a.q_stride + (int64_t)(kh * a.group + c % a.group) * D;
+        const uint16_t* qp = a.q + (u.start + token) * a.q_stride + (int64_t)(kh * a.group + c % a.group) * D;
 #pragma unroll
         for (int i = 0; i < kQSteps; ++i)
             qf[i] = *reinterpret_cast<const bf16x8_t*>(qp + (i / F::kHalves) * 2 * F::kPer + half * F::kPer + 8 * (i % F::kHalves));
@@ -608,9 +454,9 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
     }
     se12::wait_vector_loads();      // (before this block's LDS is another's)
     l += __shfl_xor(l, 32, 64);
-    if (!whole) {
+    if (u.parts > 1) {
         // the part of (unit, head, split), as the lanes hold it
-        const int64_t p = ((int64_t)rank * a.kvh + kh) * a.splits + split;
+        const int64_t p = ((int64_t)u.rank * a.kvh + kh) * a.splits + u.split;
         float4* to = reinterpret_cast<float4*>(a.part + p * kBlockColumns * D) + wave * (D / 8) * 64 + lane;
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
@@ -641,9 +487,9 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
         const int r = k * kRowsAtOnce + lane / kOutPieces, piece = lane % kOutPieces, x = c0 + r;
         if (r >= mine) continue;
         const uint4 v = *reinterpret_cast<const uint4*>(own + r * 2 * D + 16 * (piece ^ (r & kTwist)));
-        *reinterpret_cast<uint2*>(a.out + ((int64_t)(u.seq.start + x / a.group) * a.heads + kh * a.group + x % a.group) * D + 8 * piece) =
+        *reinterpret_cast<uint2*>(a.out + ((int64_t)(u.start + x / a.group) * a.heads + kh * a.group + x % a.group) * D + 8 * piece) =
             make_uint2(v.x, v.y);
-        *reinterpret_cast<uint2*>(a.out + ((int64_t)(u.seq.start + x / a.group) * a.heads + kh * a.group + x % a.group) * D + 8 * piece + 4) =
+        *reinterpret_cast<uint2*>(a.out + ((int64_t)(u.start + x / a.group) * a.heads + kh * a.group + x % a.group) * D + 8 * piece + 4) =
             make_uint2(v.z, v.w);
     }
 }
@@ -656,15 +502,13 @@ constexpr int kJoinBlocks = D / 16;
 
 template <int CT, int D>
 __global__ __launch_bounds__(kPromptThreads) void paged_prompt_join_kernel(AttendArgs a, int64_t parts) {
-    constexpr int kTile = Form<CT>::kTile, kPieces = D / 8 / kJoinBlocks<D>;
+    constexpr int kPieces = D / 8 / kJoinBlocks<D>;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31;
     const int kh = blockIdx.x % a.kvh, rank = blockIdx.x / a.kvh;
-    const Sharing sharing = sharing_of<CT, D>(a, lane);
-    Unit u;
-    if (rank >= sharing.units || !find_unit(a, rank, u)) return;
-    int t0, t1;
-    unit_tiles<kTile>(a, u, t0, t1);
-    const int length = part_tiles(a, sharing, rank, t1 - t0), count = (t1 - t0 + length - 1) / length;
+    // (a shared unit's first block; where the unit is not shared, another's or its only one)
+    const UnitWork u = unit_work(a, rank * a.splits);
+    if (u.s < 0 || u.rank != rank) return;
+    const int count = u.parts;
     const int c = u.first + wave * kWaveColumns + col;
     if (count <= 1 || c >= u.columns) return;
     const int64_t p0 = ((int64_t)rank * a.kvh + kh) * a.splits;
@@ -692,7 +536,7 @@ __global__ __launch_bounds__(kPromptThreads) void paged_prompt_join_kernel(Atten
         }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t* out = a.out + ((int64_t)(u.seq.start + c / a.group) * a.heads + kh * a.group + c % a.group) * D + 4 * (lane >> 5);
+    uint16_t* out = a.out + ((int64_t)(u.start + c / a.group) * a.heads + kh * a.group + c % a.group) * D + 4 * (lane >> 5);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i)
         store4(out + 8 * (i * kJoinBlocks<D> + blockIdx.y), o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv);
@@ -728,6 +572,12 @@ int prompt_splits(const Batch& b, int kvh, int group, int page_size) {
 bool prompt_fits(const Batch& b, int kvh, int group, int page_size) {
     return (int64_t)unit_slots(b, group) * kvh * prompt_splits(b, kvh, group, page_size) <= INT32_MAX &&
            (int64_t)b.tokens * group <= INT32_MAX;
+}
+
+int prompt_units(const Batch& b, int kvh, int group, int page_size) { return unit_slots(b, group) * prompt_splits(b, kvh, group, page_size); }
+
+int64_t prompt_unit_bytes(const Batch& b, int kvh, int group, int page_size) {
+    return ((int64_t)prompt_units(b, kvh, group, page_size) * (int64_t)sizeof(UnitWork) + 255) / 256 * 256;
 }
 
 int64_t prompt_part_bytes(const Batch& b, int kvh, int group, int page_size, int d) {
