@@ -17,7 +17,7 @@
 // Bound by the instructions of the one wave a SIMD has room for at head dim 256 (128
 // sums, 64 registers of Q): per 32 keys 388 vector instructions, a third of them
 // conversions of 8 bits, in 1,750 cycles, beside 1,030 of the matrix unit. 6,194 tokens of
-// 5 prompts behind up to 1,500 keys, 8 / 4 heads of 256, E4M3, cap: 164 us, 0.52 PFLOP/s.
+// 5 prompts behind up to 1,500 keys, 8 / 4 heads of 256, E4M3, cap: 161 us, 0.53 PFLOP/s.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -283,14 +283,16 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
     arrived(next);
     __syncthreads();
     floatx16_t d;
-    auto scores = [&]() {
+    auto scores = [&](auto beside) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) d[e] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kKeyReads; ++i)
+        for (int i = 0; i < kKeyReads; ++i) {
+            beside(i);
 #pragma unroll
             for (int h = 0; h < F::kHalves; ++h)
                 d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand<CT>(kf[i], h), qf[i * F::kHalves + h], d, 0, 0, 0);
+        }
     };
     auto cap_scores = [&](float ks) {
         const float by = a.c1 * ks;
@@ -305,7 +307,7 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
         if constexpr (kCapped) top = a.cap - 2.0f * a.cap * top;
     };
     read_keys(t0, 0);
-    scores();
+    scores([](int) {});
     read_keys(t0 + 1 / kSubs, 1 % kSubs);
     cap_scores(now.ks0);
     find_top();
@@ -411,7 +413,15 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
                 apart |= any_no_number();
             }
             if (__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0) move_maximum();
-            scores();
+            // The loads of the tiles to come, one beside every other row's products, the values'
+            // here and the keys' below: a wave waits for as long as a load is not taken.
+            // (Both below, 64 x 64 tokens behind 2,048, heads of 256: 133 us as well from E4M3
+            // pages, 194 for 170 from BF16; the values' a sub-tile later: 139 and 184.)
+            const Source vs = values_of(to_last(t + 1), (t + 1 - t0) & 1, ve);
+            if (j == 0) ve = value_entry_of(to_last(t + 2));
+            scores([&](int i) {
+                if (j == 0 && i % (kKeyReads / kLoads) == 0) load_value(vs, i / (kKeyReads / kLoads));
+            });
             weights();
             if (apart) {
                 bring_no_numbers(t, j, key0, held);
@@ -419,13 +429,9 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
                 mask_values(key0, held, 0);
                 numbers_of_values();
             }
-            // The loads of the tiles to come, one beside every other row's products: a wave
-            // waits for as long as a load is not taken.
-            static_assert(kRows == 2 * kLoads, "");
+            static_assert(kRows == 2 * kLoads && kKeyReads % kLoads == 0, "");
             const Source ks = keys_of(to_last(t + kLead + 1), (t + kLead + 1 - t0) & 1, ke);
-            const Source vs = values_of(to_last(t + 1), (t + 1 - t0) & 1, ve);
             if (j == 0) ke = key_entry_of(to_last(t + kLead + 2));
-            if (j == kSubs - 1) ve = value_entry_of(to_last(t + 2));
             __builtin_amdgcn_sched_barrier(0);
             read_keys(t + (j + 2) / kSubs, (j + 2) % kSubs);
             __builtin_amdgcn_sched_barrier(0);
@@ -442,7 +448,6 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
 #pragma unroll
                 for (int i = 0; i < kRows; ++i) {
                     if (n == 0 && j == 0 && i % 2 == 0) load_key(ks, i / 2);
-                    if (n == kValueReads - 1 && j == kSubs - 1 && i % 2 == 0) load_value(vs, i / 2);
 #pragma unroll
                     for (int h = 0; h < F::kHalves; ++h)
                         o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand<CT>(vf[i], h), pf[n + h], o[i], 0, 0, 0);
