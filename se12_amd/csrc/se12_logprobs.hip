@@ -17,9 +17,9 @@
 // second launch, where rows are too few to fill the card with a block each.
 //
 // Bound by its bytes where rows are many: 1,024 FP32 rows of 256,000 under a cap, top
-// 5, 1,049 MB in 193 us (5.4 TB/s; the arithmetic alone about 130: three instructions of
-// a quarter of the rate to a logit). One such row, top 20: 6.9 + 4.5 us, two launches'
-// latency and the rankings; 40 rows of 100,277 in BF16, top 5: 8.6 + 4.2.
+// 5, 1,049 MB in 192 us (5.5 TB/s; the arithmetic alone about 130: three instructions of
+// a quarter of the rate to a logit). One such row, top 20: 6.7 + 4.4 us, two launches'
+// latency and the rankings; 40 rows of 100,277 in BF16, top 5: 8.2 + 4.5.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
