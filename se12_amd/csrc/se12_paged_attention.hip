@@ -472,6 +472,15 @@ int64_t few_bytes(const se12_step_pages* p, const Batch& b, int group) {
 
 bool any_many(const Batch& b, int group) { return (int64_t)b.max_new * group > kFewColumns; }
 
+// what one launch holds, and what 32 bits hold of it
+const char* limits_error(const se12_step_pages* p, const Batch& b, int group) {
+    if ((int64_t)b.seqs * p->kv_heads * (kFewColumns / kColumns) > INT32_MAX || !prompt_fits(b, p->kv_heads, group, p->page_size))
+        return "too many sequences, tokens and heads for one launch";
+    if (std::min<int64_t>(b.seqs, 64) * (((int64_t)b.width * p->page_size + 31) / 32) * (kFewColumns / kColumns) * p->kv_heads > INT32_MAX)
+        return "too long a table for so many sequences and heads";
+    return nullptr;
+}
+
 int64_t part_bytes(const se12_step_pages* p, const Batch& b, int group) {
     if (!any_many(b, group)) return few_bytes(p, b, group);
     return few_bytes(p, b, group) + prompt_unit_bytes(b, p->kv_heads, group, p->page_size) +
@@ -491,9 +500,12 @@ void launch_attend(const AttendArgs& a, hipStream_t st) {
 extern "C" {
 
 int64_t se12_step_paged_attention_workspace(const se12_step_pages* pages, const se12_step_batch* batch, int32_t heads) {
-    if (const char* e = paged_error(pages, batch, heads)) return step_fail("se12_step_paged_attention_workspace", e);
+    const char* fn = "se12_step_paged_attention_workspace";
+    if (const char* e = paged_error(pages, batch, heads)) return step_fail(fn, e);
     if (batch->tokens == 0) return 0;
-    return part_bytes(pages, device_batch(batch), heads / pages->kv_heads);
+    const Batch b = device_batch(batch);
+    if (const char* e = limits_error(pages, b, heads / pages->kv_heads)) return step_fail(fn, e);
+    return part_bytes(pages, b, heads / pages->kv_heads);
 }
 
 int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batch* batch, const uint16_t* q,
@@ -509,12 +521,9 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
     if (batch->tokens == 0) return SE12_STEP_OK;
     const Batch b = device_batch(batch);
     const int group = heads / pages->kv_heads;
+    if (const char* e = limits_error(pages, b, group)) return step_fail(fn, e);
     if (reinterpret_cast<uintptr_t>(workspace) % 256 || !workspace || workspace_bytes < part_bytes(pages, b, group))
         return step_fail(fn, "workspace missing, misaligned or too small");
-    if ((int64_t)b.seqs * pages->kv_heads * (kFewColumns / kColumns) > INT32_MAX || !prompt_fits(b, pages->kv_heads, group, pages->page_size))
-        return step_fail(fn, "too many sequences, tokens and heads for one launch");
-    if (std::min<int64_t>(b.seqs, 64) * (((int64_t)b.width * pages->page_size + 31) / 32) * (kFewColumns / kColumns) * pages->kv_heads > INT32_MAX)
-        return step_fail(fn, "too long a table for so many sequences and heads");
     constexpr float kLog2E = 1.4426950408889634f;
     AttendArgs a{q, q_stride, out, pages->k, pages->v, pages->k_scale, pages->v_scale, b, heads, pages->kv_heads, group, pages->pages,
                  log2_of(pages->page_size), window, softcap > 0.0f ? 2.0f * scaling / softcap * kLog2E : scaling * kLog2E,

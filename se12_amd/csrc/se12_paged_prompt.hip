@@ -575,8 +575,8 @@ int prompt_splits(const Batch& b, int kvh, int group, int page_size) {
 }
 
 bool prompt_fits(const Batch& b, int kvh, int group, int page_size) {
-    return (int64_t)unit_slots(b, group) * kvh * prompt_splits(b, kvh, group, page_size) <= INT32_MAX &&
-           (int64_t)b.tokens * group <= INT32_MAX;
+    return (int64_t)b.tokens * group <= INT32_MAX &&
+           (int64_t)unit_slots(b, group) * kvh * prompt_splits(b, kvh, group, page_size) <= INT32_MAX;
 }
 
 int prompt_units(const Batch& b, int kvh, int group, int page_size) { return unit_slots(b, group) * prompt_splits(b, kvh, group, page_size); }

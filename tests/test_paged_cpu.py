@@ -76,6 +76,18 @@ def test_attention_refuses(change, message):
         nat.step_check(nat.lib().se12_step_paged_attention(ctypes.byref(_pages()), ctypes.byref(_batch()), *f.values(), None))
 
 
+@pytest.mark.parametrize("batch,message", [
+    (dict(tokens=1 << 30, max_new=1 << 20), "too many sequences, tokens"), (dict(tokens=1 << 28, sequences=65536), "too many"),
+    (dict(sequences=64, table_width=1 << 24, table_stride=1 << 24), "too long a table"),
+])
+def test_attention_refuses_what_one_launch_does_not_hold(batch, message):
+    lib, p, b = nat.lib(), _pages(kv_heads=8), _batch(**batch)
+    for call in (lambda: lib.se12_step_paged_attention(ctypes.byref(p), ctypes.byref(b), P, 1 << 14, P, 128, 0.1, 0.0, 0, P, 1 << 60, None),
+                 lambda: lib.se12_step_paged_attention_workspace(ctypes.byref(p), ctypes.byref(b), 128)):
+        with pytest.raises(nat.Se12Error, match=message):
+            nat.step_check(call())
+
+
 @pytest.mark.parametrize("change,message", [
     (dict(vocab=0), "bad shape"), (dict(rows=-1), "bad shape"), (dict(top=33), "top"), (dict(top=-1), "top"), (dict(vocab=4, top=5), "top"),
     (dict(logits=None), "NULL"), (dict(tokens=None), "NULL"), (dict(tl=None), "NULL"), (dict(dtype=2), "BF16 or FP32"),
