@@ -162,7 +162,7 @@ typedef struct se12_step_batch {
 
 /* Appends k and v [tokens, kv_heads, head_dim] to the cache, k rotated to its
  * position, and writes the rotated q [tokens, heads, head_dim] to q_out (BF16,
- * contiguous); q may be NULL, then nothing is. Rows `q_stride`, `k_stride`,
+ * contiguous; q itself where that is both); q may be NULL, then nothing is. Rows `q_stride`, `k_stride`,
  * `v_stride` elements apart (multiples of 4), heads of a row side by side; dtype
  * SE12_STEP_BF16 or SE12_STEP_F32 for all three, aligned to four elements. The
  * rotation takes the pair (x[i], x[i + rotary / 2]) by position * inv_freq[i],
@@ -187,8 +187,8 @@ int se12_step_paged_append(const se12_step_pages* pages, const se12_step_batch* 
  * tanh(s / softcap) * softcap when softcap > 0 (up to 1024; held to 2^-22 of
  * it); softmax and sums in FP32, weights rounded to BF16 for the product with v. q BF16 [tokens, heads,
  * head_dim], rows q_stride apart (a multiple of 8), 16-byte aligned, already
- * rotated; out BF16 [tokens, heads, head_dim] contiguous, 8-byte aligned. heads
- * a multiple of kv_heads. What a query may not see has no part in its row,
+ * rotated; out BF16 [tokens, heads, head_dim] contiguous, 8-byte aligned, apart
+ * from q. heads a multiple of kv_heads. What a query may not see has no part in its row,
  * whatever it holds (NaN too); a query that sees nothing gives zeros.
  *
  * `workspace`: se12_step_paged_attention_workspace() bytes for the shape,

@@ -532,6 +532,10 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
     if (const char* e = limits_error(pages, b, group)) return step_fail(fn, e);
     if (reinterpret_cast<uintptr_t>(workspace) % 256 || !workspace || workspace_bytes < part_bytes(pages, b, group))
         return step_fail(fn, "workspace missing, misaligned or too small");
+    // (q is read until the last wave is done with it)
+    const uint16_t *q_end = q + (b.tokens - 1) * q_stride + (int64_t)heads * pages->head_dim, *out_end = out + (int64_t)b.tokens * heads * pages->head_dim;
+    if (reinterpret_cast<uintptr_t>(q) < reinterpret_cast<uintptr_t>(out_end) && reinterpret_cast<uintptr_t>(out) < reinterpret_cast<uintptr_t>(q_end))
+        return step_fail(fn, "out overlaps q");
     constexpr float kLog2E = 1.4426950408889634f;
     AttendArgs a{q, q_stride, out, pages->k, pages->v, pages->k_scale, pages->v_scale, b, heads, pages->kv_heads, group, pages->pages,
                  log2_of(pages->page_size), window, softcap > 0.0f ? 2.0f * scaling / softcap * kLog2E : scaling * kLog2E,

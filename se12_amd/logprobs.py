@@ -31,7 +31,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, sof
     A token outside [0, vocab) has log probability -inf. Logits of -inf (tokens that are not allowed) have no part in the
     sums where there is no cap; under one, -inf counts as -softcap. A row of nothing else has log probabilities of -inf
     and entropy 0; a row with a NaN, or +inf without a cap, has NaN throughout, in its alternatives NaN comes last. Runs
-    on the current stream of the logits' device and never waits for it."""
+    on the current stream of the logits' device and never waits for it; no gradients."""
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("logits must be a bfloat16 or float32 [rows, vocab] tensor")
     if not logits.is_cuda:

@@ -172,7 +172,7 @@ class PagedKvCache:
     def append(self, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,
                inv_freq: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor | None:
         """Writes the new tokens' k and v [tokens, kv_heads, head_dim] to their pages, k rotated to its position, and
-        returns q [tokens, heads, head_dim] rotated, in BF16 (into `out` if given; None without q). BF16 or FP32, all
+        returns q [tokens, heads, head_dim] rotated, in BF16 (into `out` if given, which may be q; None without q). BF16 or FP32, all
         of one type; rows may be strided (views of one product's output). The rotation turns the pairs (i, i +
         len(inv_freq)) by position * inv_freq[i], FP32 inv_freq of up to head_dim / 2 frequencies, a multiple of 4 (the
         elements behind the pairs stay; None: no rotation), as se12_step_prefill_attention pairs them.
@@ -217,7 +217,8 @@ class PagedKvCache:
         """Attention of the new tokens' q [tokens, heads, head_dim] (BF16, rotated; rows may be strided) over their
         sequences' pages, the tokens of this call appended before: softmax(cap(q . k scaling)) . v over the keys max(0,
         p - window + 1) .. p of the query's position p, cap(s) = softcap tanh(s / softcap) where softcap > 0 (to 1024),
-        window 0 = all. Returns BF16 [tokens, heads, head_dim] (`out` if given; rows of no sequence are not written).
+        window 0 = all. Returns BF16 [tokens, heads, head_dim] (`out` if given, apart from q; rows of no sequence are not
+        written). No gradients.
 
         FP32 scores and sums; weights rounded to BF16. A query that sees nothing gives zeros. `workspace`: uint8 of at
         least `attend_workspace()` bytes for callers that must not allocate; calls that share one must not overlap."""

@@ -125,6 +125,16 @@ def test_append(gpu, x_dtype, dtype, d, page, kvh, heads, rotary, lengths, new):
     _check_append(c, before, batch, lengths, starts, table, k, v, inv, q, got)
 
 
+def test_append_rotates_q_in_place(gpu):
+    c = _cache(gpu, 4, 32, 2, 128, E4M3, 70)
+    batch, _ = _batch(gpu, [[0, 1], [2, 3]], [20, 3], [30, 1])
+    q = torch.randn((31, 8, 128), generator=_gen(71)).to(BF16).to(gpu)
+    k, v = (torch.randn((31, 2, 128), generator=_gen(72 + i)).to(BF16).to(gpu) for i in range(2))
+    inv = (10000.0 ** (-torch.arange(0, 64).float() / 64)).to(gpu)
+    apart = c.append(batch, k, v, q=q, inv_freq=inv)
+    assert c.append(batch, k, v, q=q, inv_freq=inv, out=q) is q and torch.equal(q, apart)
+
+
 def test_append_without_q_and_with_a_far_position(gpu):
     """Positions where an FP32 angle has lost every digit behind the point of a turn's hundredth."""
     lengths, new = [250_000, 131_071], [3, 2]

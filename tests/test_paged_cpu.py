@@ -67,7 +67,7 @@ def test_append_refuses(change, message):
     (dict(q=None), "NULL"), (dict(out=None), "NULL"), (dict(qs=1016), "hold all heads"), (dict(qs=1028), "multiple of 8"),
     (dict(cap=-1.0), "softcap"), (dict(cap=float("nan")), "softcap"), (dict(cap=1025.0), "softcap"), (dict(window=-1), "window"), (dict(q=P + 8), "misaligned"),
     (dict(out=P + 4), "misaligned"), (dict(ws=None), "workspace"), (dict(ws=P + 128), "workspace"), (dict(size=100), "workspace"),
-    (dict(heads=7), "kv_heads"),
+    (dict(heads=7), "kv_heads"), (dict(out=P + 3 * 2048 - 16), "overlaps"), (dict(q=P + 3 * 2048 - 16), "overlaps"), (dict(), "overlaps"),
 ])
 def test_attention_refuses(change, message):
     f = dict(q=P, qs=1024, out=P, heads=8, scaling=0.1, cap=0.0, window=0, ws=P, size=1 << 30)
