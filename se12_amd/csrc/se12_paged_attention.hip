@@ -497,10 +497,12 @@ int64_t part_bytes(const se12_step_pages* p, const Batch& b, int group) {
 
 template <int CT, int D>
 void launch_attend(const AttendArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((paged_attention_kernel<CT, D>), dim3((uint32_t)(((int64_t)a.workers + a.unit_count + 3) / (kAttendThreads / 64))), dim3(kAttendThreads), 0, st, a);
+    constexpr int kWaves = kAttendThreads / 64;
+    hipLaunchKernelGGL((paged_attention_kernel<CT, D>), dim3((uint32_t)(((int64_t)a.workers + a.unit_count + kWaves - 1) / kWaves)),
+                       dim3(kAttendThreads), 0, st, a);
     const int max_units = (int)((std::min<int64_t>((int64_t)a.b.max_new * a.group, kFewColumns) + kColumns - 1) / kColumns);
-    hipLaunchKernelGGL((paged_join_kernel<CT, D>), dim3((uint32_t)((int64_t)a.b.seqs * a.kvh * max_units), max_units > 1 ? 4 : a.columns), dim3(kAttendThreads), 0,
-                       st, a, max_units);
+    hipLaunchKernelGGL((paged_join_kernel<CT, D>), dim3((uint32_t)((int64_t)a.b.seqs * a.kvh * max_units), max_units > 1 ? 4 : a.columns),
+                       dim3(kAttendThreads), 0, st, a, max_units);
 }
 
 }  // namespace
@@ -533,8 +535,9 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
     if (reinterpret_cast<uintptr_t>(workspace) % 256 || !workspace || workspace_bytes < part_bytes(pages, b, group))
         return step_fail(fn, "workspace missing, misaligned or too small");
     // (q is read until the last wave is done with it)
-    const uint16_t *q_end = q + (b.tokens - 1) * q_stride + (int64_t)heads * pages->head_dim, *out_end = out + (int64_t)b.tokens * heads * pages->head_dim;
-    if (reinterpret_cast<uintptr_t>(q) < reinterpret_cast<uintptr_t>(out_end) && reinterpret_cast<uintptr_t>(out) < reinterpret_cast<uintptr_t>(q_end))
+    const int64_t row = (int64_t)heads * pages->head_dim;
+    if (reinterpret_cast<uintptr_t>(q) < reinterpret_cast<uintptr_t>(out + b.tokens * row) &&
+        reinterpret_cast<uintptr_t>(out) < reinterpret_cast<uintptr_t>(q + (b.tokens - 1) * q_stride + row))
         return step_fail(fn, "out overlaps q");
     constexpr float kLog2E = 1.4426950408889634f;
     AttendArgs a{q, q_stride, out, pages->k, pages->v, pages->k_scale, pages->v_scale, b, heads, pages->kv_heads, group, pages->pages,

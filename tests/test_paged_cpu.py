@@ -65,7 +65,8 @@ def test_append_refuses(change, message):
 
 @pytest.mark.parametrize("change,message", [
     (dict(q=None), "NULL"), (dict(out=None), "NULL"), (dict(qs=1016), "hold all heads"), (dict(qs=1028), "multiple of 8"),
-    (dict(cap=-1.0), "softcap"), (dict(cap=float("nan")), "softcap"), (dict(cap=1025.0), "softcap"), (dict(window=-1), "window"), (dict(q=P + 8), "misaligned"),
+    (dict(cap=-1.0), "softcap"), (dict(cap=float("nan")), "softcap"), (dict(cap=1025.0), "softcap"),
+    (dict(window=-1), "window"), (dict(q=P + 8), "misaligned"),
     (dict(out=P + 4), "misaligned"), (dict(ws=None), "workspace"), (dict(ws=P + 128), "workspace"), (dict(size=100), "workspace"),
     (dict(heads=7), "kv_heads"), (dict(out=P + 3 * 2048 - 16), "overlaps"), (dict(q=P + 3 * 2048 - 16), "overlaps"), (dict(), "overlaps"),
 ])
@@ -91,7 +92,8 @@ def test_attention_refuses_what_one_launch_does_not_hold(batch, message):
 @pytest.mark.parametrize("change,message", [
     (dict(vocab=0), "bad shape"), (dict(rows=-1), "bad shape"), (dict(top=33), "top"), (dict(top=-1), "top"), (dict(vocab=4, top=5), "top"),
     (dict(logits=None), "NULL"), (dict(tokens=None), "NULL"), (dict(tl=None), "NULL"), (dict(dtype=2), "BF16 or FP32"),
-    (dict(stride=999), "overlap"), (dict(cap=-1.0), "softcap"), (dict(cap=1025.0), "softcap"), (dict(logits=P + 2), "misaligned"), (dict(tokens=P + 4), "misaligned"),
+    (dict(stride=999), "overlap"), (dict(cap=-1.0), "softcap"), (dict(cap=1025.0), "softcap"),
+    (dict(logits=P + 2), "misaligned"), (dict(tokens=P + 4), "misaligned"),
     (dict(vocab=50000, stride=50000, ws=None), "workspace"), (dict(vocab=50000, stride=50000, size=8), "workspace"),
 ])
 def test_logprobs_refuse(change, message):
