@@ -372,8 +372,6 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
         arrived(next);
         asm volatile("" : "+v"(ke), "+v"(ve), "+v"(se.x), "+v"(se.y));
         __syncthreads();
-        after = lane_of(se);
-        se = lane_entries_of(to_last(t + 3));
 #pragma unroll
         for (int j = 0; j < kSubs; ++j) {
             const int k0 = (t * kSubs + j) * kSubTile, key0 = k0 + 16 * half;
@@ -418,7 +416,11 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
             // (Both below, 64 x 64 tokens behind 2,048, heads of 256: 133 us as well from E4M3
             // pages, 194 for 170 from BF16; the values' a sub-tile later: 139 and 184.)
             const Source vs = values_of(to_last(t + 1), (t + 1 - t0) & 1, ve);
-            if (j == 0) ve = value_entry_of(to_last(t + 2));
+            if (j == 0) {
+                ve = value_entry_of(to_last(t + 2));
+                after = lane_of(se);
+                se = lane_entries_of(to_last(t + 3));
+            }
             scores([&](int i) {
                 if (j == 0 && i % (kKeyReads / kLoads) == 0) load_value(vs, i / (kKeyReads / kLoads));
             });
