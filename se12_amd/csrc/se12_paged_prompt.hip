@@ -17,7 +17,7 @@
 // Bound by the instructions of the one wave a SIMD has room for at head dim 256 (128
 // sums, 64 registers of Q): per 32 keys 388 vector instructions, a third of them
 // conversions of 8 bits, in 1,750 cycles, beside 1,030 of the matrix unit. 6,194 tokens of
-// 5 prompts behind up to 1,500 keys, 8 / 4 heads of 256, E4M3, cap: 161 us, 0.53 PFLOP/s.
+// 5 prompts behind up to 1,500 keys, 8 / 4 heads of 256, E4M3, cap: 159 us, 0.53 PFLOP/s.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
