@@ -311,6 +311,9 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
     read_keys(t0 + 1 / kSubs, 1 % kSubs);
     cap_scores(now.ks0);
     find_top();
+    // (a buffer is written again only behind a barrier that every wave reaches after its
+    // reads: with kLead 2 the next keys go over those of t0, which all waves read above)
+    if constexpr (kLead == 2) __syncthreads();
     ke = key_entry_of(to_last(t0 + kLead));
     int ve = value_entry_of(t0);
     asm volatile("" : "+v"(ke), "+v"(ve));

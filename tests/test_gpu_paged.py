@@ -348,6 +348,16 @@ def test_more_query_heads_to_one_than_columns_of_a_block(gpu, dtype):
     _attend_case(gpu, dtype, 64, 16, 80, 1, [300, 5], [1, 2], 0.0, 70, seed=63)
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_the_first_tiles_of_prompts_from_bf16_pages(gpu, d):
+    """Keys of the tile after next go over those of the first: many units of one, two, three and four tiles of 32 keys,
+    a few times, all with the same result. (A wave ahead of the others must not overwrite what they still read.)"""
+    lengths, new = [0, 20, 31, 0, 60, 3], [32, 40, 65, 33, 60, 90]
+    c, batch, q, out = _attend_case(gpu, BF16, d, 16, 32, 16, lengths, new, 0.0, 0, seed=71, extra=0)
+    for _ in range(20):
+        assert torch.equal(c.attend(batch, q, d ** -0.5), out)
+
+
 def test_more_allowed_new_tokens_than_there_are(gpu):
     """max_new is a bound: decode steps beside kernels for prompts that find nothing to do."""
     _attend_case(gpu, E4M3, 128, 32, 8, 2, [100, 33, 0], [1, 1, 1], 0.0, 0, seed=64, max_new=500)
