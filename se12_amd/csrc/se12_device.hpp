@@ -429,9 +429,10 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 // (s_waitcnt vmcnt) before reading the LDS it fills. The compiler's own
 // waits stay correct as long as loads it tracks are only waited for by
 // count (loads complete in order, so an unseen load only makes a count
-// wait for more).
+// wait for more). A load that takes its LDS address from M0 needs a wait state
+// after a scalar write of it, which inside one asm block nobody else puts there.
 __device__ __forceinline__ void lds_load16(const void* src, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
 }
 
 // Raw BF16 pairs of chunk j of a fallback tile (tile-local order, like sm).

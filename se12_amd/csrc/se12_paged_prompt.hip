@@ -43,7 +43,7 @@ __device__ __forceinline__ int key_of_row(int m) { return (m & 3) | ((m & 8) >> 
 
 // se12::lds_load16 from a uniform address and the lane's offset
 __device__ __forceinline__ void lds_load16(const void* base, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds) : "memory", "m0");
 }
 
 // x by and x + y of a sum. At D = 256 in an accumulation register, where it is kept,

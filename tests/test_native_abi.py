@@ -281,3 +281,17 @@ def test_step_kernels_reject_invalid_arguments():
                                                            ws - 1, s))
     # the row-arrival counter after the per-row ones: 64 rows need a second 256-byte line
     assert lib.se12_step_logits_workspace(64, 2048) == 512 + 256 + 256
+
+
+def test_a_wait_state_stands_between_m0_and_the_load_that_reads_it():
+    """Inside one asm block nobody else puts it there: a scalar write of M0 and a load into LDS, which takes its address
+    from M0, need one wait state between them."""
+    found = 0
+    for path in sorted((ROOT / "se12_amd" / "csrc").glob("*.h*")):
+        for block in re.findall(r'asm volatile\(((?:\s*"[^"]*")+)', path.read_text()):
+            lines = "".join(re.findall(r'"([^"]*)"', block)).replace("\\t", "").split("\\n")
+            for i, line in enumerate(lines):
+                if re.match(r"s_mov_b32\s+m0\b", line):
+                    found += 1
+                    assert re.match(r"s_nop\b", lines[i + 1]), f"{path.name}: {lines}"
+    assert found >= 2
