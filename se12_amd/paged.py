@@ -155,13 +155,15 @@ class PagedKvCache:
             raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
         if dtype is not None and t.dtype != dtype:
             raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-        row, head, one = t.stride()
-        if (one != 1 or (head != self.head_dim and shape[1] > 1) or row % multiple or row < shape[1] * self.head_dim
+        (row, head, one), width = t.stride(), shape[1] * self.head_dim
+        apart = row >= width and row % multiple == 0
+        if (one != 1 or (head != self.head_dim and shape[1] > 1) or not (apart or shape[0] <= 1)
                 or t.data_ptr() % (multiple * t.element_size())):
-            t = t.contiguous()
+            t, apart = t.contiguous(), False
             if t.data_ptr() % (multiple * t.element_size()):
                 t = t.clone()
-        return t
+        # (of a single row any first stride is contiguous to torch)
+        return t if apart else t.as_strided(shape, (width, self.head_dim, 1))
 
     def _check(self, batch: PagedBatch) -> None:
         if not isinstance(batch, PagedBatch):

@@ -135,6 +135,25 @@ def test_append_rotates_q_in_place(gpu):
     assert c.append(batch, k, v, q=q, inv_freq=inv, out=q) is q and torch.equal(q, apart)
 
 
+def test_one_token_in_rows_of_any_distance(gpu):
+    """A single token's heads transposed, its row of an odd length: as a copy of it gives."""
+    c, d = _cache(gpu, 4, 32, 4, 128, E4M3, 73), 128
+    batch, _ = _batch(gpu, [[0, 1]], [20], [1])
+    g = _gen(74)
+    for dtype in (torch.float32, BF16):
+        x = torch.randn((1, 16, 1, d), generator=g).to(dtype).to(gpu)
+        rows = torch.randn((2, 16 * d + 3), generator=g).to(dtype).to(gpu)
+        for t in (x.transpose(1, 2)[0], rows[:1, :16 * d].view(1, 16, d), rows[1:, 3:].view(1, 16, d)):
+            q, k, v = t.split([8, 4, 4], 1)
+            got = c.append(batch, k, v, q=q)
+            state = _state(c)
+            assert torch.equal(got, c.append(batch, k.clone(), v.clone(), q=q.clone())) and torch.equal(got, q.to(BF16))
+            for a, b in zip(state, _state(c)):
+                assert torch.equal(a, b)
+            q = q.to(BF16) if dtype == BF16 else got
+            assert torch.equal(c.attend(batch, q, 0.1), c.attend(batch, q.clone(memory_format=torch.contiguous_format), 0.1))
+
+
 def test_append_without_q_and_with_a_far_position(gpu):
     """Positions where an FP32 angle has lost every digit behind the point of a turn's hundredth."""
     lengths, new = [250_000, 131_071], [3, 2]

@@ -138,6 +138,23 @@ def test_wrappers_refuse_tensors_on_the_cpu_and_bad_shapes():
         token_logprobs(torch.zeros((2, 5), dtype=torch.float16), torch.zeros(2, dtype=torch.int64))
 
 
+@pytest.mark.parametrize("multiple", [4, 8])
+def test_the_distance_of_a_single_row_to_the_next_does_not_matter(multiple):
+    """torch calls [1, heads, head_dim] contiguous whatever its first stride is, and contiguous() leaves it."""
+    from se12_amd.paged import PagedKvCache
+
+    c = PagedKvCache.__new__(PagedKvCache)
+    c.head_dim, c.device, c._index = 64, torch.device("cpu"), -1
+    whole = torch.arange(8 * 64 + 3.0)
+    for x in (whole[:512].view(1, 8, 1, 64).transpose(1, 2)[0],                  # the heads of one token, transposed
+              torch.cat([whole[:513], whole[:513]]).view(2, 513)[:1, :512].view(1, 8, 64),      # a row of an odd length
+              whole[3:515].view(1, 8, 64),                                       # from an odd offset
+              whole[:512].view(8, 64).expand(1, 8, 64), whole[:64].view(1, 1, 64).expand(1, 8, 64)):
+        r = c._rows(x, "x", 8, None, None, multiple)
+        assert torch.equal(r, x) and r.stride()[1:] == (64, 1)
+        assert r.stride(0) >= 512 and r.stride(0) % multiple == 0 and r.data_ptr() % (4 * multiple) == 0
+
+
 def test_the_oracle_rounds_as_the_type_does():
     """Every E4M3 value, every midpoint between two of them and its neighbours, against torch's conversion on the CPU."""
     values = torch.arange(0, 127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
