@@ -356,7 +356,7 @@ int se12_step_paged_append(const se12_step_pages* pages, const se12_step_batch* 
     const char* fn = "se12_step_paged_append";
     if (!pages) return step_fail(fn, "NULL argument");
     if (const char* e = paged_error(pages, batch, q ? heads : pages->kv_heads)) return step_fail(fn, e);
-    if (!k || !v || (q && !q_out) || (rotary > 0 && !inv_freq)) return step_fail(fn, "NULL argument");
+    if (batch->tokens > 0 && (!k || !v || (q && !q_out) || (rotary > 0 && !inv_freq))) return step_fail(fn, "NULL argument");
     if (dtype != SE12_STEP_BF16 && dtype != SE12_STEP_F32) return step_fail(fn, "q, k and v must be BF16 or FP32");
     if (rotary < 0 || rotary > pages->head_dim || rotary % 8) return step_fail(fn, "rotary must be a multiple of 8 up to head_dim");
     const int64_t kv_row = (int64_t)pages->kv_heads * pages->head_dim;

@@ -523,7 +523,7 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
                               int32_t window, void* workspace, int64_t workspace_bytes, void* stream) {
     const char* fn = "se12_step_paged_attention";
     if (const char* e = paged_error(pages, batch, heads)) return step_fail(fn, e);
-    if (!q || !out) return step_fail(fn, "NULL argument");
+    if (batch->tokens > 0 && (!q || !out)) return step_fail(fn, "NULL argument");
     if (q_stride < (int64_t)heads * pages->head_dim || q_stride % 8) return step_fail(fn, "q rows must be a multiple of 8 elements apart and hold all heads");
     // (the cap's form holds a score to 2^-22 of the cap)
     if (!(softcap >= 0.0f) || !(softcap <= 1024.0f) || window < 0) return step_fail(fn, "softcap must be 0 to 1024 and window 0 or more");

@@ -154,6 +154,20 @@ def test_one_token_in_rows_of_any_distance(gpu):
             assert torch.equal(c.attend(batch, q, 0.1), c.attend(batch, q.clone(memory_format=torch.contiguous_format), 0.1))
 
 
+def test_calls_without_tokens(gpu):
+    for dtype in (E4M3, BF16):
+        c = _cache(gpu, 2, 16, 2, 64, dtype, 75)
+        batch, _ = _batch(gpu, [[0], [1]], [3, 0], [0, 0], max_new=1)
+        before = _state(c)
+        k, q = torch.empty((0, 2, 64), device=gpu), torch.empty((0, 8, 64), device=gpu)
+        assert c.append(batch, k, k) is None
+        assert c.append(batch, k, k, q=q).shape == (0, 8, 64) and c.attend(batch, q.to(BF16), 0.125).shape == (0, 8, 64)
+        out = torch.empty((0, 8, 64), dtype=BF16, device=gpu)
+        assert c.append(batch, k, k, q=q, out=out) is out and c.attend(batch, q.to(BF16), 0.125, out=out) is out
+        for a, b in zip(before, _state(c)):
+            assert a is b is None or torch.equal(a, b)
+
+
 def test_append_without_q_and_with_a_far_position(gpu):
     """Positions where an FP32 angle has lost every digit behind the point of a turn's hundredth."""
     lengths, new = [250_000, 131_071], [3, 2]

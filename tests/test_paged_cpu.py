@@ -112,6 +112,15 @@ def test_calls_without_tokens_or_rows_do_nothing():
     assert lib.se12_step_logprobs(None, 0, 10, 0, 10, 0.0, None, 0, None, None, None, None, None, 0, None) == 0
 
 
+def test_calls_without_tokens_need_no_memory():
+    """Tensors of no rows have no memory: NULL."""
+    lib, p, b = nat.lib(), _pages(), _batch(tokens=0)
+    for q_out in (None, P):
+        assert lib.se12_step_paged_append(ctypes.byref(p), ctypes.byref(b), None, None, None, nat.STEP_F32, 1024, 512, 512, 8, P, 128,
+                                          q_out, None) == 0
+    assert lib.se12_step_paged_attention(ctypes.byref(p), ctypes.byref(b), None, 1024, None, 8, 0.1, 0.0, 0, None, 0, None) == 0
+
+
 def test_wrappers_refuse_tensors_on_the_cpu_and_bad_shapes():
     from se12_amd.logprobs import token_logprobs
     from se12_amd.paged import PagedBatch, PagedKvCache
