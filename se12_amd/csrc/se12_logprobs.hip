@@ -1,8 +1,9 @@
 // Log probabilities of given tokens, entropy and the most likely alternatives of
-// rows of logits. Mathematics: z = cap tanh(x / cap) or x; with a reference m,
-// S = sum e^(z - m) and W = sum e^(z - m) (m - z), both of one sign, log p_i =
-// z_i - m - log S and the entropy is log S + W / S. m is a maximum met so far, or
-// up to kLpSlack below it.
+// rows of logits. Mathematics: z = cap tanh(x / cap) or x; with the maximum m met so
+// far, S = sum e^(z - m) and W = sum e^(z - m) (m - z), both of terms of one sign,
+// log p_i = z_i - m - log S and the entropy is log S + W / S. (S is 1 at least: no log p
+// is above 0, and a likely token's has the roundings of a small number. A reference of up
+// to 8 below the maximum, which moves less often, left 1e-6 in all of them and saved nothing.)
 //
 // One pass over the logits. A wave takes kChunk of them at a time, 16 to a lane,
 // the next chunk's loads in flight. Alternatives: a key per logit, its bits in an
@@ -39,7 +40,6 @@ constexpr int kMaxTop = 32;
 constexpr int kKeys = 128;                     // of a wave's buffer: 32 best and a ballot's 64 fit
 constexpr int kBlocksWanted = 1024;            // four to a CU
 constexpr int kJoinKeys = 8;                   // that a thread of the second launch loads at once
-constexpr float kLpSlack = 8.0f;
 constexpr float kLog2E = 1.4426950408889634f;
 
 // of a part of a row: the reference, S, and W in units of log 2
@@ -266,7 +266,6 @@ __global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(LogprobArgs a) 
     Best best;
     best.reset(waves.keys[wave], a.top);
     float bar = -INFINITY;                              // no logit up to it counts
-    const float slack = kLpSlack / a.unit;
     Stats v{-INFINITY, 0.0f, 0.0f};
     uint4 next[kVecs];
     auto load = [&](int at) {
@@ -346,7 +345,7 @@ __global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(LogprobArgs a) 
             }
         }
         most = y_of(a, most);
-        if (__builtin_amdgcn_ballot_w64(most > v.m + slack) != 0) v = moved(a, v, fmaxf(v.m, wave_max(most)));
+        if (__builtin_amdgcn_ballot_w64(most > v.m) != 0) v = moved(a, v, fmaxf(v.m, wave_max(most)));
         if (v.m == -INFINITY) {
             // nothing but -inf so far, unless there is a NaN
 #pragma unroll

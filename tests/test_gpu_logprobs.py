@@ -44,6 +44,12 @@ def _check(logits, tokens, top, cap):
     assert torch.equal(fine, got.isfinite()) and ((got - want).abs()[fine] <= _tol(vocab, cap, want[fine])).all()
 
 
+def _gen(seed: int) -> torch.Generator:
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return g
+
+
 def _logits(gpu, rows, vocab, dtype, seed, scale=4.0):
     g = torch.Generator()
     g.manual_seed(seed)
@@ -120,6 +126,30 @@ def test_the_best_are_zeros(gpu, dtype):
     x[2, 9_003] = -0.0
     x[2, 15_000] = 0.0
     _check(x, t, 7, 0.0)
+
+
+@pytest.mark.parametrize("rows,cap", [(400, 0.0), (1100, 0.0), (400, 30.0)])
+def test_a_peak_that_comes_late_in_a_row(gpu, rows, cap):
+    """Two logits hold the row: one in a wave's first chunk, the peak up to 8 above it in its second. The sums are S = 1 +
+    e^-gap and W = gap e^-gap on the peak's reference: a few roundings of 2^-24 each (of the sums, a term's exponent at
+    most 8 2^-23, under the cap z by 2^-21 of it), so nothing of the size of the gap's own rounding is left in results
+    near 0. None is above 0 as a logarithm, or below as an entropy."""
+    from se12_amd.logprobs import token_logprobs
+
+    gap = torch.rand(rows, generator=_gen(8)) * 8
+    x = torch.full((rows, 9007), -1e4)
+    x[:, 5], x[:, 1500] = 3.0, 3.0 + gap
+    for order in (x, x.flip(1)):
+        r = token_logprobs(order.to(gpu), order.argmax(1).to(gpu), top=2, softcap=cap)
+        z = order.double()
+        z = cap * torch.tanh(z / cap) if cap else z
+        lp = z - torch.logsumexp(z, 1, keepdim=True)
+        want, ent = lp.amax(1), torch.special.entr(lp.exp()).sum(1)
+        tol = 2.0 ** -22 + (cap * 2.0 ** -21 + 2.0 ** -20) * (1 - want.exp()) + 2.0 ** -22 * want.abs()
+        assert (r.logprobs <= 0).all() and (r.entropy >= 0).all() and (r.top_logprobs <= 0).all()
+        assert ((r.logprobs.cpu().double() - want).abs() <= tol).all()
+        assert ((r.top_logprobs[:, 0].cpu().double() - want).abs() <= tol).all()
+        assert ((r.entropy.cpu().double() - ent).abs() <= 9 * tol).all()
 
 
 def test_rows_without_a_distribution(gpu):
