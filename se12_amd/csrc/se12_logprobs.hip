@@ -41,6 +41,7 @@ constexpr int kKeys = 128;                     // of a wave's buffer: 32 best an
 constexpr int kBlocksWanted = 1024;            // four to a CU
 constexpr int kJoinKeys = 8;                   // that a thread of the second launch loads at once
 constexpr float kLog2E = 1.4426950408889634f;
+constexpr float kFineCap = 64.0f;
 
 // of a part of a row: the reference, S, and W in units of log 2
 struct Stats {
@@ -157,8 +158,13 @@ struct Best {
 
 // What is summed: z = unit y + a constant, y = -1 / (1 + e^(2 x / cap)) under a cap (z =
 // cap + 2 cap y), else x. Differences of y are taken before the unit, so what two logits
-// close to each other, or one and itself, have in common leaves no rounding behind.
+// close to each other, or one and itself, have in common leaves no rounding behind. That
+// y is off by 2^-24 wherever x lies, z by 2^-22 of the cap: under one of 64 no more than
+// twice what FP32 leaves of logits near it. Under a larger one (z = 2 cap y) y is half the
+// hyperbolic tangent, whose error is of its own size.
+template <bool kFine>
 __device__ __forceinline__ float y_of(const LogprobArgs& a, float x) {
+    if constexpr (kFine) return 0.5f * tanhf(x * a.inv_cap2 * (0.5f / kLog2E));
     return a.cap > 0.0f ? -__builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * a.inv_cap2)) : x;
 }
 
@@ -187,10 +193,11 @@ __device__ __forceinline__ bool token_logit(const LogprobArgs& a, int row, float
 }
 
 // the row's results, by one wave, from its sums and its best keys in order
+template <bool kFine>
 __device__ __forceinline__ void finish_row(const LogprobArgs& a, int row, Stats v, const Best& best, bool valid, float x) {
     const int lane = threadIdx.x & 63;
     const float log_s = logf(v.s);
-    auto logprob = [&](float x) { return v.m == -INFINITY && v.s == 0.0f ? -INFINITY : (y_of(a, x) - v.m) * a.unit - log_s; };
+    auto logprob = [&](float x) { return v.m == -INFINITY && v.s == 0.0f ? -INFINITY : (y_of<kFine>(a, x) - v.m) * a.unit - log_s; };
     if (lane == 0) {
         // (a token that there is not: -inf, in a row of numbers)
         const float lp = valid ? logprob(x) : v.s != v.s ? v.s : -INFINITY;
@@ -246,8 +253,8 @@ __device__ __forceinline__ bool join_waves(const LogprobArgs& a, Stats& v, Best&
     return true;
 }
 
-template <int DT>
-__global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(LogprobArgs a) {
+template <int DT, bool kFine>
+__global__ __launch_bounds__(kLpThreads, kFine ? 2 : 6) void logprobs_kernel(LogprobArgs a) {
     constexpr int kVec = DT == SE12_STEP_F32 ? 4 : 8, kVecs = kLpPer / kVec, kSize = 16 / kVec;
     __shared__ Waves waves;
     __shared__ float held[kLpWaves][kChunk];
@@ -344,7 +351,7 @@ __global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(LogprobArgs a) 
                 bar = best.bar_number();
             }
         }
-        most = y_of(a, most);
+        most = y_of<kFine>(a, most);
         if (__builtin_amdgcn_ballot_w64(most > v.m) != 0) v = moved(a, v, fmaxf(v.m, wave_max(most)));
         if (v.m == -INFINITY) {
             // nothing but -inf so far, unless there is a NaN
@@ -355,7 +362,7 @@ __global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(LogprobArgs a) 
             auto add = [&](auto at_edge) {
 #pragma unroll
                 for (int k = 0; k < kLpPer; ++k) {
-                    float d = (v.m - y_of(a, x[k])) * a.unit2;
+                    float d = (v.m - y_of<kFine>(a, x[k])) * a.unit2;
                     if (at_edge.value && outside(k)) d = 1e30f;
                     const float e = __builtin_amdgcn_exp2f(-d);
                     v.s += e;
@@ -377,7 +384,7 @@ __global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(LogprobArgs a) 
     }
     if (!join_waves(a, v, best, waves)) return;
     if (a.slices == 1) {
-        finish_row(a, row, v, best, valid, token_x);
+        finish_row<kFine>(a, row, v, best, valid, token_x);
         return;
     }
     if (lane == 0) a.stats[blockIdx.x] = v;
@@ -385,7 +392,7 @@ __global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(LogprobArgs a) 
 }
 
 // the slices of a row
-template <int DT>
+template <int DT, bool kFine>
 __global__ __launch_bounds__(kLpThreads) void logprobs_join_kernel(LogprobArgs a) {
     __shared__ Waves waves;
     __shared__ uint64_t held[kLpWaves][kJoinKeys * 64];
@@ -430,7 +437,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_join_kernel(LogprobArgs a
             best.offer(i < count ? keys[i] : 0);
         }
     }
-    if (join_waves(a, v, best, waves)) finish_row(a, row, v, best, valid, token_x);
+    if (join_waves(a, v, best, waves)) finish_row<kFine>(a, row, v, best, valid, token_x);
 }
 
 }  // namespace se12step
@@ -459,6 +466,12 @@ LpLayout logprobs_layout(int32_t rows, int32_t vocab, int32_t top) {
     return l;
 }
 
+template <int DT, bool kFine>
+void launch_logprobs(const LogprobArgs& a, dim3 grid, int rows, hipStream_t st) {
+    hipLaunchKernelGGL((logprobs_kernel<DT, kFine>), grid, dim3(kLpThreads), 0, st, a);
+    if (a.slices > 1) hipLaunchKernelGGL((logprobs_join_kernel<DT, kFine>), dim3(rows), dim3(kLpThreads), 0, st, a);
+}
+
 const char* logprobs_shape_error(int32_t rows, int32_t vocab, int32_t top) {
     if (rows < 0 || vocab < 1 || vocab > (1 << 30)) return "bad shape";
     if (top < 0 || top > kMaxTop || top > vocab) return "top must be 0 to 32 and at most vocab";
@@ -483,7 +496,6 @@ int se12_step_logprobs(const void* logits, int32_t dtype, int64_t stride, int32_
     if (!logits || !tokens || !logprobs || !entropy || (top > 0 && (!top_logprobs || !top_ids))) return step_fail(fn, "NULL argument");
     if (dtype != SE12_STEP_BF16 && dtype != SE12_STEP_F32) return step_fail(fn, "logits must be BF16 or FP32");
     if (stride < vocab) return step_fail(fn, "rows overlap");
-    // (the cap's form holds z to 2^-22 of the cap)
     if (!(softcap >= 0.0f) || !(softcap <= 1024.0f)) return step_fail(fn, "softcap must be 0 to 1024");
     if (reinterpret_cast<uintptr_t>(logits) % (dtype == SE12_STEP_F32 ? 4 : 2) || reinterpret_cast<uintptr_t>(tokens) % 8 ||
         reinterpret_cast<uintptr_t>(logprobs) % 4 || reinterpret_cast<uintptr_t>(entropy) % 4 ||
@@ -499,13 +511,11 @@ int se12_step_logprobs(const void* logits, int32_t dtype, int64_t stride, int32_
                         reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + (l.slices > 1 ? l.stats_bytes : 0))};
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const dim3 grid((uint32_t)((int64_t)rows * l.slices));
-    if (dtype == SE12_STEP_F32) {
-        hipLaunchKernelGGL(logprobs_kernel<SE12_STEP_F32>, grid, dim3(kLpThreads), 0, st, a);
-        if (l.slices > 1) hipLaunchKernelGGL(logprobs_join_kernel<SE12_STEP_F32>, dim3(rows), dim3(kLpThreads), 0, st, a);
-    } else {
-        hipLaunchKernelGGL(logprobs_kernel<SE12_STEP_BF16>, grid, dim3(kLpThreads), 0, st, a);
-        if (l.slices > 1) hipLaunchKernelGGL(logprobs_join_kernel<SE12_STEP_BF16>, dim3(rows), dim3(kLpThreads), 0, st, a);
-    }
+    const bool fine = softcap > kFineCap;
+    if (dtype == SE12_STEP_F32)
+        fine ? launch_logprobs<SE12_STEP_F32, true>(a, grid, rows, st) : launch_logprobs<SE12_STEP_F32, false>(a, grid, rows, st);
+    else
+        fine ? launch_logprobs<SE12_STEP_BF16, true>(a, grid, rows, st) : launch_logprobs<SE12_STEP_BF16, false>(a, grid, rows, st);
     return step_launched();
 }
 

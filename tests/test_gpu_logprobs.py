@@ -80,6 +80,25 @@ def test_the_largest_cap(gpu):
     _check(x, t, 6, 1024.0)
 
 
+@pytest.mark.parametrize("rows,vocab", [(3, 5000), (2, 40_007), (1100, 2111)])
+@pytest.mark.parametrize("cap", [65.0, 300.0, 1024.0])
+def test_a_large_cap_leaves_small_logits_their_digits(gpu, cap, rows, vocab):
+    """z is off by a few units of 2^-24 of itself (the quotient, a hyperbolic tangent good to 2 units, the product), not
+    of the cap: logits of up to 8 here, so 2^-24 * 4 * 8 = 2^-19 beside the sums' own roundings."""
+    from se12_amd.logprobs import token_logprobs
+
+    x, t = _logits(gpu, rows, vocab, torch.float32, 9, scale=1.5)
+    x = x.clamp(-8, 8)
+    r = token_logprobs(x, t, top=3, softcap=cap)
+    z = cap * torch.tanh(x.cpu().double() / cap)
+    lp = z - torch.logsumexp(z, 1, keepdim=True)
+    want, ent = lp.gather(1, t.cpu()[:, None])[:, 0], torch.special.entr(lp.exp()).sum(1)
+    tol = lambda size: _tol(vocab, 0.0, size) + 2.0 ** -18      # noqa: E731  (of a logit and of those in the sum)
+    assert ((r.logprobs.cpu().double() - want).abs() <= tol(want)).all()
+    assert ((r.top_logprobs.cpu().double() - lp.gather(1, r.top_ids.cpu())).abs() <= tol(lp.gather(1, r.top_ids.cpu()))).all()
+    assert ((r.entropy.cpu().double() - ent).abs() <= 2 * (1 + math.log(vocab)) * tol(ent)).all()
+
+
 def test_more_rows_than_blocks_fill_the_card(gpu):
     x, t = _logits(gpu, 1500, 2100, torch.bfloat16, 2)
     _check(x, t, 3, 0.0)
