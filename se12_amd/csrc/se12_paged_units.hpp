@@ -73,7 +73,7 @@ __device__ __forceinline__ int shared_tiles(const AttendArgs& a, int lane, int r
     int64_t all = 0;
     for (int s0 = 0; s0 < a.b.seqs; s0 += 64) {
         const UnitCounts c = load_counts(a, s0, lane, capacity);
-        const int last = c.keys, first = min(c.seq.len + kBlockColumns / a.group, last), reach = a.window > 0 ? a.window + kTile : INT32_MAX;
+        const int last = c.keys, first = min(c.seq.len + kBlockColumns / a.group, last), reach = a.window > 0 ? min(a.window, INT32_MAX - kTile) + kTile : INT32_MAX;
         // (a float holds it closely enough, and is the same for every block)
         all += wave_total((int)fminf((float)c.units * (float)(min(first, reach) / 2 + min(last, reach) / 2) / kTile, 1e7f));
     }

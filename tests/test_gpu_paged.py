@@ -376,6 +376,14 @@ def test_parts_of_a_units_keys_under_a_window(gpu, dtype, d, window):
 
 
 @pytest.mark.parametrize("dtype", [E4M3, BF16])
+@pytest.mark.parametrize("heads,kvh,lengths,new", [(4, 1, [2600, 900], [70, 35]), (4, 2, [300, 70], [1, 1])])
+def test_a_window_of_the_largest_number_hides_nothing(gpu, dtype, heads, kvh, lengths, new):
+    c, batch, q, out = _attend_case(gpu, dtype, 64, 32, heads, kvh, lengths, new, 0.0, 2 ** 31 - 1, seed=67, extra=0)
+    for window in (0, 2 ** 31 - 40, 1 << 30):
+        assert torch.equal(c.attend(batch, q, 64 ** -0.5, window=window), out)
+
+
+@pytest.mark.parametrize("dtype", [E4M3, BF16])
 def test_more_query_heads_to_one_than_columns_of_a_block(gpu, dtype):
     _attend_case(gpu, dtype, 64, 16, 160, 1, [100, 5, 0], [1, 3, 1], 0.0, 0, seed=62)
     _attend_case(gpu, dtype, 64, 16, 80, 1, [300, 5], [1, 2], 0.0, 70, seed=63)
