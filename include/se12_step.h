@@ -162,8 +162,9 @@ typedef struct se12_step_batch {
 
 /* Appends k and v [tokens, kv_heads, head_dim] to the cache, k rotated to its
  * position, and writes the rotated q [tokens, heads, head_dim] to q_out (BF16,
- * contiguous; q itself where that is both); q may be NULL, then nothing is. Rows `q_stride`, `k_stride`,
- * `v_stride` elements apart (multiples of 4), heads of a row side by side; dtype
+ * contiguous; q itself where that is both, else apart from q, and apart from k and
+ * v); q may be NULL, then nothing is. Rows `q_stride`, `k_stride`, `v_stride`
+ * elements apart (multiples of 4), heads of a row side by side; dtype
  * SE12_STEP_BF16 or SE12_STEP_F32 for all three, aligned to four elements. The
  * rotation takes the pair (x[i], x[i + rotary / 2]) by position * inv_freq[i],
  * i < rotary / 2 (the angle in 64 bits, the rest in FP32); elements from

@@ -368,6 +368,15 @@ int se12_step_paged_append(const se12_step_pages* pages, const se12_step_batch* 
         reinterpret_cast<uintptr_t>(q_out) % 8 || reinterpret_cast<uintptr_t>(inv_freq) % 16)
         return step_fail(fn, "misaligned tensor");
     if (batch->tokens == 0) return SE12_STEP_OK;
+    if (q) {
+        // (blocks read and write in any order: only a value of q may be written over, by itself)
+        const int64_t q_row = (int64_t)heads * pages->head_dim, more = batch->tokens - 1, size = dtype == SE12_STEP_F32 ? 4 : 2;
+        const int64_t out_bytes = 2 * (more + 1) * q_row;
+        const bool itself = q == q_out && dtype == SE12_STEP_BF16 && (more == 0 || q_stride == q_row);
+        if ((!itself && overlap(q, size * (more * q_stride + q_row), q_out, out_bytes)) ||
+            overlap(k, size * (more * k_stride + kv_row), q_out, out_bytes) || overlap(v, size * (more * v_stride + kv_row), q_out, out_bytes))
+            return step_fail(fn, "q_out overlaps k, v or other values of q");
+    }
     AppendArgs a{q, k, v, q_stride, k_stride, v_stride, pages->k, pages->v, pages->k_scale, pages->v_scale, inv_freq, q_out,
                  device_batch(batch), 0, q ? heads : 0, pages->kv_heads, pages->pages,
                  log2_of(pages->page_size), pages->head_dim, rotary / 2};

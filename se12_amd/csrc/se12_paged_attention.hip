@@ -536,8 +536,7 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
         return step_fail(fn, "workspace missing, misaligned or too small");
     // (q is read until the last wave is done with it)
     const int64_t row = (int64_t)heads * pages->head_dim;
-    if (reinterpret_cast<uintptr_t>(q) < reinterpret_cast<uintptr_t>(out + b.tokens * row) &&
-        reinterpret_cast<uintptr_t>(out) < reinterpret_cast<uintptr_t>(q + (b.tokens - 1) * q_stride + row))
+    if (overlap(q, 2 * ((b.tokens - 1) * q_stride + row), out, 2 * b.tokens * row))
         return step_fail(fn, "out overlaps q");
     constexpr float kLog2E = 1.4426950408889634f;
     AttendArgs a{q, q_stride, out, pages->k, pages->v, pages->k_scale, pages->v_scale, b, heads, pages->kv_heads, group, pages->pages,

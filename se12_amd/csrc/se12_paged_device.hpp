@@ -169,6 +169,12 @@ inline Batch device_batch(const se12_step_batch* b) {
             b->table_width, b->sequences,   b->tokens, b->max_new < b->tokens ? b->max_new : b->tokens};
 }
 
+// host: whether `a_bytes` from a and `b_bytes` from b have a byte in common
+inline bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
+}
+
 // se12_paged_prompt.hip
 bool prompt_fits(const Batch& b, int kvh, int group, int page_size);
 int prompt_splits(const Batch& b, int kvh, int group, int page_size);

@@ -174,10 +174,11 @@ class PagedKvCache:
     def append(self, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,
                inv_freq: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor | None:
         """Writes the new tokens' k and v [tokens, kv_heads, head_dim] to their pages, k rotated to its position, and
-        returns q [tokens, heads, head_dim] rotated, in BF16 (into `out` if given, which may be q; None without q). BF16 or FP32, all
-        of one type; rows may be strided (views of one product's output). The rotation turns the pairs (i, i +
-        len(inv_freq)) by position * inv_freq[i], FP32 inv_freq of up to head_dim / 2 frequencies, a multiple of 4 (the
-        elements behind the pairs stay; None: no rotation), as se12_step_prefill_attention pairs them.
+        returns q [tokens, heads, head_dim] rotated, in BF16 (into `out` if given, which may be q, or shares no memory with
+        q, k and v; None without q). BF16 or FP32, all of one type; rows may be strided (views of one product's output).
+        The rotation turns the pairs (i, i + len(inv_freq)) by position * inv_freq[i], FP32 inv_freq of up to head_dim / 2
+        frequencies, a multiple of 4 (the elements behind the pairs stay; None: no rotation), as
+        se12_step_prefill_attention pairs them.
 
         An E4M3 page and head's scale is the least power of two (2^-100 or more) that holds its new values; with older
         tokens in the page at least what it was, and if it grows the older ones are rounded again. NaN and infinities

@@ -63,6 +63,24 @@ def test_append_refuses(change, message):
         nat.step_check(nat.lib().se12_step_paged_append(ctypes.byref(_pages()), ctypes.byref(_batch()), *f.values(), None))
 
 
+Q = 16 * P     # 3 rows of 8 heads of 128, in BF16 6,144 bytes
+
+
+@pytest.mark.parametrize("change", [
+    dict(dtype=nat.STEP_F32, q_out=Q),                                   # of another type than q
+    dict(q_out=Q + 8), dict(q_out=Q - 8), dict(q_out=Q + 6136), dict(q_out=Q - 6136),
+    dict(qs=2048, q_out=Q),                                              # q's rows apart, the output's not
+    dict(dtype=nat.STEP_F32, q_out=Q + 12280), dict(k=Q + 16 * P, q_out=Q + 16 * P + 3064), dict(v=Q + 16 * P, q_out=Q + 16 * P - 6136),
+    dict(k=Q, ks=4096),
+])
+def test_append_refuses_an_output_over_its_inputs(change):
+    """Blocks read and write in any order, so only q itself, value for value, may be written over."""
+    f = dict(q=Q, k=2 * Q, v=3 * Q, dtype=nat.STEP_BF16, qs=1024, ks=512, vs=512, heads=8, inv=P, rotary=128, q_out=Q)
+    f.update(change)
+    with pytest.raises(nat.Se12Error, match="overlaps"):
+        nat.step_check(nat.lib().se12_step_paged_append(ctypes.byref(_pages()), ctypes.byref(_batch()), *f.values(), None))
+
+
 @pytest.mark.parametrize("change,message", [
     (dict(q=None), "NULL"), (dict(out=None), "NULL"), (dict(qs=1016), "hold all heads"), (dict(qs=1028), "multiple of 8"),
     (dict(cap=-1.0), "softcap"), (dict(cap=float("nan")), "softcap"), (dict(cap=1025.0), "softcap"),
