@@ -34,12 +34,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, sof
     on the current stream of the logits' device and never waits for it; no gradients."""
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("logits must be a bfloat16 or float32 [rows, vocab] tensor")
+    rows, vocab = logits.shape
+    if not 1 <= vocab <= 2 ** 30 or rows >= 2 ** 31:
+        raise ValueError(f"logits must have 1 to 2^30 columns and below 2^31 rows, got {list(logits.shape)}")
     if not logits.is_cuda:
         raise ValueError("expected a tensor on a HIP device")
     dev = logits.device
-    rows, vocab = logits.shape
-    if vocab < 1:
-        raise ValueError("logits must have a column")
     if not isinstance(tokens, torch.Tensor) or tokens.dtype != torch.int64 or tuple(tokens.shape) != (rows,) or tokens.device != dev:
         raise ValueError(f"tokens must be an int64 [{rows}] tensor on {dev}")
     if int(top) != top or not 0 <= top <= min(MAX_TOP, vocab):

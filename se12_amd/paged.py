@@ -65,15 +65,15 @@ class PagedBatch:
     def __init__(self, page_table: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor, max_new: int = 1) -> None:
         if not isinstance(page_table, torch.Tensor) or page_table.dtype != torch.int32 or page_table.dim() != 2:
             raise ValueError("page_table must be an int32 [sequences, columns] tensor")
-        if not page_table.is_cuda:
-            raise ValueError("page_table must be on a HIP device")
         n, width = page_table.shape
-        if not 1 <= n <= 65536 or width < 1:
-            raise ValueError(f"page_table must have 1 to 65536 rows and a column, got {list(page_table.shape)}")
+        if not 1 <= n <= 65536 or not 1 <= width <= 2 ** 30:
+            raise ValueError(f"page_table must have 1 to 65536 rows and 1 to 2^30 columns, got {list(page_table.shape)}")
         if page_table.stride(1) != 1 and width > 1 or n > 1 and page_table.stride(0) < width:
             raise ValueError("page_table's rows must be contiguous and not overlap")
-        if int(max_new) < 1:
-            raise ValueError("max_new must be at least 1")
+        if int(max_new) != max_new or not 1 <= max_new < 2 ** 31:
+            raise ValueError(f"max_new must be a whole number from 1 to 2^31 - 1, got {max_new}")
+        if not page_table.is_cuda:
+            raise ValueError("page_table must be on a HIP device")
         self.device = page_table.device
         self.page_table = page_table
         self.lengths = _int32(lengths, "lengths", (n,), self.device)
@@ -88,6 +88,8 @@ class PagedBatch:
         """The C struct of a call with so many rows, by reference; the layers of a step share it."""
         last = self._last
         if last[0] != tokens:
+            if tokens >= 2 ** 31:
+                raise ValueError(f"a call holds below 2^31 tokens, got {tokens}")
             last = self._last = (tokens, ctypes.byref(nat.StepBatch(*self._fields, tokens, self.max_new)))
         return last[1]
 
@@ -253,6 +255,8 @@ class PagedKvCache:
     def attend_workspace(self, batch: PagedBatch, tokens: int, heads: int) -> int:
         """Bytes of `attend`'s workspace."""
         self._check(batch)
+        if not 0 <= tokens < 2 ** 31 or not 0 < heads < 2 ** 31:
+            raise ValueError(f"tokens and heads must be below 2^31, got {tokens}, {heads}")
         n = nat.lib().se12_step_paged_attention_workspace(self._struct, batch._struct(tokens), heads)
         if n < 0:
             nat.step_check(n)

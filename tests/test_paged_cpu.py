@@ -182,6 +182,36 @@ def test_the_distance_of_a_single_row_to_the_next_does_not_matter(multiple):
         assert r.stride(0) >= 512 and r.stride(0) % multiple == 0 and r.data_ptr() % (4 * multiple) == 0
 
 
+@pytest.mark.parametrize("max_new", [0, -1, 1.5, 2 ** 31, 2 ** 32 + 1])
+def test_a_batch_refuses_a_max_new_that_32_bits_or_whole_numbers_do_not_hold(max_new):
+    from se12_amd.paged import PagedBatch
+
+    i32 = torch.zeros((2, 3), dtype=torch.int32)
+    with pytest.raises(ValueError, match="max_new"):
+        PagedBatch(i32, i32[0, :2], i32[0], max_new=max_new)
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """Not cut to their low 32 bits on the way to the C entries (tensors without memory)."""
+    from se12_amd.logprobs import token_logprobs
+    from se12_amd.paged import PagedBatch, PagedKvCache
+
+    table = torch.empty((1, 2 ** 32 + 1), dtype=torch.int32, device="meta")
+    with pytest.raises(ValueError, match="columns"):
+        PagedBatch(table, torch.zeros(1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32))
+    for shape in ((1, 2 ** 32 + 5), (2 ** 32 + 1, 1), (1, 2 ** 30 + 1)):
+        with pytest.raises(ValueError, match="2\\^30"):
+            token_logprobs(torch.empty(shape, device="meta"), torch.empty(shape[0], dtype=torch.int64, device="meta"))
+    batch = PagedBatch.__new__(PagedBatch)
+    batch.device, batch.max_new, batch._fields, batch._last = torch.device("cpu"), 1, (P, 8, P, P, 8, 3), (-1, None)
+    c = PagedKvCache.__new__(PagedKvCache)
+    c.device, c._struct = batch.device, ctypes.byref(_pages())
+    assert c.attend_workspace(batch, 3, 8) > 0
+    for tokens, heads in ((2 ** 32 + 3, 8), (3, 2 ** 32 + 8), (2 ** 31, 8)):
+        with pytest.raises(ValueError, match="tokens"):
+            c.attend_workspace(batch, tokens, heads)
+
+
 def test_the_oracle_rounds_as_the_type_does():
     """Every E4M3 value, every midpoint between two of them and its neighbours, against torch's conversion on the CPU."""
     values = torch.arange(0, 127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
