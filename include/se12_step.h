@@ -192,8 +192,8 @@ int se12_step_paged_append(const se12_step_pages* pages, const se12_step_batch* 
  * from q. heads a multiple of kv_heads. What a query may not see has no part in its row,
  * whatever it holds (NaN too); a query that sees nothing gives zeros.
  *
- * `workspace`: se12_step_paged_attention_workspace() bytes for the shape,
- * 256-byte aligned, contents indifferent; calls sharing it (two captured graphs
+ * `workspace`: se12_step_paged_attention_workspace() bytes for the shape (or for
+ * one of more tokens), 256-byte aligned, contents indifferent; calls sharing it (two captured graphs
  * too) must not run concurrently. Two launches, four where max_new allows a
  * sequence more than 64 (token, query head) pairs to a KV head; results do not
  * depend on timing. */

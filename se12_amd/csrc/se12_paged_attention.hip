@@ -30,7 +30,6 @@
 namespace se12step {
 
 constexpr int kColumns = 16;          // columns of a unit
-constexpr int kFewColumns = 64;       // of a sequence and KV head; with more it is se12_paged_prompt.hip's
 // waves of a launch: one per SIMD of 256 CUs (3 x 65,000 keys, 28 / 4 heads of 128: 31.5
 // us, 36 with two, which have two starts and twice the parts to join)
 constexpr int kWorkersLog2 = 10, kWorkers = 1 << kWorkersLog2;
@@ -55,7 +54,7 @@ __device__ __forceinline__ SeqWork seq_work(const AttendArgs& a, Seq seq) {
     const int low = a.window > 0 ? max(0, seq.len - a.window + 1) : 0;
     w.tile0 = low / kTile;
     const int columns = seq.n * a.group;
-    w.units = columns > a.few ? 0 : (columns + kColumns - 1) / kColumns;
+    w.units = columns > kFewColumns ? 0 : (columns + kColumns - 1) / kColumns;
     w.tiles = w.units > 0 ? max((w.keys + kTile - 1) / kTile - w.tile0, 1) : 0;
     return w;
 }
@@ -311,7 +310,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : 2) void paged_attent
     const int worker = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * (kAttendThreads / 64) + (threadIdx.x >> 6)));
     // (workers come four to a block; behind them waves for the units of se12_paged_prompt.hip)
     if (worker >= a.workers) {
-        if (worker - a.workers < a.unit_count) write_unit<CT, D>(a, worker - a.workers);
+        if (worker - a.workers < a.unit_count + a.join_count) write_unit<CT, D>(a, worker - a.workers);
         return;
     }
     Chunk chunk = load_chunk<kTile>(a, 0, lane);
@@ -478,27 +477,30 @@ int64_t few_bytes(const se12_step_pages* p, const Batch& b, int group) {
     return ((int64_t)worker_count(p, b, group) * 2 * column_count(b, group) * (p->head_dim + 2) * (int64_t)sizeof(float) + 255) / 256 * 256;
 }
 
-bool any_many(const Batch& b, int group) { return (int64_t)b.max_new * group > kFewColumns; }
+PromptPlan plan_of(const se12_step_pages* p, const Batch& b, int group) {
+    if ((int64_t)b.max_new * group <= kFewColumns) return {};
+    return prompt_plan(b, p->kv_heads, group, p->page_size, p->head_dim, p->dtype == SE12_STEP_E4M3);
+}
 
 // what one launch holds, and what 32 bits hold of it
 const char* limits_error(const se12_step_pages* p, const Batch& b, int group) {
-    if ((int64_t)b.seqs * p->kv_heads * (kFewColumns / kColumns) > INT32_MAX || !prompt_fits(b, p->kv_heads, group, p->page_size))
+    if ((int64_t)b.seqs * p->kv_heads * (kFewColumns / kColumns) > INT32_MAX || (int64_t)b.tokens * group > INT32_MAX ||
+        plan_of(p, b, group).records * p->kv_heads > INT32_MAX)
         return "too many sequences, tokens and heads for one launch";
     if (std::min<int64_t>(b.seqs, 64) * (((int64_t)b.width * p->page_size + 31) / 32) * (kFewColumns / kColumns) * p->kv_heads > INT32_MAX)
         return "too long a table for so many sequences and heads";
     return nullptr;
 }
 
-int64_t part_bytes(const se12_step_pages* p, const Batch& b, int group) {
-    if (!any_many(b, group)) return few_bytes(p, b, group);
-    return few_bytes(p, b, group) + prompt_unit_bytes(b, p->kv_heads, group, p->page_size) +
-           prompt_part_bytes(b, p->kv_heads, group, p->page_size, p->head_dim);
+int64_t all_bytes(const se12_step_pages* p, const Batch& b, int group) {
+    const PromptPlan x = plan_of(p, b, group);
+    return few_bytes(p, b, group) + x.record_bytes + x.part_bytes;
 }
 
 template <int CT, int D>
 void launch_attend(const AttendArgs& a, hipStream_t st) {
     constexpr int kWaves = kAttendThreads / 64;
-    hipLaunchKernelGGL((paged_attention_kernel<CT, D>), dim3((uint32_t)(((int64_t)a.workers + a.unit_count + kWaves - 1) / kWaves)),
+    hipLaunchKernelGGL((paged_attention_kernel<CT, D>), dim3((uint32_t)(((int64_t)a.workers + a.unit_count + a.join_count + kWaves - 1) / kWaves)),
                        dim3(kAttendThreads), 0, st, a);
     const int max_units = (int)((std::min<int64_t>((int64_t)a.b.max_new * a.group, kFewColumns) + kColumns - 1) / kColumns);
     hipLaunchKernelGGL((paged_join_kernel<CT, D>), dim3((uint32_t)((int64_t)a.b.seqs * a.kvh * max_units), max_units > 1 ? 4 : a.columns),
@@ -515,7 +517,7 @@ int64_t se12_step_paged_attention_workspace(const se12_step_pages* pages, const 
     if (batch->tokens == 0) return 0;
     const Batch b = device_batch(batch);
     if (const char* e = limits_error(pages, b, heads / pages->kv_heads)) return step_fail(fn, e);
-    return part_bytes(pages, b, heads / pages->kv_heads);
+    return all_bytes(pages, b, heads / pages->kv_heads);
 }
 
 int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batch* batch, const uint16_t* q,
@@ -532,19 +534,19 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
     const Batch b = device_batch(batch);
     const int group = heads / pages->kv_heads;
     if (const char* e = limits_error(pages, b, group)) return step_fail(fn, e);
-    if (reinterpret_cast<uintptr_t>(workspace) % 256 || !workspace || workspace_bytes < part_bytes(pages, b, group))
+    if (reinterpret_cast<uintptr_t>(workspace) % 256 || !workspace || workspace_bytes < all_bytes(pages, b, group))
         return step_fail(fn, "workspace missing, misaligned or too small");
     // (q is read until the last wave is done with it)
     const int64_t row = (int64_t)heads * pages->head_dim;
     if (overlap(q, 2 * ((b.tokens - 1) * q_stride + row), out, 2 * b.tokens * row))
         return step_fail(fn, "out overlaps q");
     constexpr float kLog2E = 1.4426950408889634f;
+    const PromptPlan plan = plan_of(pages, b, group);
     AttendArgs a{q, q_stride, out, pages->k, pages->v, pages->k_scale, pages->v_scale, b, heads, pages->kv_heads, group, pages->pages,
                  log2_of(pages->page_size), window, softcap > 0.0f ? 2.0f * scaling / softcap * kLog2E : scaling * kLog2E,
-                 softcap * kLog2E, static_cast<float*>(workspace), worker_count(pages, b, group), column_count(b, group), kFewColumns,
-                 prompt_splits(b, pages->kv_heads, group, pages->page_size),
+                 softcap * kLog2E, static_cast<float*>(workspace), worker_count(pages, b, group), column_count(b, group),
                  reinterpret_cast<UnitWork*>(static_cast<char*>(workspace) + few_bytes(pages, b, group)),
-                 any_many(b, group) ? prompt_units(b, pages->kv_heads, group, pages->page_size) : 0};
+                 (int)plan.slots + plan.parts, plan.parts / 2, plan.parts, plan.most};
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const bool e4m3 = pages->dtype == SE12_STEP_E4M3;
     switch (pages->head_dim) {
@@ -557,9 +559,8 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
         default:
             e4m3 ? launch_attend<SE12_STEP_E4M3, 256>(a, st) : launch_attend<SE12_STEP_BF16, 256>(a, st);
     }
-    if (any_many(b, group)) {
-        a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + few_bytes(pages, b, group) +
-                                          prompt_unit_bytes(b, pages->kv_heads, group, pages->page_size));
+    if (plan.records > 0) {
+        a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(a.units) + plan.record_bytes);
         launch_prompt(a, e4m3, pages->head_dim, st);
     }
     return step_launched();

@@ -58,10 +58,12 @@ struct AttendArgs {
     float c1, cap;       // scores: c1 x (no cap), or cap - 2 cap / (1 + 2^(c1 x)), base 2
     float* part;         // sums of a part of a unit's keys, then their (m, l)
     int workers, columns;
-    int few;             // sequences of more columns are se12_paged_prompt.hip's
-    int splits;          // there: blocks that may share a unit's keys
-    struct UnitWork* units;   // and what its blocks are to do, `unit_count` of them
-    int unit_count;
+    // sequences of more than kFewColumns columns are se12_paged_prompt.hip's: what its
+    // blocks are to do, and the blocks that join parts (se12_paged_units.hpp)
+    struct UnitWork* units;
+    int unit_count, join_count;
+    int parts;           // blocks of a KV head that may hold parts of a unit's keys, 0 for none
+    int most;            // parts of a unit, at most
 };
 
 // What a lane holds of a tile, by the cache's type: 16 bytes of each key row's
@@ -175,12 +177,13 @@ inline bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_byt
     return x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
 }
 
-// se12_paged_prompt.hip
-bool prompt_fits(const Batch& b, int kvh, int group, int page_size);
-int prompt_splits(const Batch& b, int kvh, int group, int page_size);
-int prompt_units(const Batch& b, int kvh, int group, int page_size);
-int64_t prompt_unit_bytes(const Batch& b, int kvh, int group, int page_size);
-int64_t prompt_part_bytes(const Batch& b, int kvh, int group, int page_size, int d);
+// se12_paged_prompt.hip: what a call can have of it
+struct PromptPlan {
+    int64_t slots;               // units of a KV head, at most
+    int parts, most;             // as AttendArgs
+    int64_t records, record_bytes, part_bytes;
+};
+PromptPlan prompt_plan(const Batch& b, int kvh, int group, int page_size, int d, bool e4m3);
 void launch_prompt(const AttendArgs& a, bool e4m3, int d, hipStream_t st);
 
 inline int log2_of(int n) { return 31 - __builtin_clz((unsigned)n); }

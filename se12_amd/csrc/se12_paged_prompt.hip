@@ -465,8 +465,8 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
     se12::wait_vector_loads();      // (before this block's LDS is another's)
     l += __shfl_xor(l, 32, 64);
     if (u.parts > 1) {
-        // the part of (unit, head, split), as the lanes hold it
-        const int64_t p = ((int64_t)u.rank * a.kvh + kh) * a.splits + u.split;
+        // the part, as the lanes hold it
+        const int64_t p = part_place(a, u, kh);
         float4* to = reinterpret_cast<float4*>(a.part + p * kBlockColumns * D) + wave * (D / 8) * 64 + lane;
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
@@ -474,7 +474,7 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
             for (int g = 0; g < 4; ++g)
                 to[(4 * i + g) * 64] = make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
         if (half == 0)
-            reinterpret_cast<float2*>(a.part + (int64_t)gridDim.x * kBlockColumns * D)[p * kBlockColumns + wave * kWaveColumns + col] =
+            reinterpret_cast<float2*>(a.part + (int64_t)a.parts * a.kvh * kBlockColumns * D)[p * kBlockColumns + wave * kWaveColumns + col] =
                 make_float2(m, l);
         return;
     }
@@ -507,22 +507,26 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
 // Units whose keys were split, from their parts in order: a wave has the columns of one
 // of the unit's waves, and every kJoinBlocks-th of its lanes' pieces.
 // (Of each unit 2 pieces at D = 256: 16 units of 16 parts, 34 MB, 45 us with 4 blocks a unit.)
+// The blocks of a unit and head, which write pieces of the same lines, are 8 apart and so
+// on one XCD. (One after the other, 2,000 and 1,500 tokens, 8 heads of 64: 64 us the call,
+// 60 so; all units' first blocks in front: one unit of 64 parts 120 us, 88 so, as blocks
+// that find nothing lie between.)
 template <int D>
 constexpr int kJoinBlocks = D / 16;
 
 template <int CT, int D>
-__global__ __launch_bounds__(kPromptThreads) void paged_prompt_join_kernel(AttendArgs a, int64_t parts) {
+__global__ __launch_bounds__(kPromptThreads) void paged_prompt_join_kernel(AttendArgs a) {
     constexpr int kPieces = D / 8 / kJoinBlocks<D>;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31;
-    const int kh = blockIdx.x % a.kvh, rank = blockIdx.x / a.kvh;
-    // (a shared unit's first block; where the unit is not shared, another's or its only one)
-    const UnitWork u = unit_work(a, rank * a.splits);
-    if (u.s < 0 || u.rank != rank) return;
-    const int count = u.parts;
-    const int c = u.first + wave * kWaveColumns + col;
-    if (count <= 1 || c >= u.columns) return;
-    const int64_t p0 = ((int64_t)rank * a.kvh + kh) * a.splits;
-    const float2* ml = reinterpret_cast<const float2*>(a.part + parts * kBlockColumns * D) + p0 * kBlockColumns + wave * kWaveColumns + col;
+    const int y = (int)(blockIdx.x / 8) % kJoinBlocks<D>, x = (int)(blockIdx.x / 8) / kJoinBlocks<D> * 8 + (int)(blockIdx.x % 8);
+    if (x >= a.join_count * a.kvh) return;
+    const int kh = x % a.kvh;
+    const UnitWork u = unit_work(a, a.unit_count + x / a.kvh);
+    const int c = u.first + wave * kWaveColumns + col, count = u.parts;
+    if (u.s < 0 || count <= 1 || c >= u.columns) return;
+    const int64_t p0 = part_place(a, u, kh);
+    const float2* ml = reinterpret_cast<const float2*>(a.part + (int64_t)a.parts * a.kvh * kBlockColumns * D) + p0 * kBlockColumns +
+                       wave * kWaveColumns + col;
     const float4* from = reinterpret_cast<const float4*>(a.part + p0 * kBlockColumns * D) + wave * (D / 8) * 64 + lane;
     float m = -INFINITY;
     for (int k = 0; k < count; ++k) m = fmaxf(m, ml[k * kBlockColumns].x);
@@ -533,12 +537,12 @@ __global__ __launch_bounds__(kPromptThreads) void paged_prompt_join_kernel(Atten
     float l = 0.0f;
 #pragma unroll 4
     for (int k = 0; k < count; ++k) {
-        const float2 x = ml[k * kBlockColumns];
-        const float by = __builtin_amdgcn_exp2f(x.x - top);
-        l += by * x.y;
+        const float2 p = ml[k * kBlockColumns];
+        const float by = __builtin_amdgcn_exp2f(p.x - top);
+        l += by * p.y;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            const float4 v = from[(int64_t)k * (kBlockColumns * D / 4) + (i * kJoinBlocks<D> + blockIdx.y) * 64];
+            const float4 v = from[(int64_t)k * (kBlockColumns * D / 4) + (i * kJoinBlocks<D> + y) * 64];
             o[i].x += by * v.x;
             o[i].y += by * v.y;
             o[i].z += by * v.z;
@@ -549,58 +553,49 @@ __global__ __launch_bounds__(kPromptThreads) void paged_prompt_join_kernel(Atten
     uint16_t* out = a.out + ((int64_t)(u.start + c / a.group) * a.heads + kh * a.group + c % a.group) * D + 4 * (lane >> 5);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i)
-        store4(out + 8 * (i * kJoinBlocks<D> + blockIdx.y), o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv);
+        store4(out + 8 * (i * kJoinBlocks<D> + y), o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv);
 }
 
 namespace {
 
 template <int CT, int D>
-void launch(const AttendArgs& a, int slots, hipStream_t st) {
-    const int grid = slots * a.splits * a.kvh;
+void launch(const AttendArgs& a, hipStream_t st) {
+    const int grid = a.unit_count * a.kvh;
     if (a.cap > 0.0f)
         hipLaunchKernelGGL((paged_prompt_kernel<CT, D, true>), dim3(grid), dim3(kPromptThreads), 4 * 64 * D, st, a);
     else
         hipLaunchKernelGGL((paged_prompt_kernel<CT, D, false>), dim3(grid), dim3(kPromptThreads), 4 * 64 * D, st, a);
-    if (a.splits > 1)
-        hipLaunchKernelGGL((paged_prompt_join_kernel<CT, D>), dim3(slots * a.kvh, kJoinBlocks<D>), dim3(kPromptThreads), 0,
-                           st, a, (int64_t)grid);
+    if (a.join_count > 0)
+        hipLaunchKernelGGL((paged_prompt_join_kernel<CT, D>), dim3((a.join_count * a.kvh + 7) / 8 * 8 * kJoinBlocks<D>), dim3(kPromptThreads), 0, st, a);
 }
-
-// at most: a sequence has n group / 128 units, rounded up
-int unit_slots(const Batch& b, int group) { return (int)((int64_t)b.tokens * group / kBlockColumns) + std::min(b.seqs, b.tokens); }
 
 }  // namespace
 
-// Blocks that share a unit's keys: as many as it takes to fill the card.
-int prompt_splits(const Batch& b, int kvh, int group, int page_size) {
-    const int64_t units = std::max<int64_t>((int64_t)b.tokens * group / kBlockColumns, 1) * kvh;
-    const int64_t most = ((int64_t)b.width * page_size + 32 * kLeastTiles - 1) / (32 * kLeastTiles);
-    if (units > kSharedUnits) return 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::max<int64_t>(256 / units, 2), most));
-}
-
-bool prompt_fits(const Batch& b, int kvh, int group, int page_size) {
-    return (int64_t)b.tokens * group <= INT32_MAX &&
-           (int64_t)unit_slots(b, group) * kvh * prompt_splits(b, kvh, group, page_size) <= INT32_MAX;
-}
-
-int prompt_units(const Batch& b, int kvh, int group, int page_size) { return unit_slots(b, group) * prompt_splits(b, kvh, group, page_size); }
-
-int64_t prompt_unit_bytes(const Batch& b, int kvh, int group, int page_size) {
-    return ((int64_t)prompt_units(b, kvh, group, page_size) * (int64_t)sizeof(UnitWork) + 255) / 256 * 256;
-}
-
-int64_t prompt_part_bytes(const Batch& b, int kvh, int group, int page_size, int d) {
-    const int splits = prompt_splits(b, kvh, group, page_size);
-    return splits == 1 ? 0 : (int64_t)unit_slots(b, group) * splits * kvh * kBlockColumns * (d + 2) * (int64_t)sizeof(float);
+// A sequence has units only with more than kFewColumns columns, so at most one of so many
+// of all columns does, and its last unit holds one column at least. Parts: twice a round's
+// blocks (Sharing), or where few units can be as many as the rule for `splits` asks for.
+// Where there are many units none is shared, but the memory stays: no call takes less than
+// one of fewer tokens.
+PromptPlan prompt_plan(const Batch& b, int kvh, int group, int page_size, int d, bool e4m3) {
+    const int64_t columns = (int64_t)b.tokens * group, many = std::min<int64_t>(b.seqs, columns / (kFewColumns + 1));
+    const int64_t resident = resident_blocks(e4m3, d);
+    PromptPlan x;
+    x.slots = (columns + (kBlockColumns - 1) * many) / kBlockColumns;
+    x.most = (int)(((int64_t)b.width * page_size + 32 * kLeastTiles - 1) / (32 * kLeastTiles));
+    int64_t parts = std::min(std::min(2 * resident, std::max(resident, 2 * x.slots * kvh)) / kvh, x.slots * x.most);
+    if (x.most < 2 || parts < 2) parts = 0;
+    x.parts = columns / kBlockColumns * kvh > kSharedUnits ? 0 : (int)parts;
+    x.records = x.slots + parts + parts / 2;
+    x.record_bytes = (x.records * (int64_t)sizeof(UnitWork) + 255) / 256 * 256;
+    x.part_bytes = parts * kvh * kBlockColumns * (d + 2) * (int64_t)sizeof(float);
+    return x;
 }
 
 void launch_prompt(const AttendArgs& a, bool e4m3, int d, hipStream_t st) {
-    const int slots = unit_slots(a.b, a.group);
     switch (d) {
-        case 64: e4m3 ? launch<SE12_STEP_E4M3, 64>(a, slots, st) : launch<SE12_STEP_BF16, 64>(a, slots, st); break;
-        case 128: e4m3 ? launch<SE12_STEP_E4M3, 128>(a, slots, st) : launch<SE12_STEP_BF16, 128>(a, slots, st); break;
-        default: e4m3 ? launch<SE12_STEP_E4M3, 256>(a, slots, st) : launch<SE12_STEP_BF16, 256>(a, slots, st);
+        case 64: e4m3 ? launch<SE12_STEP_E4M3, 64>(a, st) : launch<SE12_STEP_BF16, 64>(a, st); break;
+        case 128: e4m3 ? launch<SE12_STEP_E4M3, 128>(a, st) : launch<SE12_STEP_BF16, 128>(a, st); break;
+        default: e4m3 ? launch<SE12_STEP_E4M3, 256>(a, st) : launch<SE12_STEP_BF16, 256>(a, st);
     }
 }
 

@@ -13,6 +13,7 @@
 
 namespace se12step {
 
+constexpr int kFewColumns = 64;           // of a sequence and KV head that se12_paged_attention.hip takes
 constexpr int kBlockColumns = 128;
 constexpr int kLeastTiles = 8;            // of a block, where a unit's keys are split
 
@@ -59,64 +60,40 @@ __device__ __forceinline__ UnitCounts load_counts(const AttendArgs& a, int s0, i
     c.seq = load_seq(a.b, min(s0 + lane, a.b.seqs - 1), capacity);
     c.keys = min(c.seq.len + c.seq.n, capacity);
     c.columns = s0 + lane < a.b.seqs ? c.seq.n * a.group : 0;
-    c.units = c.columns > a.few ? (c.columns + kBlockColumns - 1) / kBlockColumns : 0;
+    c.units = c.columns > kFewColumns ? (c.columns + kBlockColumns - 1) / kBlockColumns : 0;
     c.columns = c.units > 0 ? c.columns : 0;
     return c;
 }
 
-// Keys of a block where units are shared (splits > 1): about as many as make all units'
-// keys one round of blocks, those of a sequence's units taken as a run from the first
-// to the last.
-template <int kTile>
-__device__ __forceinline__ int shared_tiles(const AttendArgs& a, int lane, int resident) {
-    const int capacity = a.b.width << a.page_log2;
-    int64_t all = 0;
-    for (int s0 = 0; s0 < a.b.seqs; s0 += 64) {
-        const UnitCounts c = load_counts(a, s0, lane, capacity);
-        const int last = c.keys, first = min(c.seq.len + kBlockColumns / a.group, last), reach = a.window > 0 ? min(a.window, INT32_MAX - kTile) + kTile : INT32_MAX;
-        // (a float holds it closely enough, and is the same for every block)
-        all += wave_total((int)fminf((float)c.units * (float)(min(first, reach) / 2 + min(last, reach) / 2) / kTile, 1e7f));
+// unit `rank` of the order of 64 sequences
+__device__ __forceinline__ Unit unit_of(const AttendArgs& a, const UnitCounts& c, int s0, int rank) {
+    const int lane = threadIdx.x & 63, most = wave_most(c.units > 0 ? c.keys : 0);
+    // the largest x with more than `rank` units past 64 x (every unit is past -1)
+    int lo = -1, hi = (most + 63) / 64;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (wave_total(c.past(64 * mid, a.group)) > rank)
+            lo = mid;
+        else
+            hi = mid;
     }
-    return (int)min(all * a.kvh / resident + 1, (int64_t)INT32_MAX);
-}
-
-__device__ __forceinline__ bool find_unit(const AttendArgs& a, int rank, Unit& u) {
-    const int lane = threadIdx.x & 63, capacity = a.b.width << a.page_log2;
-    for (int s0 = 0; s0 < a.b.seqs; s0 += 64) {
-        const UnitCounts c = load_counts(a, s0, lane, capacity);
-        const int all = wave_total(c.units);
-        if (rank >= all) {
-            rank -= all;
-            continue;
-        }
-        const int most = wave_most(c.units > 0 ? c.keys : 0);
-        // the largest x with more than `rank` units past 64 x (every unit is past -1)
-        int lo = -1, hi = (most + 63) / 64;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (wave_total(c.past(64 * mid, a.group)) > rank)
-                lo = mid;
-            else
-                hi = mid;
-        }
-        const int here = lo < 0 ? c.units : c.past(64 * lo, a.group), beyond = c.past(64 * (lo + 1), a.group);
-        rank -= wave_total(beyond);
-        int upto = here - beyond;      // of this x: a sequence's are units - here .. units - beyond - 1
+    const int here = lo < 0 ? c.units : c.past(64 * lo, a.group), beyond = c.past(64 * (lo + 1), a.group);
+    rank -= wave_total(beyond);
+    int upto = here - beyond;      // of this x: a sequence's are units - here .. units - beyond - 1
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(upto, o, 64);
-            upto += lane >= o ? v : 0;
-        }
-        const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > rank));
-        auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-        u.s = s0 + l;
-        u.seq = {of(c.seq.start), of(c.seq.n), of(c.seq.len)};
-        u.keys = of(c.keys);
-        u.columns = of(c.columns);
-        u.first = kBlockColumns * (of(c.units) - of(here) + rank - (of(upto) - (of(here) - of(beyond))));
-        return true;
+    for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(upto, o, 64);
+        upto += lane >= o ? v : 0;
     }
-    return false;
+    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > rank));
+    auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+    Unit u;
+    u.s = s0 + l;
+    u.seq = {of(c.seq.start), of(c.seq.n), of(c.seq.len)};
+    u.keys = of(c.keys);
+    u.columns = of(c.columns);
+    u.first = kBlockColumns * (of(c.units) - of(here) + rank - (of(upto) - (of(here) - of(beyond))));
+    return u;
 }
 
 // the key tiles the unit's columns see
@@ -129,61 +106,83 @@ __device__ __forceinline__ void unit_tiles(const AttendArgs& a, const Unit& u, i
 }
 
 // blocks the card holds at once
-template <int CT, int D>
-constexpr int kResidentBlocks = 256 * (D == 256 || (D == 128 && CT == SE12_STEP_BF16) ? 1 : 2);
+constexpr int resident_blocks(bool e4m3, int d) { return 256 * (d == 256 || (d == 128 && !e4m3) ? 1 : 2); }
 
-// Which units are shared: the first `units` of the order, in parts of about `tiles`
-// tiles. Their parts come first, and then the others, the most keys first.
+// Which units are shared: of every 64 sequences those that see more than `tiles` tiles,
+// `units` of all at most, each in up to `splits` parts of about `tiles` tiles. Tiles: as
+// many as make all units' one round of blocks, those of a sequence's units taken as a run
+// from the first to the last, so a KV head's parts are as many as a round's blocks and the
+// shared units together, and room for twice a round's is enough (a.parts).
 struct Sharing {
-    int units, tiles;
+    int units, splits, tiles;
 };
 
 template <int CT, int D>
 __device__ __forceinline__ Sharing sharing_of(const AttendArgs& a, int lane) {
-    constexpr int kTile = Form<CT>::kTile;
-    if (a.splits == 1) return {0, INT32_MAX};
-    const int tiles = max(shared_tiles<kTile>(a, lane, kResidentBlocks<CT, D>), kLeastTiles);
-    // (all of them where their order is not that of their keys)
-    if (a.b.seqs > 64 || a.window > 0) return {INT32_MAX / a.splits, tiles};
-    return {wave_total(load_counts(a, 0, lane, a.b.width << a.page_log2).past((int)min((int64_t)tiles * kTile, (int64_t)INT32_MAX), a.group)), tiles};
+    constexpr int kTile = Form<CT>::kTile, kResident = resident_blocks(CT == SE12_STEP_E4M3, D);
+    if (a.parts < 2) return {0, 1, 1};
+    const int capacity = a.b.width << a.page_log2;
+    int64_t tiles = 0, units = 0;
+    for (int s0 = 0; s0 < a.b.seqs; s0 += 64) {
+        const UnitCounts c = load_counts(a, s0, lane, capacity);
+        const int last = c.keys, first = min(c.seq.len + kBlockColumns / a.group, last);
+        const int reach = a.window > 0 ? min(a.window, INT32_MAX - kTile) + kTile : INT32_MAX;
+        // (a float holds it closely enough, and is the same for every block)
+        tiles += wave_total((int)fminf((float)c.units * (float)(min(first, reach) / 2 + min(last, reach) / 2) / kTile, 1e7f));
+        units += wave_total(c.units);
+    }
+    const int64_t each = max(min(tiles * a.kvh / kResident + 1, (int64_t)1 << 24), (int64_t)kLeastTiles);
+    const int splits = (int)max(min(kResident / max(units * a.kvh, (int64_t)1), (int64_t)a.most), (int64_t)2);
+    return {a.parts / splits, splits, (int)each};
 }
 
-// tiles of a block of a unit that has `tiles`
-__device__ __forceinline__ int part_tiles(const AttendArgs& a, const Sharing& x, int rank, int tiles) {
-    if (rank >= x.units) return tiles;
-    const int parts = min((tiles + x.tiles - 1) / x.tiles, a.splits);
-    return (tiles + parts - 1) / parts;
-}
-
-// A block's work, for all KV heads alike: a part (`split`, of `parts`) of the unit of
-// this rank, key tiles t0 .. t1 - 1.
+// A block's work, for all KV heads alike: a part of a unit, key tiles t0 .. t1 - 1.
 struct UnitWork {
-    int s, first, start, n;        // s: -1 for none
-    int len, keys, columns, t0;
-    int t1, rank, split, parts;
+    int s, first, start, len;      // s: -1 for none
+    int keys, columns, t0, t1;
+    int rank, split, parts;        // which of its `parts`, of which of the shared units
+    int splits;                    // places for the parts of a unit
 };
 
+// where a part of a KV head's unit is held
+__device__ __forceinline__ int64_t part_place(const AttendArgs& a, const UnitWork& u, int kh) {
+    return ((int64_t)u.rank * a.kvh + kh) * u.splits + u.split;
+}
+
+// What block x does: of every 64 sequences the shared units' parts come first, then the
+// others, the most keys first. Behind the blocks' records those of the joins: the shared units.
 template <int CT, int D>
 __device__ __forceinline__ void write_unit(const AttendArgs& a, int x) {
     constexpr int kTile = Form<CT>::kTile;
-    const int lane = threadIdx.x & 63;
-    int rank = x, split = 0;
+    const int lane = threadIdx.x & 63, capacity = a.b.width << a.page_log2;
+    const bool join = x >= a.unit_count;
+    int index = join ? x - a.unit_count : x, left, before = 0;
     const Sharing sharing = sharing_of<CT, D>(a, lane);
-    if (rank < sharing.units * a.splits) {
-        split = rank % a.splits;
-        rank /= a.splits;
-    } else {
-        rank -= sharing.units * (a.splits - 1);
-    }
+    const int limit = (sharing.tiles * kTile) & ~63;      // (the order is that of 64 keys)
+    left = sharing.units;
     UnitWork w{-1, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-    Unit u;
-    if (find_unit(a, rank, u)) {
+    for (int s0 = 0; s0 < a.b.seqs; s0 += 64) {
+        const UnitCounts c = load_counts(a, s0, lane, capacity);
+        const int all = wave_total(c.units), shared = left > 0 ? min(wave_total(c.past(limit, a.group)), left) : 0;
+        const int first_alone = shared * sharing.splits, count = join ? shared : first_alone + all - shared;
+        if (index >= count) {
+            index -= count;
+            left -= shared;
+            before += shared;
+            continue;
+        }
+        const bool alone = !join && index >= first_alone;
+        const int rank = alone ? shared + index - first_alone : join ? index : index / sharing.splits;
+        const int split = alone || join ? 0 : index - rank * sharing.splits;
+        const Unit u = unit_of(a, c, s0, rank);
         int t0, t1;
         unit_tiles<kTile>(a, u, t0, t1);
-        const int length = part_tiles(a, sharing, rank, t1 - t0), parts = (t1 - t0 + length - 1) / length;
+        const int wanted = alone ? 1 : min((t1 - t0 + sharing.tiles - 1) / sharing.tiles, sharing.splits);
+        const int length = (t1 - t0 + wanted - 1) / wanted, parts = (t1 - t0 + length - 1) / length;
         if (split < parts)
-            w = {u.s, u.first, u.seq.start, u.seq.n, u.seq.len, u.keys, u.columns, t0 + split * length, min(t1, t0 + (split + 1) * length),
-                 rank, split, parts};
+            w = {u.s, u.first, u.seq.start, u.seq.len, u.keys, u.columns, t0 + split * length, min(t1, t0 + (split + 1) * length),
+                 before + rank, split, parts, sharing.splits};
+        break;
     }
     if (lane == 0) a.units[x] = w;
 }

@@ -253,7 +253,7 @@ class PagedKvCache:
         return out
 
     def attend_workspace(self, batch: PagedBatch, tokens: int, heads: int) -> int:
-        """Bytes of `attend`'s workspace."""
+        """Bytes of `attend`'s workspace for calls of so many tokens; enough for fewer as well."""
         self._check(batch)
         if not 0 <= tokens < 2 ** 31 or not 0 < heads < 2 ** 31:
             raise ValueError(f"tokens and heads must be below 2^31, got {tokens}, {heads}")

@@ -548,6 +548,54 @@ def test_workspace_and_streams(gpu):
         c.attend(batch, q, 0.0625, workspace=ws[:n - 256])
 
 
+@pytest.mark.parametrize("dtype", [E4M3, BF16])
+@pytest.mark.parametrize("d,heads,kvh,lengths,new,window", [
+    (256, 8, 4, [900, 20, 400, 3000], [1, 90, 1, 70], 0),                          # long units in parts, decode steps beside
+    (128, 28, 4, [5000, 1], [64, 1], 0),                                           # one sequence, seven heads to one
+    (64, 4, 2, [(i * 53) % 150 for i in range(100)], [90 if i in (3, 70, 99) else i % 3 for i in range(100)], 0),
+    (64, 4, 2, [(i * 253) % 1500 for i in range(130)], [90 if i in (3, 70, 129) else i % 3 for i in range(130)], 1200),
+])
+def test_what_the_workspace_of_prompts_held_does_not_matter(gpu, dtype, d, heads, kvh, lengths, new, window):
+    """Records of units, parts and statistics are all written before they are read, and none lies outside: a workspace of
+    exactly the bytes asked for, of ones or zeros, with guards around it, and used again for fewer tokens."""
+    c, batch, q, out = _attend_case(gpu, dtype, d, 64, heads, kvh, lengths, new, 0.0, window, seed=32, extra=0)
+    n = c.attend_workspace(batch, q.shape[0], heads)
+    for fill in (255, 0):
+        guarded = torch.full((n + 2048,), fill, dtype=torch.uint8, device=gpu)
+        guarded[:1024], guarded[1024 + n:] = 90, 90
+        ws = guarded[1024:1024 + n]
+        assert torch.equal(c.attend(batch, q, d ** -0.5, window=window, workspace=ws), out)
+        assert (guarded[:1024] == 90).all() and (guarded[1024 + n:] == 90).all()
+        few = [min(x, 1) for x in new]
+        step, starts = _batch(gpu, batch.page_table.tolist(), lengths, few, max_new=max(new))
+        rows = torch.tensor([s for s, x in zip(batch.starts.tolist(), new) if x], device=gpu)
+        first = c.attend(step, q[rows], d ** -0.5, window=window, workspace=ws)
+        assert torch.equal(c.attend(step, q[rows], d ** -0.5, window=window), first)
+        kp, vp, ks, vs = _state(c)
+        ref, size, _ = o.attend(kp, vp, ks, vs, batch.page_table.tolist(), lengths, starts, q[rows].cpu(), d ** -0.5, 0.0, window, 1)
+        _close(first, ref, size)
+        assert (guarded[:1024] == 90).all() and (guarded[1024 + n:] == 90).all()
+
+
+@pytest.mark.parametrize("dtype", [E4M3, BF16])
+@pytest.mark.parametrize("lengths,new,window", [
+    ([0, 6000, 0, 40], [64, 64, 33, 200], 0),                  # one unit is most of the work
+    ([2500, 10, 10, 10, 10, 10], [33, 33, 40, 50, 60, 70], 0),
+    ([4000, 10, 2000], [100, 200, 129], 1500),
+])
+def test_few_prompts_of_very_different_lengths(gpu, dtype, lengths, new, window):
+    _attend_case(gpu, dtype, 64, 16, 4, 2, lengths, new, 0.0, window, seed=33)
+
+
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+def test_prompts_with_scales_that_are_no_powers_of_two(gpu, softcap):
+    """The values' scale goes into the weight's exponent: its logarithm, of 6 at most here, is off by 2^-22."""
+    c, batch, q, _ = _attend_case(gpu, E4M3, 128, 32, 8, 4, [100, 7, 1500], [70, 1, 40], softcap, 0, seed=34, extra=0)
+    for t in (c.k_scale, c.v_scale):
+        t.mul_(1.37)
+    _again(c, batch, q, 128, softcap, 0)
+
+
 # ---------------------------------------------------------------------------
 # together
 # ---------------------------------------------------------------------------

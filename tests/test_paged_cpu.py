@@ -107,6 +107,43 @@ def test_attention_refuses_what_one_launch_does_not_hold(batch, message):
             nat.step_check(call())
 
 
+def _workspace(heads=16, pages=None, **batch):
+    f = dict(sequences=64, tokens=64, max_new=1, table_width=128, table_stride=128)
+    f.update(batch)
+    n = nat.lib().se12_step_paged_attention_workspace(ctypes.byref(_pages(**{"kv_heads": 8, "head_dim": 256, **(pages or {})})),
+                                                      ctypes.byref(_batch(**f)), heads)
+    if n < 0:
+        nat.step_check(n)
+    return n
+
+
+@pytest.mark.parametrize("batch", [
+    dict(max_new=512), dict(tokens=96, max_new=33), dict(sequences=1024, tokens=1535, max_new=512),
+    dict(tokens=64 + 511, max_new=512), dict(sequences=4096, tokens=4160, max_new=65, table_width=1024, table_stride=1024),
+    dict(tokens=6400, max_new=6400), dict(sequences=1, tokens=512, max_new=512), dict(sequences=65536, tokens=65536, max_new=4096),
+])
+@pytest.mark.parametrize("dtype", [nat.STEP_E4M3, nat.STEP_BF16])
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+def test_the_workspace_of_few_prompts_among_many_sequences(batch, dtype, head_dim):
+    """Parts of two rounds of blocks (512 of 128 columns at 256 values and two statistics, 1,024 at half as many), the
+    waves' parts of short sequences (2,048 of 16 columns), and records: a sequence of one new token adds nothing."""
+    columns = 2048 * 16 + (1 if head_dim == 256 or (head_dim == 128 and dtype == nat.STEP_BF16) else 2) * 512 * 128
+    records = (2 * batch["tokens"] // 128 + 2 * batch["tokens"] // 65 + 1600) * 48 if "tokens" in batch else 1 << 20
+    assert _workspace(pages=dict(dtype=dtype, head_dim=head_dim), **batch) <= columns * (head_dim + 2) * 4 + records + 1024
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(16, 8), (28, 4), (8, 8), (160, 1), (7, 7)])
+@pytest.mark.parametrize("sequences,width", [(1, 2000), (64, 100), (300, 4), (5, 1)])
+@pytest.mark.parametrize("page_size,dtype", [(64, nat.STEP_E4M3), (16, nat.STEP_BF16)])
+def test_a_workspace_for_more_tokens_serves_fewer(heads, kv_heads, sequences, width, page_size, dtype):
+    pages, last = dict(kv_heads=kv_heads, page_size=page_size, dtype=dtype, head_dim=128), 0
+    for max_new in (1, 2, 9, 40, 1 << 20):
+        f = dict(sequences=sequences, table_width=width, table_stride=width, max_new=max_new)
+        sizes = [_workspace(heads, pages, tokens=n, **f) for n in [*range(1, 200), *range(200, 20_000, 97), 100_000, 1_000_000]]
+        assert sizes == sorted(sizes) and sizes[-1] >= last
+        last = sizes[-1]
+
+
 @pytest.mark.parametrize("change,message", [
     (dict(vocab=0), "bad shape"), (dict(rows=-1), "bad shape"), (dict(top=33), "top"), (dict(top=-1), "top"), (dict(vocab=4, top=5), "top"),
     (dict(logits=None), "NULL"), (dict(tokens=None), "NULL"), (dict(tl=None), "NULL"), (dict(dtype=2), "BF16 or FP32"),
