@@ -147,6 +147,7 @@ typedef struct se12_step_pages {
  * [sequences + 1] ascends from 0; `tokens` is the number of rows of q, k, v and
  * out (rows from starts[sequences] on are neither read nor written), max_new at
  * least the most new tokens of a sequence (of more, the first max_new count).
+ * Lengths are 0 to 2^30 - 1 (others are taken as the nearer of these).
  * All device memory, read when the kernels run, so a captured call follows what
  * they hold then. No entry can lead outside the memory given: a page outside
  * [0, pages), or a position outside the table, holds nothing and takes nothing.

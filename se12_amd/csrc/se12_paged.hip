@@ -145,7 +145,7 @@ __device__ __forceinline__ void rotate_q(const AppendArgs& a) {
         else
             e = mid;
     }
-    const Seq seq = load_seq(a.b, s, a.b.width << a.page_log2);
+    const Seq seq = load_seq(a.b, s);
     const int i = token - seq.start;
     if (i < 0 || i >= seq.n) return;
     const int units = a.d >> 3, unit = lane & (units - 1), step = 64 / units;
@@ -211,10 +211,12 @@ __global__ __launch_bounds__(kAppendMaxThreads) void paged_append_kernel(AppendA
         s = lo;
         j = slot - (min(max(a.b.starts[s], 0), a.b.tokens) >> a.page_log2) - 2 * s;
     }
-    const Seq seq = load_seq(a.b, s, a.b.width << a.page_log2);
-    const int page = (seq.len >> a.page_log2) + j, first = page << a.page_log2;
+    const Seq seq = load_seq(a.b, s);
+    const int page = (seq.len >> a.page_log2) + j;
+    if (j < 0 || page >= a.b.width) return;
+    const int first = page << a.page_log2;
     const int from = j == 0 ? seq.len - first : 0, to = min(P, seq.len + seq.n - first);   // slots of new tokens
-    if (j < 0 || to <= from) return;
+    if (to <= from) return;
     const int id = page_of(a.b, s, page, a.pages);
     if (id < 0) return;
 

@@ -70,7 +70,7 @@ template <int kTile>
 __device__ __forceinline__ Chunk load_chunk(const AttendArgs& a, int s0, int lane) {
     Chunk c;
     const int s = s0 + lane;
-    c.seq = load_seq(a.b, min(s, a.b.seqs - 1), a.b.width << a.page_log2);
+    c.seq = load_seq(a.b, min(s, a.b.seqs - 1));
     if (s >= a.b.seqs) c.seq.n = 0;
     const SeqWork w = seq_work<kTile>(a, c.seq);
     c.tiles = w.tiles * w.units * a.kvh;

@@ -20,16 +20,16 @@ struct Batch {
 };
 
 // one sequence of a call: its new tokens are rows start .. start + n - 1, at
-// positions len ..; what the device memory says is kept inside the call's rows
-// and the table
+// positions len ..; what the device memory says is kept inside the call's rows, and
+// positions inside 31 bits (those behind the table's last column are held nowhere)
 struct Seq {
     int start, n, len;
 };
 
-__device__ __forceinline__ Seq load_seq(const Batch& b, int s, int capacity) {
+__device__ __forceinline__ Seq load_seq(const Batch& b, int s) {
     const int a = min(max(b.starts[s], 0), b.tokens);
     const int e = min(max(b.starts[s + 1], a), b.tokens);
-    return {a, min(e - a, b.max_new), min(max(b.lengths[s], 0), capacity)};
+    return {a, min(e - a, b.max_new), min(max(b.lengths[s], 0), (1 << 30) - 1)};
 }
 
 // the page holding column `c` of sequence s's table row, or -1

@@ -57,7 +57,7 @@ __device__ __forceinline__ int wave_most(int v) {
 
 __device__ __forceinline__ UnitCounts load_counts(const AttendArgs& a, int s0, int lane, int capacity) {
     UnitCounts c;
-    c.seq = load_seq(a.b, min(s0 + lane, a.b.seqs - 1), capacity);
+    c.seq = load_seq(a.b, min(s0 + lane, a.b.seqs - 1));
     c.keys = min(c.seq.len + c.seq.n, capacity);
     c.columns = s0 + lane < a.b.seqs ? c.seq.n * a.group : 0;
     c.units = c.columns > kFewColumns ? (c.columns + kBlockColumns - 1) / kBlockColumns : 0;

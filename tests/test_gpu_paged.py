@@ -513,6 +513,30 @@ def test_lengths_that_do_not_fit_the_table_stay_inside_it(gpu):
     assert (guard[4:] == 9.0).all()
 
 
+@pytest.mark.parametrize("dtype", [E4M3, BF16])
+@pytest.mark.parametrize("lengths,new", [([40, 30, 100, 5], [2, 4, 3, 1]), ([20, 32, 90, 1000], [70, 40, 33, 1])])
+@pytest.mark.parametrize("window", [0, 20, 64, 80])
+def test_positions_beyond_the_table_are_what_they_are(gpu, dtype, lengths, new, window):
+    """Tokens behind the table's last column are held nowhere, but their queries stand where they stand: turned by their
+    position, and a window reaches back from there."""
+    page, kvh, d, heads = 16, 2, 64, 4
+    table = _table(4, 2, 9, 15)
+    c = _cache(gpu, 9, page, kvh, d, dtype, 16)
+    batch, starts = _batch(gpu, table, lengths, new)
+    k, v = (torch.randn((sum(new), kvh, d), generator=_gen(17 + i)).to(gpu) for i in range(2))
+    q = torch.randn((sum(new), heads, d), generator=_gen(19)).to(gpu)
+    inv = (10000.0 ** (-torch.arange(0, d, 2).float() / d)).to(gpu)
+    before = _state(c)
+    turned = c.append(batch, k, v, q=q, inv_freq=inv)
+    _check_append(c, before, batch, lengths, starts, table, k, v, inv, q, turned)
+    kp, vp, ks, vs = _state(c)
+    ref, size, _ = o.attend(kp, vp, ks, vs, table, lengths, starts, turned.cpu(), 0.125, 0.0, window, max(new))
+    got = c.attend(batch, turned, 0.125, window=window)
+    _close(got, ref, size)
+    if window == 20:
+        assert (got[starts[2]:starts[3]] == 0).all()      # (from 90 on nothing held is within 20)
+
+
 def test_attend_with_sharp_scores_and_far_apart_tiles(gpu):
     """The maximum moves in many tiles: keys grow along the sequence; and one key holds all the weight."""
     for dtype in (E4M3, BF16):
