@@ -186,7 +186,7 @@ int se12_step_paged_append(const se12_step_pages* pages, const se12_step_batch* 
 /* Attention of the new tokens over their sequences' pages, those of the call
  * itself included (appended before): the query at position p sees keys
  * max(0, p - window + 1) .. p (window 0 = all). s = q . k * scaling, soft-capped
- * tanh(s / softcap) * softcap when softcap > 0 (up to 1024; held to 2^-22 of
+ * tanh(s / softcap) * softcap when softcap > 0 (2^-60 to 1024; held to 2^-22 of
  * it); softmax and sums in FP32, weights rounded to BF16 for the product with v. q BF16 [tokens, heads,
  * head_dim], rows q_stride apart (a multiple of 8), 16-byte aligned, already
  * rotated; out BF16 [tokens, heads, head_dim] contiguous, 8-byte aligned, apart
@@ -205,7 +205,7 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
                               int32_t window, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* What a serving program reports of logits [rows, stride] (BF16 or FP32, vocab
- * of a row used), with z = softcap tanh(logit / softcap) when softcap > 0 (up to
+ * of a row used), with z = softcap tanh(logit / softcap) when softcap > 0 (2^-60 to
  * 1024; held to 2^-22 of a cap of up to 64, of z under a larger one), else the
  * logit, and p = softmax(z) in FP32:
  *   logprobs[r]  log p of tokens[r] (-inf for a token outside [0, vocab))

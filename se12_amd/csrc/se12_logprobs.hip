@@ -496,7 +496,7 @@ int se12_step_logprobs(const void* logits, int32_t dtype, int64_t stride, int32_
     if (!logits || !tokens || !logprobs || !entropy || (top > 0 && (!top_logprobs || !top_ids))) return step_fail(fn, "NULL argument");
     if (dtype != SE12_STEP_BF16 && dtype != SE12_STEP_F32) return step_fail(fn, "logits must be BF16 or FP32");
     if (stride < vocab) return step_fail(fn, "rows overlap");
-    if (!(softcap >= 0.0f) || !(softcap <= 1024.0f)) return step_fail(fn, "softcap must be 0 to 1024");
+    if (!(softcap == 0.0f || (softcap >= 0x1p-60f && softcap <= 1024.0f))) return step_fail(fn, "softcap must be 0, or 2^-60 to 1024");
     if (reinterpret_cast<uintptr_t>(logits) % (dtype == SE12_STEP_F32 ? 4 : 2) || reinterpret_cast<uintptr_t>(tokens) % 8 ||
         reinterpret_cast<uintptr_t>(logprobs) % 4 || reinterpret_cast<uintptr_t>(entropy) % 4 ||
         reinterpret_cast<uintptr_t>(top_logprobs) % 4 || reinterpret_cast<uintptr_t>(top_ids) % 8)

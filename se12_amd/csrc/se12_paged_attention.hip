@@ -527,8 +527,10 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
     if (const char* e = paged_error(pages, batch, heads)) return step_fail(fn, e);
     if (batch->tokens > 0 && (!q || !out)) return step_fail(fn, "NULL argument");
     if (q_stride < (int64_t)heads * pages->head_dim || q_stride % 8) return step_fail(fn, "q rows must be a multiple of 8 elements apart and hold all heads");
-    // (the cap's form holds a score to 2^-22 of the cap)
-    if (!(softcap >= 0.0f) || !(softcap <= 1024.0f) || window < 0) return step_fail(fn, "softcap must be 0 to 1024 and window 0 or more");
+    if (!softcap_fits(softcap) || window < 0) return step_fail(fn, "softcap must be 0, or 2^-60 to 1024, and window 0 or more");
+    constexpr float kLog2E = 1.4426950408889634f;
+    const float c1 = softcap > 0.0f ? 2.0f * scaling / softcap * kLog2E : scaling * kLog2E;
+    if (!(c1 - c1 == 0.0f)) return step_fail(fn, "scaling, or scaling / softcap, must be finite");
     if (reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(out) % 8) return step_fail(fn, "misaligned tensor");
     if (batch->tokens == 0) return SE12_STEP_OK;
     const Batch b = device_batch(batch);
@@ -540,10 +542,9 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
     const int64_t row = (int64_t)heads * pages->head_dim;
     if (overlap(q, 2 * ((b.tokens - 1) * q_stride + row), out, 2 * b.tokens * row))
         return step_fail(fn, "out overlaps q");
-    constexpr float kLog2E = 1.4426950408889634f;
     const PromptPlan plan = plan_of(pages, b, group);
     AttendArgs a{q, q_stride, out, pages->k, pages->v, pages->k_scale, pages->v_scale, b, heads, pages->kv_heads, group, pages->pages,
-                 log2_of(pages->page_size), window, softcap > 0.0f ? 2.0f * scaling / softcap * kLog2E : scaling * kLog2E,
+                 log2_of(pages->page_size), window, c1,
                  softcap * kLog2E, static_cast<float*>(workspace), worker_count(pages, b, group), column_count(b, group),
                  reinterpret_cast<UnitWork*>(static_cast<char*>(workspace) + few_bytes(pages, b, group)),
                  (int)plan.slots + plan.parts, plan.parts / 2, plan.parts, plan.most};

@@ -177,6 +177,9 @@ inline bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_byt
     return x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
 }
 
+// host: caps whose factors FP32 holds (the cap's form holds a score to 2^-22 of the cap)
+inline bool softcap_fits(float cap) { return cap == 0.0f || (cap >= 0x1p-60f && cap <= 1024.0f); }
+
 // se12_paged_prompt.hip: what a call can have of it
 struct PromptPlan {
     int64_t slots;               // units of a KV head, at most

@@ -11,7 +11,7 @@ from typing import NamedTuple
 import torch
 
 from . import _native as nat
-from .paged import _on, _stream
+from .paged import _on, _stream, check_softcap
 
 MAX_TOP = 32
 
@@ -25,7 +25,7 @@ class TokenLogprobs(NamedTuple):
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, softcap: float = 0.0) -> TokenLogprobs:
     """Log probabilities of `tokens` int64 [rows] under softmax(z) of every row of `logits` [rows, vocab] (BF16 or FP32;
-    rows may be strided), z = softcap tanh(logits / softcap) where softcap > 0 (to 1024; a Gemma LM head's raw product),
+    rows may be strided), z = softcap tanh(logits / softcap) where softcap > 0 (2^-60 to 1024; a Gemma LM head's raw product),
     else the logits; the entropy; and the `top` (0 to 32) most likely tokens, ordered by logit, equal ones by the lower index.
 
     A token outside [0, vocab) has log probability -inf. Logits of -inf (tokens that are not allowed) have no part in the
@@ -44,8 +44,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, sof
         raise ValueError(f"tokens must be an int64 [{rows}] tensor on {dev}")
     if int(top) != top or not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"top must be 0 to {min(MAX_TOP, vocab)}, got {top}")
-    if not 0.0 <= softcap <= 1024.0:
-        raise ValueError("softcap must be 0 to 1024")
+    check_softcap(softcap)
     if (logits.stride(1) != 1 and vocab > 1) or (logits.stride(0) < vocab and rows > 1):
         logits = logits.contiguous()
     tokens = tokens.contiguous()

@@ -49,6 +49,12 @@ def _int32(t: torch.Tensor, name: str, shape: tuple, device: torch.device) -> to
     return t
 
 
+def check_softcap(softcap: float) -> None:
+    """0 for none, or 2^-60 to 1024 (FP32 holds the factors of these)."""
+    if not (softcap == 0 or 2.0 ** -60 <= softcap <= 1024.0):
+        raise ValueError(f"softcap must be 0, or 2^-60 to 1024, got {softcap}")
+
+
 class PagedBatch:
     """The new tokens of a call: sequence s holds lengths[s] tokens, rows starts[s]
     .. starts[s + 1] - 1 of q, k and v are its next ones, and its token j lies in
@@ -221,7 +227,7 @@ class PagedKvCache:
                out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of the new tokens' q [tokens, heads, head_dim] (BF16, rotated; rows may be strided) over their
         sequences' pages, the tokens of this call appended before: softmax(cap(q . k scaling)) . v over the keys max(0,
-        p - window + 1) .. p of the query's position p, cap(s) = softcap tanh(s / softcap) where softcap > 0 (to 1024),
+        p - window + 1) .. p of the query's position p, cap(s) = softcap tanh(s / softcap) where softcap > 0 (2^-60 to 1024),
         window 0 = all. Returns BF16 [tokens, heads, head_dim] (`out` if given, apart from q; rows of no sequence are not
         written). No gradients.
 
@@ -232,8 +238,9 @@ class PagedKvCache:
         tokens, heads = q.shape[0], q.shape[1]
         if heads % self.kv_heads or heads == 0:
             raise ValueError(f"q's {heads} heads are no multiple of the cache's {self.kv_heads}")
-        if not 0.0 <= softcap <= 1024.0 or int(window) != window or not 0 <= window < 2 ** 31:
-            raise ValueError("softcap must be 0 to 1024 and window 0 or more")
+        check_softcap(softcap)
+        if int(window) != window or not 0 <= window < 2 ** 31:
+            raise ValueError("window must be a whole number, 0 or more")
         out = self._out(out, tokens, heads)
         if tokens == 0:
             return out

@@ -249,6 +249,32 @@ def test_sizes_beyond_32_bits_are_refused():
             c.attend_workspace(batch, tokens, heads)
 
 
+@pytest.mark.parametrize("cap,scaling,message", [
+    (1e-40, 0.1, "softcap"), (2.0 ** -61, 0.1, "softcap"), (0.0, float("inf"), "scaling"), (0.0, float("nan"), "scaling"),
+    (0.0, 1.5 * 2.0 ** 127, "scaling"), (2.0 ** -60, 2.0 ** 70, "scaling"),
+])
+def test_caps_and_scalings_whose_factors_32_bits_do_not_hold_are_refused(cap, scaling, message):
+    """0 times an infinite factor would be a NaN."""
+    lib = nat.lib()
+    with pytest.raises(nat.Se12Error, match=message):
+        nat.step_check(lib.se12_step_paged_attention(ctypes.byref(_pages()), ctypes.byref(_batch()), P, 1024, P, 8, scaling, cap, 0, P,
+                                                     1 << 30, None))
+    if message == "softcap":
+        with pytest.raises(nat.Se12Error, match=message):
+            nat.step_check(lib.se12_step_logprobs(P, nat.STEP_F32, 1000, 2, 1000, cap, P, 5, P, P, P, P, P, 1 << 30, None))
+
+
+@pytest.mark.parametrize("cap", [-1.0, 1e-300, 1e-40, 2.0 ** -61, 1025.0, float("nan")])
+def test_wrappers_refuse_caps_before_32_bits_make_them_none(cap):
+    """(1e-300 is 0 in FP32, which stands for no cap.)"""
+    from se12_amd.paged import check_softcap
+
+    with pytest.raises(ValueError, match="softcap"):
+        check_softcap(cap)
+    for fine in (0, 0.0, 2.0 ** -60, 30.0, 1024):
+        check_softcap(fine)
+
+
 def test_the_oracle_rounds_as_the_type_does():
     """Every E4M3 value, every midpoint between two of them and its neighbours, against torch's conversion on the CPU."""
     values = torch.arange(0, 127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
