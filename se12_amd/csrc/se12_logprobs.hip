@@ -502,7 +502,7 @@ int se12_step_logprobs(const void* logits, int32_t dtype, int64_t stride, int32_
         reinterpret_cast<uintptr_t>(top_logprobs) % 4 || reinterpret_cast<uintptr_t>(top_ids) % 8)
         return step_fail(fn, "misaligned tensor");
     const LpLayout l = logprobs_layout(rows, vocab, top);
-    if ((int64_t)rows * l.slices > INT32_MAX) return step_fail(fn, "too many rows");
+    if (!grid_fits((int64_t)rows * l.slices, kLpThreads)) return step_fail(fn, "too many rows");
     if (l.total > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < l.total))
         return step_fail(fn, "workspace missing, misaligned or too small");
     const LogprobArgs a{logits, stride, vocab, top, l.slices, l.slice, softcap, softcap > 0.0f ? 2.0f * kLog2E / softcap : 0.0f,

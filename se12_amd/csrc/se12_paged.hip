@@ -388,7 +388,7 @@ int se12_step_paged_append(const se12_step_pages* pages, const se12_step_batch* 
     const int64_t slots = a.b.max_new == 1 ? a.b.seqs : (int64_t)(a.b.tokens >> a.page_log2) + 2 * (int64_t)a.b.seqs;
     const int64_t kv_blocks = slots * 2 * pages->kv_heads;
     const int64_t q_blocks = q ? ((int64_t)a.b.tokens + threads / 64 - 1) / (threads / 64) : 0;
-    if (kv_blocks + q_blocks > INT32_MAX) return step_fail(fn, "too many blocks");
+    if (!grid_fits(kv_blocks + q_blocks, threads)) return step_fail(fn, "too many tokens and heads for one launch");
     a.kv_blocks = (int)kv_blocks;
     const size_t lds = a.b.max_new < kDirectTokens
                            ? 0 : (size_t)pages->head_dim * (pages->page_size * (pages->dtype == SE12_STEP_E4M3 ? 1 : 2) + 4);

@@ -484,8 +484,9 @@ PromptPlan plan_of(const se12_step_pages* p, const Batch& b, int group) {
 
 // what one launch holds, and what 32 bits hold of it
 const char* limits_error(const se12_step_pages* p, const Batch& b, int group) {
-    if ((int64_t)b.seqs * p->kv_heads * (kFewColumns / kColumns) > INT32_MAX || (int64_t)b.tokens * group > INT32_MAX ||
-        plan_of(p, b, group).records * p->kv_heads > INT32_MAX)
+    const int64_t few = (int64_t)b.seqs * p->kv_heads * ((std::min<int64_t>((int64_t)b.max_new * group, kFewColumns) + kColumns - 1) / kColumns);
+    if ((int64_t)b.tokens * group > INT32_MAX || !grid_fits(few, kAttendThreads) ||
+        !grid_fits(plan_of(p, b, group).records * p->kv_heads, kAttendThreads))
         return "too many sequences, tokens and heads for one launch";
     if (std::min<int64_t>(b.seqs, 64) * (((int64_t)b.width * p->page_size + 31) / 32) * (kFewColumns / kColumns) * p->kv_heads > INT32_MAX)
         return "too long a table for so many sequences and heads";

@@ -94,6 +94,8 @@ __device__ __forceinline__ float block_sum(float v, float* sh) {
 int step_fail(const char* msg);
 int step_fail(const char* who, const char* msg);
 int step_launched();
+// host: whether a launch's dimension holds so many blocks (a packet counts its threads in 32 bits)
+inline bool grid_fits(int64_t blocks, int64_t threads) { return blocks <= (int64_t)UINT32_MAX / threads; }
 // host: se12_step_rmsnorm with the residual read from res_in and written to
 // res_out (the same tensor, or disjoint ones)
 int step_rmsnorm(const void* in, int32_t in_dtype, int64_t in_stride, const uint16_t* w1, const uint16_t* res_in,

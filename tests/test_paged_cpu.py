@@ -249,6 +249,19 @@ def test_sizes_beyond_32_bits_are_refused():
             c.attend_workspace(batch, tokens, heads)
 
 
+def test_grids_of_more_threads_than_32_bits_count_are_refused():
+    """Before the first launch of a call, not by the last."""
+    lib, p = nat.lib(), _pages(kv_heads=1024, pages=1 << 20)
+    b = _batch(sequences=65536, tokens=65536, max_new=1)
+    with pytest.raises(nat.Se12Error, match="too many"):
+        nat.step_check(lib.se12_step_paged_append(ctypes.byref(p), ctypes.byref(b), None, P, P, nat.STEP_F32, 0, 1 << 17, 1 << 17, 1024, None,
+                                                  0, None, None))
+    with pytest.raises(nat.Se12Error, match="too many sequences, tokens"):
+        nat.step_check(lib.se12_step_paged_attention_workspace(ctypes.byref(p), ctypes.byref(b), 1024))
+    with pytest.raises(nat.Se12Error, match="too many rows"):
+        nat.step_check(lib.se12_step_logprobs(P, nat.STEP_F32, 10, 1 << 24, 10, 0.0, P, 0, P, P, None, None, None, 0, None))
+
+
 @pytest.mark.parametrize("cap,scaling,message", [
     (1e-40, 0.1, "softcap"), (2.0 ** -61, 0.1, "softcap"), (0.0, float("inf"), "scaling"), (0.0, float("nan"), "scaling"),
     (0.0, 1.5 * 2.0 ** 127, "scaling"), (2.0 ** -60, 2.0 ** 70, "scaling"),
