@@ -187,17 +187,19 @@ int se12_step_paged_append(const se12_step_pages* pages, const se12_step_batch* 
  * itself included (appended before): the query at position p sees keys
  * max(0, p - window + 1) .. p (window 0 = all). s = q . k * scaling, soft-capped
  * tanh(s / softcap) * softcap when softcap > 0 (2^-60 to 1024; held to 2^-22 of
- * it); softmax and sums in FP32, weights rounded to BF16 for the product with v. q BF16 [tokens, heads,
- * head_dim], rows q_stride apart (a multiple of 8), 16-byte aligned, already
- * rotated; out BF16 [tokens, heads, head_dim] contiguous, 8-byte aligned, apart
- * from q. heads a multiple of kv_heads. What a query may not see has no part in its row,
- * whatever it holds (NaN too); a query that sees nothing gives zeros.
+ * it); softmax and sums in FP32, weights rounded to BF16 for the product with v.
+ * q BF16 [tokens, heads, head_dim], rows q_stride apart (a multiple of 8), 16-byte
+ * aligned, already rotated; out BF16 [tokens, heads, head_dim] contiguous, 8-byte
+ * aligned, apart from q. heads a multiple of kv_heads. What a query may not see
+ * has no part in its row, whatever it holds (NaN too); a query that sees nothing
+ * gives zeros. Any finite values of BF16 pages give finite results, those of E4M3
+ * pages where none is above 2^112 / keys.
  *
  * `workspace`: se12_step_paged_attention_workspace() bytes for the shape (or for
- * one of more tokens), 256-byte aligned, contents indifferent; calls sharing it (two captured graphs
- * too) must not run concurrently. Two launches, four where max_new allows a
- * sequence more than 64 (token, query head) pairs to a KV head; results do not
- * depend on timing. */
+ * one of more tokens), 256-byte aligned, contents indifferent; calls sharing it
+ * (two captured graphs too) must not run concurrently. Two launches, four where
+ * max_new allows a sequence more than 64 (token, query head) pairs to a KV head;
+ * results do not depend on timing. */
 int64_t se12_step_paged_attention_workspace(const se12_step_pages* pages, const se12_step_batch* batch, int32_t heads);
 
 int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batch* batch, const uint16_t* q,

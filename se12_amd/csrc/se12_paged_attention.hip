@@ -154,7 +154,7 @@ struct Attend {
         float sc[kPer], top = 0.0f, vs = 1.0f;
         bf16x8_t pf[kHalves];
         auto weights = [&]() {
-            const float base = m == -INFINITY ? 0.0f : m;
+            const float base = (m == -INFINITY ? 0.0f : m) + (CT == SE12_STEP_BF16 ? a.shift : 0.0f);
 #pragma unroll
             for (int h = 0; h < kHalves; ++h) {
                 uint32_t u[4];
@@ -544,9 +544,11 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
     if (overlap(q, 2 * ((b.tokens - 1) * q_stride + row), out, 2 * b.tokens * row))
         return step_fail(fn, "out overlaps q");
     const PromptPlan plan = plan_of(pages, b, group);
+    const int64_t held = (int64_t)b.width * pages->page_size, seen = window > 0 ? std::min<int64_t>(held, window) : held;
+    const float shift = kSlack + 1.0f + (float)(64 - __builtin_clzll((uint64_t)seen));
     AttendArgs a{q, q_stride, out, pages->k, pages->v, pages->k_scale, pages->v_scale, b, heads, pages->kv_heads, group, pages->pages,
                  log2_of(pages->page_size), window, c1,
-                 softcap * kLog2E, static_cast<float*>(workspace), worker_count(pages, b, group), column_count(b, group),
+                 softcap * kLog2E, shift, static_cast<float*>(workspace), worker_count(pages, b, group), column_count(b, group),
                  reinterpret_cast<UnitWork*>(static_cast<char*>(workspace) + few_bytes(pages, b, group)),
                  (int)plan.slots + plan.parts, plan.parts / 2, plan.parts, plan.most};
     const hipStream_t st = static_cast<hipStream_t>(stream);

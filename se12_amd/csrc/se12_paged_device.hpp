@@ -56,6 +56,11 @@ struct AttendArgs {
     Batch b;
     int heads, kvh, group, pages, page_log2, window;
     float c1, cap;       // scores: c1 x (no cap), or cap - 2 cap / (1 + 2^(c1 x)), base 2
+    // BF16 pages: weights are 2^-shift of what they are, so that they add up to less than
+    // one and sums of any finite values stay finite (the largest weight is 2^-47 at least).
+    // An E4M3 page's scale takes that range: with weights up to 2^kSlack, values of up to
+    // 2^112 / keys are safe, and pages of the least scale, 2^-100, keep weights of 2^-26.
+    float shift;
     float* part;         // sums of a part of a unit's keys, then their (m, l)
     int workers, columns;
     // sequences of more than kFewColumns columns are se12_paged_prompt.hip's: what its

@@ -221,7 +221,8 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
         return __builtin_amdgcn_ballot_w64(bad) != 0;
     };
     float sc[16], top = 0.0f;      // scores, or r of cap - 2 cap r
-    float lv = 0.0f, iv = 1.0f;    // the values' scale, in the weights' exponent: log2, and its inverse
+    // the values' scale, in the weights' exponent: log2, and its inverse
+    float lv = CT == SE12_STEP_BF16 ? -a.shift : 0.0f, iv = 1.0f;
     bf16x8_t pf[2];
     auto weights = [&]() {
         const float base = (m == -INFINITY ? 0.0f : m) - lv;

@@ -537,6 +537,24 @@ def test_positions_beyond_the_table_are_what_they_are(gpu, dtype, lengths, new, 
         assert (got[starts[2]:starts[3]] == 0).all()      # (from 90 on nothing held is within 20)
 
 
+@pytest.mark.parametrize("d,lengths,new,window", [(128, [1500, 40], [1, 1], 0), (64, [3000, 0, 700], [70, 90, 1], 0), (256, [900], [40], 300)])
+@pytest.mark.parametrize("size", [2.0 ** 127, 2.0 ** 100, 2.0 ** -70])
+def test_any_finite_values_of_bf16_pages_stay_finite(gpu, d, lengths, new, window, size):
+    """Weights add up to less than one, as weights that are normalised first: sums of the type's largest values are no
+    infinities, and keys that grow along the sequence move the maximum."""
+    c, batch, q, _ = _attend_case(gpu, BF16, d, 32, 4, 2, lengths, new, 0.0, window, seed=76, extra=0)
+    page_scale = torch.exp2(torch.arange(batch.page_table.shape[1]).float() / 8 - 3).to(gpu)
+    for row in batch.page_table.long():
+        c.k[row] = (c.k[row].float() * page_scale[:, None, None, None]).to(BF16)
+    c.v.copy_((c.v.float().sign() * (1 + c.v.float().abs().fmod(0.9))).mul(size).to(BF16))
+    kp, vp, ks, vs = _state(c)
+    table, starts = batch.page_table.tolist(), batch.starts.tolist()
+    ref, ref_size, _ = o.attend(kp, vp, ks, vs, table, lengths, starts, q.cpu(), d ** -0.5, 0.0, window, batch.max_new)
+    got = c.attend(batch, q, d ** -0.5, window=window).cpu().double()
+    # (scores reach 2^8 here, as bounded for keys that grow: 2^-24 * 256 * 2^8 in the weights' exponents)
+    assert ((got - ref).abs() <= 2.0 ** -8 * ref.abs() + (2.0 ** -8 + 2.0 ** -6) * ref_size).all()
+
+
 def test_attend_with_sharp_scores_and_far_apart_tiles(gpu):
     """The maximum moves in many tiles: keys grow along the sequence; and one key holds all the weight."""
     for dtype in (E4M3, BF16):
