@@ -232,7 +232,8 @@ class PagedKvCache:
         written). No gradients.
 
         FP32 scores and sums; weights rounded to BF16. A query that sees nothing gives zeros. `workspace`: uint8 of at
-        least `attend_workspace()` bytes for callers that must not allocate; calls that share one must not overlap."""
+        least `attend_workspace()` bytes for callers that must not allocate; calls that share one must not overlap, and
+        one that a captured call was given lives, as its other tensors, as long as the graph."""
         self._check(batch)
         q = self._rows(q, "q", None, None, torch.bfloat16, 8)
         tokens, heads = q.shape[0], q.shape[1]

@@ -620,6 +620,42 @@ def test_what_the_workspace_of_prompts_held_does_not_matter(gpu, dtype, d, heads
 
 
 @pytest.mark.parametrize("dtype", [E4M3, BF16])
+def test_captured_prompts_follow_lengths_and_starts(gpu, dtype):
+    """One captured call over other divisions of the same rows at every replay: prompts, decode steps, nothing; two
+    graphs with a workspace of their own in turn, eager calls between them."""
+    d, page, heads, kvh = 128, 32, 8, 2
+    c, batch, q, out = _attend_case(gpu, dtype, d, page, heads, kvh, [500, 900, 20, 3], [100, 1, 60, 39], 0.0, 0, seed=35, extra=0)
+    # (slots that nobody held are read below: numbers in place of the NaN there)
+    for t in (c.k, c.v, c.k_scale, c.v_scale):
+        if t is not None:
+            t.copy_(t.float().nan_to_num(0.125).to(t.dtype))
+    kp, vp, ks, vs = _state(c)
+    calls = []
+    for window in (0, 300):
+        ws = torch.full((c.attend_workspace(batch, 200, heads),), 255, dtype=torch.uint8, device=gpu)
+        y = torch.empty_like(out)
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            c.attend(batch, q, d ** -0.5, window=window, out=y, workspace=ws)
+        calls.append((window, graph, y, ws))      # (what a graph writes to lives as long as it)
+    for lengths, starts in (([500, 900, 20, 3], [0, 100, 101, 161, 200]), ([500, 800, 20, 3], [0, 1, 101, 102, 102]),
+                            ([10, 890, 40, 2], [0, 33, 34, 134, 200]), ([599, 900, 79, 41], [0, 1, 2, 3, 4]),
+                            ([500, 900, 20, 3], [0, 100, 101, 161, 200])):
+        batch.lengths.copy_(torch.tensor(lengths, dtype=torch.int32))
+        batch.starts.copy_(torch.tensor(starts, dtype=torch.int32))
+        for window, graph, y, _ in calls:
+            y.fill_(5.0)
+            graph.replay()
+            eager = c.attend(batch, q, d ** -0.5, window=window, out=torch.full_like(out, 5.0))
+            torch.cuda.synchronize()
+            assert torch.equal(y, eager) and (y[starts[-1]:] == 5.0).all()
+            ref, size, mine = o.attend(kp, vp, ks, vs, batch.page_table.tolist(), lengths, starts, q.cpu(), d ** -0.5, 0.0, window, 100)
+            _close(y, ref, size, mine)
+    assert torch.equal(calls[0][2], out)
+
+
+@pytest.mark.parametrize("dtype", [E4M3, BF16])
 @pytest.mark.parametrize("lengths,new,window", [
     ([0, 6000, 0, 40], [64, 64, 33, 200], 0),                  # one unit is most of the work
     ([2500, 10, 10, 10, 10, 10], [33, 33, 40, 50, 60, 70], 0),
