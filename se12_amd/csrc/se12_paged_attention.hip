@@ -14,6 +14,10 @@
 // 16 keys of a column in a lane. So keys, values and probabilities go from
 // memory through registers only: no LDS, no exchange between lanes, and the
 // scales (one page at least holds 16 keys) are one number per lane and tile.
+// Scores, statistics and sums are FP32; a weight, times the values' scale, is rounded to
+// BF16, the type of the second product's operands: off by 2^-8 of it at most, as the output
+// is by its own rounding, and less in a sum over many keys. (A weight in two BF16 parts
+// would double the second product.)
 //
 // Bound by the bytes of the pages: 32 sequences of up to 4,095 keys, 16 / 8 heads of 256
 // in E4M3 (309 MB) take 60 us and 4 to join, 4.9 TB/s; 24 of up to 5,000 in BF16 under a
@@ -359,11 +363,15 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : 2) void paged_attent
     }
 }
 
-// The units that several workers share, from their parts in order: one block per
-// (sequence, KV head, column unit) and column (or every fourth). D / 4 lanes take every
-// kParts-th part, the loads of four at once, or of eight where there are as many (85 parts
-// at D = 128: 6.8 us by four, 6.1 so; 12 at once are 8.0, for few parts 6.8 from 4.6); a
-// part's maximum may lie above those before it, so what is summed moves with it.
+// The units that several workers share, from their parts in order: a block (for every
+// column, or every fourth) per (sequence, KV head, column unit), or, where those are many
+// beside the workers (max_units 0), per worker, which joins the unit that the worker begins
+// and others go on with. (1,024 sequences to 1,000 keys, 16 / 8 heads of 256, a block per
+// unit: 126 us, and 848 where max_new allows 64 columns; per worker 43 and 60.) D / 4
+// lanes take every kParts-th part, the loads of four at once, or of eight where there are
+// as many (85 parts at D = 128: 6.8 us by four, 6.1 so; 12 at once are 8.0, for few parts
+// 6.8 from 4.6); a part's maximum may lie above those before it, so what is summed moves
+// with it.
 template <int CT, int D>
 __global__ __launch_bounds__(kAttendThreads) void paged_join_kernel(AttendArgs a, int max_units) {
     constexpr int kTile = Form<CT>::kTile;
@@ -371,20 +379,46 @@ __global__ __launch_bounds__(kAttendThreads) void paged_join_kernel(AttendArgs a
     __shared__ float4 sums[kAttendThreads];
     __shared__ float2 mls[kParts];
     const int tid = threadIdx.x, lane = tid & 63, part = tid / kLanes, at = tid % kLanes;
-    const int unit = (int)(blockIdx.x % max_units), kh = (int)(blockIdx.x / max_units % a.kvh), s = (int)(blockIdx.x / max_units / a.kvh);
-    Chunk chunk = load_chunk<kTile>(a, s & ~63, lane);
-    const SeqWork w = seq_work<kTile>(a, seq_of(chunk, s & 63));
-    if (unit >= w.units) return;
-    int64_t base = __builtin_amdgcn_readlane(chunk.upto, s & 63) - __builtin_amdgcn_readlane(chunk.tiles, s & 63), total = chunk.all;
-    for (int s0 = 0; s0 < a.b.seqs; s0 += 64) {
-        if (s0 == (s & ~63)) continue;
-        const int all = load_chunk<kTile>(a, s0, lane).all;
-        total += all;
-        base += s0 < s ? all : 0;
+    int unit, kh;
+    SeqWork w;
+    int64_t first, per;      // the unit's first tile, tiles of a worker
+    if (max_units > 0) {
+        unit = (int)(blockIdx.x % max_units);
+        kh = (int)(blockIdx.x / max_units % a.kvh);
+        const int s = (int)(blockIdx.x / max_units / a.kvh);
+        const Chunk chunk = load_chunk<kTile>(a, s & ~63, lane);
+        w = seq_work<kTile>(a, seq_of(chunk, s & 63));
+        if (unit >= w.units || unit * kColumns + (int)blockIdx.y >= w.seq.n * a.group) return;
+        int64_t base = __builtin_amdgcn_readlane(chunk.upto, s & 63) - __builtin_amdgcn_readlane(chunk.tiles, s & 63), total = chunk.all;
+        for (int s0 = 0; s0 < a.b.seqs; s0 += 64) {
+            if (s0 == (s & ~63)) continue;
+            const int all = load_chunk<kTile>(a, s0, lane).all;
+            total += all;
+            base += s0 < s ? all : 0;
+        }
+        per = tiles_each(total);
+        first = base + ((int64_t)kh * w.units + unit) * w.tiles;
+    } else {
+        Chunk chunk = load_chunk<kTile>(a, 0, lane);
+        int64_t total = chunk.all, before = 0;
+        for (int s0 = 64; s0 < a.b.seqs; s0 += 64) total += load_chunk<kTile>(a, s0, lane).all;
+        per = tiles_each(total);
+        const int64_t at = ((int64_t)blockIdx.x + 1) * per;      // where the next worker begins
+        if (at >= total) return;
+        for (int s0 = 64; before + chunk.all <= at; s0 += 64) {
+            before += chunk.all;
+            chunk = load_chunk<kTile>(a, s0, lane);
+        }
+        const int of = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before + chunk.upto > at));
+        w = seq_work<kTile>(a, seq_of(chunk, of));
+        const int in = (int)(at - before) - (__builtin_amdgcn_readlane(chunk.upto, of) - __builtin_amdgcn_readlane(chunk.tiles, of));
+        const int line = in / w.tiles, tile = in - line * w.tiles;
+        kh = line / w.units;
+        unit = line - kh * w.units;
+        first = at - tile;
+        if (tile == 0 || worker_of(first, per) != (int)blockIdx.x) return;
     }
-    const int64_t per = tiles_each(total);
-    const int64_t first = base + ((int64_t)kh * w.units + unit) * w.tiles, last = first + w.tiles - 1;
-    const int w0 = worker_of(first, per), w1 = worker_of(last, per);
+    const int w0 = worker_of(first, per), w1 = worker_of(first + w.tiles - 1, per);
     if (w0 == w1) return;      // one worker had it all
     const float2* mlp = reinterpret_cast<const float2*>(a.part + (int64_t)a.workers * 2 * a.columns * D);
     for (int col = blockIdx.y; col < kColumns; col += gridDim.y) {
@@ -484,9 +518,7 @@ PromptPlan plan_of(const se12_step_pages* p, const Batch& b, int group) {
 
 // what one launch holds, and what 32 bits hold of it
 const char* limits_error(const se12_step_pages* p, const Batch& b, int group) {
-    const int64_t few = (int64_t)b.seqs * p->kv_heads * ((std::min<int64_t>((int64_t)b.max_new * group, kFewColumns) + kColumns - 1) / kColumns);
-    if ((int64_t)b.tokens * group > INT32_MAX || !grid_fits(few, kAttendThreads) ||
-        !grid_fits(plan_of(p, b, group).records * p->kv_heads, kAttendThreads))
+    if ((int64_t)b.tokens * group > INT32_MAX || !grid_fits(plan_of(p, b, group).records * p->kv_heads, kAttendThreads))
         return "too many sequences, tokens and heads for one launch";
     if (std::min<int64_t>(b.seqs, 64) * (((int64_t)b.width * p->page_size + 31) / 32) * (kFewColumns / kColumns) * p->kv_heads > INT32_MAX)
         return "too long a table for so many sequences and heads";
@@ -504,8 +536,12 @@ void launch_attend(const AttendArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((paged_attention_kernel<CT, D>), dim3((uint32_t)(((int64_t)a.workers + a.unit_count + a.join_count + kWaves - 1) / kWaves)),
                        dim3(kAttendThreads), 0, st, a);
     const int max_units = (int)((std::min<int64_t>((int64_t)a.b.max_new * a.group, kFewColumns) + kColumns - 1) / kColumns);
-    hipLaunchKernelGGL((paged_join_kernel<CT, D>), dim3((uint32_t)((int64_t)a.b.seqs * a.kvh * max_units), max_units > 1 ? 4 : a.columns),
-                       dim3(kAttendThreads), 0, st, a, max_units);
+    const int64_t units = (int64_t)a.b.seqs * a.kvh * max_units;
+    // (half as many again where each can be there: 130 sequences of one token, 8 KV heads of
+    // 128, the call 29.7 us a block per unit, 30.8 per worker; 200 of 256 196 either way)
+    const bool by_unit = units <= (max_units > 1 ? a.workers : a.workers + a.workers / 2);
+    hipLaunchKernelGGL((paged_join_kernel<CT, D>), dim3(by_unit ? (uint32_t)units : (uint32_t)a.workers, max_units > 1 ? 4 : a.columns),
+                       dim3(kAttendThreads), 0, st, a, by_unit ? max_units : 0);
 }
 
 }  // namespace

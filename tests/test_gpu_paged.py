@@ -360,6 +360,18 @@ def test_many_tiles_to_a_wave(gpu, dtype, d, page, heads, kvh, softcap, window):
 
 
 @pytest.mark.parametrize("dtype", [E4M3, BF16])
+@pytest.mark.parametrize("seqs,new,max_new,length,window", [(600, (1, 1, 0), 1, 150, 0), (150, (1, 2, 1, 0), 200, 700, 0), (90, (1, 7, 25), 40, 300, 60),
+                                                            (600, (1,), 1, 20, 0), (900, (1,), 1, 90, 0)])
+def test_more_units_than_waves(gpu, dtype, seqs, new, max_new, length, window):
+    """Units that several waves share are joined by those that begin them."""
+    lengths = [(i * 271) % length for i in range(seqs)]
+    news = [new[i % len(new)] for i in range(seqs)]
+    if max_new == 200:
+        news[77], lengths[5] = 100, 6000
+    _attend_case(gpu, dtype, 64, 16, 8, 4 if seqs < 100 else 2, lengths, news, 0.0, window, seed=36, max_new=max_new)
+
+
+@pytest.mark.parametrize("dtype", [E4M3, BF16])
 @pytest.mark.parametrize("window", [0, 90])
 def test_prompts_among_more_sequences_than_a_wave_scans(gpu, dtype, window):
     """Units of prompts in the second 64 sequences too, decode steps and sequences with nothing between them."""

@@ -256,6 +256,7 @@ def test_grids_of_more_threads_than_32_bits_count_are_refused():
     with pytest.raises(nat.Se12Error, match="too many"):
         nat.step_check(lib.se12_step_paged_append(ctypes.byref(p), ctypes.byref(b), None, P, P, nat.STEP_F32, 0, 1 << 17, 1 << 17, 1024, None,
                                                   0, None, None))
+    b = _batch(sequences=65536, tokens=1 << 25, max_new=1 << 20)
     with pytest.raises(nat.Se12Error, match="too many sequences, tokens"):
         nat.step_check(lib.se12_step_paged_attention_workspace(ctypes.byref(p), ctypes.byref(b), 1024))
     with pytest.raises(nat.Se12Error, match="too many rows"):
