@@ -10,11 +10,14 @@
 // its bytes have one writer and no order to depend on; further blocks rotate q,
 // a wave per token. Angles: position * inv_freq in quarter turns, in 64 bits
 // (positions beyond 2^17 would lose a radian's third digit in FP32); sine and cosine
-// of what is beyond a whole quarter, up to pi / 4, by their series, a unit or two of
-// 2^-24 off. Bound by the bytes of q, k and v at prompt sizes: 9,001 BF16 tokens of 16
-// and 8 heads of 256 (258 MB) take 64 us (68 with a library's sine and cosine;
-// 62 with the card's instructions, whose 2^-23 change an E4M3 digit ten times as
-// often); at decode sizes by the launch: 48 tokens, 7 us.
+// of what is beyond a whole quarter, up to pi / 4, rounded once, by their series, so that
+// q and k are as close to the exact rotation as with FP32 sines and cosines of 64-bit
+// angles (in 9,001 tokens 24 E4M3 digits and 840 BF16 ones are not the exact one's; 25 and
+// 930 that way; 26 and 1,040 with the fraction turned into an angle in FP32). Bound by the
+// bytes of q, k and v at prompt sizes: 9,001 BF16 tokens of 16 and 8 heads of 256 (258 MB)
+// take 65 us (68 with a library's sine and cosine; 62 with the card's instructions, whose
+// 2^-23 change an E4M3 digit ten times as often); at decode sizes by the launch: 48
+// tokens, 7 us.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -78,9 +81,9 @@ __device__ __forceinline__ Turn turn_of(const float* inv_freq, int lo, int pos) 
         // (to a whole number in the last places of a double's 53 bits)
         const double quarters = (double)pos * (double)w[i] * 0.63661977236758134, whole = quarters + 0x1.8p52;
         const int turn = __double2loint(whole);
-        const float x = (float)(quarters - (whole - 0x1.8p52)) * 1.57079632679489662f, x2 = x * x;
+        const float x = (float)((quarters - (whole - 0x1.8p52)) * 1.57079632679489662), x2 = x * x;
         const float s = fmaf(x * x2, fmaf(x2, fmaf(x2, fmaf(x2, 1.0f / 362880, -1.0f / 5040), 1.0f / 120), -1.0f / 6), x);
-        const float c = fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, -1.0f / 3628800, 1.0f / 40320), -1.0f / 720), 1.0f / 24), -0.5f), 1.0f);
+        const float c = 1.0f + fmaf(x, -0.5f * x, x2 * x2 * fmaf(x2, fmaf(x2, fmaf(x2, -1.0f / 3628800, 1.0f / 40320), -1.0f / 720), 1.0f / 24));
         const uint32_t sn = __float_as_uint(turn & 1 ? c : s), cs = __float_as_uint(turn & 1 ? s : c);
         t.s[i] = __uint_as_float(sn ^ ((uint32_t)(turn & 2) << 30));
         t.c[i] = __uint_as_float(cs ^ ((uint32_t)((turn + 1) & 2) << 30));

@@ -185,6 +185,30 @@ def test_append_without_q_and_with_a_far_position(gpu):
     _check_append(c, before, batch, lengths, starts, table, k, v, inv)
 
 
+def test_rotations_are_as_close_as_fp32_sines_of_64_bit_angles(gpu):
+    """Of 42 million turned values, rounded to BF16, those that are not the exact rotation's: no more than of FP32
+    arithmetic with sines and cosines rounded from 64 bits, which rounds once more (a product) per value."""
+    c, d, heads = _cache(gpu, 40, 64, 8, 256, BF16, 77), 256, 8
+    lengths, new = [0, 40_000, 3], [300, 500, 224]
+    batch, starts = _batch(gpu, [[-1] * 700] * 3, lengths, new)
+    inv = (10000.0 ** (-torch.arange(0, d, 2).float() / d)).to(gpu)
+    k = torch.zeros((1024, 8, d), device=gpu)
+    pos = torch.cat([torch.arange(a, a + n) for a, n in zip(lengths, new)]).to(gpu)
+    angle = pos.double()[:, None, None] * inv.double()
+    far = [0, 0]
+    for seed in range(20):
+        q = torch.randn((1024, heads, d), generator=_gen(78 + seed)).to(gpu)
+        a, b = q[..., :128], q[..., 128:]
+        exact = torch.cat([a.double() * angle.cos() - b.double() * angle.sin(), b.double() * angle.cos() + a.double() * angle.sin()], -1)
+        cos, sin = angle.cos().float(), angle.sin().float()
+        plain = torch.cat([a * cos - b * sin, b * cos + a * sin], -1)
+        got = c.append(batch, k, k, q=q, inv_freq=inv)
+        want = exact.to(BF16)
+        far[0] += (got != want).sum().item()
+        far[1] += (plain.to(BF16) != want).sum().item()
+    assert far[0] <= far[1], far
+
+
 def test_scales_grow_and_older_tokens_are_rounded_again(gpu):
     page, kvh, d = 16, 2, 64
     c = _cache(gpu, 4, page, kvh, d, E4M3, 7)
