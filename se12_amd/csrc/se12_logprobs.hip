@@ -17,10 +17,11 @@
 // The waves of a block and the blocks of a row merge the same way, the latter in a
 // second launch, where rows are too few to fill the card with a block each.
 //
-// Bound by its bytes where rows are many: 1,024 FP32 rows of 256,000 under a cap, top
-// 5, 1,049 MB in 192 us (5.5 TB/s; the arithmetic alone about 130: three instructions of
-// a quarter of the rate to a logit). One such row, top 20: 6.7 + 4.4 us, two launches'
-// latency and the rankings; 40 rows of 100,277 in BF16, top 5: 8.2 + 4.5.
+// Bound by its bytes where rows are many and in FP32: 1,024 of 256,000, top 5, 1,049 MB in
+// 186 us, under a cap 192 (5.5 TB/s); in BF16 by its bytes without a cap, 117 us (4.5 TB/s),
+// and with one by the arithmetic, 152 (three instructions of a quarter of the rate and seven
+// others to a logit). One FP32 row, top 20: 6.9 + 4.6 us, two launches' latency and the
+// rankings; 40 rows of 100,277 in BF16, top 5: 8.2 + 4.7.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -15,9 +15,12 @@
 // piece of 16 rows take all banks once.
 //
 // Bound by the instructions of the one wave a SIMD has room for at head dim 256 (128
-// sums, 64 registers of Q): per 32 keys 388 vector instructions, a third of them
-// conversions of 8 bits, in 1,750 cycles, beside 1,030 of the matrix unit. 6,194 tokens of
-// 5 prompts behind up to 1,500 keys, 8 / 4 heads of 256, E4M3, cap: 159 us, 0.53 PFLOP/s.
+// sums, 64 registers of Q): of 3,190 cycles to 32 keys it issues for 2,230, 1,830 of them
+// 374 vector and 32 matrix instructions (a third of the vector ones convert 8 bits), and
+// waits for 680; the matrix unit is busy for 1,030, beside other instructions for the most
+// part. 6,194 tokens of 5 prompts behind up to 1,500 keys, 8 / 4 heads of 256, E4M3, cap:
+// 159 us, 0.53 PFLOP/s. BF16 pages: 5,040 cycles, 1,780 of them waits (tiles of 32 keys,
+// so twice the barriers, and twice the bytes): 64 x 64 tokens behind 2,048 160 us, 113 from E4M3.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
