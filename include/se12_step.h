@@ -177,8 +177,8 @@ typedef struct se12_step_batch {
  * least the scale they have, and if it grows they are rounded again to the new
  * one (powers of two: exact but for values that become subnormal). NaN and
  * infinities are held as NaN. Slots behind the new tokens keep their bytes. A
- * page that two sequences of a call write, or that a concurrent call reads or
- * writes, has undefined contents. */
+ * page that a call writes under two entries of the table (of two sequences, or of
+ * one), or that a concurrent call reads or writes, has undefined contents. */
 int se12_step_paged_append(const se12_step_pages* pages, const se12_step_batch* batch, const void* q, const void* k,
                            const void* v, int32_t dtype, int64_t q_stride, int64_t k_stride, int64_t v_stride,
                            int32_t heads, const float* inv_freq, int32_t rotary, uint16_t* q_out, void* stream);

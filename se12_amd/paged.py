@@ -190,7 +190,7 @@ class PagedKvCache:
 
         An E4M3 page and head's scale is the least power of two (2^-100 or more) that holds its new values; with older
         tokens in the page at least what it was, and if it grows the older ones are rounded again. NaN and infinities
-        are held as NaN. A page that two sequences share must not be written by a call."""
+        are held as NaN. A page that two entries of the table name must not be written by a call."""
         self._check(batch)
         if not isinstance(k, torch.Tensor) or k.dtype not in (torch.bfloat16, torch.float32):
             raise ValueError("k must be a bfloat16 or float32 tensor")
