@@ -208,8 +208,7 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
 
 /* What a serving program reports of logits [rows, stride] (BF16 or FP32, vocab
  * of a row used), with z = softcap tanh(logit / softcap) when softcap > 0 (2^-60 to
- * 1024; held to 2^-22 of a cap of up to 64, of z under a larger one), else the
- * logit, and p = softmax(z) in FP32:
+ * 1024; held to 2^-22 of itself), else the logit, and p = softmax(z) in FP32:
  *   logprobs[r]  log p of tokens[r] (-inf for a token outside [0, vocab))
  *   entropy[r]   -sum p log p
  *   top_logprobs, top_ids [rows, top]  the `top` (0 .. 32) most likely tokens,

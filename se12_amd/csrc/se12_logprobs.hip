@@ -19,9 +19,9 @@
 //
 // Bound by its bytes where rows are many and in FP32: 1,024 of 256,000, top 5, 1,049 MB in
 // 186 us, under a cap 192 (5.5 TB/s); in BF16 by its bytes without a cap, 117 us (4.5 TB/s),
-// and with one by the arithmetic, 152 (three instructions of a quarter of the rate and seven
-// others to a logit). One FP32 row, top 20: 6.9 + 4.6 us, two launches' latency and the
-// rankings; 40 rows of 100,277 in BF16, top 5: 8.2 + 4.7.
+// and with one by the arithmetic, 145 (an instruction of a quarter of the rate and eleven
+// others to a logit). One FP32 row, top 20: 6.6 + 4.6 us, two launches' latency and the
+// rankings; 40 rows of 100,277 in BF16, top 5: 8.0 + 4.6.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -42,9 +42,8 @@ constexpr int kKeys = 128;                     // of a wave's buffer: 32 best an
 constexpr int kBlocksWanted = 1024;            // four to a CU
 constexpr int kJoinKeys = 8;                   // that a thread of the second launch loads at once
 constexpr float kLog2E = 1.4426950408889634f;
-constexpr float kFineCap = 64.0f;
 
-// of a part of a row: the reference, S, and W in units of log 2
+// of a part of a row: the maximum (of capped logits in units of log 2), S, and W in units of log 2
 struct Stats {
     float m, s, w;
 };
@@ -53,8 +52,9 @@ struct LogprobArgs {
     const void* logits;
     int64_t stride;
     int vocab, top, slices, slice;             // slice: logits of a block, a multiple of kLpWaves * kChunk
-    float cap, inv_cap2;                       // inv_cap2: 2 log2(e) / cap
-    float unit, unit2;                         // of y: 2 cap or 1, and that times log2(e)
+    float cap, half, inv_cap2;                 // base 2: the cap; |x| of the polynomial; 2 log2(e) / cap
+    float unit, unit2;                         // of z: to units of 1, and of log 2
+    float k[5];                                // the polynomial's coefficients
     const int64_t* tokens;
     float* logprobs;
     float* entropy;
@@ -157,19 +157,23 @@ struct Best {
     }
 };
 
-// What is summed: z = unit y + a constant, y = -1 / (1 + e^(2 x / cap)) under a cap (z =
-// cap + 2 cap y), else x. Differences of y are taken before the unit, so what two logits
-// close to each other, or one and itself, have in common leaves no rounding behind. That
-// y is off by 2^-24 wherever x lies, z by 2^-22 of the cap: under one of 64 no more than
-// twice what FP32 leaves of logits near it. Under a larger one (z = 2 cap y) y is half the
-// hyperbolic tangent, whose error is of its own size.
-template <bool kFine>
-__device__ __forceinline__ float y_of(const LogprobArgs& a, float x) {
-    if constexpr (kFine) return 0.5f * tanhf(x * a.inv_cap2 * (0.5f / kLog2E));
-    return a.cap > 0.0f ? -__builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * a.inv_cap2)) : x;
+// Capped logits in units of log 2, z = log2(e) cap tanh(u), u = x / cap, off by 3 units of
+// 2^-24 of themselves: up to cap / 2 as x p(x^2), p fitted (kTanh), beyond from e^(2 |u|).
+// The same x has the same z wherever it is taken (the product is rounded, not made part of
+// a difference), so a maximum's own term is 1.
+__device__ __forceinline__ float z_near(const LogprobArgs& a, float x) {
+#pragma clang fp contract(off)
+    const float q = x * x;
+    return x * fmaf(q, fmaf(q, fmaf(q, fmaf(q, a.k[4], a.k[3]), a.k[2]), a.k[1]), a.k[0]);
 }
 
-// sums on a reference moved up to `to`
+__device__ __forceinline__ float z_of(const LogprobArgs& a, float x) {
+    if (a.cap == 0.0f) return x;
+    const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(fabsf(x) * a.inv_cap2));
+    return fabsf(x) < a.half ? z_near(a, x) : copysignf(fmaf(-2.0f * a.cap, r, a.cap), x);
+}
+
+// sums on a maximum moved up to `to`
 __device__ __forceinline__ Stats moved(const LogprobArgs& a, Stats v, float to) {
     // (of m = -inf there is no sum; a NaN stays one)
     const float d = v.m == -INFINITY ? 0.0f : (to - v.m) * a.unit2, f = __builtin_amdgcn_exp2f(-d);
@@ -194,11 +198,10 @@ __device__ __forceinline__ bool token_logit(const LogprobArgs& a, int row, float
 }
 
 // the row's results, by one wave, from its sums and its best keys in order
-template <bool kFine>
 __device__ __forceinline__ void finish_row(const LogprobArgs& a, int row, Stats v, const Best& best, bool valid, float x) {
     const int lane = threadIdx.x & 63;
     const float log_s = logf(v.s);
-    auto logprob = [&](float x) { return v.m == -INFINITY && v.s == 0.0f ? -INFINITY : (y_of<kFine>(a, x) - v.m) * a.unit - log_s; };
+    auto logprob = [&](float x) { return v.m == -INFINITY && v.s == 0.0f ? -INFINITY : (z_of(a, x) - v.m) * a.unit - log_s; };
     if (lane == 0) {
         // (a token that there is not: -inf, in a row of numbers)
         const float lp = valid ? logprob(x) : v.s != v.s ? v.s : -INFINITY;
@@ -254,8 +257,8 @@ __device__ __forceinline__ bool join_waves(const LogprobArgs& a, Stats& v, Best&
     return true;
 }
 
-template <int DT, bool kFine>
-__global__ __launch_bounds__(kLpThreads, kFine ? 2 : 6) void logprobs_kernel(LogprobArgs a) {
+template <int DT>
+__global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(LogprobArgs a) {
     constexpr int kVec = DT == SE12_STEP_F32 ? 4 : 8, kVecs = kLpPer / kVec, kSize = 16 / kVec;
     __shared__ Waves waves;
     __shared__ float held[kLpWaves][kChunk];
@@ -352,32 +355,40 @@ __global__ __launch_bounds__(kLpThreads, kFine ? 2 : 6) void logprobs_kernel(Log
                 bar = best.bar_number();
             }
         }
-        most = y_of<kFine>(a, most);
+        most = z_of(a, most);
         if (__builtin_amdgcn_ballot_w64(most > v.m) != 0) v = moved(a, v, fmaxf(v.m, wave_max(most)));
         if (v.m == -INFINITY) {
             // nothing but -inf so far, unless there is a NaN
 #pragma unroll
             for (int k = 0; k < kLpPer; ++k) v.s = x[k] != x[k] ? x[k] : v.s;
         } else if (a.cap > 0.0f) {
-            // (three instructions of a quarter of the rate and seven others to a logit)
-            auto add = [&](auto at_edge) {
+            // (a logit within cap / 2 takes an instruction of a quarter of the rate and eleven
+            // others, one beyond three and sixteen: 1,024 BF16 rows of 256,000 145 us; 152 with
+            // the second form, in cap - 2 cap r, off by 2^-22 of the cap, for all)
+            float far = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kLpPer; ++k) far = fmaxf(far, fabsf(x[k]));
+            auto add = [&](auto near, auto at_edge) {
 #pragma unroll
                 for (int k = 0; k < kLpPer; ++k) {
-                    float d = (v.m - y_of<kFine>(a, x[k])) * a.unit2;
+                    float d = v.m - (near.value ? z_near(a, x[k]) : z_of(a, x[k]));
                     if (at_edge.value && outside(k)) d = 1e30f;
                     const float e = __builtin_amdgcn_exp2f(-d);
                     v.s += e;
                     v.w = fmaf(e, d, v.w);
                 }
             };
+            // (a NaN that the maximum leaves out stays one either way)
             if (edge)
-                add(std::true_type{});
+                add(std::false_type{}, std::true_type{});
+            else if (__builtin_amdgcn_ballot_w64(far >= a.half) != 0)
+                add(std::false_type{}, std::false_type{});
             else
-                add(std::false_type{});
+                add(std::true_type{}, std::false_type{});
         } else {
 #pragma unroll
             for (int k = 0; k < kLpPer; ++k) {
-                const float d = (v.m - x[k]) * a.unit2, e = __builtin_amdgcn_exp2f(-d);
+                const float d = (v.m - x[k]) * kLog2E, e = __builtin_amdgcn_exp2f(-d);
                 v.s += e;
                 v.w = fmaf(e, fminf(d, 1e30f), v.w);
             }
@@ -385,7 +396,7 @@ __global__ __launch_bounds__(kLpThreads, kFine ? 2 : 6) void logprobs_kernel(Log
     }
     if (!join_waves(a, v, best, waves)) return;
     if (a.slices == 1) {
-        finish_row<kFine>(a, row, v, best, valid, token_x);
+        finish_row(a, row, v, best, valid, token_x);
         return;
     }
     if (lane == 0) a.stats[blockIdx.x] = v;
@@ -393,7 +404,7 @@ __global__ __launch_bounds__(kLpThreads, kFine ? 2 : 6) void logprobs_kernel(Log
 }
 
 // the slices of a row
-template <int DT, bool kFine>
+template <int DT>
 __global__ __launch_bounds__(kLpThreads) void logprobs_join_kernel(LogprobArgs a) {
     __shared__ Waves waves;
     __shared__ uint64_t held[kLpWaves][kJoinKeys * 64];
@@ -438,7 +449,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_join_kernel(LogprobArgs a
             best.offer(i < count ? keys[i] : 0);
         }
     }
-    if (join_waves(a, v, best, waves)) finish_row<kFine>(a, row, v, best, valid, token_x);
+    if (join_waves(a, v, best, waves)) finish_row(a, row, v, best, valid, token_x);
 }
 
 }  // namespace se12step
@@ -446,6 +457,10 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_join_kernel(LogprobArgs a
 using namespace se12step;
 
 namespace {
+
+// (tanh(u) / u - 1) / u^2 in powers of u^2, |u| <= 1/2: least squares with weights moved to
+// where tanh(u) is furthest off (2^-26 of it)
+constexpr double kTanh[4] = {-0.33333149552345276, 0.1332598775625229, -0.05305296927690506, 0.01725703850388527};
 
 struct LpLayout {
     int slices, slice;
@@ -465,12 +480,6 @@ LpLayout logprobs_layout(int32_t rows, int32_t vocab, int32_t top) {
     l.stats_bytes = ((int64_t)rows * l.slices * (int64_t)sizeof(Stats) + 15) / 16 * 16;
     l.total = l.slices == 1 ? 0 : l.stats_bytes + (int64_t)rows * l.slices * top * (int64_t)sizeof(uint64_t);
     return l;
-}
-
-template <int DT, bool kFine>
-void launch_logprobs(const LogprobArgs& a, dim3 grid, int rows, hipStream_t st) {
-    hipLaunchKernelGGL((logprobs_kernel<DT, kFine>), grid, dim3(kLpThreads), 0, st, a);
-    if (a.slices > 1) hipLaunchKernelGGL((logprobs_join_kernel<DT, kFine>), dim3(rows), dim3(kLpThreads), 0, st, a);
 }
 
 const char* logprobs_shape_error(int32_t rows, int32_t vocab, int32_t top) {
@@ -506,17 +515,43 @@ int se12_step_logprobs(const void* logits, int32_t dtype, int64_t stride, int32_
     if (!grid_fits((int64_t)rows * l.slices, kLpThreads)) return step_fail(fn, "too many rows");
     if (l.total > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < l.total))
         return step_fail(fn, "workspace missing, misaligned or too small");
-    const LogprobArgs a{logits, stride, vocab, top, l.slices, l.slice, softcap, softcap > 0.0f ? 2.0f * kLog2E / softcap : 0.0f,
-                        softcap > 0.0f ? 2.0f * softcap : 1.0f, softcap > 0.0f ? 2.0f * softcap * kLog2E : kLog2E,
-                        tokens, logprobs, entropy, top_logprobs, top_ids, static_cast<Stats*>(workspace),
-                        reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + (l.slices > 1 ? l.stats_bytes : 0))};
+    LogprobArgs a{};
+    a.logits = logits;
+    a.stride = stride;
+    a.vocab = vocab;
+    a.top = top;
+    a.slices = l.slices;
+    a.slice = l.slice;
+    a.cap = softcap * kLog2E;
+    a.unit = softcap > 0.0f ? 1.0f / kLog2E : 1.0f;
+    a.unit2 = softcap > 0.0f ? 1.0f : kLog2E;
+    if (softcap > 0.0f) {
+        a.inv_cap2 = 2.0f * kLog2E / softcap;
+        // (of smaller caps FP32 does not hold the coefficients, and no z is above 2^-14)
+        a.half = softcap >= 0x1p-14f ? 0.5f * softcap : 0.0f;
+        double k = 1.4426950408889634;
+        a.k[0] = (float)k;
+        for (int i = 0; i < 4 && a.half > 0.0f; ++i) {
+            k /= (double)softcap * softcap;
+            a.k[i + 1] = (float)(k * kTanh[i]);
+        }
+    }
+    a.tokens = tokens;
+    a.logprobs = logprobs;
+    a.entropy = entropy;
+    a.top_logprobs = top_logprobs;
+    a.top_ids = top_ids;
+    a.stats = static_cast<Stats*>(workspace);
+    a.keys = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + (l.slices > 1 ? l.stats_bytes : 0));
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const dim3 grid((uint32_t)((int64_t)rows * l.slices));
-    const bool fine = softcap > kFineCap;
-    if (dtype == SE12_STEP_F32)
-        fine ? launch_logprobs<SE12_STEP_F32, true>(a, grid, rows, st) : launch_logprobs<SE12_STEP_F32, false>(a, grid, rows, st);
-    else
-        fine ? launch_logprobs<SE12_STEP_BF16, true>(a, grid, rows, st) : launch_logprobs<SE12_STEP_BF16, false>(a, grid, rows, st);
+    if (dtype == SE12_STEP_F32) {
+        hipLaunchKernelGGL(logprobs_kernel<SE12_STEP_F32>, grid, dim3(kLpThreads), 0, st, a);
+        if (l.slices > 1) hipLaunchKernelGGL(logprobs_join_kernel<SE12_STEP_F32>, dim3(rows), dim3(kLpThreads), 0, st, a);
+    } else {
+        hipLaunchKernelGGL(logprobs_kernel<SE12_STEP_BF16>, grid, dim3(kLpThreads), 0, st, a);
+        if (l.slices > 1) hipLaunchKernelGGL(logprobs_join_kernel<SE12_STEP_BF16>, dim3(rows), dim3(kLpThreads), 0, st, a);
+    }
     return step_launched();
 }
 

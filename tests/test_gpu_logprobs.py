@@ -99,6 +99,26 @@ def test_a_large_cap_leaves_small_logits_their_digits(gpu, cap, rows, vocab):
     assert ((r.entropy.cpu().double() - ent).abs() <= 2 * (1 + math.log(vocab)) * tol(ent)).all()
 
 
+@pytest.mark.parametrize("cap", [20.0, 30.0, 64.0, 1000.0])
+def test_two_capped_logits_keep_their_digits(gpu, cap):
+    """Rows of two logits of up to 4: each z is off by 3 units of 2^-24 of itself at most (2 of its form, one of rounding),
+    their difference d by 2^-24 * 24, log p = -log(1 + e^d) by no more and a few units of its own. Rows of larger ones,
+    up to 1.5 caps: 4 units of the cap's half each (the quotient counts once more beyond cap / 2)."""
+    from se12_amd.logprobs import token_logprobs
+
+    for scale, off in ((1.0, 24 * 2.0 ** -24), (cap, 8 * cap * 2.0 ** -24)):
+        x = (torch.rand((4096, 2), generator=_gen(10)) * 2 - 1) * (4.0 if scale == 1.0 else 1.5 * cap)
+        t = torch.randint(0, 2, (4096,), generator=_gen(11))
+        r = token_logprobs(x.to(gpu), t.to(gpu), top=2, softcap=cap)
+        lp = torch.log_softmax(cap * torch.tanh(x.double() / cap), 1)
+        want, ent = lp.gather(1, t[:, None])[:, 0], torch.special.entr(lp.exp()).sum(1)
+        tol = off + 2.0 ** -22 * (1 + want.abs())
+        assert ((r.logprobs.cpu().double() - want).abs() <= tol).all(), ((r.logprobs.cpu().double() - want).abs() / tol).max()
+        assert (r.logprobs <= 0).all() and (r.entropy >= 0).all()
+        # (the entropy's derivative by d is d p (1 - p), below 1/2)
+        assert ((r.entropy.cpu().double() - ent).abs() <= off + 2.0 ** -21).all()
+
+
 def test_more_rows_than_blocks_fill_the_card(gpu):
     x, t = _logits(gpu, 1500, 2100, torch.bfloat16, 2)
     _check(x, t, 3, 0.0)
