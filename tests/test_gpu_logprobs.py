@@ -119,6 +119,25 @@ def test_two_capped_logits_keep_their_digits(gpu, cap):
         assert ((r.entropy.cpu().double() - ent).abs() <= off + 2.0 ** -21).all()
 
 
+@pytest.mark.parametrize("cap", [2.0 ** -60, 2.0 ** -15, 2.0 ** -14, 1e-3, 1.0])
+def test_small_caps(gpu, cap):
+    """Both sides of the least cap whose coefficients FP32 holds, and the least of all."""
+    from se12_amd.logprobs import token_logprobs
+
+    x, t = _logits(gpu, 3, 5000, torch.float32, 12)
+    x[1] *= cap
+    x[2, :2500] *= cap / 8
+    r = token_logprobs(x, t, top=4, softcap=cap)
+    z = cap * torch.tanh(x.cpu().double() / cap)
+    lp = z - torch.logsumexp(z, 1, keepdim=True)
+    want = lp.gather(1, t.cpu()[:, None])[:, 0]
+    assert ((r.logprobs.cpu().double() - want).abs() <= _tol(5000, 0.0, want)).all()
+    ent = torch.special.entr(lp.exp()).sum(1)
+    assert ((r.entropy.cpu().double() - ent).abs() <= 2 * (1 + math.log(5000)) * _tol(5000, 0.0, ent)).all()
+    ids = torch.sort(x.cpu(), dim=1, descending=True, stable=True).indices[:, :4]
+    assert torch.equal(r.top_ids.cpu(), ids)
+
+
 def test_more_rows_than_blocks_fill_the_card(gpu):
     x, t = _logits(gpu, 1500, 2100, torch.bfloat16, 2)
     _check(x, t, 3, 0.0)

@@ -450,6 +450,13 @@ def test_sequences_that_share_pages(gpu):
         _again(c, batch, q, 128, 0.0, 0)
 
 
+@pytest.mark.parametrize("cap", [2.0 ** -60, 0.01])
+@pytest.mark.parametrize("new", [1, 50])
+def test_small_caps(gpu, cap, new):
+    for dtype in (E4M3, BF16):
+        _attend_case(gpu, dtype, 64, 32, 4, 2, [600, 3], [new, 1], cap, 0, seed=51, extra=0)
+
+
 @pytest.mark.parametrize("new", [1, 50])
 def test_the_largest_cap(gpu, new):
     """A score is held to 2^-22 of the cap, here 2^-12, twice in a quotient of sums."""
