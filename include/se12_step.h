@@ -29,6 +29,9 @@ extern "C" {
 /* element type of a paged cache besides SE12_STEP_BF16: 8 bits (OCP E4M3, no
  * infinities), one FP32 scale per page and KV head */
 #define SE12_STEP_E4M3 2
+/* and 4 bits (E2M1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign), one 8-bit scale per 32
+ * columns of a token and KV head */
+#define SE12_STEP_E2M1 3
 
 const char* se12_step_last_error(void);
 
@@ -130,6 +133,13 @@ int se12_step_prefill_attention(uint16_t* qkv, int64_t stride, const uint16_t* c
  *   k_scale, v_scale [pages, kv_heads] FP32 (SE12_STEP_E4M3; else ignored): a
  *   held value stands for itself times the scale of its page and head, a positive
  *   number (se12_step_paged_append writes powers of two)
+ * SE12_STEP_E2M1, two values to a byte, the first in its low half:
+ *   k [pages, kv_heads, page_size, head_dim / 2]
+ *   v [pages, kv_heads, page_size / 16, head_dim, 8]: 16 tokens of a column
+ *   k_scale, v_scale uint8 [pages, kv_heads, head_dim / 32, page_size], 16-byte
+ *   aligned: the byte's bits are bits 14 .. 7 of an FP16 number (5 of exponent, 3
+ *   of fraction), which 32 columns of a token are times; 255: one of the 32 is no
+ *   number, and all of them count as NaN
  * head_dim 64, 128 or 256; k and v 16-byte aligned. */
 typedef struct se12_step_pages {
     void* k;
@@ -178,10 +188,53 @@ typedef struct se12_step_batch {
  * one (powers of two: exact but for values that become subnormal). NaN and
  * infinities are held as NaN. Slots behind the new tokens keep their bytes. A
  * page that a call writes under two entries of the table (of two sequences, or of
- * one), or that a concurrent call reads or writes, has undefined contents. */
+ * one), or that a concurrent call reads or writes, has undefined contents.
+ * SE12_STEP_E2M1: as se12_step_paged_append_rotated. */
 int se12_step_paged_append(const se12_step_pages* pages, const se12_step_batch* batch, const void* q, const void* k,
                            const void* v, int32_t dtype, int64_t q_stride, int64_t k_stride, int64_t v_stride,
                            int32_t heads, const float* inv_freq, int32_t rotary, uint16_t* q_out, void* stream);
+
+/* How q and k are made from a projection's rows, head by head:
+ *   n = x rsqrt(mean(x^2) + eps) (offset + w) where a norm weight w [head_dim] (BF16
+ *   or FP32, 16-byte aligned) is given, q_norm for q and k_norm for k, else x;
+ *   the pairs (n[i], n[i + rotary / 2]), or (n[2 i], n[2 i + 1]) where interleaved,
+ *   i < rotary / 2, by position * inv_freq[i], sine and cosine times `scale`;
+ *   elements from `rotary` on stay (a multiple of 8 up to head_dim, 0 for none).
+ * Sums of squares and angles in 64 bits, the rest in FP32. */
+typedef struct se12_step_rotation {
+    const float* inv_freq;
+    const void* q_norm;
+    const void* k_norm;
+    double scale, eps;
+    float offset;
+    int32_t norm_dtype, rotary, interleaved;
+} se12_step_rotation;
+
+/* se12_step_paged_append for a cache of SE12_STEP_E2M1, with norms and any rotation.
+ * Of 32 columns of a token the scale is the one nearest to a sixth of the largest
+ * value (ties to the even byte; at most 10240, so values beyond 61440 are held as
+ * that, and where the largest is below 2^-16 all are zero); a value the nearest code, ties to
+ * even. 32 columns with a NaN or an infinity are held as NaN. A token's codes and
+ * scales depend on that token alone. One launch. */
+int se12_step_paged_append_rotated(const se12_step_pages* pages, const se12_step_batch* batch, const void* q, const void* k,
+                                   const void* v, int32_t dtype, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                                   int32_t heads, const se12_step_rotation* rotation, uint16_t* q_out, void* stream);
+
+/* What a cache of any type holds of the batch's tokens (rows starts[s] .. of
+ * positions lengths[s] ..): k and v [tokens, kv_heads, head_dim] BF16, contiguous, 16-byte
+ * aligned, apart from each other; rounded once (exact from SE12_STEP_E2M1 and
+ * SE12_STEP_BF16, and from SE12_STEP_E4M3 under power-of-two scales). A token
+ * held nowhere gives zeros; rows of no sequence are not written. One launch. */
+int se12_step_paged_read(const se12_step_pages* pages, const se12_step_batch* batch, uint16_t* k, uint16_t* v, void* stream);
+
+/* The batch's q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] (none
+ * where kv_heads is 0) normed and rotated, into q_out and k_out (out_dtype BF16 or
+ * FP32, contiguous, 16-byte aligned; each may be its input where that has the same
+ * type and rows, else all apart). The batch's page table is not read. head_dim a multiple of
+ * 8 up to 256; strides multiples of 4, rows aligned to 4 values. One launch. */
+int se12_step_rotate_heads(const se12_step_batch* batch, const void* q, const void* k, int32_t dtype, int64_t q_stride,
+                           int64_t k_stride, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                           const se12_step_rotation* rotation, void* q_out, void* k_out, int32_t out_dtype, void* stream);
 
 /* Attention of the new tokens over their sequences' pages, those of the call
  * itself included (appended before): the query at position p sees keys
@@ -193,7 +246,9 @@ int se12_step_paged_append(const se12_step_pages* pages, const se12_step_batch* 
  * aligned, apart from q. heads a multiple of kv_heads. What a query may not see
  * has no part in its row, whatever it holds (NaN too); a query that sees nothing
  * gives zeros. Any finite values of BF16 pages give finite results, those of E4M3
- * pages where none is above 2^112 / keys.
+ * pages where none is above 2^112 / keys. SE12_STEP_E2M1 pages: the products' operands
+ * are FP16, which holds keys and values exactly, a query to 2^-38 of its largest value, and a
+ * weight to 2^-12 of itself or 2^-32 of the row's largest.
  *
  * `workspace`: se12_step_paged_attention_workspace() bytes for the shape (or for
  * one of more tokens), 256-byte aligned, contents indifferent; calls sharing it

@@ -124,6 +124,20 @@ class StepBatch(ctypes.Structure):
     ]
 
 
+class StepRotation(ctypes.Structure):
+    _fields_ = [
+        ("inv_freq", c_void_p),
+        ("q_norm", c_void_p),
+        ("k_norm", c_void_p),
+        ("scale", ctypes.c_double),
+        ("eps", ctypes.c_double),
+        ("offset", ctypes.c_float),
+        ("norm_dtype", c_i32),
+        ("rotary", c_i32),
+        ("interleaved", c_i32),
+    ]
+
+
 # name -> (restype, argtypes): every symbol include/se12_gfx950.h and
 # include/se12_step.h declare
 SIGNATURES = {
@@ -229,6 +243,13 @@ SIGNATURES = {
         c_i32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_i32, c_i64, c_i64, c_i64, c_i32, c_void_p, c_i32, c_void_p,
                 c_void_p],
     ),
+    "se12_step_paged_append_rotated": (
+        c_i32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_i32, c_i64, c_i64, c_i64, c_i32, c_void_p, c_void_p, c_void_p],
+    ),
+    "se12_step_paged_read": (c_i32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "se12_step_rotate_heads": (
+        c_i32, [c_void_p, c_void_p, c_void_p, c_i32, c_i64, c_i64, c_i32, c_i32, c_i32, c_void_p, c_void_p, c_void_p, c_i32, c_void_p],
+    ),
     "se12_step_paged_attention_workspace": (c_i64, [c_void_p, c_void_p, c_i32]),
     "se12_step_paged_attention": (
         c_i32, [c_void_p, c_void_p, c_void_p, c_i64, c_void_p, c_i32, ctypes.c_float, ctypes.c_float, c_i32, c_void_p, c_i64,
@@ -244,6 +265,7 @@ SIGNATURES = {
 STEP_BF16 = 0
 STEP_F32 = 1
 STEP_E4M3 = 2
+STEP_E2M1 = 3
 
 _lib: ctypes.CDLL | None = None
 

@@ -23,7 +23,8 @@ LIBDIR = PKG / "_lib"
 LIBNAME = "libse12_gfx950.so"
 SOURCES = ("se12_abi.hip", "se12_gemv.hip", "se12_gemm.hip", "se12_decode.hip", "se12_encode.hip", "se12_step.hip",
            "se12_probe.hip", "se12_gemm_rx.hip", "se12_prefill.hip", "se12_paged.hip", "se12_paged_attention.hip",
-           "se12_paged_prompt.hip", "se12_logprobs.hip")
+           "se12_paged_prompt.hip", "se12_paged_prompt4.hip", "se12_paged_e2m1.hip", "se12_paged_rotate.hip",
+           "se12_logprobs.hip")
 ARCH = "gfx950"
 
 # Packed-FP32 VALU forms are disabled for every HIP unit (hipcc's host pass

@@ -361,26 +361,14 @@ int se12_step_paged_append(const se12_step_pages* pages, const se12_step_batch* 
     const char* fn = "se12_step_paged_append";
     if (!pages) return step_fail(fn, "NULL argument");
     if (const char* e = paged_error(pages, batch, q ? heads : pages->kv_heads)) return step_fail(fn, e);
-    if (batch->tokens > 0 && (!k || !v || (q && !q_out) || (rotary > 0 && !inv_freq))) return step_fail(fn, "NULL argument");
-    if (dtype != SE12_STEP_BF16 && dtype != SE12_STEP_F32) return step_fail(fn, "q, k and v must be BF16 or FP32");
+    if (batch->tokens > 0 && rotary > 0 && !inv_freq) return step_fail(fn, "NULL argument");
     if (rotary < 0 || rotary > pages->head_dim || rotary % 8) return step_fail(fn, "rotary must be a multiple of 8 up to head_dim");
-    const int64_t kv_row = (int64_t)pages->kv_heads * pages->head_dim;
-    if (k_stride < kv_row || v_stride < kv_row || k_stride % 4 || v_stride % 4 ||
-        (q && (q_stride < (int64_t)heads * pages->head_dim || q_stride % 4)))
-        return step_fail(fn, "rows must be a multiple of 4 elements apart and hold all heads");
-    const uintptr_t piece = dtype == SE12_STEP_F32 ? 16 : 8;
-    if (reinterpret_cast<uintptr_t>(q) % piece || reinterpret_cast<uintptr_t>(k) % piece || reinterpret_cast<uintptr_t>(v) % piece ||
-        reinterpret_cast<uintptr_t>(q_out) % 8 || reinterpret_cast<uintptr_t>(inv_freq) % 16)
-        return step_fail(fn, "misaligned tensor");
+    if (reinterpret_cast<uintptr_t>(inv_freq) % 16) return step_fail(fn, "misaligned tensor");
+    if (const char* e = append_error(pages, batch, q, k, v, dtype, q_stride, k_stride, v_stride, heads, q_out)) return step_fail(fn, e);
     if (batch->tokens == 0) return SE12_STEP_OK;
-    if (q) {
-        // (blocks read and write in any order: only a value of q may be written over, by itself)
-        const int64_t q_row = (int64_t)heads * pages->head_dim, more = batch->tokens - 1, size = dtype == SE12_STEP_F32 ? 4 : 2;
-        const int64_t out_bytes = 2 * (more + 1) * q_row;
-        const bool itself = q == q_out && dtype == SE12_STEP_BF16 && (more == 0 || q_stride == q_row);
-        if ((!itself && overlap(q, size * (more * q_stride + q_row), q_out, out_bytes)) ||
-            overlap(k, size * (more * k_stride + kv_row), q_out, out_bytes) || overlap(v, size * (more * v_stride + kv_row), q_out, out_bytes))
-            return step_fail(fn, "q_out overlaps k, v or other values of q");
+    if (pages->dtype == SE12_STEP_E2M1) {
+        const se12_step_rotation r{inv_freq, nullptr, nullptr, 1.0, 0.0, 0.0f, SE12_STEP_BF16, rotary, 0};
+        return se12_step_paged_append_rotated(pages, batch, q, k, v, dtype, q_stride, k_stride, v_stride, heads, &r, q_out, stream);
     }
     AppendArgs a{q, k, v, q_stride, k_stride, v_stride, pages->k, pages->v, pages->k_scale, pages->v_scale, inv_freq, q_out,
                  device_batch(batch), 0, q ? heads : 0, pages->kv_heads, pages->pages,

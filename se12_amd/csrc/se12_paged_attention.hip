@@ -29,6 +29,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "se12_paged_attend4.hpp"
 #include "se12_paged_units.hpp"
 
 namespace se12step {
@@ -101,6 +102,7 @@ __device__ __forceinline__ Seq seq_of(const Chunk& c, int l) {
     return {__builtin_amdgcn_readlane(c.seq.start, l), __builtin_amdgcn_readlane(c.seq.n, l), __builtin_amdgcn_readlane(c.seq.len, l)};
 }
 
+// (of E2M1: se12_paged_attend4.hpp)
 template <int CT, int D>
 struct Attend {
     using F = Form<CT>;
@@ -110,6 +112,14 @@ struct Attend {
     static constexpr int kRows = D / 16;             // 16-column parts of the output
     floatx4_t o[kRows];
     float m, l;
+
+    // what the lane holds of its column: runs of four
+    template <typename Store>
+    __device__ __forceinline__ void each_part(Store store) const {
+        const int quarter = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) store(16 * i + 4 * quarter, o[i]);
+    }
 
     // one run of tiles of a unit
     __device__ __forceinline__ void run(const AttendArgs& a, int s, const SeqWork& w, int kh, int unit, int tile, int tiles) {
@@ -343,15 +353,11 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : 2) void paged_attent
         if (c < w.seq.n * a.group) {
             if (tiles == w.tiles) {
                 const float inv = x.l == 0.0f ? 0.0f : 1.0f / x.l;
-                uint16_t* out = a.out + ((int64_t)(w.seq.start + c / a.group) * a.heads + kh * a.group + c % a.group) * D + 4 * quarter;
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i)
-                    store4(out + 16 * i, x.o[i][0] * inv, x.o[i][1] * inv, x.o[i][2] * inv, x.o[i][3] * inv);
+                uint16_t* out = a.out + ((int64_t)(w.seq.start + c / a.group) * a.heads + kh * a.group + c % a.group) * D;
+                x.each_part([&](int at, floatx4_t v) { store4(out + at, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv); });
             } else {
                 const int64_t p = part_at(a, worker, tile > 0 ? 0 : 1) + col;
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i)
-                    *reinterpret_cast<floatx4_t*>(a.part + p * D + 16 * i + 4 * quarter) = x.o[i];
+                x.each_part([&](int at, floatx4_t v) { *reinterpret_cast<floatx4_t*>(a.part + p * D + at) = v; });
                 if (quarter == 0) {
                     float* ml = a.part + (int64_t)a.workers * 2 * a.columns * D + 2 * p;
                     ml[0] = x.m;
@@ -513,7 +519,7 @@ int64_t few_bytes(const se12_step_pages* p, const Batch& b, int group) {
 
 PromptPlan plan_of(const se12_step_pages* p, const Batch& b, int group) {
     if ((int64_t)b.max_new * group <= kFewColumns) return {};
-    return prompt_plan(b, p->kv_heads, group, p->page_size, p->head_dim, p->dtype == SE12_STEP_E4M3);
+    return prompt_plan(b, p->kv_heads, group, p->page_size, p->head_dim, p->dtype);
 }
 
 // what one launch holds, and what 32 bits hold of it
@@ -542,6 +548,15 @@ void launch_attend(const AttendArgs& a, hipStream_t st) {
     const bool by_unit = units <= (max_units > 1 ? a.workers : a.workers + a.workers / 2);
     hipLaunchKernelGGL((paged_join_kernel<CT, D>), dim3(by_unit ? (uint32_t)units : (uint32_t)a.workers, max_units > 1 ? 4 : a.columns),
                        dim3(kAttendThreads), 0, st, a, by_unit ? max_units : 0);
+}
+
+template <int CT>
+void launch_attend_of(const AttendArgs& a, int d, hipStream_t st) {
+    switch (d) {
+        case 64: launch_attend<CT, 64>(a, st); break;
+        case 128: launch_attend<CT, 128>(a, st); break;
+        default: launch_attend<CT, 256>(a, st);
+    }
 }
 
 }  // namespace
@@ -588,20 +603,14 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
                  reinterpret_cast<UnitWork*>(static_cast<char*>(workspace) + few_bytes(pages, b, group)),
                  (int)plan.slots + plan.parts, plan.parts / 2, plan.parts, plan.most};
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const bool e4m3 = pages->dtype == SE12_STEP_E4M3;
-    switch (pages->head_dim) {
-        case 64:
-            e4m3 ? launch_attend<SE12_STEP_E4M3, 64>(a, st) : launch_attend<SE12_STEP_BF16, 64>(a, st);
-            break;
-        case 128:
-            e4m3 ? launch_attend<SE12_STEP_E4M3, 128>(a, st) : launch_attend<SE12_STEP_BF16, 128>(a, st);
-            break;
-        default:
-            e4m3 ? launch_attend<SE12_STEP_E4M3, 256>(a, st) : launch_attend<SE12_STEP_BF16, 256>(a, st);
+    switch (pages->dtype) {
+        case SE12_STEP_E2M1: launch_attend_of<SE12_STEP_E2M1>(a, pages->head_dim, st); break;
+        case SE12_STEP_E4M3: launch_attend_of<SE12_STEP_E4M3>(a, pages->head_dim, st); break;
+        default: launch_attend_of<SE12_STEP_BF16>(a, pages->head_dim, st);
     }
     if (plan.records > 0) {
         a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(a.units) + plan.record_bytes);
-        launch_prompt(a, e4m3, pages->head_dim, st);
+        launch_prompt(a, pages->dtype, pages->head_dim, st);
     }
     return step_launched();
 }

@@ -42,6 +42,8 @@ __device__ __forceinline__ int page_of(const Batch& b, int s, int c, int pages) 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef float floatx4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 halfx2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 halfx8_t __attribute__((ext_vector_type(8)));
 
 constexpr float kSlack = 16.0f;       // how far a score may pass the maximum it is taken from, base 2
 
@@ -72,10 +74,11 @@ struct AttendArgs {
 };
 
 // What a lane holds of a tile, by the cache's type: 16 bytes of each key row's
-// 64-byte part, and the lane's keys of a value column, 16 bytes as well.
+// 64-byte part, and the lane's keys of a value column, 16 bytes as well. (Of E2M1 16
+// keys too, and what goes by them; its bytes are laid out in kernels of their own.)
 template <int CT>
 struct Form {
-    static constexpr int kPer = CT == SE12_STEP_E4M3 ? 16 : 8;   // values of 16 bytes, and keys of a lane
+    static constexpr int kPer = CT == SE12_STEP_BF16 ? 8 : 16;   // values of 16 bytes, and keys of a lane
     static constexpr int kTile = 4 * kPer;                        // keys of a tile
     static constexpr int kHalves = kPer / 8;                      // matrix operands of a piece
     static constexpr int kWord = kPer / 4;                        // values of a 32-bit word
@@ -143,6 +146,22 @@ __device__ __forceinline__ uint32_t where_no_number(uint32_t w, int kind) {
     return is * 0x7Fu;
 }
 
+// E2M1: a scale is the upper byte of an FP16 number behind its sign (byte << 7: 5 bits of
+// exponent, 3 of fraction), 255 where one of its 32 values is no number
+__device__ __forceinline__ float e2m1_scale(uint32_t byte) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(byte << 7)); }
+
+// bit 7 of every byte that is no scale
+__device__ __forceinline__ uint32_t no_scales(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & w & 0x80808080u; }
+
+// the 8 codes of a word times their scales (of two at a time), in FP16: exact
+__device__ __forceinline__ halfx8_t e2m1_operand(uint32_t w, const halfx2_t by[4]) {
+    const halfx2_t x0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 0) * by[0];
+    const halfx2_t x1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 1) * by[1];
+    const halfx2_t x2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 2) * by[2];
+    const halfx2_t x3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 3) * by[3];
+    return halfx8_t{x0.x, x0.y, x1.x, x1.y, x2.x, x2.y, x3.x, x3.y};
+}
+
 __device__ __forceinline__ void store4(uint16_t* p, float a, float b, float c, float d) {
     *reinterpret_cast<uint2*>(p) = make_uint2(f_to_bf16x2(a, b), f_to_bf16x2(c, d));
 }
@@ -151,8 +170,9 @@ __device__ __forceinline__ void store4(uint16_t* p, float a, float b, float c, f
 inline const char* paged_error(const se12_step_pages* p, const se12_step_batch* b, int32_t heads) {
     if (!p || !b) return "NULL argument";
     if (!p->k || !p->v) return "NULL cache";
-    if (p->dtype != SE12_STEP_BF16 && p->dtype != SE12_STEP_E4M3) return "the cache must be BF16 or E4M3";
-    if (p->dtype == SE12_STEP_E4M3 && (!p->k_scale || !p->v_scale)) return "an E4M3 cache needs scales";
+    if (p->dtype != SE12_STEP_BF16 && p->dtype != SE12_STEP_E4M3 && p->dtype != SE12_STEP_E2M1)
+        return "the cache must be BF16 or E4M3 or E2M1";
+    if (p->dtype != SE12_STEP_BF16 && (!p->k_scale || !p->v_scale)) return "an E4M3 or E2M1 cache needs scales";
     if (p->page_size != 16 && p->page_size != 32 && p->page_size != 64 && p->page_size != 128)
         return "page_size must be 16, 32, 64 or 128";
     if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256) return "head_dim must be 64, 128 or 256";
@@ -168,6 +188,8 @@ inline const char* paged_error(const se12_step_pages* p, const se12_step_batch* 
         reinterpret_cast<uintptr_t>(b->starts) % 4 || reinterpret_cast<uintptr_t>(p->k_scale) % 4 ||
         reinterpret_cast<uintptr_t>(p->v_scale) % 4)
         return "misaligned tensor";
+    if (p->dtype == SE12_STEP_E2M1 && (reinterpret_cast<uintptr_t>(p->k_scale) % 16 || reinterpret_cast<uintptr_t>(p->v_scale) % 16))
+        return "scales of an E2M1 cache not 16-byte aligned";
     return nullptr;
 }
 
@@ -182,6 +204,29 @@ inline bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_byt
     return x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
 }
 
+// host: the first thing wrong with the rows of an append, or NULL
+inline const char* append_error(const se12_step_pages* p, const se12_step_batch* b, const void* q, const void* k, const void* v,
+                                int32_t dtype, int64_t q_stride, int64_t k_stride, int64_t v_stride, int32_t heads,
+                                const uint16_t* q_out) {
+    if (b->tokens > 0 && (!k || !v || (q && !q_out))) return "NULL argument";
+    if (dtype != SE12_STEP_BF16 && dtype != SE12_STEP_F32) return "q, k and v must be BF16 or FP32";
+    const int64_t kv_row = (int64_t)p->kv_heads * p->head_dim, q_row = (int64_t)heads * p->head_dim;
+    if (k_stride < kv_row || v_stride < kv_row || k_stride % 4 || v_stride % 4 || (q && (q_stride < q_row || q_stride % 4)))
+        return "rows must be a multiple of 4 elements apart and hold all heads";
+    const uintptr_t piece = dtype == SE12_STEP_F32 ? 16 : 8;
+    if (reinterpret_cast<uintptr_t>(q) % piece || reinterpret_cast<uintptr_t>(k) % piece || reinterpret_cast<uintptr_t>(v) % piece ||
+        reinterpret_cast<uintptr_t>(q_out) % 8)
+        return "misaligned tensor";
+    if (!q || b->tokens == 0) return nullptr;
+    // (blocks read and write in any order: only a value of q may be written over, by itself)
+    const int64_t more = b->tokens - 1, size = dtype == SE12_STEP_F32 ? 4 : 2, out_bytes = 2 * (more + 1) * q_row;
+    const bool itself = q == q_out && dtype == SE12_STEP_BF16 && (more == 0 || q_stride == q_row);
+    if ((!itself && overlap(q, size * (more * q_stride + q_row), q_out, out_bytes)) ||
+        overlap(k, size * (more * k_stride + kv_row), q_out, out_bytes) || overlap(v, size * (more * v_stride + kv_row), q_out, out_bytes))
+        return "q_out overlaps k, v or other values of q";
+    return nullptr;
+}
+
 // host: caps whose factors FP32 holds (the cap's form holds a score to 2^-22 of the cap)
 inline bool softcap_fits(float cap) { return cap == 0.0f || (cap >= 0x1p-60f && cap <= 1024.0f); }
 
@@ -191,8 +236,10 @@ struct PromptPlan {
     int parts, most;             // as AttendArgs
     int64_t records, record_bytes, part_bytes;
 };
-PromptPlan prompt_plan(const Batch& b, int kvh, int group, int page_size, int d, bool e4m3);
-void launch_prompt(const AttendArgs& a, bool e4m3, int d, hipStream_t st);
+PromptPlan prompt_plan(const Batch& b, int kvh, int group, int page_size, int d, int dtype);
+void launch_prompt(const AttendArgs& a, int dtype, int d, hipStream_t st);
+// se12_paged_prompt4.hip: the launches of pages of E2M1
+void launch_prompt4(const AttendArgs& a, int d, hipStream_t st);
 
 inline int log2_of(int n) { return 31 - __builtin_clz((unsigned)n); }
 

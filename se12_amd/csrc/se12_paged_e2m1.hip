@@ -1,0 +1,351 @@
+// Appending to a paged cache of E2M1 (4 bits, a scale to 32 columns of a token and
+// head), and reading a cache of any type back. Mathematics: rows of q and k normed and
+// rotated (se12_paged_rotation.hpp); of 32 columns s = the 8-bit scale nearest to
+// max |x| / 6, at most 10240, and each value the E2M1 nearest to x / s, ties to even,
+// 6 at most. A code has 2 significant bits and a scale 4, so what is held is a number of
+// FP16 and of BF16 alike. A scale is that of its token alone: no later token changes it,
+// and nothing is rounded twice.
+//
+// A block has 16 positions of a sequence and one KV head: its keys, its values and the
+// query heads that read it, so a value column's 8 bytes (16 tokens) have one writer and
+// the angles serve all its rows. Values meet in LDS, where a column's tokens lie apart.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "se12_paged_rotation.hpp"
+
+namespace se12step {
+
+constexpr int kRowThreads = 256;
+
+struct Append4Args {
+    const void* q;
+    const void* k;
+    const void* v;
+    int64_t q_stride, k_stride, v_stride;
+    uint8_t* kc;
+    uint8_t* vc;
+    uint8_t* k_scale;
+    uint8_t* v_scale;
+    uint16_t* q_out;
+    Batch b;
+    Rotation r;
+    int group, kvh, pages, page_log2;      // group: query heads of a KV head, 0 without q
+};
+
+// the scale nearest to amax / 6 (ties to an even byte), and its byte; amax by its bits
+__device__ __forceinline__ uint32_t scale_byte(uint32_t amax) {
+    if (amax >= 0x7F800000u) return 255u;
+    const float a = __uint_as_float(amax), sixth = a * (1.0f / 6.0f);
+    // below it (cut to 3 bits of fraction) and half a step on, six times: both exact
+    uint32_t byte;
+    if (sixth >= 0x1p-14f)
+        byte = min((__float_as_uint(sixth) >> 20) - (112u << 3), 226u);
+    else
+        byte = (uint32_t)(sixth * 0x1p17f);
+    const int e = max((int)(byte >> 3), 1);
+    const float s = e2m1_scale(byte), middle = 6.0f * (s + __uint_as_float((uint32_t)(e - 19 + 127) << 23));
+    byte += a > middle || (a == middle && (byte & 1));
+    return min(byte, 226u);
+}
+
+// 8 values as codes, the first in the lowest bits
+__device__ __forceinline__ uint32_t e2m1x8(const float x[8], float s) {
+    if (!(s > 0.0f)) return 0u;            // (NaN: the scale says so)
+    const float inv = 1.0f / s;
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        // the quotient to its last bit, or a tie would go by the inverse's rounding
+        const float t = x[i] * inv;
+        y[i] = __builtin_amdgcn_fmed3f(fmaf(fmaf(-t, s, x[i]), inv, t), -6.0f, 6.0f);
+    }
+    uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, y[0], y[1], 1.0f, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[2], y[3], 1.0f, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[4], y[5], 1.0f, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[6], y[7], 1.0f, 3);
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(kRowThreads) void paged_append4_kernel(Append4Args a) {
+    constexpr int kLanes = D / 8, kRows = kRowThreads / kLanes;
+    __shared__ __attribute__((aligned(16))) float2 cs[16 * D / 2];
+    __shared__ __attribute__((aligned(16))) float rows[kRows * D];
+    __shared__ uint32_t codes[16][kLanes];                       // of the values
+    __shared__ __attribute__((aligned(16))) uint8_t scales[2][D / 32][16];
+    const int tid = threadIdx.x, kh = (int)blockIdx.x % a.kvh;
+    const Run16 u = run16_of(a.b, (int)blockIdx.x / a.kvh);
+    const int n = u.to - u.from;
+    if (n <= 0) return;
+    const int64_t row0 = u.seq.start + u.first + u.from - u.seq.len;      // of the first token
+    const int half = a.r.half;
+    for (int i = tid; i < n * half; i += kRowThreads) {
+        const int t = i / half, f = i - t * half;
+        cs[t * half + f] = turn_at(u.first + u.from + t, a.r.inv_freq[f], a.r.scale);
+    }
+    const int P = 1 << a.page_log2, page = page_of(a.b, u.s, u.first >> a.page_log2, a.pages);
+    const int64_t page_head = (int64_t)max(page, 0) * a.kvh + kh;
+    const int slot0 = u.first & (P - 1);
+    __syncthreads();
+
+    // rows: values, keys, then the query heads, each of n tokens
+    const int lane = tid % kLanes, c0 = 8 * lane;
+    float* own = rows + (tid / kLanes) * D;
+    for (int i = tid / kLanes; i < (2 + a.group) * n; i += kRows) {
+        const int what = i / n, t = i - what * n;
+        const int64_t row = row0 + t;
+        float x[8];
+        if (what == 0) {
+            load8<DT>(a.v, row * a.v_stride + kh * D + c0, x);
+        } else {
+            const int head = what == 1 ? kh : kh * a.group + what - 2;
+            load8<DT>(what == 1 ? a.k : a.q, row * (what == 1 ? a.k_stride : a.q_stride) + (int64_t)head * D + c0, x);
+            const void* w = what == 1 ? a.r.k_norm : a.r.q_norm;
+            if (w) norm_row<kLanes>(x, a.r, w, c0, D);
+            if (half > 0) turn_row(x, own, cs + t * half, c0, half, a.r.interleaved);
+            if (what > 1) {
+                uint16_t* o = a.q_out + (row * a.group * a.kvh + head) * D + c0;
+                const uint4 v = bf16x8(x);
+                reinterpret_cast<uint2*>(o)[0] = make_uint2(v.x, v.y);
+                reinterpret_cast<uint2*>(o)[1] = make_uint2(v.z, v.w);
+                continue;
+            }
+        }
+        uint32_t amax = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) amax = max(amax, __float_as_uint(x[k]) & 0x7FFFFFFFu);
+        amax = max(amax, (uint32_t)__builtin_amdgcn_mov_dpp((int)amax, 0xB1, 0xF, 0xF, true));       // of four lanes
+        amax = max(amax, (uint32_t)__builtin_amdgcn_mov_dpp((int)amax, 0x4E, 0xF, 0xF, true));
+        const uint32_t byte = scale_byte(amax), w = e2m1x8(x, e2m1_scale(byte));
+        const int slot = u.from + t;
+        if (lane % 4 == 0) scales[what][lane / 4][slot] = (uint8_t)byte;
+        if (what == 0)
+            codes[slot][lane] = w;
+        else if (page >= 0)
+            *reinterpret_cast<uint32_t*>(a.kc + (page_head * P + slot0 + slot) * (D / 2) + c0 / 2) = w;
+    }
+    __syncthreads();
+    if (page < 0) return;
+    for (int c = tid; c < D; c += kRowThreads) {
+        uint2* p = reinterpret_cast<uint2*>(a.vc + ((page_head << (a.page_log2 - 4)) + slot0 / 16) * (8 * D)) + c;
+        uint32_t w[2] = {0, 0}, m[2] = {0, 0};
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+            const bool mine = t >= u.from && t < u.to;
+            const uint32_t v = (codes[t][c / 8] >> (4 * (c % 8))) & 15u;
+            w[t / 8] |= mine ? v << (4 * (t % 8)) : 0u;
+            m[t / 8] |= mine ? 15u << (4 * (t % 8)) : 0u;
+        }
+        if (n < 16) {
+            const uint2 was = *p;
+            w[0] |= was.x & ~m[0];
+            w[1] |= was.y & ~m[1];
+        }
+        *p = make_uint2(w[0], w[1]);
+    }
+    for (int i = tid; i < 2 * (D / 32); i += kRowThreads) {
+        const int what = i / (D / 32), g = i % (D / 32);
+        uint8_t* p = (what == 0 ? a.v_scale : a.k_scale) + (page_head * (D / 32) + g) * P + slot0;
+        if (n == 16)
+            *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(scales[what][g]);
+        else
+            for (int t = u.from; t < u.to; ++t) p[t] = scales[what][g][t];
+    }
+}
+
+// ---------------------------------------------------------------------------
+// reading back
+// ---------------------------------------------------------------------------
+
+struct ReadArgs {
+    const uint8_t* kc;
+    const uint8_t* vc;
+    const void* k_scale;
+    const void* v_scale;
+    uint16_t* k;
+    uint16_t* v;
+    Batch b;
+    int kvh, pages, page_log2;
+};
+
+// four values of 8 bits times s, in BF16
+__device__ __forceinline__ uint2 e4m3x4_values(uint32_t w, float s) {
+    typedef float f2_t __attribute__((ext_vector_type(2)));
+    const f2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    return make_uint2(f_to_bf16x2(a.x * s, a.y * s), f_to_bf16x2(b.x * s, b.y * s));
+}
+
+// the two codes of byte `which` of w, times a and b, in BF16
+template <int kByte>
+__device__ __forceinline__ uint32_t e2m1_values(uint32_t w, float a, float b) {
+    typedef float f2_t __attribute__((ext_vector_type(2)));
+    const f2_t x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, kByte);
+    return f_to_bf16x2(x.x * a, x.y * b);
+}
+
+template <int CT, int D>
+__global__ __launch_bounds__(kRowThreads) void paged_read_kernel(ReadArgs a) {
+    constexpr int kLanes = D / 8, kRows = kRowThreads / kLanes;
+    __shared__ __attribute__((aligned(16))) uint16_t tile[16 * (D + 8)];      // values, a token to a row
+    const int tid = threadIdx.x, kh = (int)blockIdx.x % a.kvh;
+    const Run16 u = run16_of(a.b, (int)blockIdx.x / a.kvh);
+    if (u.to <= u.from) return;
+    const int P = 1 << a.page_log2, page = page_of(a.b, u.s, u.first >> a.page_log2, a.pages);
+    const int64_t page_head = (int64_t)max(page, 0) * a.kvh + kh;
+    const int slot0 = u.first & (P - 1), lane = tid % kLanes;
+    const int64_t out0 = ((u.seq.start + (int64_t)u.first - u.seq.len) * a.kvh + kh) * D + 8 * lane;       // of slot 0
+    // values: two columns to a thread, 16 tokens
+    for (int c = 2 * tid; c < D; c += 2 * kRowThreads) {
+        uint32_t x[16];      // (token's two columns)
+        if constexpr (CT == SE12_STEP_E2M1) {
+            const uint4 w = *reinterpret_cast<const uint4*>(a.vc + ((page_head << (a.page_log2 - 4)) + slot0 / 16) * (8 * D) + 8 * c);
+            const uint4 sb = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.v_scale) + (page_head * (D / 32) + c / 32) * P + slot0);
+            const uint32_t ws[4] = {w.x, w.y, w.z, w.w}, bs[4] = {sb.x, sb.y, sb.z, sb.w};
+            uint32_t y[2][8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t b = bs[k / 2] >> (16 * (k & 1));
+                const float s0 = e2m1_scale(b & 255u), s1 = e2m1_scale((b >> 8) & 255u);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t v = ws[2 * j + k / 4];
+                    y[j][k] = (k & 3) == 0 ? e2m1_values<0>(v, s0, s1) : (k & 3) == 1 ? e2m1_values<1>(v, s0, s1)
+                              : (k & 3) == 2 ? e2m1_values<2>(v, s0, s1) : e2m1_values<3>(v, s0, s1);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                x[2 * k] = __builtin_amdgcn_perm(y[1][k], y[0][k], 0x05040100u);
+                x[2 * k + 1] = __builtin_amdgcn_perm(y[1][k], y[0][k], 0x07060302u);
+            }
+        } else {
+            uint32_t y[2][8];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint8_t* p = a.vc + ((page_head * D + c + j) * P + slot0) * (CT == SE12_STEP_BF16 ? 2 : 1);
+                if constexpr (CT == SE12_STEP_BF16) {
+                    const uint4 v0 = reinterpret_cast<const uint4*>(p)[0], v1 = reinterpret_cast<const uint4*>(p)[1];
+                    const uint32_t v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) y[j][k] = v[k];
+                } else {
+                    const float s = static_cast<const float*>(a.v_scale)[page_head];
+                    const uint4 v0 = *reinterpret_cast<const uint4*>(p);
+                    const uint32_t v[4] = {v0.x, v0.y, v0.z, v0.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint2 z = e4m3x4_values(v[k], s);
+                        y[j][2 * k] = z.x;
+                        y[j][2 * k + 1] = z.y;
+                    }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                x[2 * k] = __builtin_amdgcn_perm(y[1][k], y[0][k], 0x05040100u);
+                x[2 * k + 1] = __builtin_amdgcn_perm(y[1][k], y[0][k], 0x07060302u);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 16; ++t) *reinterpret_cast<uint32_t*>(tile + t * (D + 8) + c) = x[t];
+    }
+    for (int t = u.from + tid / kLanes; t < u.to; t += kRows) {
+        uint4 x;
+        const int64_t at = (page_head * P + slot0 + t) * D + 8 * lane;
+        if constexpr (CT == SE12_STEP_E2M1) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(a.kc + at / 2);
+            const float s = e2m1_scale(static_cast<const uint8_t*>(a.k_scale)[(page_head * (D / 32) + lane / 4) * P + slot0 + t]);
+            x = make_uint4(e2m1_values<0>(w, s, s), e2m1_values<1>(w, s, s), e2m1_values<2>(w, s, s), e2m1_values<3>(w, s, s));
+        } else if constexpr (CT == SE12_STEP_E4M3) {
+            const uint2 w = *reinterpret_cast<const uint2*>(a.kc + at);
+            const float s = static_cast<const float*>(a.k_scale)[page_head];
+            const uint2 x0 = e4m3x4_values(w.x, s), x1 = e4m3x4_values(w.y, s);
+            x = make_uint4(x0.x, x0.y, x1.x, x1.y);
+        } else {
+            x = *reinterpret_cast<const uint4*>(a.kc + 2 * at);
+        }
+        *reinterpret_cast<uint4*>(a.k + out0 + (int64_t)t * a.kvh * D) = page >= 0 ? x : make_uint4(0, 0, 0, 0);
+    }
+    __syncthreads();
+    for (int t = u.from + tid / kLanes; t < u.to; t += kRows) {
+        const uint4 x = *reinterpret_cast<const uint4*>(tile + t * (D + 8) + 8 * lane);
+        *reinterpret_cast<uint4*>(a.v + out0 + (int64_t)t * a.kvh * D) = page >= 0 ? x : make_uint4(0, 0, 0, 0);
+    }
+}
+
+}  // namespace se12step
+
+using namespace se12step;
+
+namespace {
+
+template <int DT>
+void launch_append4(const Append4Args& a, int d, uint32_t blocks, hipStream_t st) {
+    switch (d) {
+        case 64: hipLaunchKernelGGL((paged_append4_kernel<DT, 64>), dim3(blocks), dim3(kRowThreads), 0, st, a); break;
+        case 128: hipLaunchKernelGGL((paged_append4_kernel<DT, 128>), dim3(blocks), dim3(kRowThreads), 0, st, a); break;
+        default: hipLaunchKernelGGL((paged_append4_kernel<DT, 256>), dim3(blocks), dim3(kRowThreads), 0, st, a);
+    }
+}
+
+template <int CT>
+void launch_read(const ReadArgs& a, int d, uint32_t blocks, hipStream_t st) {
+    switch (d) {
+        case 64: hipLaunchKernelGGL((paged_read_kernel<CT, 64>), dim3(blocks), dim3(kRowThreads), 0, st, a); break;
+        case 128: hipLaunchKernelGGL((paged_read_kernel<CT, 128>), dim3(blocks), dim3(kRowThreads), 0, st, a); break;
+        default: hipLaunchKernelGGL((paged_read_kernel<CT, 256>), dim3(blocks), dim3(kRowThreads), 0, st, a);
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+int se12_step_paged_append_rotated(const se12_step_pages* pages, const se12_step_batch* batch, const void* q, const void* k,
+                                   const void* v, int32_t dtype, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                                   int32_t heads, const se12_step_rotation* rotation, uint16_t* q_out, void* stream) {
+    const char* fn = "se12_step_paged_append_rotated";
+    if (!pages) return step_fail(fn, "NULL argument");
+    if (const char* e = paged_error(pages, batch, q ? heads : pages->kv_heads)) return step_fail(fn, e);
+    if (pages->dtype != SE12_STEP_E2M1) return step_fail(fn, "the cache must be E2M1");
+    if (const char* e = rotation_error(rotation, pages->head_dim)) return step_fail(fn, e);
+    if (const char* e = append_error(pages, batch, q, k, v, dtype, q_stride, k_stride, v_stride, heads, q_out)) return step_fail(fn, e);
+    if (batch->tokens == 0) return SE12_STEP_OK;
+    const Append4Args a{q, k, v, q_stride, k_stride, v_stride, static_cast<uint8_t*>(pages->k), static_cast<uint8_t*>(pages->v),
+                        reinterpret_cast<uint8_t*>(pages->k_scale), reinterpret_cast<uint8_t*>(pages->v_scale), q_out,
+                        device_batch(batch), device_rotation(rotation), q ? heads / pages->kv_heads : 0, pages->kv_heads,
+                        pages->pages, log2_of(pages->page_size)};
+    const int64_t blocks = run16_blocks(a.b) * pages->kv_heads;
+    if (!grid_fits(blocks, kRowThreads)) return step_fail(fn, "too many tokens and heads for one launch");
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (dtype == SE12_STEP_F32)
+        launch_append4<SE12_STEP_F32>(a, pages->head_dim, (uint32_t)blocks, st);
+    else
+        launch_append4<SE12_STEP_BF16>(a, pages->head_dim, (uint32_t)blocks, st);
+    return step_launched();
+}
+
+int se12_step_paged_read(const se12_step_pages* pages, const se12_step_batch* batch, uint16_t* k, uint16_t* v, void* stream) {
+    const char* fn = "se12_step_paged_read";
+    if (!pages) return step_fail(fn, "NULL argument");
+    if (const char* e = paged_error(pages, batch, pages->kv_heads)) return step_fail(fn, e);
+    if (batch->tokens == 0) return SE12_STEP_OK;
+    if (!k || !v) return step_fail(fn, "NULL argument");
+    if (reinterpret_cast<uintptr_t>(k) % 16 || reinterpret_cast<uintptr_t>(v) % 16) return step_fail(fn, "misaligned tensor");
+    const int64_t bytes = 2 * (int64_t)batch->tokens * pages->kv_heads * pages->head_dim;
+    if (overlap(k, bytes, v, bytes)) return step_fail(fn, "k overlaps v");
+    const ReadArgs a{static_cast<const uint8_t*>(pages->k), static_cast<const uint8_t*>(pages->v), pages->k_scale, pages->v_scale, k, v,
+                     device_batch(batch), pages->kv_heads, pages->pages, log2_of(pages->page_size)};
+    const int64_t blocks = run16_blocks(a.b) * pages->kv_heads;
+    if (!grid_fits(blocks, kRowThreads)) return step_fail(fn, "too many tokens and heads for one launch");
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (pages->dtype == SE12_STEP_E2M1)
+        launch_read<SE12_STEP_E2M1>(a, pages->head_dim, (uint32_t)blocks, st);
+    else if (pages->dtype == SE12_STEP_E4M3)
+        launch_read<SE12_STEP_E4M3>(a, pages->head_dim, (uint32_t)blocks, st);
+    else
+        launch_read<SE12_STEP_BF16>(a, pages->head_dim, (uint32_t)blocks, st);
+    return step_launched();
+}
+
+}  // extern "C"

@@ -518,7 +518,7 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
 template <int D>
 constexpr int kJoinBlocks = D / 16;
 
-template <int CT, int D>
+template <int D>
 __global__ __launch_bounds__(kPromptThreads) void paged_prompt_join_kernel(AttendArgs a) {
     constexpr int kPieces = D / 8 / kJoinBlocks<D>;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31;
@@ -562,6 +562,12 @@ __global__ __launch_bounds__(kPromptThreads) void paged_prompt_join_kernel(Atten
 
 namespace {
 
+template <int D>
+void launch_join(const AttendArgs& a, hipStream_t st) {
+    if (a.join_count > 0)
+        hipLaunchKernelGGL((paged_prompt_join_kernel<D>), dim3((a.join_count * a.kvh + 7) / 8 * 8 * kJoinBlocks<D>), dim3(kPromptThreads), 0, st, a);
+}
+
 template <int CT, int D>
 void launch(const AttendArgs& a, hipStream_t st) {
     const int grid = a.unit_count * a.kvh;
@@ -569,8 +575,7 @@ void launch(const AttendArgs& a, hipStream_t st) {
         hipLaunchKernelGGL((paged_prompt_kernel<CT, D, true>), dim3(grid), dim3(kPromptThreads), 4 * 64 * D, st, a);
     else
         hipLaunchKernelGGL((paged_prompt_kernel<CT, D, false>), dim3(grid), dim3(kPromptThreads), 4 * 64 * D, st, a);
-    if (a.join_count > 0)
-        hipLaunchKernelGGL((paged_prompt_join_kernel<CT, D>), dim3((a.join_count * a.kvh + 7) / 8 * 8 * kJoinBlocks<D>), dim3(kPromptThreads), 0, st, a);
+    launch_join<D>(a, st);
 }
 
 }  // namespace
@@ -580,9 +585,9 @@ void launch(const AttendArgs& a, hipStream_t st) {
 // blocks (Sharing), or where few units can be as many as the rule for `splits` asks for.
 // Where there are many units none is shared, but the memory stays: no call takes less than
 // one of fewer tokens.
-PromptPlan prompt_plan(const Batch& b, int kvh, int group, int page_size, int d, bool e4m3) {
+PromptPlan prompt_plan(const Batch& b, int kvh, int group, int page_size, int d, int dtype) {
     const int64_t columns = (int64_t)b.tokens * group, many = std::min<int64_t>(b.seqs, columns / (kFewColumns + 1));
-    const int64_t resident = resident_blocks(e4m3, d);
+    const int64_t resident = resident_blocks(dtype, d);
     PromptPlan x;
     x.slots = (columns + (kBlockColumns - 1) * many) / kBlockColumns;
     x.most = (int)(((int64_t)b.width * page_size + 32 * kLeastTiles - 1) / (32 * kLeastTiles));
@@ -595,7 +600,13 @@ PromptPlan prompt_plan(const Batch& b, int kvh, int group, int page_size, int d,
     return x;
 }
 
-void launch_prompt(const AttendArgs& a, bool e4m3, int d, hipStream_t st) {
+void launch_prompt(const AttendArgs& a, int dtype, int d, hipStream_t st) {
+    if (dtype == SE12_STEP_E2M1) {
+        launch_prompt4(a, d, st);
+        d == 64 ? launch_join<64>(a, st) : d == 128 ? launch_join<128>(a, st) : launch_join<256>(a, st);
+        return;
+    }
+    const bool e4m3 = dtype == SE12_STEP_E4M3;
     switch (d) {
         case 64: e4m3 ? launch<SE12_STEP_E4M3, 64>(a, st) : launch<SE12_STEP_BF16, 64>(a, st); break;
         case 128: e4m3 ? launch<SE12_STEP_E4M3, 128>(a, st) : launch<SE12_STEP_BF16, 128>(a, st); break;

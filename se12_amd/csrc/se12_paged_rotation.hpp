@@ -1,0 +1,192 @@
+// Norm and position rotation of a token's heads, shared by the append to E2M1 pages
+// (se12_paged_e2m1.hip) and the rotation by itself (se12_paged_rotate.hip).
+// Mathematics: n = x rsqrt(mean(x^2) + eps) (offset + w), then the pair (a, b) of n by
+// angle = position * inv_freq: (a cos - b sin, b cos + a sin) times `scale`; pairs (i, i +
+// rotary / 2), or (2 i, 2 i + 1) where interleaved.
+//
+// A row (token and head) is 8 columns to a lane. Sums of squares and angles in 64 bits,
+// each rounded to FP32 once (the mean's root, sine and cosine times scale); all else in
+// single FP32 operations, no product kept longer than the next rounding. So keys are the
+// same bits whatever the launch, and those of the formula in FP32: a digit of a quantised
+// key does not depend on how the work was cut.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "se12_paged_device.hpp"
+
+namespace se12step {
+
+struct Rotation {
+    const float* inv_freq;
+    const void* q_norm;
+    const void* k_norm;
+    double scale, eps;
+    float offset;
+    int half;              // rotary / 2
+    bool f32_norm, interleaved;
+};
+
+template <int DT>
+__device__ __forceinline__ void load8(const void* p, int64_t i, float x[8]) {
+    if constexpr (DT == SE12_STEP_F32) {
+        const float4* v = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+        const float4 a = v[0], b = v[1];
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+        // (rows are 4 values' bytes apart at least, not 16)
+        const uint2* v = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+        const uint2 a = v[0], b = v[1];
+        const uint32_t w[4] = {a.x, a.y, b.x, b.y};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            x[2 * k] = __uint_as_float(w[k] << 16);
+            x[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+        }
+    }
+}
+
+// cos and sin of pos * freq, times scale
+__device__ __forceinline__ float2 turn_at(int pos, float freq, double scale) {
+    // what is beyond a whole number of quarter turns, in two parts of pi / 2, by the series
+    // of sine and cosine: 2^-53 of the angle's own rounding
+    const double angle = (double)pos * (double)freq, whole = angle * 0.63661977236758134 + 0x1.8p52, k = whole - 0x1.8p52;
+    const int turn = __double2loint(whole);
+    const double x = fma(-k, 6.123233995736766e-17, fma(-k, 1.5707963267948966, angle)), x2 = x * x;
+    double s = -1.0 / 1307674368000, c = 1.0 / 20922789888000;
+    s = fma(s, x2, 1.0 / 6227020800);
+    c = fma(c, x2, -1.0 / 87178291200);
+    s = fma(s, x2, -1.0 / 39916800);
+    c = fma(c, x2, 1.0 / 479001600);
+    s = fma(s, x2, 1.0 / 362880);
+    c = fma(c, x2, -1.0 / 3628800);
+    s = fma(s, x2, -1.0 / 5040);
+    c = fma(c, x2, 1.0 / 40320);
+    s = fma(s, x2, 1.0 / 120);
+    c = fma(c, x2, -1.0 / 720);
+    s = fma(s, x2, -1.0 / 6);
+    c = fma(c, x2, 1.0 / 24);
+    s = fma(s * x2, x, x);
+    c = fma(c, x2, -0.5);
+    c = fma(c, x2, 1.0);
+    const double sn = turn & 1 ? c : s, cs = turn & 1 ? s : c;
+    return make_float2((float)((turn + 1) & 2 ? -cs * scale : cs * scale), (float)(turn & 2 ? -sn * scale : sn * scale));
+}
+
+// x[8] of a row whose kLanes lanes lie side by side, normed with weights w
+template <int kLanes>
+__device__ __forceinline__ void norm_row(float x[8], const Rotation& r, const void* w, int c0, int d) {
+#pragma clang fp contract(off)
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += (double)x[i] * (double)x[i];
+#pragma unroll
+    for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor(sum, o, 64);
+    const float inv = (float)(1.0 / sqrt(sum / d + r.eps));
+    float f[8];
+    if (r.f32_norm)
+        load8<SE12_STEP_F32>(w, c0, f);
+    else
+        load8<SE12_STEP_BF16>(w, c0, f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (x[i] * inv) * (r.offset + f[i]);
+}
+
+// x[8], columns c0 .. of a row, turned by the angles cs[half] of its token; `row`: the
+// row's place in LDS, read and written by the wave's own lanes alone
+__device__ __forceinline__ void turn_row(float x[8], float* row, const float2* cs, int c0, int half, bool interleaved) {
+#pragma clang fp contract(off)
+    if (interleaved) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            if (c0 + 2 * p >= 2 * half) break;
+            const float2 t = cs[c0 / 2 + p];
+            const float a = x[2 * p], b = x[2 * p + 1];
+            x[2 * p] = a * t.x - b * t.y;
+            x[2 * p + 1] = b * t.x + a * t.y;
+        }
+        return;
+    }
+    *reinterpret_cast<float4*>(row + c0) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(row + c0 + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int c = c0 + 4 * i;
+        if (c >= 2 * half) break;
+        const bool first = c < half;
+        const float4 other = *reinterpret_cast<const float4*>(row + (first ? c + half : c - half));
+        const float4* t = reinterpret_cast<const float4*>(cs + (first ? c : c - half));
+        const float4 t0 = t[0], t1 = t[1];
+        const float o[4] = {other.x, other.y, other.z, other.w}, cos[4] = {t0.x, t0.z, t1.x, t1.z}, sin[4] = {t0.y, t0.w, t1.y, t1.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float a = x[4 * i + k] * cos[k], b = o[k] * sin[k];
+            x[4 * i + k] = first ? a - b : a + b;
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
+__device__ __forceinline__ uint4 bf16x8(const float x[8]) {
+    return make_uint4(f_to_bf16x2(x[0], x[1]), f_to_bf16x2(x[2], x[3]), f_to_bf16x2(x[4], x[5]), f_to_bf16x2(x[6], x[7]));
+}
+
+// The calls' blocks: each has 16 positions side by side of one sequence. A sequence of
+// n new tokens touches at most n / 16 + 2 such runs, so sequence s may have blocks
+// starts[s] / 16 + 2 s onwards; at one token each, block s.
+struct Run16 {
+    Seq seq;
+    int s, first;        // sequence, first position of the run (a multiple of 16)
+    int from, to;        // its new tokens: first + from .. first + to - 1
+};
+
+__device__ __forceinline__ Run16 run16_of(const Batch& b, int slot) {
+    int s = slot, j = 0;
+    if (b.max_new > 1) {
+        auto block0 = [&](int i) { return (min(max(b.starts[i], 0), b.tokens) >> 4) + 2 * i; };
+        int lo = 0, hi = b.seqs;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (block0(mid) <= slot)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        s = lo;
+        j = slot - block0(s);
+    }
+    Run16 r;
+    r.s = s;
+    r.seq = load_seq(b, s);
+    const int64_t first = ((int64_t)(r.seq.len >> 4) + j) << 4, left = (int64_t)r.seq.len + r.seq.n - first;
+    r.first = (int)first;
+    r.from = j == 0 ? r.seq.len - r.first : 0;
+    r.to = j < 0 ? 0 : (int)max(min(left, (int64_t)16), (int64_t)0);
+    return r;
+}
+
+// host
+inline int64_t run16_blocks(const Batch& b) {
+    return b.max_new == 1 ? b.seqs : (int64_t)(b.tokens >> 4) + 2 * (int64_t)b.seqs;
+}
+
+inline const char* rotation_error(const se12_step_rotation* r, int head_dim) {
+    if (!r) return "NULL argument";
+    if (r->rotary < 0 || r->rotary > head_dim || r->rotary % 8) return "rotary must be a multiple of 8 up to head_dim";
+    if (r->rotary > 0 && !r->inv_freq) return "NULL argument";
+    if (r->norm_dtype != SE12_STEP_BF16 && r->norm_dtype != SE12_STEP_F32) return "norm weights must be BF16 or FP32";
+    if (!(r->scale - r->scale == 0.0) || !(r->eps >= 0.0) || !(r->eps - r->eps == 0.0) || !(r->offset - r->offset == 0.0f))
+        return "scale, eps and offset must be finite, eps not below 0";
+    if (reinterpret_cast<uintptr_t>(r->inv_freq) % 16 || reinterpret_cast<uintptr_t>(r->q_norm) % 16 ||
+        reinterpret_cast<uintptr_t>(r->k_norm) % 16)
+        return "misaligned tensor";
+    return nullptr;
+}
+
+inline Rotation device_rotation(const se12_step_rotation* r) {
+    return {r->inv_freq, r->q_norm, r->k_norm, r->scale, r->eps, r->offset, r->rotary / 2, r->norm_dtype == SE12_STEP_F32, r->interleaved != 0};
+}
+
+}  // namespace se12step

@@ -106,7 +106,7 @@ __device__ __forceinline__ void unit_tiles(const AttendArgs& a, const Unit& u, i
 }
 
 // blocks the card holds at once
-constexpr int resident_blocks(bool e4m3, int d) { return 256 * (d == 256 || (d == 128 && !e4m3) ? 1 : 2); }
+constexpr int resident_blocks(int dtype, int d) { return 256 * (d == 256 || (d == 128 && dtype == SE12_STEP_BF16) ? 1 : 2); }
 
 // Which units are shared: of every 64 sequences those that see more than `tiles` tiles,
 // `units` of all at most, each in up to `splits` parts of about `tiles` tiles. Tiles: as
@@ -119,7 +119,7 @@ struct Sharing {
 
 template <int CT, int D>
 __device__ __forceinline__ Sharing sharing_of(const AttendArgs& a, int lane) {
-    constexpr int kTile = Form<CT>::kTile, kResident = resident_blocks(CT == SE12_STEP_E4M3, D);
+    constexpr int kTile = Form<CT>::kTile, kResident = resident_blocks(CT, D);
     if (a.parts < 2) return {0, 1, 1};
     const int capacity = a.b.width << a.page_log2;
     int64_t tiles = 0, units = 0;

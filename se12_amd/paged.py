@@ -1,7 +1,8 @@
 """A key/value cache in pages, for programs that decode sequences of different
-lengths in one batch: any page of a pool holds any part of any sequence, in BF16
-or in 8 bits (E4M3) with one power-of-two scale per page and KV head. (The static
-cache of `gemma2.Gemma2Decoder` has one length for the whole batch.)
+lengths in one batch: any page of a pool holds any part of any sequence, in BF16,
+in 8 bits (E4M3) with one power-of-two scale per page and KV head, or in 4 bits
+(E2M1) with an 8-bit scale per 32 columns of a token. (The static cache of
+`gemma2.Gemma2Decoder` has one length for the whole batch.)
 
     cache = PagedKvCache(pages=4096, page_size=64, kv_heads=4, head_dim=256, device=dev)  # one per layer
     batch = PagedBatch(page_table, lengths, starts, max_new=1)      # shared by the layers
@@ -10,17 +11,22 @@ cache of `gemma2.Gemma2Decoder` has one length for the whole batch.)
     ...                                                             # after the last layer
     lengths += starts.diff()
 
-Both calls run on the current stream of the cache's device, read the batch's
+`append` norms q and k per head and rotates them in either layout of pairs;
+`rotate_heads` does that by itself; `PagedKvCache.read` gives back what is held.
+
+All calls run on the current stream of the cache's device, read the batch's
 tensors when their kernels run (a captured call follows what they hold at its
 replay) and never wait for the device. No counterpart in the reference, whose
-runtime leaves the cache to the framework. Kernels: se12_step_paged_append and
-se12_step_paged_attention (include/se12_step.h).
+runtime leaves the cache to the framework. Kernels: se12_step_paged_append,
+se12_step_paged_append_rotated, se12_step_paged_attention, se12_step_paged_read and
+se12_step_rotate_heads (include/se12_step.h).
 """
 
 from __future__ import annotations
 
 import contextlib
 import ctypes
+import math
 
 import torch
 
@@ -28,6 +34,7 @@ from . import _native as nat
 
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128, 256)
+_DTYPES = {torch.bfloat16: nat.STEP_BF16, torch.float8_e4m3fn: nat.STEP_E4M3, torch.float4_e2m1fn_x2: nat.STEP_E2M1}
 _NO_GUARD = contextlib.nullcontext()
 
 
@@ -39,6 +46,60 @@ def _on(device: torch.device):
 def _stream(device: torch.device) -> int:
     """The handle of the device's current stream."""
     return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _row_view(t, name: str, head_dim: int, index: int, device, heads: int | None, tokens: int | None, dtype: torch.dtype | None,
+              multiple: int, owner: str = "the cache") -> torch.Tensor:
+    """t [tokens, heads, head_dim] with heads side by side and rows `multiple` elements apart: itself, or a copy."""
+    shape = t.shape if isinstance(t, torch.Tensor) else ()
+    if len(shape) != 3 or shape[2] != head_dim or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{name} must be [tokens, {'heads' if heads is None else heads}, {head_dim}]")
+    if tokens is not None and shape[0] != tokens:
+        raise ValueError(f"{name} has {shape[0]} rows, k has {tokens}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, {owner} on {device}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    (row, head, one), width = t.stride(), shape[1] * head_dim
+    apart = row >= width and row % multiple == 0
+    if (one != 1 or (head != head_dim and shape[1] > 1) or not (apart or shape[0] <= 1)
+            or t.data_ptr() % (multiple * t.element_size())):
+        t, apart = t.contiguous(), False
+        if t.data_ptr() % (multiple * t.element_size()):
+            t = t.clone()
+    # (of a single row any first stride is contiguous to torch)
+    return t if apart else t.as_strided(shape, (width, head_dim, 1))
+
+
+def _rotation(head_dim: int, device, inv_freq, interleaved, rotary_scale, q_norm, k_norm, norm_eps, norm_offset):
+    """The C struct of a rotation and norms, by reference, and the tensors it points to."""
+    rotary = 0
+    if inv_freq is not None:
+        if (not isinstance(inv_freq, torch.Tensor) or inv_freq.device != device or inv_freq.dtype != torch.float32 or inv_freq.dim() != 1
+                or not inv_freq.is_contiguous()):
+            raise ValueError(f"inv_freq must be a contiguous float32 vector on {device}")
+        rotary = 2 * inv_freq.numel()
+        if rotary % 8 or not 0 < rotary <= head_dim:
+            raise ValueError(f"inv_freq must hold a multiple of 4, at most {head_dim // 2} frequencies, got {inv_freq.numel()}")
+        if inv_freq.data_ptr() % 16:
+            inv_freq = inv_freq.clone()
+    held, dtypes = [inv_freq], set()
+    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if w is not None:
+            if (not isinstance(w, torch.Tensor) or w.device != device or w.dtype not in (torch.bfloat16, torch.float32)
+                    or tuple(w.shape) != (head_dim,) or not w.is_contiguous()):
+                raise ValueError(f"{name} must be a contiguous bfloat16 or float32 [{head_dim}] tensor on {device}")
+            dtypes.add(w.dtype)
+            if w.data_ptr() % 16:
+                w = w.clone()
+        held.append(w)
+    if len(dtypes) > 1:
+        raise ValueError("q_norm and k_norm must be of one type")
+    if not (math.isfinite(rotary_scale) and math.isfinite(norm_eps) and norm_eps >= 0 and abs(norm_offset) < 2.0 ** 127):
+        raise ValueError("rotary_scale, norm_eps and norm_offset must be finite, norm_eps not below 0")
+    pointers = [None if t is None else t.data_ptr() for t in held]
+    return ctypes.byref(nat.StepRotation(*pointers, rotary_scale, norm_eps, norm_offset,
+                                         nat.STEP_F32 if torch.float32 in dtypes else nat.STEP_BF16, rotary, int(bool(interleaved)))), held
 
 
 def _int32(t: torch.Tensor, name: str, shape: tuple, device: torch.device) -> torch.Tensor:
@@ -105,15 +166,27 @@ class PagedKvCache:
     kv_heads, head_dim, page_size] (a value column's tokens side by side, as the
     attention's matrix operands take them), dtype float8_e4m3fn or bfloat16; with
     float8_e4m3fn `k_scale` and `v_scale` FP32 [pages, kv_heads], positive numbers by
-    which a held value is multiplied. page_size 16, 32, 64 or 128, head_dim 64, 128 or 256."""
+    which a held value is multiplied. page_size 16, 32, 64 or 128, head_dim 64, 128 or 256.
+
+    dtype float4_e2m1fn_x2 (two values to an element, the first in the low half): `k`
+    [pages, kv_heads, page_size, head_dim / 2], `v` [pages, kv_heads, page_size / 16,
+    head_dim, 8] (16 tokens of a column side by side), `k_scale` and `v_scale` uint8
+    [pages, kv_heads, head_dim / 32, page_size], one to 32 columns of a token: an FP16
+    number's bits 14 .. 7 (5 of exponent, 3 of fraction); 255 stands for no number."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.float8_e4m3fn,
                  device=None) -> None:
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-        k = torch.zeros((pages, kv_heads, page_size, head_dim), dtype=dtype, device=device)
-        scales = [torch.ones((pages, kv_heads), dtype=torch.float32, device=device) for _ in range(2)] \
-            if dtype == torch.float8_e4m3fn else [None, None]
-        self._bind(k, torch.zeros((pages, kv_heads, head_dim, page_size), dtype=dtype, device=device), *scales)
+        if dtype == torch.float4_e2m1fn_x2:
+            shapes = ((pages, kv_heads, page_size, head_dim // 2), (pages, kv_heads, page_size // 16, head_dim, 8))
+            k, v = (torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype) for shape in shapes)
+            scales = [torch.zeros((pages, kv_heads, head_dim // 32, page_size), dtype=torch.uint8, device=device) for _ in range(2)]
+        else:
+            k = torch.zeros((pages, kv_heads, page_size, head_dim), dtype=dtype, device=device)
+            v = torch.zeros((pages, kv_heads, head_dim, page_size), dtype=dtype, device=device)
+            scales = [torch.ones((pages, kv_heads), dtype=torch.float32, device=device) for _ in range(2)] \
+                if dtype == torch.float8_e4m3fn else [None, None]
+        self._bind(k, v, *scales)
 
     @classmethod
     def from_tensors(cls, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
@@ -124,21 +197,25 @@ class PagedKvCache:
         return self
 
     def _bind(self, k, v, k_scale, v_scale) -> None:
-        if not isinstance(k, torch.Tensor) or k.dim() != 4 or k.dtype not in (torch.float8_e4m3fn, torch.bfloat16):
-            raise ValueError("k must be a float8_e4m3fn or bfloat16 [pages, kv_heads, page_size, head_dim] tensor")
+        if not isinstance(k, torch.Tensor) or k.dim() != 4 or k.dtype not in _DTYPES:
+            raise ValueError("k must be a float4_e2m1fn_x2, float8_e4m3fn or bfloat16 [pages, kv_heads, page_size, head_dim] tensor")
         pages, kv_heads, page_size, head_dim = k.shape
+        e2m1, e4m3 = k.dtype == torch.float4_e2m1fn_x2, k.dtype == torch.float8_e4m3fn
+        head_dim *= 2 if e2m1 else 1
         if page_size not in PAGE_SIZES or head_dim not in HEAD_DIMS:
             raise ValueError(f"page_size must be one of {PAGE_SIZES} and head_dim one of {HEAD_DIMS}, got {page_size}, {head_dim}")
         if pages < 1 or not 1 <= kv_heads <= 1024 or pages > 2 ** 31 - 1:
             raise ValueError("the cache needs a page and 1 to 1024 heads")
-        if not isinstance(v, torch.Tensor) or v.dtype != k.dtype or tuple(v.shape) != (pages, kv_heads, head_dim, page_size):
-            raise ValueError(f"v must be {k.dtype} {[pages, kv_heads, head_dim, page_size]}")
-        e4m3 = k.dtype == torch.float8_e4m3fn
+        v_shape = (pages, kv_heads, page_size // 16, head_dim, 8) if e2m1 else (pages, kv_heads, head_dim, page_size)
+        if not isinstance(v, torch.Tensor) or v.dtype != k.dtype or tuple(v.shape) != v_shape:
+            raise ValueError(f"v must be {k.dtype} {list(v_shape)}")
+        scaled, kind = e2m1 or e4m3, "an E2M1" if e2m1 else "an E4M3"
+        scale_shape, scale_dtype = ((pages, kv_heads, head_dim // 32, page_size), torch.uint8) if e2m1 else ((pages, kv_heads), torch.float32)
         for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-            if (t is not None) != e4m3:
-                raise ValueError(f"{name} goes with an E4M3 cache" if t is not None else f"an E4M3 cache needs {name}")
-            if e4m3 and (t.dtype != torch.float32 or tuple(t.shape) != (pages, kv_heads)):
-                raise ValueError(f"{name} must be float32 {[pages, kv_heads]}")
+            if (t is not None) != scaled:
+                raise ValueError(f"{name} goes with an E4M3 or E2M1 cache" if t is not None else f"{kind} cache needs {name}")
+            if scaled and (t.dtype != scale_dtype or tuple(t.shape) != scale_shape):
+                raise ValueError(f"{name} must be {scale_dtype} {list(scale_shape)}")
         tensors = [t for t in (k, v, k_scale, v_scale) if t is not None]
         if any(not t.is_contiguous() for t in tensors):
             raise ValueError("a cache's tensors must be contiguous")
@@ -147,31 +224,12 @@ class PagedKvCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.device, self.dtype, self._index = k.device, k.dtype, k.get_device()
         self.pages, self.kv_heads, self.page_size, self.head_dim = pages, kv_heads, page_size, head_dim
-        self._struct = ctypes.byref(nat.StepPages(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if e4m3 else None,
-                                     v_scale.data_ptr() if e4m3 else None, nat.STEP_E4M3 if e4m3 else nat.STEP_BF16, pages,
-                                     page_size, kv_heads, head_dim))
+        self._struct = ctypes.byref(nat.StepPages(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if scaled else None,
+                                     v_scale.data_ptr() if scaled else None, _DTYPES[k.dtype], pages, page_size, kv_heads, head_dim))
 
     def _rows(self, t: torch.Tensor, name: str, heads: int | None, tokens: int | None, dtype: torch.dtype | None,
               multiple: int) -> torch.Tensor:
-        """t [tokens, heads, head_dim] with heads side by side and rows `multiple` elements apart: itself, or a copy."""
-        shape = t.shape if isinstance(t, torch.Tensor) else ()
-        if len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
-            raise ValueError(f"{name} must be [tokens, {'heads' if heads is None else heads}, {self.head_dim}]")
-        if tokens is not None and shape[0] != tokens:
-            raise ValueError(f"{name} has {shape[0]} rows, k has {tokens}")
-        if t.get_device() != self._index:
-            raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
-        if dtype is not None and t.dtype != dtype:
-            raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-        (row, head, one), width = t.stride(), shape[1] * self.head_dim
-        apart = row >= width and row % multiple == 0
-        if (one != 1 or (head != self.head_dim and shape[1] > 1) or not (apart or shape[0] <= 1)
-                or t.data_ptr() % (multiple * t.element_size())):
-            t, apart = t.contiguous(), False
-            if t.data_ptr() % (multiple * t.element_size()):
-                t = t.clone()
-        # (of a single row any first stride is contiguous to torch)
-        return t if apart else t.as_strided(shape, (width, self.head_dim, 1))
+        return _row_view(t, name, self.head_dim, self._index, self.device, heads, tokens, dtype, multiple)
 
     def _check(self, batch: PagedBatch) -> None:
         if not isinstance(batch, PagedBatch):
@@ -180,15 +238,24 @@ class PagedKvCache:
             raise ValueError(f"the batch is on {batch.device}, the cache on {self.device}")
 
     def append(self, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,
-               inv_freq: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor | None:
+               inv_freq: torch.Tensor | None = None, out: torch.Tensor | None = None, *, interleaved: bool = False,
+               rotary_scale: float = 1.0, q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None,
+               norm_eps: float = 1e-6, norm_offset: float = 0.0) -> torch.Tensor | None:
         """Writes the new tokens' k and v [tokens, kv_heads, head_dim] to their pages, k rotated to its position, and
         returns q [tokens, heads, head_dim] rotated, in BF16 (into `out` if given, which may be q, or shares no memory with
         q, k and v; None without q). BF16 or FP32, all of one type; rows may be strided (views of one product's output).
         The rotation turns the pairs (i, i + len(inv_freq)) by position * inv_freq[i], FP32 inv_freq of up to head_dim / 2
         frequencies, a multiple of 4 (the elements behind the pairs stay; None: no rotation), as
-        se12_step_prefill_attention pairs them.
+        se12_step_prefill_attention pairs them; or the pairs (2 i, 2 i + 1) where `interleaved`; sine and cosine times
+        `rotary_scale`. With `q_norm` and `k_norm` [head_dim] (BF16 or FP32) q's and k's heads are normed before: x
+        rsqrt(mean(x^2) + norm_eps) (norm_offset + w). (`rotary.rotary_frequencies` stretches inv_freq to longer contexts.)
 
-        An E4M3 page and head's scale is the least power of two (2^-100 or more) that holds its new values; with older
+        An E2M1 cache holds 32 columns of a token as codes times the 8-bit scale nearest to a sixth of their largest
+        value, 10240 at most (so values up to 61440), each value as the nearest code; 32 columns with a NaN or an infinity
+        as NaN. What a token is held as depends on that token alone.
+
+        (Norms, interleaved pairs and a scale for a cache of BF16 or E4M3 take a launch more for each of q and k, and
+        memory for k and v in FP32.) An E4M3 page and head's scale is the least power of two (2^-100 or more) that holds its new values; with older
         tokens in the page at least what it was, and if it grows the older ones are rounded again. NaN and infinities
         are held as NaN. A page that two entries of the table name must not be written by a call."""
         self._check(batch)
@@ -197,15 +264,8 @@ class PagedKvCache:
         k = self._rows(k, "k", self.kv_heads, None, None, 4)
         tokens = k.shape[0]
         v = self._rows(v, "v", self.kv_heads, tokens, k.dtype, 4)
-        rotary = 0
-        if inv_freq is not None:
-            if inv_freq.device != self.device or inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
-                raise ValueError(f"inv_freq must be a contiguous float32 vector on {self.device}")
-            rotary = 2 * inv_freq.numel()
-            if rotary % 8 or not 0 < rotary <= self.head_dim:
-                raise ValueError(f"inv_freq must hold a multiple of 4, at most {self.head_dim // 2} frequencies, got {inv_freq.numel()}")
-            if inv_freq.data_ptr() % 16:
-                inv_freq = inv_freq.clone()
+        rotation, held = _rotation(self.head_dim, self.device, inv_freq, interleaved, rotary_scale, q_norm, k_norm, norm_eps, norm_offset)
+        inv_freq = held[0]
         heads, q_stride = self.kv_heads, 0
         if q is not None:
             q = self._rows(q, "q", None, tokens, k.dtype, 4)
@@ -215,13 +275,63 @@ class PagedKvCache:
             out = self._out(out, tokens, heads)
         elif out is not None:
             raise ValueError("out goes with q")
+        elif q_norm is not None:
+            raise ValueError("q_norm goes with q")
+        lib, new = nat.lib(), batch._struct(tokens)
+        dtype = nat.STEP_F32 if k.dtype == torch.float32 else nat.STEP_BF16
         with _on(self.device):
-            nat.step_check(nat.lib().se12_step_paged_append(
-                self._struct, batch._struct(tokens), None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                nat.STEP_F32 if k.dtype == torch.float32 else nat.STEP_BF16, q_stride, k.stride(0), v.stride(0), heads,
-                None if inv_freq is None else inv_freq.data_ptr(), rotary, None if q is None else out.data_ptr(),
-                _stream(self.device)))
+            stream = _stream(self.device)
+            if self.dtype == torch.float4_e2m1fn_x2:
+                nat.step_check(lib.se12_step_paged_append_rotated(
+                    self._struct, new, None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype, q_stride, k.stride(0),
+                    v.stride(0), heads, rotation, None if q is None else out.data_ptr(), stream))
+                return out
+            if q_norm is not None or k_norm is not None or interleaved or rotary_scale != 1.0:
+                return self._append_turned(batch, q, k, v, out, inv_freq, interleaved, rotary_scale, q_norm, k_norm, norm_eps, norm_offset)
+            nat.step_check(lib.se12_step_paged_append(
+                self._struct, new, None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype, q_stride, k.stride(0), v.stride(0),
+                heads, None if inv_freq is None else inv_freq.data_ptr(), 0 if inv_freq is None else 2 * inv_freq.numel(),
+                None if q is None else out.data_ptr(), stream))
         return out
+
+    def _append_turned(self, batch, q, k, v, out, inv_freq, interleaved, rotary_scale, q_norm, k_norm, norm_eps, norm_offset):
+        """append for a cache of BF16 or E4M3 whose kernel does not norm: q and k turned before, k kept in FP32."""
+        if q is not None:
+            spans = [(t.data_ptr(), t.data_ptr() + t.element_size() * ((t.shape[0] - 1) * t.stride(0) + t.shape[1] * t.shape[2]))
+                     for t in (out, k, v) if t.shape[0]]
+            if any(lo < spans[0][1] and spans[0][0] < hi for lo, hi in spans[1:]):
+                raise ValueError("out overlaps k or v")
+        turn = dict(interleaved=interleaved, rotary_scale=rotary_scale, norm_eps=norm_eps, norm_offset=norm_offset)
+        turned, _ = rotate_heads(batch, k, None, inv_freq, q_norm=k_norm, dtype=torch.float32, **turn)
+        self.append(batch, turned, v.float())
+        if q is not None:
+            # (q's kernel writes 16 bytes at once)
+            fits = out.data_ptr() % 16 == 0
+            got, _ = rotate_heads(batch, q, None, inv_freq, q_norm=q_norm, out=(out if fits else out.clone(), None), **turn)
+            if not fits:
+                out.copy_(got)
+        return out
+
+    def read(self, batch: PagedBatch, tokens: int, out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """What the cache holds of the batch's tokens, in BF16: (k, v) [tokens, kv_heads, head_dim], rows starts[s] ..
+        starts[s + 1] - 1 of positions lengths[s] .. (lengths of zero and starts that add the sequences' tokens up: whole
+        sequences; max_new the longest). Into `out` if given, two tensors apart. Rounded once: E2M1, BF16 and E4M3 under
+        power-of-two scales are exact. A token held nowhere gives zeros; rows of no sequence are not written."""
+        self._check(batch)
+        if int(tokens) != tokens or not 0 <= tokens < 2 ** 31:
+            raise ValueError(f"tokens must be a whole number from 0 to 2^31 - 1, got {tokens}")
+        shape = (int(tokens), self.kv_heads, self.head_dim)
+        if out is None:
+            out = torch.empty((2, *shape), dtype=torch.bfloat16, device=self.device).unbind()
+        k, v = out
+        for t in (k, v):
+            if not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype != torch.bfloat16 or tuple(t.shape) != shape or not t.is_contiguous():
+                raise ValueError(f"out must be two contiguous bfloat16 {list(shape)} tensors on {self.device}")
+            if t.data_ptr() % 16:
+                raise ValueError("out must be 16-byte aligned")
+        with _on(self.device):
+            nat.step_check(nat.lib().se12_step_paged_read(self._struct, batch._struct(shape[0]), k.data_ptr(), v.data_ptr(), _stream(self.device)))
+        return k, v
 
     def attend(self, batch: PagedBatch, q: torch.Tensor, scaling: float, softcap: float = 0.0, window: int = 0,
                out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
@@ -231,7 +341,7 @@ class PagedKvCache:
         window 0 = all. Returns BF16 [tokens, heads, head_dim] (`out` if given, apart from q; rows of no sequence are not
         written). No gradients.
 
-        FP32 scores and sums; weights rounded to BF16. A query that sees nothing gives zeros. `workspace`: uint8 of at
+        FP32 scores and sums; weights rounded to BF16 (over an E2M1 cache to FP16). A query that sees nothing gives zeros. `workspace`: uint8 of at
         least `attend_workspace()` bytes for callers that must not allocate; calls that share one must not overlap, and
         one that a captured call was given lives, as its other tensors, as long as the graph."""
         self._check(batch)
@@ -279,3 +389,57 @@ class PagedKvCache:
         if out.data_ptr() % 8:
             raise ValueError("out must be 8-byte aligned")
         return out
+
+
+def rotate_heads(batch: PagedBatch, q: torch.Tensor, k: torch.Tensor | None = None, inv_freq: torch.Tensor | None = None, *,
+                 interleaved: bool = False, rotary_scale: float = 1.0, q_norm: torch.Tensor | None = None,
+                 k_norm: torch.Tensor | None = None, norm_eps: float = 1e-6, norm_offset: float = 0.0,
+                 dtype: torch.dtype = torch.bfloat16, out: tuple | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """The batch's q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] (BF16 or FP32, both of one type; rows
+    may be strided) normed and rotated to their positions as `PagedKvCache.append` does, in `dtype` (bfloat16 or float32):
+    (q, k), k None without k. Into `out` = (q, k) if given; each may be its own input, and is apart from the rest
+    otherwise. head_dim a multiple of 8 up to 256. The batch's page table is not read; rows of no sequence are
+    not written. No gradients."""
+    if not isinstance(batch, PagedBatch):
+        raise ValueError("batch must be a PagedBatch")
+    if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("q must be a bfloat16 or float32 [tokens, heads, head_dim] tensor")
+    tokens, heads, head_dim = q.shape
+    if head_dim % 8 or not 8 <= head_dim <= 256 or not 1 <= heads <= 65535:
+        raise ValueError(f"q must have 1 to 65535 heads and a head_dim of a multiple of 8 up to 256, got {heads}, {head_dim}")
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"dtype must be bfloat16 or float32, got {dtype}")
+    index = batch.page_table.get_device()
+    q = _row_view(q, "q", head_dim, index, batch.device, None, None, None, 4, "the batch")
+    if k is not None:
+        if isinstance(k, torch.Tensor) and k.dim() == 3 and not 1 <= k.shape[1] <= 65535:
+            raise ValueError(f"k must have 1 to 65535 heads, got {k.shape[1]}")
+        if isinstance(k, torch.Tensor) and k.dim() == 3 and k.shape[0] != tokens:
+            raise ValueError(f"k has {k.shape[0]} rows, q has {tokens}")
+        k = _row_view(k, "k", head_dim, index, batch.device, None, None, q.dtype, 4, "the batch")
+    elif k_norm is not None:
+        raise ValueError("k_norm goes with k")
+    outs = []
+    for i, t in enumerate((q, k)):
+        given = None if out is None else out[i]
+        if t is None:
+            if given is not None:
+                raise ValueError("out's second tensor goes with k")
+            outs.append(None)
+        elif given is None:
+            outs.append(torch.empty(tuple(t.shape), dtype=dtype, device=batch.device))
+        else:
+            if not isinstance(given, torch.Tensor) or given.device != batch.device or given.dtype != dtype or given.shape != t.shape or not given.is_contiguous():
+                raise ValueError(f"out must hold contiguous {dtype} tensors of q's and k's shapes on {batch.device}")
+            if given.data_ptr() % 16:
+                raise ValueError("out must be 16-byte aligned")
+            outs.append(given)
+    rotation, held = _rotation(head_dim, batch.device, inv_freq, interleaved, rotary_scale, q_norm, k_norm, norm_eps, norm_offset)
+    types = {torch.float32: nat.STEP_F32, torch.bfloat16: nat.STEP_BF16}
+    with _on(batch.device):
+        nat.step_check(nat.lib().se12_step_rotate_heads(
+            batch._struct(tokens), q.data_ptr(), None if k is None else k.data_ptr(), types[q.dtype], q.stride(0),
+            0 if k is None else k.stride(0), heads, 0 if k is None else k.shape[1], head_dim, rotation, outs[0].data_ptr(),
+            None if k is None else outs[1].data_ptr(), types[dtype], _stream(batch.device)))
+    del held      # (read by the call; the stream keeps the order with what is made of their memory)
+    return outs[0], outs[1]
