@@ -31,18 +31,12 @@
 
 namespace se12step {
 
-typedef float floatx16_t __attribute__((ext_vector_type(16)));
-
 constexpr int kPromptThreads = 256;
 constexpr int kPromptWaves = kPromptThreads / 64;
 constexpr int kWaveColumns = 32;
 static_assert(kBlockColumns == kPromptWaves * kWaveColumns, "");
 constexpr int kSubTile = 32;              // keys of a first product
 constexpr int kSharedUnits = 1024;        // with more, blocks end close enough to each other as they are
-
-// the key (of 32) of row m of the first product's A operand: lane half h = bit 2 of
-// m takes keys 16 h ..
-__device__ __forceinline__ int key_of_row(int m) { return (m & 3) | ((m & 8) >> 1) | ((m & 16) >> 1) | ((m & 4) << 2); }
 
 // se12::lds_load16 from a uniform address and the lane's offset
 __device__ __forceinline__ void lds_load16(const void* base, uint32_t offset, uint32_t lds) {

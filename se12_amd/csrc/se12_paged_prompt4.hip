@@ -1,234 +1,181 @@
 // Attention over pages of E2M1 for sequences with many new tokens: the units, columns and
-// order of keys of se12_paged_prompt.hip, the operands of se12_paged_attend4.hpp.
+// parts of se12_paged_prompt.hip, the operands of se12_paged_attend4.hpp, tiles of 64 keys.
 //
-// A block takes 128 columns, 32 a wave, and walks the tiles of 64 keys they see. Each
-// value of a tile is turned into FP16 once a block, on its way into LDS, not once a wave
-// as it is read: 4 bits take a conversion and a product to two values, and four waves read
-// each. The tile after next is asked for and the next one turned while the products of this one
-// run; two tiles stand in LDS. v_mfma_f32_32x32x16_f16; keys' rows in the order that leaves a
-// lane's scores the second product's operand. The 16-byte pieces of an LDS row lie in an
-// order of its own, so that neither the lanes that read the same piece of 8 rows nor those
-// that write 8 pieces of a row meet in a bank.
+// Each value of a tile is turned into FP16 once a block of 128 columns, on its way into LDS
+// (se12_paged_tile4.hpp), not once a wave as it is read: 4 bits take a conversion and a packed
+// product to two values, and all waves read each. Two tiles stand in LDS, the one after is
+// on its way. Scores of keys to come are worked out beside the weights of those before, and the
+// product of weights and values beside what becomes of the next scores.
+//
+// Head dim 64 and 128: four waves of 32 columns (v_mfma_f32_32x32x16_f16), two blocks to a CU.
+// Head dim 256: a wave's sums and queries for 32 columns leave room for one wave to a SIMD, which
+// waits for each of its own instructions; eight waves of 16 columns (v_mfma_f32_16x16x32_f16)
+// read each operand twice as often from LDS, but two share a SIMD. (6,194 tokens of 5 prompts
+// behind up to 1,500 keys, 84.7 GFLOP: heads of 256 144 us the call, 173 the other way; heads of 128
+// 139, 173 the other way.)
+//
+// Bound by the vector instructions between the products, half of the time issued, and the
+// waits of waves for each other's: at 256, of 265,000 cycles 144,000 issue vector instructions (48
+// of 309 to 64 keys of 16 columns exponentials and inverses, at half the rate) and the matrix
+// unit is busy for 88,000.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include <type_traits>
 
-#include "se12_paged_attend4.hpp"
-#include "se12_paged_units.hpp"
+#include "se12_paged_tile4.hpp"
 
 namespace se12step {
 
-typedef float floatx16_t __attribute__((ext_vector_type(16)));
+// a wave's columns of a unit and what they see
+struct Columns4 {
+    int c0, mine, pos, pos_min, pos_max, reach;      // (mine: may be none; pos -1 sees nothing)
+    const uint16_t* q;
+};
 
-constexpr int kPrompt4Threads = 256, kWave4Columns = 32, kTile4 = 64;
+template <int D>
+__device__ __forceinline__ Columns4 columns_of(const AttendArgs& a, const UnitWork& u, int kh, int first, int most, int col) {
+    Columns4 x;
+    x.c0 = u.first + first;
+    x.mine = min(most, u.columns - x.c0);
+    const bool live = col < x.mine;
+    const int c = live ? x.c0 + col : u.first, token = c / a.group;
+    x.pos = live ? u.len + token : -1;
+    x.pos_min = u.len + x.c0 / a.group;
+    x.pos_max = x.mine > 0 ? u.len + (x.c0 + x.mine - 1) / a.group : -1;
+    x.reach = a.window > 0 ? a.window : INT32_MAX;
+    x.q = a.q + (u.start + token) * a.q_stride + (int64_t)(kh * a.group + c % a.group) * D;
+    return x;
+}
 
-// the key (of 32) of row m of the first product's A operand
-__device__ __forceinline__ int key_of_row4(int m) { return (m & 3) | ((m & 8) >> 1) | ((m & 16) >> 1) | ((m & 4) << 2); }
+// of two weights, in FP16: into place `at` of the product's operands, their sum added to l
+template <int kAt>
+__device__ __forceinline__ void put_weights(halfx8_t (&pf)[2], float& l, float p0, float p1) {
+    const halfx2_t w = {(_Float16)p0, (_Float16)p1};
+    pf[kAt / 8][kAt % 8] = w.x;
+    pf[kAt / 8][kAt % 8 + 1] = w.y;
+    // (the sum of what the product takes: two at once, times 1)
+    l = __builtin_amdgcn_fdot2(w, halfx2_t{(_Float16)1.0f, (_Float16)1.0f}, l, false);
+}
+
+// a wave's rows of the output, kCols of D / 8 pieces each, from `own` in LDS
+template <int D, int kCols>
+__device__ __forceinline__ void write_rows(const AttendArgs& a, const UnitWork& u, int kh, const Columns4& x, const uint8_t* own) {
+    constexpr int kPieces = D / 8, kTwist = kPieces < 16 ? kPieces - 1 : 15, kAtOnce = 64 / kPieces;
+    const int lane = threadIdx.x & 63;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int k = 0; k < kCols / kAtOnce; ++k) {
+        const int r = k * kAtOnce + lane / kPieces, piece = lane % kPieces, c = x.c0 + r;
+        if (r >= x.mine) continue;
+        const uint4 v = *reinterpret_cast<const uint4*>(own + r * 2 * D + 16 * (piece ^ (r & kTwist)));
+        uint2* to = reinterpret_cast<uint2*>(a.out + ((int64_t)(u.start + c / a.group) * a.heads + kh * a.group + c % a.group) * D + 8 * piece);
+        to[0] = make_uint2(v.x, v.y);
+        to[1] = make_uint2(v.z, v.w);
+    }
+}
 
 template <int D, bool kCapped>
-__global__ __launch_bounds__(kPrompt4Threads, D == 256 ? 1 : 2) void paged_prompt4_kernel(AttendArgs a) {
-    constexpr int kGroups = D / 32, kRows = D / 32, kQSteps = D / 16;
-    constexpr int kKeyPieces = D / 8;                        // 16-byte pieces of a key's row in LDS
-    constexpr int kWords = D >= 128 ? 4 : 2;                 // of a thread's piece of a key as it is held
-    constexpr int kKeyLoads = kTile4 * D / 8 / kWords / kPrompt4Threads;       // pieces of a thread
-    constexpr int kHeldPieces = D / (8 * kWords);            // of a key
-    constexpr int kValueLoads = kTile4 * D / 32 / kPrompt4Threads;             // pieces of 16 tokens of two columns
-    constexpr int kValueThreads = kValueLoads > 0 ? kPrompt4Threads : kTile4 * D / 32;
-    constexpr int kKeyBytes = kTile4 * D * 2, kBuffer = 2 * kKeyBytes;
-    static_assert(kKeyLoads >= 1, "");
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];     // [2][keys, values], then the values' scales that are none
+__global__ __launch_bounds__(256, 2) void paged_prompt4_kernel(AttendArgs a) {
+    using Tile = Tile4<D, 256, false>;
+    constexpr int kRows = D / 32, kN = D / 16;                // rows of 32 columns of the output; steps of either product
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kh = blockIdx.x % a.kvh;
     const UnitWork u = unit_work(a, blockIdx.x / a.kvh);
     if (u.s < 0) return;
-    const int t0 = u.t0, t1 = u.t1;
-    uint16_t* const bad = reinterpret_cast<uint16_t*>(lds + 2 * kBuffer);      // [2][4 runs of 16 tokens][8 groups]
-
-    const int col = lane & 31, half = lane >> 5;
-    const int c0 = u.first + wave * kWave4Columns, mine = min(kWave4Columns, u.columns - c0);   // (may be none)
-    const bool live = col < mine;
-    const int c = live ? c0 + col : u.first, token = c / a.group;
-    const int pos = live ? u.len + token : -1;
-    const int pos_min = u.len + c0 / a.group, pos_max = mine > 0 ? u.len + (c0 + mine - 1) / a.group : -1;
-    const int reach = a.window > 0 ? a.window : INT32_MAX;
-
-    const int P = 1 << a.page_log2;
-    const int32_t* table = a.b.table + u.s * a.b.table_stride;
-    auto entry = [&](int key) { return table[min(key >> a.page_log2, a.b.width - 1)]; };
-    auto in_pool = [&](int e) { return (uint32_t)e < (uint32_t)a.pages ? e : 0; };
+    const int t0 = u.t0, t1 = u.t1, col = lane & 31, half = lane >> 5;
+    const Columns4 x = columns_of<D>(a, u, kh, 32 * wave, 32, col);
     auto to_last = [&](int t) { return min(t, t1 - 1); };
-    const uint8_t* const kc = static_cast<const uint8_t*>(a.kc);
-    const uint8_t* const vc = static_cast<const uint8_t*>(a.vc);
-    const uint8_t* const k_scale = reinterpret_cast<const uint8_t*>(a.k_scale);
-    const uint8_t* const v_scale = reinterpret_cast<const uint8_t*>(a.v_scale);
 
-    // What a thread brings of a tile. Keys: pieces of rows; values: columns 2 x, 2 x + 1 of a run.
-    struct Held {
-        uint32_t k[kKeyLoads][kWords];
-        uint32_t ks[kKeyLoads];
-        uint4 v[kValueLoads > 0 ? kValueLoads : 1], vs[kValueLoads > 0 ? kValueLoads : 1];
-    } held;
-    auto key_row = [&](int i) { return (tid + i * kPrompt4Threads) / kHeldPieces; };
-    auto run_of = [&](int i) { return (tid + i * kPrompt4Threads) / (D / 2); };
-    struct Entries {
-        int k[kKeyLoads], v[kValueLoads > 0 ? kValueLoads : 1];
-    } entries;
-    auto load_entries = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < kKeyLoads; ++i) entries.k[i] = entry(t * kTile4 + key_row(i));
-#pragma unroll
-        for (int i = 0; i < (kValueLoads > 0 ? kValueLoads : 1); ++i) entries.v[i] = entry(t * kTile4 + 16 * min(run_of(i), 3));
-    };
-    auto load_held = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < kKeyLoads; ++i) {
-            const int r = key_row(i), piece = (tid + i * kPrompt4Threads) % kHeldPieces, slot = (t * kTile4 + r) & (P - 1);
-            const int64_t head_page = (int64_t)in_pool(entries.k[i]) * a.kvh + kh;
-            const uint8_t* p = kc + (head_page * P + slot) * (D / 2) + 4 * kWords * piece;
-            if constexpr (kWords == 4) {
-                const uint4 x = *reinterpret_cast<const uint4*>(p);
-                held.k[i][0] = x.x, held.k[i][1] = x.y, held.k[i][2] = x.z, held.k[i][3] = x.w;
-            } else {
-                const uint2 x = *reinterpret_cast<const uint2*>(p);
-                held.k[i][0] = x.x, held.k[i][1] = x.y;
-            }
-            held.ks[i] = k_scale[(head_page * kGroups + piece * 8 * kWords / 32) * P + slot];
-        }
-#pragma unroll
-        for (int i = 0; i < (kValueLoads > 0 ? kValueLoads : 1); ++i) {
-            const int run = min(run_of(i), 3), x = (tid + i * kPrompt4Threads) % (D / 2), slot = (t * kTile4 + 16 * run) & (P - 1);
-            const int64_t head_page = (int64_t)in_pool(entries.v[i]) * a.kvh + kh;
-            held.v[i] = *reinterpret_cast<const uint4*>(vc + ((head_page << (a.page_log2 - 4)) + (slot >> 4)) * (8 * D) + 16 * x);
-            held.vs[i] = *reinterpret_cast<const uint4*>(v_scale + (head_page * kGroups + x / 16) * P + slot);
-        }
-    };
-    // where piece p of a key's row, or of a value column, lies
-    auto key_place = [](int r, int p) {
-        const int twist = kKeyPieces >= 16 ? (r & 7) | ((r & 16) >> 1) : ((r & 7) | ((r & 16) >> 1)) >> 1;
-        const int q = p ^ ((p >> 2) & 7);
-        return r * (kKeyPieces * 16) + 16 * (q ^ twist);
-    };
-    auto value_place = [](int r, int p) { return r * 128 + 16 * (p ^ (r & 7) ^ ((r >> 3) & 1)); };
-    auto put_keys = [&](int buffer) {
-        uint8_t* to = lds + buffer * kBuffer;
-#pragma unroll
-        for (int i = 0; i < kKeyLoads; ++i) {
-            const int r = key_row(i), piece = (tid + i * kPrompt4Threads) % kHeldPieces;
-            const halfx2_t s2 = __builtin_bit_cast(halfx2_t, held.ks[i] * 0x00800080u);
-            const halfx2_t by[4] = {s2, s2, s2, s2};
-#pragma unroll
-            for (int h = 0; h < kWords; ++h)
-                *reinterpret_cast<halfx8_t*>(to + key_place(r, kWords * piece + h)) = e2m1_operand(held.k[i][h], by);
-        }
-    };
-    auto put_values = [&](int buffer) {
-        uint8_t* to = lds + buffer * kBuffer + kKeyBytes;
-        if (tid >= kValueThreads) return;
-#pragma unroll
-        for (int i = 0; i < (kValueLoads > 0 ? kValueLoads : 1); ++i) {
-            const int run = run_of(i), x = (tid + i * kPrompt4Threads) % (D / 2);
-            uint32_t s[4] = {held.vs[i].x, held.vs[i].y, held.vs[i].z, held.vs[i].w};
-            // (a scale that is no number leaves the product: 0 x NaN is NaN)
-            uint32_t none = 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint32_t b = no_scales(s[k]) >> 7;
-                s[k] &= ~(b * 255u);
-                none |= ((b * 0x01020408u) >> 24 & 15u) << (4 * k);
-            }
-            if (x % 16 == 0) bad[buffer * 32 + run * 8 + x / 16] = (uint16_t)none;
-            halfx2_t pair[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                pair[k] = __builtin_bit_cast(halfx2_t, __builtin_amdgcn_perm(0u, s[k / 2], k & 1 ? 0x0C030C02u : 0x0C010C00u) << 7);
-            const uint32_t w[4] = {held.v[i].x, held.v[i].y, held.v[i].z, held.v[i].w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<halfx8_t*>(to + value_place(2 * x + j / 2, 2 * run + (j & 1))) = e2m1_operand(w[j], pair + 4 * (j & 1));
-        }
-    };
-
-    load_entries(t0);
-    load_held(t0);
-    load_entries(to_last(t0 + 1));
-    if (tid < 64) bad[tid] = 0;
+    // The walk, in halves of 32 keys. Operands are read from LDS half a half ahead, so keys are
+    // two tiles ahead of the products in LDS, values one, and a barrier a tile is enough: what is
+    // written in a tile's time goes over what every wave had read before its start.
+    Tile tile(a, u, kh, lds);
+    int ke = tile.key_entry(t0), ve = tile.value_entry(t0);
+    auto page_entries = [&](int t) { return make_int2(tile.entry(t * kTile4 + 16 * half), tile.entry(t * kTile4 + 32 + 16 * half)); };
+    int2 pages = page_entries(t0);
+    tile.load_keys(t0, ke);
+    tile.load_values(t0, ve);
+    ke = tile.key_entry(to_last(t0 + 1));
+    ve = tile.value_entry(to_last(t0 + 1));
+    if (tid < 64) tile.bad[tid] = 0;
+    halfx8_t qf[kN];
+    const float by = load_query<kN, 16, 32>(qf, x.q + 8 * half, a.c1);
     __syncthreads();
-    halfx8_t qf[kQSteps];
-    float by;
-    {
-        // the queries, times 2^lift
-        const uint16_t* qp = a.q + (u.start + token) * a.q_stride + (int64_t)(kh * a.group + c % a.group) * D + 8 * half;
-        uint4 x[kQSteps];
-        uint32_t most = 0;
-#pragma unroll
-        for (int i = 0; i < kQSteps; ++i) {
-            x[i] = *reinterpret_cast<const uint4*>(qp + 16 * i);
-            for (const uint32_t v : {x[i].x, x[i].y, x[i].z, x[i].w}) most = max(most, max((v << 16) & 0x7FFF0000u, v & 0x7FFF0000u));
-        }
-        most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
-        const int lift = 14 + 127 - (int)(most >> 23);
-        by = ldexpf(a.c1, -lift);
-#pragma unroll
-        for (int i = 0; i < kQSteps; ++i) {
-            const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                qf[i][2 * k] = (_Float16)ldexpf(__uint_as_float(v[k] << 16), lift);
-                qf[i][2 * k + 1] = (_Float16)ldexpf(__uint_as_float(v[k] & 0xFFFF0000u), lift);
-            }
-        }
-    }
-    put_keys(0);
-    put_values(0);
-    load_held(to_last(t0 + 1));
-    load_entries(to_last(t0 + 2));
+    tile.put_keys(0);
+    tile.note_none(0);
+    tile.put_values(0);
+    tile.load_keys(to_last(t0 + 1), ke);
+    tile.load_values(to_last(t0 + 1), ve);
+    ke = tile.key_entry(to_last(t0 + 2));
+    ve = tile.value_entry(to_last(t0 + 2));
+    tile.put_keys(1);
+    tile.load_keys(to_last(t0 + 2), ke);
+    ke = tile.key_entry(to_last(t0 + 3));
+    __syncthreads();
 
-    floatx16_t o[kRows];
+    floatx16_t o[kRows], d;
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
     float m = -INFINITY, l = 0.0f;
-    uint32_t none_seen = 0;       // groups of which the column saw what is no number
-    const int key_row0 = key_of_row4(col);
+    uint32_t none_seen = 0;       // groups of which the column sees what is no number
+    halfx8_t kf[kN], vf[kRows][2];
+    const int lds0 = (int)se12::lds_address(lds);
+    const int key_at0 = lds0 + Tile::key_place(key_of_row(col), half), value_at0 = lds0 + Tile::value_place(col, 2 * half);
+    // (order(p) of piece p = 2 i + half is order(2 i) ^ half)
+    auto read_key = [&](int at, int i, int j) { return lds_get((at ^ (16 * Tile::key_order(2 * i))) + j * 32 * 16 * Tile::kKeyPieces); };
+    float sc[16], top, p[2];      // scores, or r of cap - 2 cap r; two weights
+    auto cap_score = [&](int e) { sc[e] = kCapped ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(d[e] * by)) : d[e] * by; };
+    auto find_top = [&]() {
+        top = sc[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) top = kCapped ? fminf(top, sc[e]) : fmaxf(top, sc[e]);
+        if constexpr (kCapped) top = a.cap - 2.0f * a.cap * top;
+    };
+    auto no_scores = [&]() {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) d[e] = 0.0f;
+    };
+    no_scores();
+#pragma unroll
+    for (int i = 0; i < kN; ++i) d = __builtin_amdgcn_mfma_f32_32x32x16_f16(read_key(key_at0, i, 0), qf[i], d, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < kN; ++i) kf[i] = read_key(key_at0, i, 1);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) cap_score(e);
+    find_top();
     for (int t = t0; t < t1; ++t) {
         const int buffer = (t - t0) & 1;
-        __syncthreads();          // this tile has come, and every wave is done with the other buffer
-        const uint8_t* const keys = lds + buffer * kBuffer;
-        const uint8_t* const values = keys + kKeyBytes;
-        floatx16_t d[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) d[j][e] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kQSteps; ++i) {
-                const halfx8_t k = *reinterpret_cast<const halfx8_t*>(keys + key_place(32 * j + key_row0, 2 * i + half));
-                d[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[i], d[j], 0, 0, 0);
-            }
-        }
-        put_keys(buffer ^ 1);
-        put_values(buffer ^ 1);
-        load_held(to_last(t + 2));
-        load_entries(to_last(t + 3));
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int k0 = t * kTile4 + 32 * j, key0 = k0 + 16 * half;
-            float sc[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-                sc[e] = kCapped ? a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(d[j][e] * by)) : d[j][e] * by;
-            const bool here = (uint32_t)entry(key0) < (uint32_t)a.pages;
-            const bool inside = (k0 + 31 <= pos_min) & (k0 + 32 <= u.keys) & (pos_max - k0 < reach) & (__builtin_amdgcn_ballot_w64(!here) == 0);
+        __syncthreads();
+        const uint4 none0 = tile.none_of(buffer, half), none1 = tile.none_of(buffer, 2 + half);
+        const uint32_t any_none = none0.x | none0.y | none0.z | none0.w | none1.x | none1.y | none1.z | none1.w;
+        const int2 here = pages;
+        pages = page_entries(to_last(t + 1));
+        each_of<2>([&](auto j) {
+            const int k0 = t * kTile4 + 32 * j.value, key0 = k0 + 16 * half;
+            const bool held = (uint32_t)(j.value ? here.y : here.x) < (uint32_t)a.pages;
+            const bool inside = (k0 + 31 <= x.pos_min) & (k0 + 32 <= u.keys) & (x.pos_max - k0 < x.reach) & (__builtin_amdgcn_ballot_w64(!held) == 0);
             if (!inside) {
-                const int since = max(pos - reach + 1, 0) - key0, to = here ? min(pos + 1, u.keys) - key0 : 0;
+                asm volatile("");      // (left to the halves that need it)
+                const int since = max(x.pos - x.reach + 1, 0) - key0, to = held ? min(x.pos + 1, u.keys) - key0 : 0;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) sc[e] = (e < since || e >= to) ? -INFINITY : sc[e];
+                for (int e = 0; e < 16; ++e) sc[e] = (e < since || e >= to) ? (kCapped ? INFINITY : -INFINITY) : sc[e];
+                find_top();
             }
-            float top = sc[0];
+            if (j.value == 1) tile.note_none(buffer ^ 1);
+            if (j.value == 1 && __builtin_amdgcn_ballot_w64(any_none != 0) != 0) {
+                asm volatile("");
 #pragma unroll
-            for (int e = 1; e < 16; ++e) top = fmaxf(top, sc[e]);
+                for (int i = 0; i < 2; ++i) {
+                    const int first = t * kTile4 + 32 * i + 16 * half;
+                    const bool there = (uint32_t)(i ? here.y : here.x) < (uint32_t)a.pages;
+                    none_seen |= Tile::groups_of(tile.none_of(buffer, 2 * i + half), max(x.pos - x.reach + 1, 0) - first,
+                                                 there ? min(x.pos + 1, u.keys) - first : 0);
+                }
+            }
             if (__builtin_amdgcn_ballot_w64(top > m + kSlack4) != 0) {
                 const float to = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
                 const float scale = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
@@ -237,32 +184,60 @@ __global__ __launch_bounds__(kPrompt4Threads, D == 256 ? 1 : 2) void paged_promp
 #pragma unroll
                 for (int i = 0; i < kRows; ++i) o[i] *= scale;
             }
+            // Beside each matrix instruction as much of the rest as it takes time for, in this
+            // order (left to itself the compiler puts reads, conversions and exponentials into runs of
+            // their own, the matrix unit idle).
+            constexpr int kEach = 16 / kN, kPuts = j.value == 0 ? Tile::kWords : 4, kLast = 2 * kN - 2;
+            constexpr int kAhead = kN / 2 > 4 ? kN / 2 : 4;      // values' pieces read before their product
             const float base = (m == -INFINITY ? 0.0f : m) - kLift4;
             halfx8_t pf[2];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float p = __builtin_amdgcn_exp2f(sc[e] - base);
-                l += p;
-                pf[e / 8][e % 8] = (_Float16)p;
-            }
-            const uint4 none = *reinterpret_cast<const uint4*>(bad + buffer * 32 + (2 * j + half) * 8);
-            if (__builtin_amdgcn_ballot_w64((none.x | none.y | none.z | none.w) != 0) != 0) {
-                const uint32_t w[4] = {none.x, none.y, none.z, none.w};
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const bool seen = !((float)pf[e / 8][e % 8] <= 0.0f);
-#pragma unroll
-                    for (int g = 0; g < kGroups; ++g) none_seen |= seen && (w[g / 2] >> (16 * (g & 1) + e) & 1u) ? 1u << g : 0u;
+            int key_at = key_at0 + (buffer ^ 1) * Tile::kBuffer, value_at = value_at0 + buffer * Tile::kBuffer;
+            asm volatile("" : "+v"(key_at), "+v"(value_at));      // (addresses, not one for every piece over the walk)
+            auto read_value = [&](int i) { vf[i / 2][i % 2] = lds_get((value_at ^ (16 * (4 * j.value + i % 2))) + 4096 * (i / 2)); };
+            auto put_beside = [&](auto step) {      // of 2 kN steps
+                constexpr int at = (step.value * kPuts + kLast - 1) / kLast, end = ((step.value + 1) * kPuts + kLast - 1) / kLast;
+                if constexpr (at < end && at < kPuts) {
+                    if constexpr (j.value == 0)
+                        tile.template put_key<at>(buffer);
+                    else
+                        tile.template put_value<at>(buffer ^ 1);
                 }
-            }
-#pragma unroll
-            for (int i = 0; i < kRows; ++i)
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const halfx8_t v = *reinterpret_cast<const halfx8_t*>(values + value_place(32 * i + col, 4 * j + 2 * half + n));
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pf[n], o[i], 0, 0, 0);
+                if constexpr (step.value == kLast) {
+                    if constexpr (j.value == 0) {
+                        tile.load_keys(to_last(t + 3), ke);
+                        ke = tile.key_entry(to_last(t + 4));
+                    } else {
+                        tile.load_values(to_last(t + 2), ve);
+                        ve = tile.value_entry(to_last(t + 3));
+                    }
                 }
-        }
+            };
+            no_scores();
+            each_of<kN>([&](auto step) {
+                constexpr int i = step.value;
+                d = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i], qf[i], d, 0, 0, 0);
+                if constexpr (i >= kN - kAhead) read_value(i - (kN - kAhead));
+                each_of<kEach>([&](auto each) {
+                    constexpr int e = i * kEach + each.value;
+                    p[e & 1] = __builtin_amdgcn_exp2f(kCapped ? (a.cap - base) - 2.0f * a.cap * sc[e] : sc[e] - base);
+                    if constexpr (e & 1) put_weights<e - 1>(pf, l, p[0], p[1]);
+                });
+                put_beside(std::integral_constant<int, i>{});
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            each_of<kN>([&](auto step) {
+                constexpr int i = step.value, lag = kN > 4 ? 2 : 0;
+                o[i / 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i / 2][i % 2], pf[i % 2], o[i / 2], 0, 0, 0);
+                kf[i] = read_key(key_at, i, j.value);
+                if constexpr (i + kAhead < kN) read_value(i + kAhead);
+                put_beside(std::integral_constant<int, kN + i>{});
+                // (the scores are there two products on)
+#pragma unroll
+                for (int e = max(i - lag, 0) * kEach; e < (i + 1 == kN ? 16 : max(i + 1 - lag, 0) * kEach); ++e) cap_score(e);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            find_top();
+        });
     }
     l += __shfl_xor(l, 32, 64);
     none_seen |= (uint32_t)__shfl_xor((int)none_seen, 32, 64);
@@ -272,22 +247,21 @@ __global__ __launch_bounds__(kPrompt4Threads, D == 256 ? 1 : 2) void paged_promp
     }
     if (u.parts > 1) {
         // the part, as the lanes hold it
-        const int64_t p = part_place(a, u, kh);
-        float4* to = reinterpret_cast<float4*>(a.part + p * kBlockColumns * D) + wave * (D / 8) * 64 + lane;
+        const int64_t part = part_place(a, u, kh);
+        float4* to = reinterpret_cast<float4*>(a.part + part * kBlockColumns * D) + wave * (D / 8) * 64 + lane;
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
 #pragma unroll
             for (int g = 0; g < 4; ++g)
                 to[(4 * i + g) * 64] = make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
         if (half == 0)
-            reinterpret_cast<float2*>(a.part + (int64_t)a.parts * a.kvh * kBlockColumns * D)[p * kBlockColumns + wave * kWave4Columns + col] =
-                make_float2(m, l);
+            reinterpret_cast<float2*>(a.part + (int64_t)a.parts * a.kvh * kBlockColumns * D)[part * kBlockColumns + 32 * wave + col] = make_float2(m, l);
         return;
     }
     // through LDS to whole rows
     __syncthreads();
-    constexpr int kOutPieces = D / 8, kTwist = kOutPieces < 16 ? kOutPieces - 1 : 15, kRowsAtOnce = 64 / kOutPieces;
-    uint8_t* own = lds + wave * kWave4Columns * 2 * D;
+    constexpr int kTwist = D / 8 < 16 ? D / 8 - 1 : 15;
+    uint8_t* own = lds + wave * 32 * 2 * D;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
@@ -295,37 +269,197 @@ __global__ __launch_bounds__(kPrompt4Threads, D == 256 ? 1 : 2) void paged_promp
         for (int g = 0; g < 4; ++g)
             store4(reinterpret_cast<uint16_t*>(own + col * 2 * D + 16 * ((4 * i + g) ^ (col & kTwist)) + 8 * half), o[i][4 * g] * inv,
                    o[i][4 * g + 1] * inv, o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    write_rows<D, 32>(a, u, kh, x, own);
+}
+
+// Eight waves of 16 columns. Row r of the first product's step g is key 16 (r / 4) + 4 g + r % 4,
+// so a lane's scores are those of 16 keys in a row of its column.
+template <int D, bool kCapped>
+__global__ __launch_bounds__(512, 2) void paged_prompt4_wide_kernel(AttendArgs a) {
+    using Tile = Tile4<D, 512, true>;
+    constexpr int kRows = D / 16, kSteps = D / 32, kN = D / 8;      // kN: products of either kind
+    constexpr int kAhead = 8;                                       // operands read ahead of theirs
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int kh = blockIdx.x % a.kvh;
+    const UnitWork u = unit_work(a, blockIdx.x / a.kvh);
+    if (u.s < 0) return;
+    const int t0 = u.t0, t1 = u.t1, col = lane & 15, quarter = lane >> 4;
+    const Columns4 x = columns_of<D>(a, u, kh, 16 * wave, 16, col);
+    auto to_last = [&](int t) { return min(t, t1 - 1); };
+
+    // The walk: scores of the next tile beside the weights of this one, then the product of its
+    // weights and values beside what becomes of the next scores. In LDS keys are two tiles ahead of
+    // that product and values one, so a barrier a tile is enough: what is written in a tile's time
+    // goes over what every wave had read before its start.
+    Tile tile(a, u, kh, lds);
+    int ke = tile.key_entry(t0), ve = tile.value_entry(t0), page_entry = tile.entry(t0 * kTile4 + 16 * quarter);
+    tile.load_keys(t0, ke);
+    tile.load_values(t0, ve);
+    ke = tile.key_entry(to_last(t0 + 1));
+    ve = tile.value_entry(to_last(t0 + 1));
+    if (tid < 64) tile.bad[tid] = 0;
+    halfx8_t qf[kSteps];
+    const float by = load_query<kSteps, 32, 16>(qf, x.q + 8 * quarter, a.c1);
+    __syncthreads();
+    tile.put_keys(0);
+    tile.note_none(0);
+    tile.put_values(0);
+    tile.load_keys(to_last(t0 + 1), ke);
+    tile.load_values(to_last(t0 + 1), ve);
+    ke = tile.key_entry(to_last(t0 + 2));
+    ve = tile.value_entry(to_last(t0 + 2));
+    tile.put_keys(1);
+    tile.load_keys(to_last(t0 + 2), ke);
+    ke = tile.key_entry(to_last(t0 + 3));
+    __syncthreads();
+
+    floatx4_t o[kRows], d[4];
 #pragma unroll
-    for (int k = 0; k < kWave4Columns / kRowsAtOnce; ++k) {
-        const int r = k * kRowsAtOnce + lane / kOutPieces, piece = lane % kOutPieces, x = c0 + r;
-        if (r >= mine) continue;
-        const uint4 v = *reinterpret_cast<const uint4*>(own + r * 2 * D + 16 * (piece ^ (r & kTwist)));
-        uint2* to = reinterpret_cast<uint2*>(a.out + ((int64_t)(u.start + x / a.group) * a.heads + kh * a.group + x % a.group) * D + 8 * piece);
-        to[0] = make_uint2(v.x, v.y);
-        to[1] = make_uint2(v.z, v.w);
+    for (int i = 0; i < kRows; ++i) o[i] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+    uint32_t none_seen = 0;       // groups of which the column sees what is no number
+    const int lds0 = (int)se12::lds_address(lds);
+    const int key_at0 = lds0 + Tile::key_place(16 * (col >> 2) + (col & 3), quarter), value_at0 = lds0 + Tile::value_place(col, 2 * quarter);
+    float sc[16], top, p[2];      // scores, or r of cap - 2 cap r; two weights
+    auto cap_score = [&](int e) {
+        const float v = d[e / 4][e % 4] * by;
+        sc[e] = kCapped ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v)) : v;
+    };
+    auto find_top = [&]() {
+        top = sc[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) top = kCapped ? fminf(top, sc[e]) : fmaxf(top, sc[e]);
+        if constexpr (kCapped) top = a.cap - 2.0f * a.cap * top;
+    };
+    // product n of the scores: step n / 4 of the inner dimension, of the rows step n % 4 (order(p)
+    // of piece p = 4 s + quarter is order(4 s) ^ quarter)
+    auto read_key = [&](int at, int n) { return lds_get((at ^ (16 * Tile::key_order(4 * (n / 4)))) + (n % 4) * 4 * 16 * Tile::kKeyPieces); };
+    auto score_step = [&](int n, halfx8_t k) {
+        d[n % 4] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[n / 4], n < 4 ? floatx4_t{0.0f, 0.0f, 0.0f, 0.0f} : d[n % 4], 0, 0, 0);
+    };
+#pragma unroll
+    for (int n = 0; n < kN; ++n) score_step(n, read_key(key_at0, n));
+#pragma unroll
+    for (int e = 0; e < 16; ++e) cap_score(e);
+    find_top();
+    for (int t = t0; t < t1; ++t) {
+        const int buffer = (t - t0) & 1;
+        __syncthreads();
+        const uint4 none = tile.none_of(buffer, quarter);
+        int key_at = key_at0 + (buffer ^ 1) * Tile::kBuffer, value_at = value_at0 + buffer * Tile::kBuffer;
+        asm volatile("" : "+v"(key_at), "+v"(value_at));      // (addresses, not one for every piece over the walk)
+        halfx8_t ring[kAhead];
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) ring[n] = read_key(key_at, n);
+        const int k0 = t * kTile4, key0 = k0 + 16 * quarter;
+        const bool held = (uint32_t)page_entry < (uint32_t)a.pages;
+        page_entry = tile.entry(to_last(t + 1) * kTile4 + 16 * quarter);
+        tile.note_none(buffer ^ 1);
+        const bool inside = (k0 + kTile4 - 1 <= x.pos_min) & (k0 + kTile4 <= u.keys) & (x.pos_max - k0 < x.reach) & (__builtin_amdgcn_ballot_w64(!held) == 0);
+        const int since = max(x.pos - x.reach + 1, 0) - key0, to = held ? min(x.pos + 1, u.keys) - key0 : 0;
+        if (!inside) {
+            asm volatile("");      // (left to the tiles that need it)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[e] = (e < since || e >= to) ? (kCapped ? INFINITY : -INFINITY) : sc[e];
+            find_top();
+        }
+        if (__builtin_amdgcn_ballot_w64((none.x | none.y | none.z | none.w) != 0) != 0) {
+            asm volatile("");
+            none_seen |= Tile::groups_of(none, since, to);
+        }
+        if (__builtin_amdgcn_ballot_w64(top > m + kSlack4) != 0) {
+            asm volatile("");
+            float next = fmaxf(top, __shfl_xor(top, 16, 64));
+            next = fmaxf(m, fmaxf(next, __shfl_xor(next, 32, 64)));
+            const float scale = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - next);
+            m = next;
+            l *= scale;
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) o[i] *= scale;
+        }
+        const float base = (m == -INFINITY ? 0.0f : m) - kLift4;
+        halfx8_t pf[2];
+        auto read_value = [&](int n) { return lds_get((value_at ^ (16 * (n % 2))) + 2048 * (n / 2)); };
+        each_of<kN>([&](auto step) {
+            constexpr int n = step.value, from = 16 * n / kN, upto = 16 * (n + 1) / kN;
+            score_step(n, ring[n % kAhead]);
+            ring[n % kAhead] = n + kAhead < kN ? read_key(key_at, n + kAhead) : read_value(n + kAhead - kN);
+            each_of<upto - from>([&](auto each) {
+                constexpr int e = from + each.value;
+                p[e & 1] = __builtin_amdgcn_exp2f(kCapped ? (a.cap - base) - 2.0f * a.cap * sc[e] : sc[e] - base);
+                if constexpr (e & 1) put_weights<e - 1>(pf, l, p[0], p[1]);
+            });
+            if constexpr (n < 4) tile.template put_value<n>(buffer ^ 1);
+            if constexpr (n == 4) {
+                tile.load_values(to_last(t + 2), ve);
+                ve = tile.value_entry(to_last(t + 3));
+            }
+        });
+        each_of<kN>([&](auto step) {
+            constexpr int n = step.value, from = 16 * n / kN, upto = 16 * (n + 1) / kN;
+            o[n / 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ring[n % kAhead], pf[n % 2], o[n / 2], 0, 0, 0);
+            if constexpr (n + kAhead < kN) ring[n % kAhead] = read_value(n + kAhead);
+#pragma unroll
+            for (int e = from; e < upto; ++e) cap_score(e);
+            if constexpr (n < Tile::kWords) tile.template put_key<n>(buffer);
+            if constexpr (n == Tile::kWords) {
+                tile.load_keys(to_last(t + 3), ke);
+                ke = tile.key_entry(to_last(t + 4));
+            }
+        });
+        find_top();
     }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    none_seen |= (uint32_t)__shfl_xor((int)none_seen, 16, 64);
+    none_seen |= (uint32_t)__shfl_xor((int)none_seen, 32, 64);
+    if (__builtin_amdgcn_ballot_w64(none_seen != 0) != 0) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) o[i] += (none_seen >> (i / 2) & 1u) ? __builtin_nanf("") : 0.0f;
+    }
+    if (u.parts > 1) {
+        // the part, where a lane of a wave of 32 columns would hold it
+        const int64_t part = part_place(a, u, kh);
+        const int column = 16 * wave + col;
+        float4* to = reinterpret_cast<float4*>(a.part + part * kBlockColumns * D) + ((column / 32) * (D / 8) + (quarter >> 1)) * 64 + column % 32 + 32 * (quarter & 1);
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) to[2 * i * 64] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+        if (quarter == 0)
+            reinterpret_cast<float2*>(a.part + (int64_t)a.parts * a.kvh * kBlockColumns * D)[part * kBlockColumns + column] = make_float2(m, l);
+        return;
+    }
+    // through LDS to whole rows
+    __syncthreads();
+    constexpr int kTwist = D / 8 < 16 ? D / 8 - 1 : 15;
+    uint8_t* own = lds + wave * 16 * 2 * D;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+        store4(reinterpret_cast<uint16_t*>(own + col * 2 * D + 16 * ((2 * i + (quarter >> 1)) ^ (col & kTwist)) + 8 * (quarter & 1)), o[i][0] * inv,
+               o[i][1] * inv, o[i][2] * inv, o[i][3] * inv);
+    write_rows<D, 16>(a, u, kh, x, own);
 }
 
 namespace {
 
-template <int D>
+template <int D, bool kCapped>
 void launch4(const AttendArgs& a, hipStream_t st) {
     const dim3 grid(a.unit_count * a.kvh);
-    constexpr size_t kLds = 2 * 2 * kTile4 * D * 2 + 2 * 32 * sizeof(uint16_t);
-    if (a.cap > 0.0f)
-        hipLaunchKernelGGL((paged_prompt4_kernel<D, true>), grid, dim3(kPrompt4Threads), kLds, st, a);
+    if constexpr (D == 256)
+        hipLaunchKernelGGL((paged_prompt4_wide_kernel<D, kCapped>), grid, dim3(512), (Tile4<D, 512, true>::kBytes), st, a);
     else
-        hipLaunchKernelGGL((paged_prompt4_kernel<D, false>), grid, dim3(kPrompt4Threads), kLds, st, a);
+        hipLaunchKernelGGL((paged_prompt4_kernel<D, kCapped>), grid, dim3(256), (Tile4<D, 256, false>::kBytes), st, a);
 }
 
 }  // namespace
 
 void launch_prompt4(const AttendArgs& a, int d, hipStream_t st) {
+    const bool capped = a.cap > 0.0f;
     switch (d) {
-        case 64: launch4<64>(a, st); break;
-        case 128: launch4<128>(a, st); break;
-        default: launch4<256>(a, st);
+        case 64: capped ? launch4<64, true>(a, st) : launch4<64, false>(a, st); break;
+        case 128: capped ? launch4<128, true>(a, st) : launch4<128, false>(a, st); break;
+        default: capped ? launch4<256, true>(a, st) : launch4<256, false>(a, st);
     }
 }
 

@@ -17,6 +17,12 @@ constexpr int kFewColumns = 64;           // of a sequence and KV head that se12
 constexpr int kBlockColumns = 128;
 constexpr int kLeastTiles = 8;            // of a block, where a unit's keys are split
 
+typedef float floatx16_t __attribute__((ext_vector_type(16)));      // sums of v_mfma_f32_32x32x16
+
+// the key (of 32) of row m of the first product's A operand: lane half h = bit 2 of
+// m takes keys 16 h ..
+__device__ __forceinline__ int key_of_row(int m) { return (m & 3) | ((m & 8) >> 1) | ((m & 16) >> 1) | ((m & 4) << 2); }
+
 // one unit: 128 columns of a sequence and KV head
 struct Unit {
     int s, first;          // sequence, its first column of the unit
