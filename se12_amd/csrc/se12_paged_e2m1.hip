@@ -52,13 +52,14 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t amax) {
 // 8 values as codes, the first in the lowest bits
 __device__ __forceinline__ uint32_t e2m1x8(const float x[8], float s) {
     if (!(s > 0.0f)) return 0u;            // (NaN: the scale says so)
-    const float inv = 1.0f / s;
+    const float inv = __builtin_amdgcn_rcpf(s);
     float y[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        // the quotient to its last bit, or a tie would go by the inverse's rounding
+        // the quotient to its last bit, or a tie would go by the inverse's rounding (beyond 6
+        // the conversion gives 6)
         const float t = x[i] * inv;
-        y[i] = __builtin_amdgcn_fmed3f(fmaf(fmaf(-t, s, x[i]), inv, t), -6.0f, 6.0f);
+        y[i] = fmaf(fmaf(-t, s, x[i]), inv, t);
     }
     uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, y[0], y[1], 1.0f, 0);
     w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[2], y[3], 1.0f, 1);
@@ -71,6 +72,7 @@ __global__ __launch_bounds__(kRowThreads) void paged_append4_kernel(Append4Args 
     constexpr int kLanes = D / 8, kRows = kRowThreads / kLanes;
     __shared__ __attribute__((aligned(16))) float2 cs[16 * D / 2];
     __shared__ __attribute__((aligned(16))) float rows[kRows * D];
+    __shared__ __attribute__((aligned(16))) float weights[2][D]; // of q's norm and k's
     __shared__ uint32_t codes[16][kLanes];                       // of the values
     __shared__ __attribute__((aligned(16))) uint8_t scales[2][D / 32][16];
     const int tid = threadIdx.x, kh = (int)blockIdx.x % a.kvh;
@@ -79,41 +81,53 @@ __global__ __launch_bounds__(kRowThreads) void paged_append4_kernel(Append4Args 
     if (n <= 0) return;
     const int64_t row0 = u.seq.start + u.first + u.from - u.seq.len;      // of the first token
     const int half = a.r.half;
-    for (int i = tid; i < n * half; i += kRowThreads) {
-        const int t = i / half, f = i - t * half;
-        cs[t * half + f] = turn_at(u.first + u.from + t, a.r.inv_freq[f], a.r.scale);
-    }
+    turn_run16<kRowThreads>(cs, a.r, u.first, u.from, u.to);
+    if (a.r.q_norm && a.group > 0) load_weights<kRowThreads>(weights[0], a.r, a.r.q_norm, D);
+    if (a.r.k_norm) load_weights<kRowThreads>(weights[1], a.r, a.r.k_norm, D);
     const int P = 1 << a.page_log2, page = page_of(a.b, u.s, u.first >> a.page_log2, a.pages);
     const int64_t page_head = (int64_t)max(page, 0) * a.kvh + kh;
     const int slot0 = u.first & (P - 1);
-    __syncthreads();
 
-    // rows: values, keys, then the query heads, each of n tokens
-    const int lane = tid % kLanes, c0 = 8 * lane;
+    // rows: values, keys, then the query heads, n tokens of each (in places for a power of
+    // two); the next one is on its way while one is worked on
+    const int lane = tid % kLanes, c0 = 8 * lane, places = n > 1 ? 32 - __builtin_clz(n - 1) : 0, count = (2 + a.group) << places;
     float* own = rows + (tid / kLanes) * D;
-    for (int i = tid / kLanes; i < (2 + a.group) * n; i += kRows) {
-        const int what = i / n, t = i - what * n;
-        const int64_t row = row0 + t;
+    auto load = [&](int i) {
+        const int what = i >> places, t = i & ((1 << places) - 1);
+        const void* from = what == 0 ? a.v : what == 1 ? a.k : a.q;
+        const int64_t stride = what == 0 ? a.v_stride : what == 1 ? a.k_stride : a.q_stride;
+        Eight<DT> v;
+        v.load(from, (row0 + min(t, n - 1)) * stride + (int64_t)(what < 2 ? kh : kh * a.group + what - 2) * D + c0);
+        return v;
+    };
+    int i = tid / kLanes;
+    Eight<DT> next;
+    if (i < count) next = load(i);
+    __syncthreads();
+    for (; i < count; i += kRows) {
+        const int what = i >> places, t = i & ((1 << places) - 1);
         float x[8];
-        if (what == 0) {
-            load8<DT>(a.v, row * a.v_stride + kh * D + c0, x);
-        } else {
-            const int head = what == 1 ? kh : kh * a.group + what - 2;
-            load8<DT>(what == 1 ? a.k : a.q, row * (what == 1 ? a.k_stride : a.q_stride) + (int64_t)head * D + c0, x);
+        next.values(x);
+        if (i + kRows < count) next = load(i + kRows);
+        if (t >= n) continue;
+        const int64_t row = row0 + t;
+        if (what > 0) {
             const void* w = what == 1 ? a.r.k_norm : a.r.q_norm;
-            if (w) norm_row<kLanes>(x, a.r, w, c0, D);
+            if (w) norm_row<kLanes>(x, a.r.eps, weights[what == 1] + c0, 1.0 / D);
             if (half > 0) turn_row(x, own, cs + t * half, c0, half, a.r.interleaved);
             if (what > 1) {
-                uint16_t* o = a.q_out + (row * a.group * a.kvh + head) * D + c0;
+                uint16_t* o = a.q_out + (row * a.group * a.kvh + kh * a.group + what - 2) * D + c0;
                 const uint4 v = bf16x8(x);
                 reinterpret_cast<uint2*>(o)[0] = make_uint2(v.x, v.y);
                 reinterpret_cast<uint2*>(o)[1] = make_uint2(v.z, v.w);
                 continue;
             }
         }
-        uint32_t amax = 0;
+        // (the larger one, and NaN if there is one: by bits a NaN is above all numbers)
+        float most = fabsf(x[0]);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) amax = max(amax, __float_as_uint(x[k]) & 0x7FFFFFFFu);
+        for (int k = 1; k < 8; ++k) most = __builtin_elementwise_maximum(most, fabsf(x[k]));
+        uint32_t amax = __float_as_uint(most) & 0x7FFFFFFFu;
         amax = max(amax, (uint32_t)__builtin_amdgcn_mov_dpp((int)amax, 0xB1, 0xF, 0xF, true));       // of four lanes
         amax = max(amax, (uint32_t)__builtin_amdgcn_mov_dpp((int)amax, 0x4E, 0xF, 0xF, true));
         const uint32_t byte = scale_byte(amax), w = e2m1x8(x, e2m1_scale(byte));
@@ -128,18 +142,15 @@ __global__ __launch_bounds__(kRowThreads) void paged_append4_kernel(Append4Args 
     if (page < 0) return;
     for (int c = tid; c < D; c += kRowThreads) {
         uint2* p = reinterpret_cast<uint2*>(a.vc + ((page_head << (a.page_log2 - 4)) + slot0 / 16) * (8 * D)) + c;
-        uint32_t w[2] = {0, 0}, m[2] = {0, 0};
+        uint2 was = make_uint2(0, 0);
+        if (n < 16) was = *p;
+        uint32_t w[2] = {0, 0};
 #pragma unroll
-        for (int t = 0; t < 16; ++t) {
-            const bool mine = t >= u.from && t < u.to;
-            const uint32_t v = (codes[t][c / 8] >> (4 * (c % 8))) & 15u;
-            w[t / 8] |= mine ? v << (4 * (t % 8)) : 0u;
-            m[t / 8] |= mine ? 15u << (4 * (t % 8)) : 0u;
-        }
-        if (n < 16) {
-            const uint2 was = *p;
-            w[0] |= was.x & ~m[0];
-            w[1] |= was.y & ~m[1];
+        for (int t = 0; t < 16; ++t) w[t / 8] |= ((codes[t][c / 8] >> (4 * (c % 8))) & 15u) << (4 * (t % 8));
+        if (n < 16) {      // slots that are not new keep what they hold
+            const uint64_t fresh = ((1ull << (4 * n)) - 1) << (4 * u.from);
+            w[0] = (w[0] & (uint32_t)fresh) | (was.x & ~(uint32_t)fresh);
+            w[1] = (w[1] & (uint32_t)(fresh >> 32)) | (was.y & ~(uint32_t)(fresh >> 32));
         }
         *p = make_uint2(w[0], w[1]);
     }

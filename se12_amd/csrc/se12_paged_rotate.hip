@@ -19,12 +19,14 @@ struct RotateArgs {
     Batch b;
     Rotation r;
     int heads, kvh, d, tokens;      // tokens of a block
+    double share;                   // 1 / d
 };
 
 template <int DT, int OT, int kLanes>
 __global__ __launch_bounds__(kRotateThreads) void rotate_heads_kernel(RotateArgs a) {
     constexpr int kRows = kRotateThreads / kLanes;
     __shared__ __attribute__((aligned(16))) float rows[kRows * kLanes * 8];
+    __shared__ __attribute__((aligned(16))) float weights[2 * kLanes * 8];      // of q's norm and k's
     extern __shared__ __attribute__((aligned(16))) float2 cs[];      // [tokens][half], then positions
     const int tid = threadIdx.x, half = a.r.half, first = (int)blockIdx.x * a.tokens, n = min(a.tokens, a.b.tokens - first);
     int* pos = reinterpret_cast<int*>(cs + a.tokens * half);
@@ -42,6 +44,8 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_heads_kernel(RotateArgs
         const int i = first + tid - seq.start;
         pos[tid] = i >= 0 && i < seq.n ? seq.len + i : -1;
     }
+    if (a.r.q_norm) load_weights<kRotateThreads>(weights, a.r, a.r.q_norm, a.d);
+    if (a.r.k_norm) load_weights<kRotateThreads>(weights + kLanes * 8, a.r, a.r.k_norm, a.d);
     __syncthreads();
     for (int i = tid; i < n * half; i += kRotateThreads) {
         const int t = i / half, f = i - t * half;
@@ -60,7 +64,7 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_heads_kernel(RotateArgs
         float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         if (live) load8<DT>(is_q ? a.q : a.k, row * (is_q ? a.q_stride : a.k_stride) + (int64_t)head * a.d + c0, x);
         const void* w = is_q ? a.r.q_norm : a.r.k_norm;
-        if (w) norm_row<kLanes>(x, a.r, w, live ? c0 : 0, a.d);
+        if (w) norm_row<kLanes>(x, a.r.eps, weights + (is_q ? 0 : kLanes * 8) + c0, a.share);
         if (half > 0) turn_row(x, own, cs + t * half, c0, half, a.r.interleaved);
         if (!live) continue;
         const int64_t to = (row * (is_q ? a.heads : a.kvh) + head) * a.d + c0;
@@ -135,7 +139,7 @@ extern "C" int se12_step_rotate_heads(const se12_step_batch* batch, const void* 
     const Batch b{nullptr, 0, batch->lengths, batch->starts, 0, batch->sequences, batch->tokens,
                   batch->max_new < batch->tokens ? batch->max_new : batch->tokens};
     // tokens of a block: four share the start, where there are enough blocks all the same
-    RotateArgs a{q, k, q_stride, k_stride, q_out, k_out, b, device_rotation(rotation), heads, kv_heads, head_dim, batch->tokens >= 4096 ? 4 : 1};
+    RotateArgs a{q, k, q_stride, k_stride, q_out, k_out, b, device_rotation(rotation), heads, kv_heads, head_dim, batch->tokens >= 4096 ? 4 : 1, 1.0 / head_dim};
     const int64_t blocks = ((int64_t)b.tokens + a.tokens - 1) / a.tokens;
     if (!grid_fits(blocks, kRotateThreads) || (int64_t)a.tokens * (heads + kv_heads) > INT32_MAX)
         return step_fail(fn, "too many tokens and heads for one launch");

@@ -14,6 +14,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "se12_paged_device.hpp"
 
 namespace se12step {
@@ -28,30 +30,43 @@ struct Rotation {
     bool f32_norm, interleaved;
 };
 
+// eight values as they are loaded (rows are 4 values' bytes apart at least, not 16)
 template <int DT>
-__device__ __forceinline__ void load8(const void* p, int64_t i, float x[8]) {
-    if constexpr (DT == SE12_STEP_F32) {
-        const float4* v = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-        const float4 a = v[0], b = v[1];
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-        // (rows are 4 values' bytes apart at least, not 16)
-        const uint2* v = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
-        const uint2 a = v[0], b = v[1];
-        const uint32_t w[4] = {a.x, a.y, b.x, b.y};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            x[2 * k] = __uint_as_float(w[k] << 16);
-            x[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+struct Eight {
+    uint32_t w[DT == SE12_STEP_F32 ? 8 : 4];
+    __device__ __forceinline__ void load(const void* p, int64_t i) {
+        if constexpr (DT == SE12_STEP_F32) {
+            const uint4* v = reinterpret_cast<const uint4*>(static_cast<const float*>(p) + i);
+            const uint4 a = v[0], b = v[1];
+            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+        } else {
+            const uint2* v = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+            const uint2 a = v[0], b = v[1];
+            w[0] = a.x, w[1] = a.y, w[2] = b.x, w[3] = b.y;
         }
     }
+    __device__ __forceinline__ void values(float x[8]) const {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            x[k] = __uint_as_float(DT == SE12_STEP_F32 ? w[k] : k & 1 ? w[k / 2] & 0xFFFF0000u : w[k / 2] << 16);
+    }
+};
+
+template <int DT>
+__device__ __forceinline__ void load8(const void* p, int64_t i, float x[8]) {
+    Eight<DT> v;
+    v.load(p, i);
+    v.values(x);
 }
 
-// cos and sin of pos * freq, times scale
-__device__ __forceinline__ float2 turn_at(int pos, float freq, double scale) {
+struct Angle {
+    double c, s;      // its cosine and sine
+};
+
+__device__ __forceinline__ Angle angle_of(double angle) {
     // what is beyond a whole number of quarter turns, in two parts of pi / 2, by the series
-    // of sine and cosine: 2^-53 of the angle's own rounding
-    const double angle = (double)pos * (double)freq, whole = angle * 0.63661977236758134 + 0x1.8p52, k = whole - 0x1.8p52;
+    // of sine and cosine: 2^-52 of a whole turn, beside the angle's own rounding
+    const double whole = angle * 0.63661977236758134 + 0x1.8p52, k = whole - 0x1.8p52;
     const int turn = __double2loint(whole);
     const double x = fma(-k, 6.123233995736766e-17, fma(-k, 1.5707963267948966, angle)), x2 = x * x;
     double s = -1.0 / 1307674368000, c = 1.0 / 20922789888000;
@@ -71,26 +86,84 @@ __device__ __forceinline__ float2 turn_at(int pos, float freq, double scale) {
     c = fma(c, x2, -0.5);
     c = fma(c, x2, 1.0);
     const double sn = turn & 1 ? c : s, cs = turn & 1 ? s : c;
-    return make_float2((float)((turn + 1) & 2 ? -cs * scale : cs * scale), (float)(turn & 2 ? -sn * scale : sn * scale));
+    return {(turn + 1) & 2 ? -cs : cs, turn & 2 ? -sn : sn};
 }
 
-// x[8] of a row whose kLanes lanes lie side by side, normed with weights w
+__device__ __forceinline__ Angle operator+(Angle a, Angle b) { return {fma(a.c, b.c, -a.s * b.s), fma(a.s, b.c, a.c * b.s)}; }
+
+__device__ __forceinline__ float2 turn_of(Angle a, double scale) { return make_float2((float)(a.c * scale), (float)(a.s * scale)); }
+
+// cos and sin of pos * freq, times scale
+__device__ __forceinline__ float2 turn_at(int pos, float freq, double scale) { return turn_of(angle_of((double)pos * (double)freq), scale); }
+
+// Those of positions first + from .. first + to - 1 of a run of 16 (first a multiple of 16),
+// cs[position][half], by a block's kThreads: the run's first angle, and what a place is
+// beyond it, by the places' bits, the high ones first. (An angle for every place: a quarter of the
+// append's vector instructions; so a place's is the same whatever else of its run is worked out.)
+template <int kThreads>
+__device__ __forceinline__ void turn_run16(float2* cs, const Rotation& r, int first, int from, int to) {
+    const int half = r.half;
+    if (half == 0) return;
+    int parts = 16;                                  // of the run, each a thread's
+    while (parts > 1 && parts * half > kThreads) parts >>= 1;
+    const int part = (int)threadIdx.x / half, f = (int)threadIdx.x - part * half, each = 16 / parts;
+    if (part >= parts) return;
+    const double freq = (double)r.inv_freq[f];
+    const Angle one = angle_of(freq), two = one + one, four = two + two, eight = four + four;
+    const Angle start = angle_of((double)first * freq);
+    for (int i = max(part * each, from); i < min((part + 1) * each, to); ++i) {
+        Angle x = start;
+        if (i & 8) x = x + eight;
+        if (i & 4) x = x + four;
+        if (i & 2) x = x + two;
+        if (i & 1) x = x + one;
+        cs[(i - from) * half + f] = turn_of(x, r.scale);
+    }
+}
+
+// the sum over 16 lanes side by side, in each of them
+__device__ __forceinline__ double row16_sum(double v) {
+    auto add = [&](auto control) {
+        const int lo = __builtin_amdgcn_mov_dpp(__double2loint(v), control.value, 0xF, 0xF, true);
+        const int hi = __builtin_amdgcn_mov_dpp(__double2hiint(v), control.value, 0xF, 0xF, true);
+        v += __hiloint2double(hi, lo);
+    };
+    add(std::integral_constant<int, 0xB1>{});       // (as row16_reduce of se12_step_math.hpp)
+    add(std::integral_constant<int, 0x4E>{});
+    add(std::integral_constant<int, 0x141>{});
+    add(std::integral_constant<int, 0x140>{});
+    return v;
+}
+
+// offset + w of d weights, in FP32
+template <int kThreads>
+__device__ __forceinline__ void load_weights(float* to, const Rotation& r, const void* w, int d) {
+    for (int i = threadIdx.x; i < d; i += kThreads)
+        to[i] = r.offset + (r.f32_norm ? static_cast<const float*>(w)[i] : bf16_to_f(static_cast<const uint16_t*>(w)[i]));
+}
+
+// x[8] of a row whose kLanes lanes lie side by side, normed; w: the 8 weights of its columns, share: 1 / head_dim
 template <int kLanes>
-__device__ __forceinline__ void norm_row(float x[8], const Rotation& r, const void* w, int c0, int d) {
+__device__ __forceinline__ void norm_row(float x[8], double eps, const float* w, double share) {
 #pragma clang fp contract(off)
+    static_assert(kLanes == 8 || kLanes == 16 || kLanes == 32, "");
     double sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum += (double)x[i] * (double)x[i];
+    for (int i = 0; i < 8; ++i) sum = fma((double)x[i], (double)x[i], sum);
+    if constexpr (kLanes == 8) {
 #pragma unroll
-    for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor(sum, o, 64);
-    const float inv = (float)(1.0 / sqrt(sum / d + r.eps));
-    float f[8];
-    if (r.f32_norm)
-        load8<SE12_STEP_F32>(w, c0, f);
-    else
-        load8<SE12_STEP_BF16>(w, c0, f);
+        for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor(sum, o, 64);
+    } else {
+        sum = row16_sum(sum);
+        if constexpr (kLanes == 32) sum += __shfl_xor(sum, 16, 64);
+    }
+    // the inverse root to 2^-45: the card's, and one step of Newton's
+    const double mean = sum * share + eps, root = __builtin_amdgcn_rsq(mean);
+    const float inv = (float)(root > 0.0 && root < INFINITY ? fma(0.5 * root, fma(-mean * root, root, 1.0), root) : root);
+    const float4 w0 = *reinterpret_cast<const float4*>(w), w1 = *reinterpret_cast<const float4*>(w + 4);
+    const float f[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (x[i] * inv) * (r.offset + f[i]);
+    for (int i = 0; i < 8; ++i) x[i] = (x[i] * inv) * f[i];
 }
 
 // x[8], columns c0 .. of a row, turned by the angles cs[half] of its token; `row`: the
@@ -111,20 +184,28 @@ __device__ __forceinline__ void turn_row(float x[8], float* row, const float2* c
     *reinterpret_cast<float4*>(row + c0) = make_float4(x[0], x[1], x[2], x[3]);
     *reinterpret_cast<float4*>(row + c0 + 4) = make_float4(x[4], x[5], x[6], x[7]);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int c = c0 + 4 * i;
-        if (c >= 2 * half) break;
-        const bool first = c < half;
-        const float4 other = *reinterpret_cast<const float4*>(row + (first ? c + half : c - half));
-        const float4* t = reinterpret_cast<const float4*>(cs + (first ? c : c - half));
+    // four columns at `at`: with those half a rotation on, or back (a - b is a + -b)
+    auto turn4 = [&](float* y, int at) {
+        const bool first = at < half;
+        const uint32_t sign = first ? 0x80000000u : 0u;
+        const float4 other = *reinterpret_cast<const float4*>(row + (first ? at + half : at - half));
+        const float4* t = reinterpret_cast<const float4*>(cs + (first ? at : at - half));
         const float4 t0 = t[0], t1 = t[1];
         const float o[4] = {other.x, other.y, other.z, other.w}, cos[4] = {t0.x, t0.z, t1.x, t1.z}, sin[4] = {t0.y, t0.w, t1.y, t1.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const float a = x[4 * i + k] * cos[k], b = o[k] * sin[k];
-            x[4 * i + k] = first ? a - b : a + b;
+            const float b = o[k] * __uint_as_float(__float_as_uint(sin[k]) ^ sign);
+            y[k] = y[k] * cos[k] + b;
         }
+    };
+    if (half % 8 == 0) {
+        if (c0 < 2 * half) {
+            turn4(x, c0);
+            turn4(x + 4, c0 + 4);
+        }
+    } else {
+        if (c0 < 2 * half) turn4(x, c0);
+        if (c0 + 4 < 2 * half) turn4(x + 4, c0 + 4);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
