@@ -96,28 +96,49 @@ __device__ __forceinline__ float2 turn_of(Angle a, double scale) { return make_f
 // cos and sin of pos * freq, times scale
 __device__ __forceinline__ float2 turn_at(int pos, float freq, double scale) { return turn_of(angle_of((double)pos * (double)freq), scale); }
 
-// Those of positions first + from .. first + to - 1 of a run of 16 (first a multiple of 16),
-// cs[position][half], by a block's kThreads: the run's first angle, and what a place is
-// beyond it, by the places' bits, the high ones first. (An angle for every place: a quarter of the
-// append's vector instructions; so a place's is the same whatever else of its run is worked out.)
+// The angles of kEach places of a run of 16 from place `at`, whose angle is x: halves of them
+// in turn, so a place's is its run's first, and then the powers of two it is beyond it, the
+// high ones first. `beyond`: 1, 2, 4, 8 places.
+template <int kEach, typename Put>
+__device__ __forceinline__ void places_of(Angle x, int at, const Angle* beyond, Put put) {
+    if constexpr (kEach == 1) {
+        put(at, x);
+    } else {
+        constexpr int kHalf = kEach / 2, kPower = kHalf == 1 ? 0 : kHalf == 2 ? 1 : kHalf == 4 ? 2 : 3;
+        places_of<kHalf>(x, at, beyond, put);
+        places_of<kHalf>(x + beyond[kPower], at + kHalf, beyond, put);
+    }
+}
+
+// cos and sin of positions first + from .. first + to - 1 of a run of 16 (first a multiple of
+// 16), cs[position][half], by a block's kThreads. (An angle worked out for every place was a
+// quarter of the append's vector instructions. A place's is the same whatever else of its run is
+// worked out.)
 template <int kThreads>
 __device__ __forceinline__ void turn_run16(float2* cs, const Rotation& r, int first, int from, int to) {
+    static_assert(kThreads >= 256, "");
     const int half = r.half;
     if (half == 0) return;
     int parts = 16;                                  // of the run, each a thread's
     while (parts > 1 && parts * half > kThreads) parts >>= 1;
-    const int part = (int)threadIdx.x / half, f = (int)threadIdx.x - part * half, each = 16 / parts;
-    if (part >= parts) return;
+    const int part = (int)threadIdx.x / half, f = (int)threadIdx.x - part * half, each = 16 / parts, at = part * each;
+    if (part >= parts || at >= to || at + each <= from) return;
     const double freq = (double)r.inv_freq[f];
-    const Angle one = angle_of(freq), two = one + one, four = two + two, eight = four + four;
-    const Angle start = angle_of((double)first * freq);
-    for (int i = max(part * each, from); i < min((part + 1) * each, to); ++i) {
-        Angle x = start;
-        if (i & 8) x = x + eight;
-        if (i & 4) x = x + four;
-        if (i & 2) x = x + two;
-        if (i & 1) x = x + one;
-        cs[(i - from) * half + f] = turn_of(x, r.scale);
+    Angle beyond[4] = {angle_of(freq)}, x = angle_of((double)first * freq);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) beyond[i] = beyond[i - 1] + beyond[i - 1];
+    if (at & 8) x = x + beyond[3];
+    if (at & 4) x = x + beyond[2];
+    if (at & 2) x = x + beyond[1];
+    if (at & 1) x = x + beyond[0];
+    auto put = [&](int i, Angle y) {
+        if (i >= from && i < to) cs[(i - from) * half + f] = turn_of(y, r.scale);
+    };
+    switch (each) {
+        case 1: places_of<1>(x, at, beyond, put); break;
+        case 2: places_of<2>(x, at, beyond, put); break;
+        case 4: places_of<4>(x, at, beyond, put); break;
+        default: places_of<8>(x, at, beyond, put);      // (half is 128 at most, threads 256)
     }
 }
 
