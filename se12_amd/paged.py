@@ -71,35 +71,40 @@ def _row_view(t, name: str, head_dim: int, index: int, device, heads: int | None
     return t if apart else t.as_strided(shape, (width, head_dim, 1))
 
 
-def _rotation(head_dim: int, device, inv_freq, interleaved, rotary_scale, q_norm, k_norm, norm_eps, norm_offset):
+def _norm_weight(w, name: str, head_dim: int, index: int, device) -> torch.Tensor:
+    if not (isinstance(w, torch.Tensor) and w.get_device() == index and w.dtype in (torch.bfloat16, torch.float32) and w.shape == (head_dim,)
+            and w.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous bfloat16 or float32 [{head_dim}] tensor on {device}")
+    return w if w.data_ptr() % 16 == 0 else w.clone()
+
+
+def _rotation(head_dim: int, index: int, device, inv_freq, interleaved, rotary_scale, q_norm, k_norm, norm_eps, norm_offset):
     """The C struct of a rotation and norms, by reference, and the tensors it points to."""
-    rotary = 0
+    rotary, f, dtype = 0, None, nat.STEP_BF16
     if inv_freq is not None:
-        if (not isinstance(inv_freq, torch.Tensor) or inv_freq.device != device or inv_freq.dtype != torch.float32 or inv_freq.dim() != 1
-                or not inv_freq.is_contiguous()):
+        if not (isinstance(inv_freq, torch.Tensor) and inv_freq.get_device() == index and inv_freq.dtype == torch.float32 and inv_freq.dim() == 1
+                and inv_freq.is_contiguous()):
             raise ValueError(f"inv_freq must be a contiguous float32 vector on {device}")
         rotary = 2 * inv_freq.numel()
         if rotary % 8 or not 0 < rotary <= head_dim:
             raise ValueError(f"inv_freq must hold a multiple of 4, at most {head_dim // 2} frequencies, got {inv_freq.numel()}")
-        if inv_freq.data_ptr() % 16:
+        f = inv_freq.data_ptr()
+        if f % 16:
             inv_freq = inv_freq.clone()
-    held, dtypes = [inv_freq], set()
-    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if w is not None:
-            if (not isinstance(w, torch.Tensor) or w.device != device or w.dtype not in (torch.bfloat16, torch.float32)
-                    or tuple(w.shape) != (head_dim,) or not w.is_contiguous()):
-                raise ValueError(f"{name} must be a contiguous bfloat16 or float32 [{head_dim}] tensor on {device}")
-            dtypes.add(w.dtype)
-            if w.data_ptr() % 16:
-                w = w.clone()
-        held.append(w)
-    if len(dtypes) > 1:
-        raise ValueError("q_norm and k_norm must be of one type")
+            f = inv_freq.data_ptr()
+    if q_norm is not None:
+        q_norm = _norm_weight(q_norm, "q_norm", head_dim, index, device)
+    if k_norm is not None:
+        k_norm = _norm_weight(k_norm, "k_norm", head_dim, index, device)
+        if q_norm is not None and q_norm.dtype != k_norm.dtype:
+            raise ValueError("q_norm and k_norm must be of one type")
+    w = q_norm if q_norm is not None else k_norm
+    if w is not None and w.dtype == torch.float32:
+        dtype = nat.STEP_F32
     if not (math.isfinite(rotary_scale) and math.isfinite(norm_eps) and norm_eps >= 0 and abs(norm_offset) < 2.0 ** 127):
         raise ValueError("rotary_scale, norm_eps and norm_offset must be finite, norm_eps not below 0")
-    pointers = [None if t is None else t.data_ptr() for t in held]
-    return ctypes.byref(nat.StepRotation(*pointers, rotary_scale, norm_eps, norm_offset,
-                                         nat.STEP_F32 if torch.float32 in dtypes else nat.STEP_BF16, rotary, int(bool(interleaved)))), held
+    return ctypes.byref(nat.StepRotation(f, None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(),
+                                         rotary_scale, norm_eps, norm_offset, dtype, rotary, 1 if interleaved else 0)), (inv_freq, q_norm, k_norm)
 
 
 def _int32(t: torch.Tensor, name: str, shape: tuple, device: torch.device) -> torch.Tensor:
@@ -264,7 +269,7 @@ class PagedKvCache:
         k = self._rows(k, "k", self.kv_heads, None, None, 4)
         tokens = k.shape[0]
         v = self._rows(v, "v", self.kv_heads, tokens, k.dtype, 4)
-        rotation, held = _rotation(self.head_dim, self.device, inv_freq, interleaved, rotary_scale, q_norm, k_norm, norm_eps, norm_offset)
+        rotation, held = _rotation(self.head_dim, self._index, self.device, inv_freq, interleaved, rotary_scale, q_norm, k_norm, norm_eps, norm_offset)
         inv_freq = held[0]
         heads, q_stride = self.kv_heads, 0
         if q is not None:
@@ -322,9 +327,10 @@ class PagedKvCache:
             raise ValueError(f"tokens must be a whole number from 0 to 2^31 - 1, got {tokens}")
         shape = (int(tokens), self.kv_heads, self.head_dim)
         if out is None:
-            out = torch.empty((2, *shape), dtype=torch.bfloat16, device=self.device).unbind()
-        k, v = out
-        for t in (k, v):
+            k, v = torch.empty((2, *shape), dtype=torch.bfloat16, device=self.device).unbind()
+        else:
+            k, v = out
+        for t in () if out is None else (k, v):
             if not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype != torch.bfloat16 or tuple(t.shape) != shape or not t.is_contiguous():
                 raise ValueError(f"out must be two contiguous bfloat16 {list(shape)} tensors on {self.device}")
             if t.data_ptr() % 16:
@@ -409,37 +415,37 @@ def rotate_heads(batch: PagedBatch, q: torch.Tensor, k: torch.Tensor | None = No
         raise ValueError(f"q must have 1 to 65535 heads and a head_dim of a multiple of 8 up to 256, got {heads}, {head_dim}")
     if dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"dtype must be bfloat16 or float32, got {dtype}")
-    index = batch.page_table.get_device()
-    q = _row_view(q, "q", head_dim, index, batch.device, None, None, None, 4, "the batch")
+    index, device = batch.page_table.get_device(), batch.device
+    q = _row_view(q, "q", head_dim, index, device, None, None, None, 4, "the batch")
+    q_out, k_out = (None, None) if out is None else out
+    q_out = _turned_out(q_out, q.shape, dtype, device)
+    kv_heads = k_stride = k_at = k_out_at = 0
     if k is not None:
-        if isinstance(k, torch.Tensor) and k.dim() == 3 and not 1 <= k.shape[1] <= 65535:
-            raise ValueError(f"k must have 1 to 65535 heads, got {k.shape[1]}")
-        if isinstance(k, torch.Tensor) and k.dim() == 3 and k.shape[0] != tokens:
-            raise ValueError(f"k has {k.shape[0]} rows, q has {tokens}")
-        k = _row_view(k, "k", head_dim, index, batch.device, None, None, q.dtype, 4, "the batch")
-    elif k_norm is not None:
-        raise ValueError("k_norm goes with k")
-    outs = []
-    for i, t in enumerate((q, k)):
-        given = None if out is None else out[i]
-        if t is None:
-            if given is not None:
-                raise ValueError("out's second tensor goes with k")
-            outs.append(None)
-        elif given is None:
-            outs.append(torch.empty(tuple(t.shape), dtype=dtype, device=batch.device))
-        else:
-            if not isinstance(given, torch.Tensor) or given.device != batch.device or given.dtype != dtype or given.shape != t.shape or not given.is_contiguous():
-                raise ValueError(f"out must hold contiguous {dtype} tensors of q's and k's shapes on {batch.device}")
-            if given.data_ptr() % 16:
-                raise ValueError("out must be 16-byte aligned")
-            outs.append(given)
-    rotation, held = _rotation(head_dim, batch.device, inv_freq, interleaved, rotary_scale, q_norm, k_norm, norm_eps, norm_offset)
-    types = {torch.float32: nat.STEP_F32, torch.bfloat16: nat.STEP_BF16}
-    with _on(batch.device):
+        if isinstance(k, torch.Tensor) and k.dim() == 3:
+            if not 1 <= k.shape[1] <= 65535:
+                raise ValueError(f"k must have 1 to 65535 heads, got {k.shape[1]}")
+            if k.shape[0] != tokens:
+                raise ValueError(f"k has {k.shape[0]} rows, q has {tokens}")
+        k = _row_view(k, "k", head_dim, index, device, None, None, q.dtype, 4, "the batch")
+        k_out = _turned_out(k_out, k.shape, dtype, device)
+        kv_heads, k_stride, k_at, k_out_at = k.shape[1], k.stride(0), k.data_ptr(), k_out.data_ptr()
+    elif k_norm is not None or k_out is not None:
+        raise ValueError("k_norm and out's second tensor go with k")
+    rotation, held = _rotation(head_dim, index, device, inv_freq, interleaved, rotary_scale, q_norm, k_norm, norm_eps, norm_offset)
+    with _on(device):
         nat.step_check(nat.lib().se12_step_rotate_heads(
-            batch._struct(tokens), q.data_ptr(), None if k is None else k.data_ptr(), types[q.dtype], q.stride(0),
-            0 if k is None else k.stride(0), heads, 0 if k is None else k.shape[1], head_dim, rotation, outs[0].data_ptr(),
-            None if k is None else outs[1].data_ptr(), types[dtype], _stream(batch.device)))
-    del held      # (read by the call; the stream keeps the order with what is made of their memory)
-    return outs[0], outs[1]
+            batch._struct(tokens), q.data_ptr(), k_at or None, nat.STEP_F32 if q.dtype == torch.float32 else nat.STEP_BF16, q.stride(0), k_stride,
+            heads, kv_heads, head_dim, rotation, q_out.data_ptr(), k_out_at or None, nat.STEP_F32 if dtype == torch.float32 else nat.STEP_BF16,
+            _stream(device)))
+    del held      # (until the call has been made)
+    return q_out, k_out
+
+
+def _turned_out(out, shape, dtype: torch.dtype, device) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if not isinstance(out, torch.Tensor) or out.device != device or out.dtype != dtype or out.shape != shape or not out.is_contiguous():
+        raise ValueError(f"out must hold contiguous {dtype} tensors of q's and k's shapes on {device}")
+    if out.data_ptr() % 16:
+        raise ValueError("out must be 16-byte aligned")
+    return out
