@@ -138,8 +138,9 @@ int se12_step_prefill_attention(uint16_t* qkv, int64_t stride, const uint16_t* c
  *   v [pages, kv_heads, page_size / 16, head_dim, 8]: 16 tokens of a column
  *   k_scale, v_scale uint8 [pages, kv_heads, head_dim / 32, page_size], 16-byte
  *   aligned: the byte's bits are bits 14 .. 7 of an FP16 number (5 of exponent, 3
- *   of fraction), which 32 columns of a token are times; 255: one of the 32 is no
- *   number, and all of them count as NaN
+ *   of fraction), which 32 columns of a token are times, 0 to 226 (10240); 255: one
+ *   of the 32 is no number, and all of them count as NaN. (Of slots that hold no
+ *   token the bytes may be any.)
  * head_dim 64, 128 or 256; k and v 16-byte aligned. */
 typedef struct se12_step_pages {
     void* k;

@@ -150,8 +150,9 @@ __device__ __forceinline__ uint32_t where_no_number(uint32_t w, int kind) {
 // exponent, 3 of fraction), 255 where one of its 32 values is no number
 __device__ __forceinline__ float e2m1_scale(uint32_t byte) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(byte << 7)); }
 
-// bit 7 of every byte that is no scale (of exponent 31)
-__device__ __forceinline__ uint32_t no_scales(uint32_t w) { return ((w & 0x78787878u) + 0x08080808u) & w & 0x80808080u; }
+// bit 7 of every byte that is no scale: 255, and what nobody writes, from 227 on (a slot that
+// is not held may have any bytes, and FP16 does not hold 6 times those)
+__device__ __forceinline__ uint32_t no_scales(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x1D1D1D1Du) & w & 0x80808080u; }
 
 // the 8 codes of a word times their scales (of two at a time), in FP16: exact
 __device__ __forceinline__ halfx8_t e2m1_operand(uint32_t w, const halfx2_t by[4]) {

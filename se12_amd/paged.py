@@ -177,7 +177,7 @@ class PagedKvCache:
     [pages, kv_heads, page_size, head_dim / 2], `v` [pages, kv_heads, page_size / 16,
     head_dim, 8] (16 tokens of a column side by side), `k_scale` and `v_scale` uint8
     [pages, kv_heads, head_dim / 32, page_size], one to 32 columns of a token: an FP16
-    number's bits 14 .. 7 (5 of exponent, 3 of fraction); 255 stands for no number."""
+    number's bits 14 .. 7 (5 of exponent, 3 of fraction), 0 to 226; 255 stands for no number."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.float8_e4m3fn,
                  device=None) -> None:
@@ -308,13 +308,13 @@ class PagedKvCache:
                 raise ValueError("out overlaps k or v")
         turn = dict(interleaved=interleaved, rotary_scale=rotary_scale, norm_eps=norm_eps, norm_offset=norm_offset)
         turned, _ = rotate_heads(batch, k, None, inv_freq, q_norm=k_norm, dtype=torch.float32, **turn)
-        self.append(batch, turned, v.float())
         if q is not None:
             # (q's kernel writes 16 bytes at once)
             fits = out.data_ptr() % 16 == 0
             got, _ = rotate_heads(batch, q, None, inv_freq, q_norm=q_norm, out=(out if fits else out.clone(), None), **turn)
             if not fits:
                 out.copy_(got)
+        self.append(batch, turned, v.float())
         return out
 
     def read(self, batch: PagedBatch, tokens: int, out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
