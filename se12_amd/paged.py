@@ -27,6 +27,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -35,7 +36,10 @@ from . import _native as nat
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128, 256)
 _DTYPES = {torch.bfloat16: nat.STEP_BF16, torch.float8_e4m3fn: nat.STEP_E4M3, torch.float4_e2m1fn_x2: nat.STEP_E2M1}
+_KINDS = {torch.bfloat16: nat.STEP_BF16, torch.float32: nat.STEP_F32}
 _NO_GUARD = contextlib.nullcontext()
+# a se12_step_rotation (packed a microsecond faster than a ctypes structure is filled)
+_ROTATION = struct.Struct("@3P2df3i").pack
 
 
 def _on(device: torch.device):
@@ -71,40 +75,47 @@ def _row_view(t, name: str, head_dim: int, index: int, device, heads: int | None
     return t if apart else t.as_strided(shape, (width, head_dim, 1))
 
 
-def _norm_weight(w, name: str, head_dim: int, index: int, device) -> torch.Tensor:
+def _norm_weight(w, name: str, head_dim: int, index: int, device) -> tuple[torch.Tensor, int]:
+    """(w, its address)"""
     if not (isinstance(w, torch.Tensor) and w.get_device() == index and w.dtype in (torch.bfloat16, torch.float32) and w.shape == (head_dim,)
             and w.is_contiguous()):
         raise ValueError(f"{name} must be a contiguous bfloat16 or float32 [{head_dim}] tensor on {device}")
-    return w if w.data_ptr() % 16 == 0 else w.clone()
+    at = w.data_ptr()
+    if at % 16:
+        w = w.clone()
+        at = w.data_ptr()
+    return w, at
 
 
-def _rotation(head_dim: int, index: int, device, inv_freq, interleaved, rotary_scale, q_norm, k_norm, norm_eps, norm_offset):
-    """The C struct of a rotation and norms, by reference, and the tensors it points to."""
-    rotary, f, dtype = 0, None, nat.STEP_BF16
-    if inv_freq is not None:
-        if not (isinstance(inv_freq, torch.Tensor) and inv_freq.get_device() == index and inv_freq.dtype == torch.float32 and inv_freq.dim() == 1
-                and inv_freq.is_contiguous()):
-            raise ValueError(f"inv_freq must be a contiguous float32 vector on {device}")
-        rotary = 2 * inv_freq.numel()
-        if rotary % 8 or not 0 < rotary <= head_dim:
-            raise ValueError(f"inv_freq must hold a multiple of 4, at most {head_dim // 2} frequencies, got {inv_freq.numel()}")
-        f = inv_freq.data_ptr()
-        if f % 16:
-            inv_freq = inv_freq.clone()
-            f = inv_freq.data_ptr()
+def _frequencies(inv_freq, head_dim: int, index: int, device) -> tuple[torch.Tensor, int, int]:
+    """(inv_freq, its address, the columns it turns)"""
+    if not (isinstance(inv_freq, torch.Tensor) and inv_freq.get_device() == index and inv_freq.dtype == torch.float32 and inv_freq.dim() == 1
+            and inv_freq.is_contiguous()):
+        raise ValueError(f"inv_freq must be a contiguous float32 vector on {device}")
+    rotary = 2 * inv_freq.numel()
+    if rotary % 8 or not 0 < rotary <= head_dim:
+        raise ValueError(f"inv_freq must hold a multiple of 4, at most {head_dim // 2} frequencies, got {inv_freq.numel()}")
+    at = inv_freq.data_ptr()
+    if at % 16:
+        inv_freq = inv_freq.clone()
+        at = inv_freq.data_ptr()
+    return inv_freq, at, rotary
+
+
+def _rotation(head_dim: int, index: int, device, at: int, rotary: int, interleaved, rotary_scale, q_norm, k_norm, norm_eps, norm_offset):
+    """A se12_step_rotation's bytes, and the weights that it points to."""
+    q_at, k_at, dtype = 0, 0, torch.bfloat16
     if q_norm is not None:
-        q_norm = _norm_weight(q_norm, "q_norm", head_dim, index, device)
+        q_norm, q_at = _norm_weight(q_norm, "q_norm", head_dim, index, device)
+        dtype = q_norm.dtype
     if k_norm is not None:
-        k_norm = _norm_weight(k_norm, "k_norm", head_dim, index, device)
-        if q_norm is not None and q_norm.dtype != k_norm.dtype:
+        k_norm, k_at = _norm_weight(k_norm, "k_norm", head_dim, index, device)
+        if q_norm is not None and k_norm.dtype != dtype:
             raise ValueError("q_norm and k_norm must be of one type")
-    w = q_norm if q_norm is not None else k_norm
-    if w is not None and w.dtype == torch.float32:
-        dtype = nat.STEP_F32
+        dtype = k_norm.dtype
     if not (math.isfinite(rotary_scale) and math.isfinite(norm_eps) and norm_eps >= 0 and abs(norm_offset) < 2.0 ** 127):
         raise ValueError("rotary_scale, norm_eps and norm_offset must be finite, norm_eps not below 0")
-    return ctypes.byref(nat.StepRotation(f, None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(),
-                                         rotary_scale, norm_eps, norm_offset, dtype, rotary, 1 if interleaved else 0)), (inv_freq, q_norm, k_norm)
+    return _ROTATION(at, q_at, k_at, rotary_scale, norm_eps, norm_offset, _KINDS[dtype], rotary, 1 if interleaved else 0), (q_norm, k_norm)
 
 
 def _int32(t: torch.Tensor, name: str, shape: tuple, device: torch.device) -> torch.Tensor:
@@ -266,37 +277,39 @@ class PagedKvCache:
         self._check(batch)
         if not isinstance(k, torch.Tensor) or k.dtype not in (torch.bfloat16, torch.float32):
             raise ValueError("k must be a bfloat16 or float32 tensor")
-        k = self._rows(k, "k", self.kv_heads, None, None, 4)
+        head_dim, index, device, dtype = self.head_dim, self._index, self.device, k.dtype
+        k = _row_view(k, "k", head_dim, index, device, self.kv_heads, None, None, 4)
         tokens = k.shape[0]
-        v = self._rows(v, "v", self.kv_heads, tokens, k.dtype, 4)
-        rotation, held = _rotation(self.head_dim, self._index, self.device, inv_freq, interleaved, rotary_scale, q_norm, k_norm, norm_eps, norm_offset)
-        inv_freq = held[0]
-        heads, q_stride = self.kv_heads, 0
+        v = _row_view(v, "v", head_dim, index, device, self.kv_heads, tokens, dtype, 4)
+        inv_freq, inv_at, rotary = (None, 0, 0) if inv_freq is None else _frequencies(inv_freq, head_dim, index, device)
+        heads, q_stride, q_at, out_at = self.kv_heads, 0, None, None
         if q is not None:
-            q = self._rows(q, "q", None, tokens, k.dtype, 4)
-            heads, q_stride = q.shape[1], q.stride(0)
+            q = _row_view(q, "q", head_dim, index, device, None, tokens, dtype, 4)
+            heads, q_stride, q_at = q.shape[1], q.stride(0), q.data_ptr()
             if heads % self.kv_heads or heads == 0:
                 raise ValueError(f"q's {heads} heads are no multiple of the cache's {self.kv_heads}")
             out = self._out(out, tokens, heads)
+            out_at = out.data_ptr()
         elif out is not None:
             raise ValueError("out goes with q")
         elif q_norm is not None:
             raise ValueError("q_norm goes with q")
-        lib, new = nat.lib(), batch._struct(tokens)
-        dtype = nat.STEP_F32 if k.dtype == torch.float32 else nat.STEP_BF16
-        with _on(self.device):
-            stream = _stream(self.device)
-            if self.dtype == torch.float4_e2m1fn_x2:
+        e2m1 = self.dtype == torch.float4_e2m1fn_x2
+        plain = q_norm is None and k_norm is None and not interleaved and rotary_scale == 1.0
+        if e2m1 or not plain or norm_eps != 1e-6 or norm_offset != 0.0:
+            rotation, held = _rotation(head_dim, index, device, inv_at, rotary, interleaved, rotary_scale, q_norm, k_norm, norm_eps, norm_offset)
+        lib, new, kind = nat.lib(), batch._struct(tokens), _KINDS[dtype]
+        with _on(device):
+            if e2m1:
                 nat.step_check(lib.se12_step_paged_append_rotated(
-                    self._struct, new, None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype, q_stride, k.stride(0),
-                    v.stride(0), heads, rotation, None if q is None else out.data_ptr(), stream))
+                    self._struct, new, q_at, k.data_ptr(), v.data_ptr(), kind, q_stride, k.stride(0), v.stride(0), heads, rotation, out_at,
+                    _stream(device)))
                 return out
-            if q_norm is not None or k_norm is not None or interleaved or rotary_scale != 1.0:
-                return self._append_turned(batch, q, k, v, out, inv_freq, interleaved, rotary_scale, q_norm, k_norm, norm_eps, norm_offset)
+            if not plain:
+                return self._append_turned(batch, q, k, v, out, inv_freq, interleaved, rotary_scale, *held, norm_eps, norm_offset)
             nat.step_check(lib.se12_step_paged_append(
-                self._struct, new, None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype, q_stride, k.stride(0), v.stride(0),
-                heads, None if inv_freq is None else inv_freq.data_ptr(), 0 if inv_freq is None else 2 * inv_freq.numel(),
-                None if q is None else out.data_ptr(), stream))
+                self._struct, new, q_at, k.data_ptr(), v.data_ptr(), kind, q_stride, k.stride(0), v.stride(0), heads, inv_at or None, rotary,
+                out_at, _stream(device)))
         return out
 
     def _append_turned(self, batch, q, k, v, out, inv_freq, interleaved, rotary_scale, q_norm, k_norm, norm_eps, norm_offset):
@@ -408,36 +421,40 @@ def rotate_heads(batch: PagedBatch, q: torch.Tensor, k: torch.Tensor | None = No
     not written. No gradients."""
     if not isinstance(batch, PagedBatch):
         raise ValueError("batch must be a PagedBatch")
-    if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype not in (torch.bfloat16, torch.float32):
+    if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype not in _KINDS:
         raise ValueError("q must be a bfloat16 or float32 [tokens, heads, head_dim] tensor")
-    tokens, heads, head_dim = q.shape
+    shape, kind = q.shape, q.dtype
+    tokens, heads, head_dim = shape
     if head_dim % 8 or not 8 <= head_dim <= 256 or not 1 <= heads <= 65535:
         raise ValueError(f"q must have 1 to 65535 heads and a head_dim of a multiple of 8 up to 256, got {heads}, {head_dim}")
-    if dtype not in (torch.bfloat16, torch.float32):
+    if dtype not in _KINDS:
         raise ValueError(f"dtype must be bfloat16 or float32, got {dtype}")
     index, device = batch.page_table.get_device(), batch.device
     q = _row_view(q, "q", head_dim, index, device, None, None, None, 4, "the batch")
     q_out, k_out = (None, None) if out is None else out
-    q_out = _turned_out(q_out, q.shape, dtype, device)
-    kv_heads = k_stride = k_at = k_out_at = 0
+    q_out = _turned_out(q_out, shape, dtype, device)
+    kv_heads = k_stride = 0
+    k_at = k_out_at = None
     if k is not None:
         if isinstance(k, torch.Tensor) and k.dim() == 3:
-            if not 1 <= k.shape[1] <= 65535:
-                raise ValueError(f"k must have 1 to 65535 heads, got {k.shape[1]}")
-            if k.shape[0] != tokens:
-                raise ValueError(f"k has {k.shape[0]} rows, q has {tokens}")
-        k = _row_view(k, "k", head_dim, index, device, None, None, q.dtype, 4, "the batch")
-        k_out = _turned_out(k_out, k.shape, dtype, device)
-        kv_heads, k_stride, k_at, k_out_at = k.shape[1], k.stride(0), k.data_ptr(), k_out.data_ptr()
+            shape = k.shape
+            kv_heads = shape[1]
+            if not 1 <= kv_heads <= 65535:
+                raise ValueError(f"k must have 1 to 65535 heads, got {kv_heads}")
+            if shape[0] != tokens:
+                raise ValueError(f"k has {shape[0]} rows, q has {tokens}")
+        k = _row_view(k, "k", head_dim, index, device, None, None, kind, 4, "the batch")
+        k_out = _turned_out(k_out, shape, dtype, device)
+        k_stride, k_at, k_out_at = k.stride(0), k.data_ptr(), k_out.data_ptr()
     elif k_norm is not None or k_out is not None:
         raise ValueError("k_norm and out's second tensor go with k")
-    rotation, held = _rotation(head_dim, index, device, inv_freq, interleaved, rotary_scale, q_norm, k_norm, norm_eps, norm_offset)
+    inv_freq, inv_at, rotary = (None, 0, 0) if inv_freq is None else _frequencies(inv_freq, head_dim, index, device)
+    rotation, held = _rotation(head_dim, index, device, inv_at, rotary, interleaved, rotary_scale, q_norm, k_norm, norm_eps, norm_offset)
     with _on(device):
         nat.step_check(nat.lib().se12_step_rotate_heads(
-            batch._struct(tokens), q.data_ptr(), k_at or None, nat.STEP_F32 if q.dtype == torch.float32 else nat.STEP_BF16, q.stride(0), k_stride,
-            heads, kv_heads, head_dim, rotation, q_out.data_ptr(), k_out_at or None, nat.STEP_F32 if dtype == torch.float32 else nat.STEP_BF16,
-            _stream(device)))
-    del held      # (until the call has been made)
+            batch._struct(tokens), q.data_ptr(), k_at, _KINDS[kind], q.stride(0), k_stride, heads, kv_heads, head_dim, rotation, q_out.data_ptr(),
+            k_out_at, _KINDS[dtype], _stream(device)))
+    del inv_freq, held      # (until the call has been made)
     return q_out, k_out
 
 
