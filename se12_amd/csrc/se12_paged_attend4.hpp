@@ -253,7 +253,7 @@ struct Attend<SE12_STEP_E2M1, D> {
             if (t >= t1) break;
             // The rare tile, outside the loop: the maximum moves, and what is summed with it;
             // 0 x NaN is NaN, so a scale that is no number leaves the product, and what it
-            // scales comes back as a NaN in the columns that give its key a weight.
+            // scales comes back as a NaN in the columns that see its key, whatever its weight.
             const float to = fmaxf(m, column_max(top));
             const float scale = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
             m = to;
@@ -275,7 +275,7 @@ struct Attend<SE12_STEP_E2M1, D> {
                     for (int k = 0; k < 4; ++k) {
                         const uint32_t x = of_row16<i>(bad[k]);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) seen |= ((x >> (8 * e)) & 1u) != 0 && (float)pf[k / 2][4 * (k % 2) + e] > 0.0f;
+                        for (int e = 0; e < 4; ++e) seen |= ((x >> (8 * e)) & 1u) != 0 && sc[4 * k + e] != -INFINITY;
                     }
                     seen |= __shfl_xor(seen, 16, 64);
                     seen |= __shfl_xor(seen, 32, 64);

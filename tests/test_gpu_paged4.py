@@ -715,6 +715,23 @@ def test_what_a_query_may_not_see_has_no_part_in_its_row(gpu, d, many):
             r += 1
 
 
+@pytest.mark.parametrize("d,new", [(64, 1), (256, 1), (128, 9), (64, 60), (256, 60)])
+def test_values_that_are_no_numbers_are_seen_whatever_their_weight(gpu, d, new):
+    """A key of great size beside the others: its weight is all or nothing, by the sign of its score."""
+    c, batch, q, _ = _attend_case(gpu, d, 16, 8, 2, [150, 3], [new, 1], 0.0, 0, seed=84, extra=0)
+    page = batch.page_table[0, 4].item()
+    c.k_scale[page, :, :, 3] = 200                       # (2^10: scores of thousands)
+    before = c.attend(batch, q, d ** -0.5 / 4)
+    k = e.pools(c)[0][page, :, 3]
+    scores = q[:new].cpu().double().view(new, 2, 4, d) @ k[None, :, :, None]
+    assert (scores > 1000).any() and (scores < -1000).any() and before.isfinite().all()
+    c.v_scale[page, :, 1, 3] = 255
+    got = c.attend(batch, q, d ** -0.5 / 4)
+    assert got[:new, :, 32:64].isnan().all()
+    assert torch.equal(got[:new, :, :32], before[:new, :, :32]) and torch.equal(got[:new, :, 64:], before[:new, :, 64:])
+    assert torch.equal(got[new:], before[new:])
+
+
 @pytest.mark.parametrize("d,lengths,new,window", [(64, [200, 13], [1, 1], 60), (256, [200, 13], [40, 5], 60), (128, [77], [70], 0), (64, [0, 130], [65, 3], 20)])
 def test_slots_that_are_not_seen_may_hold_any_bytes(gpu, d, lengths, new, window):
     page = 32
@@ -955,3 +972,39 @@ def test_rows_beyond_32_bit_offsets(gpu):
     for r in (0, 1_048_575, 1_048_576, n - 4, n - 1):
         one, _ = _batch(gpu, [[0]], [r], [1])
         assert torch.equal(rotate_heads(one, k[r:r + 1], None, inv)[0], turned[r:r + 1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, BF16])
+def test_norms_for_caches_of_other_types_in_a_graph(gpu, dtype):
+    """Steps of a cache that norms before it appends, replayed with eager work between, against the same one by one."""
+    from se12_amd.paged import PagedBatch, PagedKvCache
+
+    d, kvh, heads = 64, 2, 4
+    inv = (10000.0 ** (-torch.arange(0, d, 2).float() / d)).to(gpu)
+    w = (torch.rand(d, generator=_gen(90)) + 0.5).to(gpu)
+    as32 = lambda v: torch.tensor(v, dtype=torch.int32, device=gpu)  # noqa: E731
+    outs = []
+    for captured in (False, True):
+        c = PagedKvCache(6, 16, kvh, d, dtype=dtype, device=gpu)
+        lengths = as32([14, 0])
+        batch = PagedBatch(as32([[0, 2, 4], [1, 3, 5]]), lengths, as32([0, 1, 2]))
+        x, y, g = torch.empty((2, heads + 2 * kvh, d), dtype=BF16, device=gpu), torch.empty((2, heads, d), dtype=BF16, device=gpu), _gen(91)
+
+        def step():
+            q, k, v = x.split([heads, kvh, kvh], 1)
+            c.attend(batch, c.append(batch, k, v, q=q, inv_freq=inv, interleaved=True, q_norm=w, k_norm=w), 0.125, out=y)
+            lengths.add_(1)
+
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            torch.cuda.synchronize()
+            with torch.cuda.graph(graph):
+                step()
+        for _ in range(6):
+            x.copy_(torch.randn(x.shape, generator=g))
+            graph.replay() if captured else step()
+            outs.append((y.cpu(), c.k.float().cpu(), c.v.float().cpu()))
+            torch.randn(1000, device=gpu).sum().item()
+    for a, b in zip(outs[:6], outs[6:]):
+        for s, t in zip(a, b):
+            assert torch.equal(s, t)
