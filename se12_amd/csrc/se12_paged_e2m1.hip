@@ -78,6 +78,7 @@ __device__ __forceinline__ uint32_t e2m1x8(const float x[8], float s) {
 template <int DT, int D, bool kFew>
 __global__ __launch_bounds__(kRowThreads) void paged_append4_kernel(Append4Args a) {
     constexpr int kLanes = D / 8, kRows = kRowThreads / kLanes;
+    static_assert(16 <= 2 * kRows, "");
     __shared__ __attribute__((aligned(16))) float2 cs[16 * D / 2];
     __shared__ __attribute__((aligned(16))) float rows[kRows * D];
     __shared__ __attribute__((aligned(16))) float weights[2][D]; // of q's norm and k's
@@ -101,11 +102,11 @@ __global__ __launch_bounds__(kRowThreads) void paged_append4_kernel(Append4Args 
     // power of two): 3 of 32 / 8 heads of 128 for 40 sequences 6.8 us, 10.6 one at a time; 9,001
     // of 16 / 8 heads of 256 76 one at a time, 90 several, where each lane finds its own.
     // The next row is on its way while one is worked on.
-    const int lane = tid % kLanes, c0 = 8 * lane, place = tid / kLanes, what_end = 2 + a.group, turns = (n + kRows - 1) / kRows;
-    const int places = n > 1 ? 32 - __builtin_clz(n - 1) : 0;
+    const int lane = tid % kLanes, c0 = 8 * lane, place = tid / kLanes, what_end = 2 + a.group;
+    const int turns_log2 = n > kRows ? 1 : 0, places = n > 1 ? 32 - __builtin_clz(n - 1) : 0;
     float* own = rows + place * D;
-    auto what_of = [&](int k) { return kFew ? (k * kRows + place) >> places : k / turns; };
-    auto token_of = [&](int k) { return kFew ? (k * kRows + place) & ((1 << places) - 1) : k % turns * kRows + place; };
+    auto what_of = [&](int k) { return kFew ? (k * kRows + place) >> places : k >> turns_log2; };
+    auto token_of = [&](int k) { return kFew ? (k * kRows + place) & ((1 << places) - 1) : (k & turns_log2) * kRows + place; };
     auto load = [&](int k) {
         const int what = what_of(k), t = min(token_of(k), n - 1);
         Eight<DT> v;
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(kRowThreads) void paged_append4_kernel(Append4Args 
             v.load(a.q, (row0 + t) * a.q_stride + (int64_t)(kh * a.group + what - 2) * D + c0);
         return v;
     };
-    const int count = kFew ? ((what_end << places) + kRows - 1) / kRows : what_end * turns;
+    const int count = kFew ? ((what_end << places) + kRows - 1) / kRows : what_end << turns_log2;
     Eight<DT> next = {};
     if (what_of(0) < what_end) next = load(0);
     __syncthreads();
