@@ -80,7 +80,6 @@ __global__ __launch_bounds__(kRowThreads) void paged_append4_kernel(Append4Args 
     constexpr int kLanes = D / 8, kRows = kRowThreads / kLanes;
     static_assert(16 <= 2 * kRows, "");
     __shared__ __attribute__((aligned(16))) float2 cs[16 * D / 2];
-    __shared__ __attribute__((aligned(16))) float rows[kRows * D];
     __shared__ __attribute__((aligned(16))) float weights[2][D]; // of q's norm and k's
     __shared__ uint32_t codes[16][kLanes];                       // of the values
     __shared__ __attribute__((aligned(16))) uint8_t scales[2][D / 32][16];
@@ -99,16 +98,15 @@ __global__ __launch_bounds__(kRowThreads) void paged_append4_kernel(Append4Args 
 
     // Rows: values (0), keys (1), then the query heads, n tokens of each. A block's threads take
     // kRows tokens of one of them at a time, or of few tokens those of several (in places for a
-    // power of two): 3 of 32 / 8 heads of 128 for 40 sequences 6.8 us, 10.6 one at a time; 9,001
-    // of 16 / 8 heads of 256 76 one at a time, 90 several, where each lane finds its own.
-    // The next row is on its way while one is worked on.
+    // power of two): 57 of 40 sequences, 32 / 8 heads of 128, 6.4 us, 10.6 one at a time; 9,001 of
+    // 16 / 8 heads of 256 14 us less one at a time than several, where each lane finds its own. The
+    // next rows are on their way while some are worked on (16 tokens of a head of 256 in two turns,
+    // both asked for at once: 3 us of 9,001 tokens').
+    constexpr int kTurns = kFew ? 1 : kRows >= 16 ? 1 : 16 / kRows;
     const int lane = tid % kLanes, c0 = 8 * lane, place = tid / kLanes, what_end = 2 + a.group;
-    const int turns_log2 = n > kRows ? 1 : 0, places = n > 1 ? 32 - __builtin_clz(n - 1) : 0;
-    float* own = rows + place * D;
-    auto what_of = [&](int k) { return kFew ? (k * kRows + place) >> places : k >> turns_log2; };
-    auto token_of = [&](int k) { return kFew ? (k * kRows + place) & ((1 << places) - 1) : (k & turns_log2) * kRows + place; };
-    auto load = [&](int k) {
-        const int what = what_of(k), t = min(token_of(k), n - 1);
+    const int places = n > 1 ? 32 - __builtin_clz(n - 1) : 0;
+    auto load = [&](int what, int token) {
+        const int t = min(token, n - 1);
         Eight<DT> v;
         if (what == 0)
             v.load(a.v, (row0 + t) * a.v_stride + (int64_t)kh * D + c0);
@@ -118,27 +116,21 @@ __global__ __launch_bounds__(kRowThreads) void paged_append4_kernel(Append4Args 
             v.load(a.q, (row0 + t) * a.q_stride + (int64_t)(kh * a.group + what - 2) * D + c0);
         return v;
     };
-    const int count = kFew ? ((what_end << places) + kRows - 1) / kRows : what_end << turns_log2;
-    Eight<DT> next = {};
-    if (what_of(0) < what_end) next = load(0);
-    __syncthreads();
-    for (int k = 0; k < count; ++k) {
-        const int what = what_of(k), t = token_of(k);
+    auto work = [&](const Eight<DT>& from, int what, int t) {
+        if (what >= what_end || t >= n) return;
         float x[8];
-        next.values(x);
-        if (k + 1 < count && what_of(k + 1) < what_end) next = load(k + 1);
-        if (what >= what_end || t >= n) continue;
+        from.values(x);
         const int64_t row = row0 + t;
         if (what > 0) {
             const void* w = what == 1 ? a.r.k_norm : a.r.q_norm;
             if (w) norm_row<kLanes>(x, a.r.eps, weights[what == 1] + c0, 1.0 / D);
-            if (half > 0) turn_row(x, own, cs + t * half, c0, half, a.r.interleaved);
+            if (half > 0) turn_row(x, cs + t * half, c0, half, a.r.interleaved);
             if (what > 1) {
                 uint16_t* o = a.q_out + (row * a.group * a.kvh + kh * a.group + what - 2) * D + c0;
                 const uint4 v = bf16x8(x);
                 reinterpret_cast<uint2*>(o)[0] = make_uint2(v.x, v.y);
                 reinterpret_cast<uint2*>(o)[1] = make_uint2(v.z, v.w);
-                continue;
+                return;
             }
         }
         // (the larger one, and NaN if there is one: by bits a NaN is above all numbers)
@@ -155,6 +147,33 @@ __global__ __launch_bounds__(kRowThreads) void paged_append4_kernel(Append4Args 
             codes[slot][lane] = w;
         else if (page >= 0)
             *reinterpret_cast<uint32_t*>(a.kc + (page_head * P + slot0 + slot) * (D / 2) + c0 / 2) = w;
+    };
+    Eight<DT> next[kTurns] = {};
+    if constexpr (kFew) {
+        auto what_of = [&](int k) { return (k * kRows + place) >> places; };
+        auto token_of = [&](int k) { return (k * kRows + place) & ((1 << places) - 1); };
+        const int count = ((what_end << places) + kRows - 1) / kRows;
+        if (what_of(0) < what_end) next[0] = load(what_of(0), token_of(0));
+        __syncthreads();
+        for (int k = 0; k < count; ++k) {
+            const Eight<DT> here = next[0];
+            if (k + 1 < count && what_of(k + 1) < what_end) next[0] = load(what_of(k + 1), token_of(k + 1));
+            work(here, what_of(k), token_of(k));
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kTurns; ++j) next[j] = load(0, j * kRows + place);
+        __syncthreads();
+        for (int what = 0; what < what_end; ++what) {
+            Eight<DT> here[kTurns];
+#pragma unroll
+            for (int j = 0; j < kTurns; ++j) {
+                here[j] = next[j];
+                if (what + 1 < what_end) next[j] = load(what + 1, j * kRows + place);
+            }
+#pragma unroll
+            for (int j = 0; j < kTurns; ++j) work(here[j], what, j * kRows + place);
+        }
     }
     __syncthreads();
     if (page < 0) return;

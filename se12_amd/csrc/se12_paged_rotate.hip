@@ -27,7 +27,6 @@ struct RotateArgs {
 template <int DT, int OT, int kLanes>
 __global__ __launch_bounds__(kRotateThreads) void rotate_heads_kernel(RotateArgs a) {
     constexpr int kRows = kRotateThreads / kLanes;
-    __shared__ __attribute__((aligned(16))) float rows[kRows * kLanes * 8];
     __shared__ __attribute__((aligned(16))) float weights[2 * kLanes * 8];      // of q's norm and k's
     extern __shared__ __attribute__((aligned(16))) float2 cs[];      // [tokens][half], then positions
     const int tid = threadIdx.x, half = a.r.half, first = (int)blockIdx.x * a.tokens, n = min(a.tokens, a.b.tokens - first);
@@ -56,7 +55,6 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_heads_kernel(RotateArgs
     __syncthreads();
     const int lane = tid % kLanes, c0 = 8 * lane, all = a.heads + a.kvh;
     const bool live = c0 < a.d;
-    float* own = rows + (tid / kLanes) * kLanes * 8;
     for (int i = tid / kLanes; i < n * all; i += kRows) {
         const int t = i / all, h = i - t * all;
         const bool is_q = h < a.heads;
@@ -67,7 +65,7 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_heads_kernel(RotateArgs
         if (live) load8<DT>(is_q ? a.q : a.k, row * (is_q ? a.q_stride : a.k_stride) + (int64_t)head * a.d + c0, x);
         const void* w = is_q ? a.r.q_norm : a.r.k_norm;
         if (w) norm_row<kLanes>(x, a.r.eps, weights + (is_q ? 0 : kLanes * 8) + c0, a.share);
-        if (half > 0) turn_row(x, own, cs + t * half, c0, half, a.r.interleaved);
+        if (half > 0) turn_row(x, cs + t * half, c0, half, a.r.interleaved);
         if (!live) continue;
         const int64_t to = (row * (is_q ? a.heads : a.kvh) + head) * a.d + c0;
         if constexpr (OT == SE12_STEP_F32) {

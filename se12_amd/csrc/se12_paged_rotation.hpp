@@ -187,48 +187,54 @@ __device__ __forceinline__ void norm_row(float x[8], double eps, const float* w,
     for (int i = 0; i < 8; ++i) x[i] = (x[i] * inv) * f[i];
 }
 
-// x[8], columns c0 .. of a row, turned by the angles cs[half] of its token; `row`: the
-// row's place in LDS, read and written by the wave's own lanes alone
-__device__ __forceinline__ void turn_row(float x[8], float* row, const float2* cs, int c0, int half, bool interleaved) {
+// x[8], columns c0 .. of a row whose lanes lie side by side, turned by the angles cs[half] of
+// its token
+__device__ __forceinline__ void turn_row(float x[8], const float2* cs, int c0, int half, bool interleaved) {
 #pragma clang fp contract(off)
+    if (c0 >= 2 * half) return;
     if (interleaved) {
+        const float4* t = reinterpret_cast<const float4*>(cs + c0 / 2);
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            if (c0 + 2 * p >= 2 * half) break;
-            const float2 t = cs[c0 / 2 + p];
-            const float a = x[2 * p], b = x[2 * p + 1];
-            x[2 * p] = a * t.x - b * t.y;
-            x[2 * p + 1] = b * t.x + a * t.y;
+        for (int p = 0; p < 2; ++p) {
+            const float4 u = t[p];
+            const float a = x[4 * p], b = x[4 * p + 1], c = x[4 * p + 2], d = x[4 * p + 3];
+            x[4 * p] = a * u.x - b * u.y;
+            x[4 * p + 1] = b * u.x + a * u.y;
+            x[4 * p + 2] = c * u.z - d * u.w;
+            x[4 * p + 3] = d * u.z + c * u.w;
         }
         return;
     }
-    *reinterpret_cast<float4*>(row + c0) = make_float4(x[0], x[1], x[2], x[3]);
-    *reinterpret_cast<float4*>(row + c0 + 4) = make_float4(x[4], x[5], x[6], x[7]);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    // four columns at `at`: with those half a rotation on, or back (a - b is a + -b)
-    auto turn4 = [&](float* y, int at) {
-        const bool first = at < half;
-        const uint32_t sign = first ? 0x80000000u : 0u;
-        const float4 other = *reinterpret_cast<const float4*>(row + (first ? at + half : at - half));
-        const float4* t = reinterpret_cast<const float4*>(cs + (first ? at : at - half));
-        const float4 t0 = t[0], t1 = t[1];
-        const float o[4] = {other.x, other.y, other.z, other.w}, cos[4] = {t0.x, t0.z, t1.x, t1.z}, sin[4] = {t0.y, t0.w, t1.y, t1.w};
+    // The columns half a rotation on, or back, are another lane's: its same four, or where half
+    // is no multiple of 8 its other four.
+    float o[8];
+    auto bring = [&](auto swapped) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float b = o[k] * __uint_as_float(__float_as_uint(sin[k]) ^ sign);
-            y[k] = y[k] * cos[k] + b;
+        for (int j = 0; j < 2; ++j) {
+            const int at = c0 + 4 * j, from = 4 * ((int)(threadIdx.x & 63) + (at < half ? at + half : at - half) / 8 - c0 / 8);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                o[4 * j + k] = __int_as_float(__builtin_amdgcn_ds_bpermute(from, __float_as_int(x[(swapped.value ? 4 - 4 * j : 4 * j) + k])));
         }
     };
-    if (half % 8 == 0) {
-        if (c0 < 2 * half) {
-            turn4(x, c0);
-            turn4(x + 4, c0 + 4);
+    if (half % 8 == 0)
+        bring(std::false_type{});
+    else
+        bring(std::true_type{});
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int at = c0 + 4 * j;
+        const bool first = at < half;
+        const uint32_t sign = first ? 0x80000000u : 0u;      // (a - b is a + -b)
+        const float4* t = reinterpret_cast<const float4*>(cs + (first ? at : at - half));
+        const float4 t0 = t[0], t1 = t[1];
+        const float cos[4] = {t0.x, t0.z, t1.x, t1.z}, sin[4] = {t0.y, t0.w, t1.y, t1.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float b = o[4 * j + k] * __uint_as_float(__float_as_uint(sin[k]) ^ sign);
+            x[4 * j + k] = x[4 * j + k] * cos[k] + b;
         }
-    } else {
-        if (c0 < 2 * half) turn4(x, c0);
-        if (c0 + 4 < 2 * half) turn4(x + 4, c0 + 4);
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
 __device__ __forceinline__ uint4 bf16x8(const float x[8]) {
