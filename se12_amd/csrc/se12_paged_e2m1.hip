@@ -10,9 +10,9 @@
 // query heads that read it, so a value column's 8 bytes (16 tokens) have one writer and
 // the angles serve all its rows. Values meet in LDS, where a column's tokens lie apart.
 //
-// Append: 9,001 tokens of 7 prompts, 16 / 8 heads of 256 normed and rotated, BF16 in: 241 MB in 76
-// us (3.2 TB/s; a copy 5.0, so 48). Bound by vector instructions, 1,590 to a
-// wave of 16 rows, issued 73% of the time. One token 4.6 us, 57 of 40 sequences 6.5: starts, lengths, table
+// Append: 9,001 tokens of 7 prompts, 16 / 8 heads of 256 normed and rotated, BF16 in: 241 MB in 57 to
+// 60 us (4.1 TB/s; a copy 5.0, so 48), the vector units busy for most of it (with the angles in
+// every thread, 1,470 instructions to a wave of 16 rows, 89% of 66 us). One token 4.6 us, 57 of 40 sequences 6.5: starts, lengths, table
 // entry and rows, one after the other.
 // Read: bound by bytes. 47,604 tokens of 8 heads of 256 from pages of 4 bits: 494 MB in 104 us (4.75
 // TB/s; a copy 5.0). Values turn in LDS, so that rows are written whole.
@@ -74,24 +74,29 @@ __device__ __forceinline__ uint32_t e2m1x8(const float x[8], float s) {
     return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[6], y[7], 1.0f, 3);
 }
 
-// kFew: a run's new tokens are half of the rows that the block works on at once, or fewer
-template <int DT, int D, bool kFew>
-__global__ __launch_bounds__(kRowThreads) void paged_append4_kernel(Append4Args a) {
-    constexpr int kLanes = D / 8, kRows = kRowThreads / kLanes;
+// kFew: a run's new tokens are half of the rows that kRowThreads work on at once, or fewer.
+// kHeads: KV heads of a block, each with kRowThreads of its own (two share the angles: 9,001
+// tokens of 8 heads 2 us less than one to a block; few tokens have blocks to spare)
+template <int DT, int D, bool kFew, int kHeads>
+__global__ __launch_bounds__(kHeads * kRowThreads) void paged_append4_kernel(Append4Args a) {
+    constexpr int kLanes = D / 8, kRows = kRowThreads / kLanes, kThreads = kHeads * kRowThreads;
     static_assert(16 <= 2 * kRows, "");
     __shared__ __attribute__((aligned(16))) float2 cs[16 * D / 2];
     __shared__ __attribute__((aligned(16))) float weights[2][D]; // of q's norm and k's
-    __shared__ uint32_t codes[16][kLanes];                       // of the values
-    __shared__ __attribute__((aligned(16))) uint8_t scales[2][D / 32][16];
-    const int tid = threadIdx.x, kh = (int)blockIdx.x % a.kvh;
-    const Run16 u = run16_of(a.b, (int)blockIdx.x / a.kvh);
+    __shared__ uint32_t all_codes[kHeads][16][kLanes];           // of the values
+    __shared__ __attribute__((aligned(16))) uint8_t all_scales[kHeads][2][D / 32][16];
+    const int sub = kHeads == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kRowThreads), tid = threadIdx.x % kRowThreads;
+    auto& codes = all_codes[sub];
+    auto& scales = all_scales[sub];
+    const int groups = (a.kvh + kHeads - 1) / kHeads, kh = (int)blockIdx.x % groups * kHeads + sub;
+    const Run16 u = run16_of(a.b, (int)blockIdx.x / groups);
     const int n = u.to - u.from;
     if (n <= 0) return;
     const int64_t row0 = u.seq.start + u.first + u.from - u.seq.len;      // of the first token
     const int half = a.r.half;
-    turn_run16<kRowThreads>(cs, a.r, u.first, u.from, u.to);
-    if (a.r.q_norm && a.group > 0) load_weights<kRowThreads>(weights[0], a.r, a.r.q_norm, D);
-    if (a.r.k_norm) load_weights<kRowThreads>(weights[1], a.r, a.r.k_norm, D);
+    turn_run16<kThreads, !kFew>(cs, a.r, u.first, u.from, u.to);
+    if (a.r.q_norm && a.group > 0) load_weights<kThreads>(weights[0], a.r, a.r.q_norm, D);
+    if (a.r.k_norm) load_weights<kThreads>(weights[1], a.r, a.r.k_norm, D);
     const int P = 1 << a.page_log2, page = page_of(a.b, u.s, u.first >> a.page_log2, a.pages);
     const int64_t page_head = (int64_t)max(page, 0) * a.kvh + kh;
     const int slot0 = u.first & (P - 1);
@@ -103,7 +108,7 @@ __global__ __launch_bounds__(kRowThreads) void paged_append4_kernel(Append4Args 
     // next rows are on their way while some are worked on (16 tokens of a head of 256 in two turns,
     // both asked for at once: 3 us of 9,001 tokens').
     constexpr int kTurns = kFew ? 1 : kRows >= 16 ? 1 : 16 / kRows;
-    const int lane = tid % kLanes, c0 = 8 * lane, place = tid / kLanes, what_end = 2 + a.group;
+    const int lane = tid % kLanes, c0 = 8 * lane, place = tid / kLanes, what_end = kh < a.kvh ? 2 + a.group : 0;
     const int places = n > 1 ? 32 - __builtin_clz(n - 1) : 0;
     auto load = [&](int what, int token) {
         const int t = min(token, n - 1);
@@ -162,7 +167,8 @@ __global__ __launch_bounds__(kRowThreads) void paged_append4_kernel(Append4Args 
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < kTurns; ++j) next[j] = load(0, j * kRows + place);
+        for (int j = 0; j < kTurns; ++j)
+            if (what_end > 0) next[j] = load(0, j * kRows + place);
         __syncthreads();
         for (int what = 0; what < what_end; ++what) {
             Eight<DT> here[kTurns];
@@ -176,7 +182,7 @@ __global__ __launch_bounds__(kRowThreads) void paged_append4_kernel(Append4Args 
         }
     }
     __syncthreads();
-    if (page < 0) return;
+    if (page < 0 || kh >= a.kvh) return;
     for (int c = tid; c < D; c += kRowThreads) {
         uint2* p = reinterpret_cast<uint2*>(a.vc + ((page_head << (a.page_log2 - 4)) + slot0 / 16) * (8 * D)) + c;
         uint2 was = make_uint2(0, 0);
@@ -328,19 +334,21 @@ using namespace se12step;
 namespace {
 
 template <int DT, int D>
-void launch_append4_of(const Append4Args& a, uint32_t blocks, hipStream_t st) {
+void launch_append4_of(const Append4Args& a, uint32_t runs, hipStream_t st) {
     if (2 * (a.b.max_new < 16 ? a.b.max_new : 16) <= kRowThreads / (D / 8))
-        hipLaunchKernelGGL((paged_append4_kernel<DT, D, true>), dim3(blocks), dim3(kRowThreads), 0, st, a);
+        hipLaunchKernelGGL((paged_append4_kernel<DT, D, true, 1>), dim3(runs * a.kvh), dim3(kRowThreads), 0, st, a);
+    else if (a.kvh == 1)
+        hipLaunchKernelGGL((paged_append4_kernel<DT, D, false, 1>), dim3(runs), dim3(kRowThreads), 0, st, a);
     else
-        hipLaunchKernelGGL((paged_append4_kernel<DT, D, false>), dim3(blocks), dim3(kRowThreads), 0, st, a);
+        hipLaunchKernelGGL((paged_append4_kernel<DT, D, false, 2>), dim3(runs * ((a.kvh + 1) / 2)), dim3(2 * kRowThreads), 0, st, a);
 }
 
 template <int DT>
-void launch_append4(const Append4Args& a, int d, uint32_t blocks, hipStream_t st) {
+void launch_append4(const Append4Args& a, int d, uint32_t runs, hipStream_t st) {
     switch (d) {
-        case 64: launch_append4_of<DT, 64>(a, blocks, st); break;
-        case 128: launch_append4_of<DT, 128>(a, blocks, st); break;
-        default: launch_append4_of<DT, 256>(a, blocks, st);
+        case 64: launch_append4_of<DT, 64>(a, runs, st); break;
+        case 128: launch_append4_of<DT, 128>(a, runs, st); break;
+        default: launch_append4_of<DT, 256>(a, runs, st);
     }
 }
 
@@ -371,13 +379,13 @@ int se12_step_paged_append_rotated(const se12_step_pages* pages, const se12_step
                         reinterpret_cast<uint8_t*>(pages->k_scale), reinterpret_cast<uint8_t*>(pages->v_scale), q_out,
                         device_batch(batch), device_rotation(rotation), q ? heads / pages->kv_heads : 0, pages->kv_heads,
                         pages->pages, log2_of(pages->page_size)};
-    const int64_t blocks = run16_blocks(a.b) * pages->kv_heads;
-    if (!grid_fits(blocks, kRowThreads)) return step_fail(fn, "too many tokens and heads for one launch");
+    const int64_t runs = run16_blocks(a.b);
+    if (!grid_fits(runs * (pages->kv_heads + 1), kRowThreads)) return step_fail(fn, "too many tokens and heads for one launch");
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (dtype == SE12_STEP_F32)
-        launch_append4<SE12_STEP_F32>(a, pages->head_dim, (uint32_t)blocks, st);
+        launch_append4<SE12_STEP_F32>(a, pages->head_dim, (uint32_t)runs, st);
     else
-        launch_append4<SE12_STEP_BF16>(a, pages->head_dim, (uint32_t)blocks, st);
+        launch_append4<SE12_STEP_BF16>(a, pages->head_dim, (uint32_t)runs, st);
     return step_launched();
 }
 

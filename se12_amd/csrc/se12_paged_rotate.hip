@@ -1,7 +1,7 @@
 // Norm and rotation of a call's q and k by themselves (for caches of BF16 and E4M3, or a
 // program's own): se12_paged_rotation.hpp for the mathematics. A block takes a few tokens
 // with all their heads, whose angles it works out once. Bound by the bytes of q and k: 7,987
-// tokens of 32 / 8 heads of 128, BF16, normed: 164 MB in 35 us (4.6 TB/s; a copy 5.0). 24 tokens 6.1
+// tokens of 32 / 8 heads of 128, BF16, normed: 164 MB in 35 us (4.7 TB/s; a copy 5.0). 24 tokens 6.1
 // us: starts, lengths and rows, one after the other.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
