@@ -378,8 +378,9 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : 2) void paged_attent
 // as many (85 parts at D = 128: 6.8 us by four, 6.1 so; 12 at once are 8.0, for few parts
 // 6.8 from 4.6); a part's maximum may lie above those before it, so what is summed moves
 // with it.
+// Of a grid of blocks [nx][ny] (max_units 0: x a worker) block x, y.
 template <int CT, int D>
-__global__ __launch_bounds__(kAttendThreads) void paged_join_kernel(AttendArgs a, int max_units) {
+__device__ __forceinline__ void join_columns(const AttendArgs& a, int max_units, int x, int y, int ny) {
     constexpr int kTile = Form<CT>::kTile;
     constexpr int kLanes = D / 4, kParts = kAttendThreads / kLanes;
     __shared__ float4 sums[kAttendThreads];
@@ -389,12 +390,12 @@ __global__ __launch_bounds__(kAttendThreads) void paged_join_kernel(AttendArgs a
     SeqWork w;
     int64_t first, per;      // the unit's first tile, tiles of a worker
     if (max_units > 0) {
-        unit = (int)(blockIdx.x % max_units);
-        kh = (int)(blockIdx.x / max_units % a.kvh);
-        const int s = (int)(blockIdx.x / max_units / a.kvh);
+        unit = x % max_units;
+        kh = x / max_units % a.kvh;
+        const int s = x / max_units / a.kvh;
         const Chunk chunk = load_chunk<kTile>(a, s & ~63, lane);
         w = seq_work<kTile>(a, seq_of(chunk, s & 63));
-        if (unit >= w.units || unit * kColumns + (int)blockIdx.y >= w.seq.n * a.group) return;
+        if (unit >= w.units || unit * kColumns + y >= w.seq.n * a.group) return;
         int64_t base = __builtin_amdgcn_readlane(chunk.upto, s & 63) - __builtin_amdgcn_readlane(chunk.tiles, s & 63), total = chunk.all;
         for (int s0 = 0; s0 < a.b.seqs; s0 += 64) {
             if (s0 == (s & ~63)) continue;
@@ -409,7 +410,7 @@ __global__ __launch_bounds__(kAttendThreads) void paged_join_kernel(AttendArgs a
         int64_t total = chunk.all, before = 0;
         for (int s0 = 64; s0 < a.b.seqs; s0 += 64) total += load_chunk<kTile>(a, s0, lane).all;
         per = tiles_each(total);
-        const int64_t at = ((int64_t)blockIdx.x + 1) * per;      // where the next worker begins
+        const int64_t at = ((int64_t)x + 1) * per;      // where the next worker begins
         if (at >= total) return;
         for (int s0 = 64; before + chunk.all <= at; s0 += 64) {
             before += chunk.all;
@@ -422,12 +423,12 @@ __global__ __launch_bounds__(kAttendThreads) void paged_join_kernel(AttendArgs a
         kh = line / w.units;
         unit = line - kh * w.units;
         first = at - tile;
-        if (tile == 0 || worker_of(first, per) != (int)blockIdx.x) return;
+        if (tile == 0 || worker_of(first, per) != x) return;
     }
     const int w0 = worker_of(first, per), w1 = worker_of(first + w.tiles - 1, per);
     if (w0 == w1) return;      // one worker had it all
     const float2* mlp = reinterpret_cast<const float2*>(a.part + (int64_t)a.workers * 2 * a.columns * D);
-    for (int col = blockIdx.y; col < kColumns; col += gridDim.y) {
+    for (int col = y; col < kColumns; col += ny) {
         const int c = unit * kColumns + col;
         if (c >= w.seq.n * a.group) break;
         float m = -INFINITY, l = 0.0f;
@@ -494,6 +495,24 @@ __global__ __launch_bounds__(kAttendThreads) void paged_join_kernel(AttendArgs a
     }
 }
 
+template <int CT, int D>
+__global__ __launch_bounds__(kAttendThreads) void paged_join_kernel(AttendArgs a, int max_units) {
+    join_columns<CT, D>(a, max_units, (int)blockIdx.x, (int)blockIdx.y, (int)gridDim.y);
+}
+
+// Both joins of a call that may have prompts, behind their kernel: the prompts' units, then the
+// others' columns (a launch each: 302 tokens of 4 sequences 41 us for 39).
+template <int CT, int D>
+__global__ __launch_bounds__(kAttendThreads) void paged_joins_kernel(AttendArgs a, float* prompt_part, int prompt_blocks, int max_units, int nx, int ny) {
+    const int block = (int)blockIdx.x - prompt_blocks;
+    if (block < 0) {
+        a.part = prompt_part;
+        join_unit<D>(a, (int)blockIdx.x);
+    } else {
+        join_columns<CT, D>(a, max_units, block % nx, block / nx, ny);
+    }
+}
+
 }  // namespace se12step
 
 using namespace se12step;
@@ -536,8 +555,9 @@ int64_t all_bytes(const se12_step_pages* p, const Batch& b, int group) {
     return few_bytes(p, b, group) + x.record_bytes + x.part_bytes;
 }
 
+// part: of the prompts' units, NULL where no sequence can have any
 template <int CT, int D>
-void launch_attend(const AttendArgs& a, hipStream_t st) {
+void launch_attend(const AttendArgs& a, float* part, hipStream_t st) {
     constexpr int kWaves = kAttendThreads / 64;
     hipLaunchKernelGGL((paged_attention_kernel<CT, D>), dim3((uint32_t)(((int64_t)a.workers + a.unit_count + a.join_count + kWaves - 1) / kWaves)),
                        dim3(kAttendThreads), 0, st, a);
@@ -546,16 +566,24 @@ void launch_attend(const AttendArgs& a, hipStream_t st) {
     // (half as many again where each can be there: 130 sequences of one token, 8 KV heads of
     // 128, the call 29.7 us a block per unit, 30.8 per worker; 200 of 256 196 either way)
     const bool by_unit = units <= (max_units > 1 ? a.workers : a.workers + a.workers / 2);
-    hipLaunchKernelGGL((paged_join_kernel<CT, D>), dim3(by_unit ? (uint32_t)units : (uint32_t)a.workers, max_units > 1 ? 4 : a.columns),
-                       dim3(kAttendThreads), 0, st, a, by_unit ? max_units : 0);
+    const int nx = by_unit ? (int)units : a.workers, ny = max_units > 1 ? 4 : a.columns;
+    if (!part) {
+        hipLaunchKernelGGL((paged_join_kernel<CT, D>), dim3(nx, ny), dim3(kAttendThreads), 0, st, a, by_unit ? max_units : 0);
+        return;
+    }
+    AttendArgs prompts = a;
+    prompts.part = part;
+    launch_prompt(prompts, CT, D, st);
+    const int blocks = join_blocks<D>(a);
+    hipLaunchKernelGGL((paged_joins_kernel<CT, D>), dim3(blocks + nx * ny), dim3(kAttendThreads), 0, st, a, part, blocks, by_unit ? max_units : 0, nx, ny);
 }
 
 template <int CT>
-void launch_attend_of(const AttendArgs& a, int d, hipStream_t st) {
+void launch_attend_of(const AttendArgs& a, float* part, int d, hipStream_t st) {
     switch (d) {
-        case 64: launch_attend<CT, 64>(a, st); break;
-        case 128: launch_attend<CT, 128>(a, st); break;
-        default: launch_attend<CT, 256>(a, st);
+        case 64: launch_attend<CT, 64>(a, part, st); break;
+        case 128: launch_attend<CT, 128>(a, part, st); break;
+        default: launch_attend<CT, 256>(a, part, st);
     }
 }
 
@@ -603,14 +631,11 @@ int se12_step_paged_attention(const se12_step_pages* pages, const se12_step_batc
                  reinterpret_cast<UnitWork*>(static_cast<char*>(workspace) + few_bytes(pages, b, group)),
                  (int)plan.slots + plan.parts, plan.parts / 2, plan.parts, plan.most};
     const hipStream_t st = static_cast<hipStream_t>(stream);
+    float* part = plan.records > 0 ? reinterpret_cast<float*>(reinterpret_cast<char*>(a.units) + plan.record_bytes) : nullptr;
     switch (pages->dtype) {
-        case SE12_STEP_E2M1: launch_attend_of<SE12_STEP_E2M1>(a, pages->head_dim, st); break;
-        case SE12_STEP_E4M3: launch_attend_of<SE12_STEP_E4M3>(a, pages->head_dim, st); break;
-        default: launch_attend_of<SE12_STEP_BF16>(a, pages->head_dim, st);
-    }
-    if (plan.records > 0) {
-        a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(a.units) + plan.record_bytes);
-        launch_prompt(a, pages->dtype, pages->head_dim, st);
+        case SE12_STEP_E2M1: launch_attend_of<SE12_STEP_E2M1>(a, part, pages->head_dim, st); break;
+        case SE12_STEP_E4M3: launch_attend_of<SE12_STEP_E4M3>(a, part, pages->head_dim, st); break;
+        default: launch_attend_of<SE12_STEP_BF16>(a, part, pages->head_dim, st);
     }
     return step_launched();
 }

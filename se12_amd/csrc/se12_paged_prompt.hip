@@ -502,65 +502,7 @@ __global__ __launch_bounds__(kPromptThreads, D == 64 || (D == 128 && CT == SE12_
     }
 }
 
-// Units whose keys were split, from their parts in order: a wave has the columns of one
-// of the unit's waves, and every kJoinBlocks-th of its lanes' pieces.
-// (Of each unit 2 pieces at D = 256: 16 units of 16 parts, 34 MB, 45 us with 4 blocks a unit.)
-// The blocks of a unit and head, which write pieces of the same lines, are 8 apart and so
-// on one XCD. (One after the other, 2,000 and 1,500 tokens, 8 heads of 64: 64 us the call,
-// 60 so; all units' first blocks in front: one unit of 64 parts 120 us, 88 so, as blocks
-// that find nothing lie between.)
-template <int D>
-constexpr int kJoinBlocks = D / 16;
-
-template <int D>
-__global__ __launch_bounds__(kPromptThreads) void paged_prompt_join_kernel(AttendArgs a) {
-    constexpr int kPieces = D / 8 / kJoinBlocks<D>;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31;
-    const int y = (int)(blockIdx.x / 8) % kJoinBlocks<D>, x = (int)(blockIdx.x / 8) / kJoinBlocks<D> * 8 + (int)(blockIdx.x % 8);
-    if (x >= a.join_count * a.kvh) return;
-    const int kh = x % a.kvh;
-    const UnitWork u = unit_work(a, a.unit_count + x / a.kvh);
-    const int c = u.first + wave * kWaveColumns + col, count = u.parts;
-    if (u.s < 0 || count <= 1 || c >= u.columns) return;
-    const int64_t p0 = part_place(a, u, kh);
-    const float2* ml = reinterpret_cast<const float2*>(a.part + (int64_t)a.parts * a.kvh * kBlockColumns * D) + p0 * kBlockColumns +
-                       wave * kWaveColumns + col;
-    const float4* from = reinterpret_cast<const float4*>(a.part + p0 * kBlockColumns * D) + wave * (D / 8) * 64 + lane;
-    float m = -INFINITY;
-    for (int k = 0; k < count; ++k) m = fmaxf(m, ml[k * kBlockColumns].x);
-    const float top = m == -INFINITY ? 0.0f : m;
-    float4 o[kPieces];
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float l = 0.0f;
-#pragma unroll 4
-    for (int k = 0; k < count; ++k) {
-        const float2 p = ml[k * kBlockColumns];
-        const float by = __builtin_amdgcn_exp2f(p.x - top);
-        l += by * p.y;
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            const float4 v = from[(int64_t)k * (kBlockColumns * D / 4) + (i * kJoinBlocks<D> + y) * 64];
-            o[i].x += by * v.x;
-            o[i].y += by * v.y;
-            o[i].z += by * v.z;
-            o[i].w += by * v.w;
-        }
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t* out = a.out + ((int64_t)(u.start + c / a.group) * a.heads + kh * a.group + c % a.group) * D + 4 * (lane >> 5);
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i)
-        store4(out + 8 * (i * kJoinBlocks<D> + y), o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv);
-}
-
 namespace {
-
-template <int D>
-void launch_join(const AttendArgs& a, hipStream_t st) {
-    if (a.join_count > 0)
-        hipLaunchKernelGGL((paged_prompt_join_kernel<D>), dim3((a.join_count * a.kvh + 7) / 8 * 8 * kJoinBlocks<D>), dim3(kPromptThreads), 0, st, a);
-}
 
 template <int CT, int D>
 void launch(const AttendArgs& a, hipStream_t st) {
@@ -569,7 +511,6 @@ void launch(const AttendArgs& a, hipStream_t st) {
         hipLaunchKernelGGL((paged_prompt_kernel<CT, D, true>), dim3(grid), dim3(kPromptThreads), 4 * 64 * D, st, a);
     else
         hipLaunchKernelGGL((paged_prompt_kernel<CT, D, false>), dim3(grid), dim3(kPromptThreads), 4 * 64 * D, st, a);
-    launch_join<D>(a, st);
 }
 
 }  // namespace
@@ -595,11 +536,7 @@ PromptPlan prompt_plan(const Batch& b, int kvh, int group, int page_size, int d,
 }
 
 void launch_prompt(const AttendArgs& a, int dtype, int d, hipStream_t st) {
-    if (dtype == SE12_STEP_E2M1) {
-        launch_prompt4(a, d, st);
-        d == 64 ? launch_join<64>(a, st) : d == 128 ? launch_join<128>(a, st) : launch_join<256>(a, st);
-        return;
-    }
+    if (dtype == SE12_STEP_E2M1) return launch_prompt4(a, d, st);
     const bool e4m3 = dtype == SE12_STEP_E4M3;
     switch (d) {
         case 64: e4m3 ? launch<SE12_STEP_E4M3, 64>(a, st) : launch<SE12_STEP_BF16, 64>(a, st); break;
