@@ -15,7 +15,7 @@ namespace se12step {
 
 constexpr int kFewColumns = 64;           // of a sequence and KV head that se12_paged_attention.hip takes
 constexpr int kBlockColumns = 128;
-constexpr int kLeastTiles = 8;            // of a block, where a unit's keys are split
+constexpr int kLeastTiles = 8;            // of a block, where a unit's keys are split (E2M1: sharing_of)
 
 typedef float floatx16_t __attribute__((ext_vector_type(16)));      // sums of v_mfma_f32_32x32x16
 
@@ -137,7 +137,12 @@ __device__ __forceinline__ Sharing sharing_of(const AttendArgs& a, int lane) {
         tiles += wave_total((int)fminf((float)c.units * (float)(min(first, reach) / 2 + min(last, reach) / 2) / kTile, 1e7f));
         units += wave_total(c.units);
     }
-    const int64_t each = max(min(tiles * a.kvh / kResident + 1, (int64_t)1 << 24), (int64_t)kLeastTiles);
+    // (E2M1, whose parts start sooner: 4 tiles, or what makes 12 parts of a unit, as the join takes
+    // them one after the other. 302 tokens of 4 sequences behind 800, 16 / 8 heads of 256: 34.6 us, with
+    // 8 tiles 39.5; 500 tokens from the start, 4 heads: 24.6, 30.3; units of 92 tiles, 59 tokens
+    // behind 5,839, 8 heads on one of 128: 31.3 so and with 8, 32.5 with 4.)
+    const int64_t least = CT == SE12_STEP_E2M1 ? min(max(tiles / max(units, (int64_t)1) / 12, (int64_t)4), (int64_t)kLeastTiles) : kLeastTiles;
+    const int64_t each = max(min(tiles * a.kvh / kResident + 1, (int64_t)1 << 24), least);
     const int splits = (int)max(min(kResident / max(units * a.kvh, (int64_t)1), (int64_t)a.most), (int64_t)2);
     return {a.parts / splits, splits, (int)each};
 }
