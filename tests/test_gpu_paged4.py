@@ -1008,3 +1008,65 @@ def test_norms_for_caches_of_other_types_in_a_graph(gpu, dtype):
     for a, b in zip(outs[:6], outs[6:]):
         for s, t in zip(a, b):
             assert torch.equal(s, t)
+
+
+@pytest.mark.parametrize("d,page,kvh,heads,rotary,interleaved,norm,lengths,new", [
+    (256, 64, 3, 3, 256, False, BF16, [5, 130], [40, 17]),                 # heads in pairs, one left
+    (128, 16, 5, 10, 64, True, torch.float32, [0, 33], [70, 12]),
+    (64, 32, 3, 12, 56, False, None, [1], [100]),
+    (256, 128, 1, 2, 248, False, BF16, [9], [31]),                         # one head; pairs apart by no multiple of 8
+    (64, 16, 2, 2, 8, False, torch.float32, [3, 14], [33, 20]),
+    (128, 64, 7, 7, 0, False, BF16, [60], [75]),
+])
+def test_append_of_odd_numbers_of_heads(gpu, d, page, kvh, heads, rotary, interleaved, norm, lengths, new):
+    columns = max((a + n + page - 1) // page for a, n in zip(lengths, new))
+    pages = len(new) * columns + 1
+    table = _table(len(new), columns, pages, 92)
+    c = _cache(gpu, pages, page, kvh, d, 93)
+    batch, starts = _batch(gpu, table, lengths, new)
+    g = _gen(94)
+    x = torch.randn((starts[-1], heads + 2 * kvh, d), generator=g).to(BF16).to(gpu)
+    q, k, v = x.split([heads, kvh, kvh], 1)
+    inv = (10000.0 ** (-torch.arange(0, rotary, 2).float() / rotary)).to(gpu) if rotary else None
+    w = [None, None] if norm is None else [(torch.rand(d, generator=g) + 0.5).to(norm).to(gpu) for _ in range(2)]
+    before = _snapshot(c)
+    got = c.append(batch, k, v, q=q, inv_freq=inv, interleaved=interleaved, q_norm=w[0], k_norm=w[1])
+    _check_append(c, before, batch, lengths, starts, table, q, k, v, got, dict(inv_freq=inv, interleaved=interleaved, q_norm=w[0], k_norm=w[1]))
+
+
+def test_a_cache_in_the_callers_tensors_and_values_at_odd_addresses(gpu):
+    """from_tensors holds them in place; frequencies and weights need not be aligned."""
+    from se12_amd.paged import PagedKvCache, rotate_heads
+
+    c = _cache(gpu, 4, 16, 2, 64, 95)
+    other = PagedKvCache.from_tensors(c.k, c.v, c.k_scale, c.v_scale)
+    batch, _ = _batch(gpu, [[0, 2], [1, 3]], [3, 0], [20, 1])
+    g = _gen(96)
+    q, k, v = (torch.randn((21, h, 64), generator=g).to(gpu) for h in (4, 2, 2))
+    inv = 10000.0 ** (-torch.arange(0, 64, 2).float() / 64)
+    w = torch.rand(64, generator=g)
+    odd = [torch.cat([torch.zeros(1), t]).to(gpu)[1:] for t in (inv, w)]
+    assert all(t.data_ptr() % 16 for t in odd)
+    a = other.append(batch, k, v, q=q, inv_freq=odd[0], q_norm=odd[1], k_norm=odd[1])
+    state = _snapshot(c)
+    b = c.append(batch, k, v, q=q, inv_freq=inv.to(gpu), q_norm=w.to(gpu), k_norm=w.to(gpu))
+    assert torch.equal(a, b) and all(torch.equal(x, y) for x, y in zip(state, _snapshot(c)))
+    assert torch.equal(other.attend(batch, a, 0.125), c.attend(batch, a, 0.125))
+    for x, y in zip(rotate_heads(batch, q, k, odd[0], q_norm=odd[1]), rotate_heads(batch, q, k, inv.to(gpu), q_norm=w.to(gpu))):
+        assert torch.equal(x, y)
+
+
+def test_the_plain_append_entry_serves_4_bits_too(gpu):
+    import ctypes
+
+    from se12_amd import _native as nat
+
+    batch, _ = _batch(gpu, [[0, 2], [1, 3]], [3, 0], [20, 1])
+    q, k, v = (torch.randn((21, h, 64), generator=_gen(97)).to(gpu) for h in (4, 2, 2))
+    inv = (10000.0 ** (-torch.arange(0, 32, 2).float() / 32)).to(gpu)
+    a, b = _cache(gpu, 4, 16, 2, 64, 98), _cache(gpu, 4, 16, 2, 64, 98)
+    out = torch.empty((21, 4, 64), dtype=BF16, device=gpu)
+    nat.step_check(nat.lib().se12_step_paged_append(a._struct, batch._struct(21), q.data_ptr(), k.data_ptr(), v.data_ptr(), nat.STEP_F32, 256, 128, 128, 4,
+                                                    inv.data_ptr(), 32, out.data_ptr(), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+    assert torch.equal(out, b.append(batch, k, v, q=q, inv_freq=inv))
+    assert all(torch.equal(x, y) for x, y in zip(_snapshot(a), _snapshot(b)))
