@@ -140,6 +140,14 @@ def test_calls_without_tokens_need_no_memory():
                                       None) == 0
 
 
+def test_blocks_of_prompts_are_twice_as_large_and_counted_so():
+    lib, b = nat.lib(), _batch(sequences=200, tokens=1 << 27, max_new=1 << 20)
+    assert lib.se12_step_paged_attention_workspace(ctypes.byref(_pages(kv_heads=1, head_dim=256)), ctypes.byref(b), 8) > 0
+    p = _pages4(kv_heads=1, head_dim=256)
+    _refused("too many", lambda: lib.se12_step_paged_attention_workspace(ctypes.byref(p), ctypes.byref(b), 8))
+    _refused("too many", lambda: lib.se12_step_paged_attention(ctypes.byref(p), ctypes.byref(b), P, 1 << 14, P, 8, 0.1, 0.0, 0, P, 1 << 60, None))
+
+
 @pytest.mark.parametrize("heads,kv_heads", [(8, 4), (16, 8), (28, 4), (1, 1), (160, 1)])
 @pytest.mark.parametrize("sequences,width,page_size,head_dim", [(1, 6000, 16, 256), (64, 20, 64, 128), (300, 4, 128, 64), (3, 100, 32, 256)])
 def test_a_workspace_for_more_tokens_serves_fewer(heads, kv_heads, sequences, width, page_size, head_dim):
