@@ -16,7 +16,7 @@
 //
 // Bound by the bytes of the pages: 32 sequences to 8,191 keys, 16 / 8 heads of 256, 328 MB in 66 us and
 // 5 of the join (5.0 TB/s, a copy's rate); 3 to 130,000, 28 / 4 heads of 128, 159 MB in 32 + 6. 1,024
-// waves as for the other types: with 2,048 the calls took 75 and 44 for 68 and 40.
+// waves as for the other types: with 2,048 the calls took 75 and 44 for 68 and 40, in 256 registers 91.
 #pragma once
 
 #include "se12_paged_device.hpp"
