@@ -249,7 +249,8 @@ int se12_step_rotate_heads(const se12_step_batch* batch, const void* q, const vo
  * gives zeros. Any finite values of BF16 pages give finite results, those of E4M3
  * pages where none is above 2^112 / keys. SE12_STEP_E2M1 pages: the products' operands
  * are FP16, which holds keys and values exactly, a query to 2^-38 of its largest value, and a
- * weight to 2^-12 of itself or 2^-32 of the row's largest.
+ * weight to 2^-12 of itself or 2^-32 of the row's largest; scores beyond FP32's range
+ * keep their order.
  *
  * `workspace`: se12_step_paged_attention_workspace() bytes for the shape (or for
  * one of more tokens), 256-byte aligned, contents indifferent; calls sharing it

@@ -26,6 +26,11 @@ namespace se12step {
 constexpr float kSlack4 = 8.0f;
 constexpr float kLift4 = 7.0f;
 
+// What the scores of a query times 2^lift are to be multiplied by, 2^80 at most: sums of products are
+// multiples of 2^-42 (a query's and a key's least steps) below 2^39, so those that differ do by 2^38
+// all the same, the largest stay finite, and those of 0 are 0.
+__device__ __forceinline__ float score_factor(float c1, int lift) { return fminf(fmaxf(ldexpf(c1, -lift), -0x1p80f), 0x1p80f); }
+
 template <int CT, int D>
 struct Attend;
 
@@ -137,7 +142,7 @@ struct Attend<SE12_STEP_E2M1, D> {
             top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
             top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
             const int lift = 14 + 127 - (int)(top >> 23);
-            by = ldexpf(a.c1, -lift);
+            by = score_factor(a.c1, lift);
 #pragma unroll
             for (int i = 0; i < kChunks; ++i)
 #pragma unroll

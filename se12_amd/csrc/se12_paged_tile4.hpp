@@ -38,7 +38,7 @@ __device__ __forceinline__ float load_query(halfx8_t (&q)[kPieces], const uint16
             q[i][2 * k + 1] = (_Float16)ldexpf(__uint_as_float(v[k] & 0xFFFF0000u), lift);
         }
     }
-    return ldexpf(c1, -lift);
+    return score_factor(c1, lift);
 }
 
 // kRows16: keys are read 16 rows at a time (16 r / 4 + r % 4), else 32 in key_of_row's order

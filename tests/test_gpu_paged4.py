@@ -1070,3 +1070,31 @@ def test_the_plain_append_entry_serves_4_bits_too(gpu):
                                                     inv.data_ptr(), 32, out.data_ptr(), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
     assert torch.equal(out, b.append(batch, k, v, q=q, inv_freq=inv))
     assert all(torch.equal(x, y) for x, y in zip(_snapshot(a), _snapshot(b)))
+
+
+@pytest.mark.parametrize("d,new", [(64, 1), (128, 7), (256, 1), (64, 70), (128, 60), (256, 50)])
+@pytest.mark.parametrize("scaling,softcap", [(2.0 ** 100, 0.0), (-2.0 ** 100, 0.0), (2.0 ** 100, 50.0)])
+def test_scores_beyond_fp32(gpu, d, new, scaling, softcap):
+    """Queries and a scaling whose product FP32 does not hold: the largest score has all the weight (those alike share it; of
+    capped ones all above 0), and a key of zeros a score of 0. Sums of whole numbers up to 3 times codes times scales of 4
+    bits: exact."""
+    c, batch, q, _ = _attend_case(gpu, d, 32, 4, 2, [90, 300], [new, 1], 0.0, 0, seed=87, extra=0)
+    table = batch.page_table.tolist()
+    for s, slot in ((0, 3), (1, 40)):
+        c.k_scale[table[s][slot // 32], :, :, slot % 32] = 0
+    y = (torch.randint(-3, 4, q.shape, generator=_gen(88)) * 2.0 ** 100).to(BF16).to(gpu)
+    y[-1, 2] = 0
+    got = _again(c, batch, y, scaling, softcap)
+    assert got.isfinite().all()
+    # (where nothing is above 0 but the key of zeros, it is the largest)
+    pid = table[1][1]
+    one = _batch(gpu, [[pid]], [9], [1])[0]
+    k = c.k.view(torch.uint8)
+    k[pid, :, :10] = 0x22
+    k[pid, :, 8] = 0
+    c.k_scale[pid, :, :, :10] = 120
+    c.v_scale[pid, :, :, :10] = 120
+    down = torch.full((1, 4, d), -2.0 ** 100, dtype=BF16, device=gpu)
+    got = c.attend(one, down, abs(scaling))
+    _, v = c.read(_batch(gpu, [[pid]], [8], [1])[0], 1)
+    assert torch.equal(got, v.repeat_interleave(2, 1))
