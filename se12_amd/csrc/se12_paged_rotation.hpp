@@ -68,7 +68,9 @@ __device__ __forceinline__ Angle angle_of(double angle) {
     // of sine and cosine: 2^-52 of a whole turn, beside the angle's own rounding
     const double whole = angle * 0.63661977236758134 + 0x1.8p52, k = whole - 0x1.8p52;
     const int turn = __double2loint(whole);
-    const double x = fma(-k, 6.123233995736766e-17, fma(-k, 1.5707963267948966, angle)), x2 = x * x;
+    // (beyond 2^52 quarters a double is whole ones: none left over)
+    const double over = fma(-k, 6.123233995736766e-17, fma(-k, 1.5707963267948966, angle));
+    const double x = fabs(over) <= 2.0 ? over : angle - angle, x2 = x * x;
     double s = -1.0 / 1307674368000, c = 1.0 / 20922789888000;
     s = fma(s, x2, 1.0 / 6227020800);
     c = fma(c, x2, -1.0 / 87178291200);

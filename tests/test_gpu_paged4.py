@@ -1098,3 +1098,33 @@ def test_scores_beyond_fp32(gpu, d, new, scaling, softcap):
     got = c.attend(one, down, abs(scaling))
     _, v = c.read(_batch(gpu, [[pid]], [8], [1])[0], 1)
     assert torch.equal(got, v.repeat_interleave(2, 1))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_angles_of_any_size(gpu, interleaved):
+    """Frequencies up to FP32's largest: a rotation keeps a pair's length whatever its angle, and below 2^51 quarter turns it
+    is that of the angle in 64 bits."""
+    from se12_amd.paged import rotate_heads
+
+    d, heads, kvh = 64, 4, 2
+    inv = 2.0 ** torch.linspace(-20, 127, 32)
+    inv[-1] = torch.finfo(torch.float32).max
+    lengths, new = [0, 1001, 1 << 29], [20, 3, 17]
+    batch, starts = _batch(gpu, [[0] * 70, [1] * 70, [2] * 70], lengths, new)
+    g = _gen(89)
+    q, k, v = (torch.randn((40, h, d), generator=g).to(gpu) for h in (heads, kvh, kvh))
+    turned = rotate_heads(batch, q, k, inv.to(gpu), interleaved=interleaved, dtype=torch.float32)
+    c = _cache(gpu, 9, 16, kvh, d, 90)
+    appended = c.append(batch, k, v, q=q, inv_freq=inv.to(gpu), interleaved=interleaved)
+    pairs = (lambda t: t.unflatten(-1, (32, 2))) if interleaved else (lambda t: t.unflatten(-1, (2, 32)).transpose(-2, -1))
+    pos = torch.cat([torch.arange(a, a + n) for a, n in zip(lengths, new)]).double()
+    small = pos[:, None] * inv.double() < 2.0 ** 51
+    for got, x, step in ((turned[0], q, 0.0), (turned[1], k, 0.0), (appended, q, 2.0 ** -8)):
+        got, x = got.cpu().double(), x.cpu()
+        a, b = pairs(got), pairs(x.double())
+        # (FP32: a cosine, a sine, two products and a sum, each 2^-24 of itself: 2^-21 of |a| + |b|)
+        size = b.abs().sum(-1)
+        assert ((a.square().sum(-1).sqrt() - b.square().sum(-1).sqrt()).abs() <= (2 * step + 2.0 ** -20) * size).all()
+        ref = pairs(torch.stack([e.turned(x[r], pos[r].item(), inv, interleaved) for r in range(40)]))
+        off = (a - ref).abs() <= step * ref.abs() + 2.0 ** -20 * size[..., None]
+        assert off.transpose(1, 2).flatten(2)[small].all()
