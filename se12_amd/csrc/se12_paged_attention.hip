@@ -543,7 +543,7 @@ PromptPlan plan_of(const se12_step_pages* p, const Batch& b, int group) {
 
 // what one launch holds, and what 32 bits hold of it
 const char* limits_error(const se12_step_pages* p, const Batch& b, int group) {
-    const int most_threads = (p->dtype == SE12_STEP_E2M1 ? 2 : 1) * kAttendThreads;      // (of a block of prompts)
+    const int most_threads = (p->dtype == SE12_STEP_E2M1 && p->head_dim == 256 ? 2 : 1) * kAttendThreads;      // (of a block of prompts)
     if ((int64_t)b.tokens * group > INT32_MAX || !grid_fits(plan_of(p, b, group).records * p->kv_heads, most_threads))
         return "too many sequences, tokens and heads for one launch";
     if (std::min<int64_t>(b.seqs, 64) * (((int64_t)b.width * p->page_size + 31) / 32) * (kFewColumns / kColumns) * p->kv_heads > INT32_MAX)

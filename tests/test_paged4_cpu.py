@@ -148,6 +148,17 @@ def test_blocks_of_prompts_are_twice_as_large_and_counted_so():
     _refused("too many", lambda: lib.se12_step_paged_attention(ctypes.byref(p), ctypes.byref(b), P, 1 << 14, P, 8, 0.1, 0.0, 0, P, 1 << 60, None))
 
 
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_blocks_of_prompts_of_smaller_heads_are_not(head_dim):
+    """As many calls as over a cache of BF16, whose blocks have as many threads."""
+    lib = nat.lib()
+    for tokens in (1 << 27, 1 << 28, (1 << 28) - (1 << 16), 1 << 29):
+        b, fits = _batch(sequences=200, tokens=tokens, max_new=1 << 20), []
+        for p in (_pages4(kv_heads=1, head_dim=head_dim), _pages(kv_heads=1, head_dim=head_dim, dtype=nat.STEP_BF16)):
+            fits.append(lib.se12_step_paged_attention_workspace(ctypes.byref(p), ctypes.byref(b), 8) > 0)
+        assert fits[0] == fits[1]
+
+
 @pytest.mark.parametrize("heads,kv_heads", [(8, 4), (16, 8), (28, 4), (1, 1), (160, 1)])
 @pytest.mark.parametrize("sequences,width,page_size,head_dim", [(1, 6000, 16, 256), (64, 20, 64, 128), (300, 4, 128, 64), (3, 100, 32, 256)])
 def test_a_workspace_for_more_tokens_serves_fewer(heads, kv_heads, sequences, width, page_size, head_dim):
