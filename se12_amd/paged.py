@@ -35,7 +35,8 @@ from . import _native as nat
 
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128, 256)
-_DTYPES = {torch.bfloat16: nat.STEP_BF16, torch.float8_e4m3fn: nat.STEP_E4M3, torch.float4_e2m1fn_x2: nat.STEP_E2M1}
+_E2M1 = getattr(torch, "float4_e2m1fn_x2", object())      # (a torch without the type: equal to none)
+_DTYPES = {torch.bfloat16: nat.STEP_BF16, torch.float8_e4m3fn: nat.STEP_E4M3, _E2M1: nat.STEP_E2M1}
 _KINDS = {torch.bfloat16: nat.STEP_BF16, torch.float32: nat.STEP_F32}
 _NO_GUARD = contextlib.nullcontext()
 # a se12_step_rotation (packed a microsecond faster than a ctypes structure is filled)
@@ -193,7 +194,7 @@ class PagedKvCache:
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.float8_e4m3fn,
                  device=None) -> None:
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-        if dtype == torch.float4_e2m1fn_x2:
+        if dtype == _E2M1:
             shapes = ((pages, kv_heads, page_size, head_dim // 2), (pages, kv_heads, page_size // 16, head_dim, 8))
             k, v = (torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype) for shape in shapes)
             scales = [torch.zeros((pages, kv_heads, head_dim // 32, page_size), dtype=torch.uint8, device=device) for _ in range(2)]
@@ -216,7 +217,7 @@ class PagedKvCache:
         if not isinstance(k, torch.Tensor) or k.dim() != 4 or k.dtype not in _DTYPES:
             raise ValueError("k must be a float4_e2m1fn_x2, float8_e4m3fn or bfloat16 [pages, kv_heads, page_size, head_dim] tensor")
         pages, kv_heads, page_size, head_dim = k.shape
-        e2m1, e4m3 = k.dtype == torch.float4_e2m1fn_x2, k.dtype == torch.float8_e4m3fn
+        e2m1, e4m3 = k.dtype == _E2M1, k.dtype == torch.float8_e4m3fn
         head_dim *= 2 if e2m1 else 1
         if page_size not in PAGE_SIZES or head_dim not in HEAD_DIMS:
             raise ValueError(f"page_size must be one of {PAGE_SIZES} and head_dim one of {HEAD_DIMS}, got {page_size}, {head_dim}")
@@ -294,7 +295,7 @@ class PagedKvCache:
             raise ValueError("out goes with q")
         elif q_norm is not None:
             raise ValueError("q_norm goes with q")
-        e2m1 = self.dtype == torch.float4_e2m1fn_x2
+        e2m1 = self.dtype == _E2M1
         plain = q_norm is None and k_norm is None and not interleaved and rotary_scale == 1.0
         if e2m1 or not plain or norm_eps != 1e-6 or norm_offset != 0.0:
             rotation, held = _rotation(head_dim, index, device, inv_at, rotary, interleaved, rotary_scale, q_norm, k_norm, norm_eps, norm_offset)

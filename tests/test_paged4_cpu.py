@@ -342,3 +342,22 @@ def test_frequencies_refuse(args, message):
 
     with pytest.raises(ValueError, match=message):
         rotary_frequencies(*args)
+
+
+def test_the_other_caches_need_no_torch_with_types_of_4_bits(monkeypatch):
+    import importlib.util
+
+    from se12_amd import paged
+
+    monkeypatch.delattr(torch, "float4_e2m1fn_x2")
+    spec = importlib.util.spec_from_file_location("se12_amd.paged_of_8_bits", paged.__file__)
+    other = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(other)
+    k, v, s = torch.zeros((4, 2, 16, 64)), torch.zeros((4, 2, 64, 16)), torch.ones((4, 2))
+    for dtype, scales in ((torch.bfloat16, ()), (torch.float8_e4m3fn, (s, s))):
+        with pytest.raises(ValueError, match="HIP device"):
+            other.PagedKvCache.from_tensors(k.to(dtype), v.to(dtype), *scales)
+    with pytest.raises(ValueError, match="k must be"):
+        other.PagedKvCache.from_tensors(k, v)
+    with pytest.raises(ValueError, match="k must be"):
+        other.PagedKvCache(4, 16, 2, 64, dtype=None, device="cpu")
