@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import pathlib
+import struct
 
 import torch  # noqa: F401  (loads the HIP runtime this library binds to)
 
@@ -136,6 +137,10 @@ class StepRotation(ctypes.Structure):
         ("rotary", c_i32),
         ("interleaved", c_i32),
     ]
+
+
+# its bytes from its fields in order (a microsecond faster than the structure is filled)
+pack_rotation = struct.Struct("@" + "".join(kind._type_ for _, kind in StepRotation._fields_)).pack
 
 
 # name -> (restype, argtypes): every symbol include/se12_gfx950.h and

@@ -27,7 +27,6 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
-import struct
 
 import torch
 
@@ -39,8 +38,6 @@ _E2M1 = getattr(torch, "float4_e2m1fn_x2", object())      # (a torch without the
 _DTYPES = {torch.bfloat16: nat.STEP_BF16, torch.float8_e4m3fn: nat.STEP_E4M3, _E2M1: nat.STEP_E2M1}
 _KINDS = {torch.bfloat16: nat.STEP_BF16, torch.float32: nat.STEP_F32}
 _NO_GUARD = contextlib.nullcontext()
-# a se12_step_rotation (packed a microsecond faster than a ctypes structure is filled)
-_ROTATION = struct.Struct("@3P2df3i").pack
 
 
 def _on(device: torch.device):
@@ -116,7 +113,7 @@ def _rotation(head_dim: int, index: int, device, at: int, rotary: int, interleav
         dtype = k_norm.dtype
     if not (math.isfinite(rotary_scale) and math.isfinite(norm_eps) and norm_eps >= 0 and abs(norm_offset) < 2.0 ** 127):
         raise ValueError("rotary_scale, norm_eps and norm_offset must be finite, norm_eps not below 0")
-    return _ROTATION(at, q_at, k_at, rotary_scale, norm_eps, norm_offset, _KINDS[dtype], rotary, 1 if interleaved else 0), (q_norm, k_norm)
+    return nat.pack_rotation(at, q_at, k_at, rotary_scale, norm_eps, norm_offset, _KINDS[dtype], rotary, 1 if interleaved else 0), (q_norm, k_norm)
 
 
 def _int32(t: torch.Tensor, name: str, shape: tuple, device: torch.device) -> torch.Tensor:

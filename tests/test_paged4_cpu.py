@@ -361,3 +361,8 @@ def test_the_other_caches_need_no_torch_with_types_of_4_bits(monkeypatch):
         other.PagedKvCache.from_tensors(k, v)
     with pytest.raises(ValueError, match="k must be"):
         other.PagedKvCache(4, 16, 2, 64, dtype=None, device="cpu")
+
+
+def test_rotations_go_to_the_kernels_as_the_struct_they_are():
+    values = (1 << 40, 1 << 41, 1 << 42, 1.25, 1e-6, 0.5, nat.STEP_F32, 120, 1)
+    assert nat.pack_rotation(*values) == bytes(nat.StepRotation(*values))
