@@ -199,7 +199,8 @@ int se12_step_paged_append(const se12_step_pages* pages, const se12_step_batch* 
  *   n = x rsqrt(mean(x^2) + eps) (offset + w) where a norm weight w [head_dim] (BF16
  *   or FP32, 16-byte aligned) is given, q_norm for q and k_norm for k, else x;
  *   the pairs (n[i], n[i + rotary / 2]), or (n[2 i], n[2 i + 1]) where interleaved,
- *   i < rotary / 2, by position * inv_freq[i], sine and cosine times `scale`;
+ *   i < rotary / 2, by position * inv_freq[i], sine and cosine times `scale` (below
+ *   2^127);
  *   elements from `rotary` on stay (a multiple of 8 up to head_dim, 0 for none).
  * Sums of squares and angles in 64 bits, the rest in FP32. */
 typedef struct se12_step_rotation {

@@ -306,8 +306,8 @@ inline const char* rotation_error(const se12_step_rotation* r, int head_dim) {
     if (r->rotary < 0 || r->rotary > head_dim || r->rotary % 8) return "rotary must be a multiple of 8 up to head_dim";
     if (r->rotary > 0 && !r->inv_freq) return "NULL argument";
     if (r->norm_dtype != SE12_STEP_BF16 && r->norm_dtype != SE12_STEP_F32) return "norm weights must be BF16 or FP32";
-    if (!(r->scale - r->scale == 0.0) || !(r->eps >= 0.0) || !(r->eps - r->eps == 0.0) || !(r->offset - r->offset == 0.0f))
-        return "scale, eps and offset must be finite, eps not below 0";
+    if (!(fabs(r->scale) < 0x1p127) || !(r->eps >= 0.0) || !(r->eps - r->eps == 0.0) || !(r->offset - r->offset == 0.0f))
+        return "scale, eps and offset must be finite (scale below 2^127), eps not below 0";
     if (reinterpret_cast<uintptr_t>(r->inv_freq) % 16 || reinterpret_cast<uintptr_t>(r->q_norm) % 16 ||
         reinterpret_cast<uintptr_t>(r->k_norm) % 16)
         return "misaligned tensor";

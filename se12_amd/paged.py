@@ -111,8 +111,8 @@ def _rotation(head_dim: int, index: int, device, at: int, rotary: int, interleav
         if q_norm is not None and k_norm.dtype != dtype:
             raise ValueError("q_norm and k_norm must be of one type")
         dtype = k_norm.dtype
-    if not (math.isfinite(rotary_scale) and math.isfinite(norm_eps) and norm_eps >= 0 and abs(norm_offset) < 2.0 ** 127):
-        raise ValueError("rotary_scale, norm_eps and norm_offset must be finite, norm_eps not below 0")
+    if not (abs(rotary_scale) < 2.0 ** 127 and math.isfinite(norm_eps) and norm_eps >= 0 and abs(norm_offset) < 2.0 ** 127):
+        raise ValueError("rotary_scale, norm_eps and norm_offset must be finite (the first and last below 2^127), norm_eps not below 0")
     return nat.pack_rotation(at, q_at, k_at, rotary_scale, norm_eps, norm_offset, _KINDS[dtype], rotary, 1 if interleaved else 0), (q_norm, k_norm)
 
 

@@ -366,3 +366,16 @@ def test_the_other_caches_need_no_torch_with_types_of_4_bits(monkeypatch):
 def test_rotations_go_to_the_kernels_as_the_struct_they_are():
     values = (1 << 40, 1 << 41, 1 << 42, 1.25, 1e-6, 0.5, nat.STEP_F32, 120, 1)
     assert nat.pack_rotation(*values) == bytes(nat.StepRotation(*values))
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e300, 2.0 ** 127])
+def test_a_factor_that_fp32_does_not_hold_is_refused(scale):
+    from se12_amd.paged import rotate_heads
+
+    lib, b, r = nat.lib(), _batch(), _turn(scale=scale)
+    _refused("finite", lambda: lib.se12_step_paged_append_rotated(ctypes.byref(_pages4()), ctypes.byref(b), P, P, P, nat.STEP_F32, 1024, 512, 512, 8,
+                                                                  ctypes.byref(r), None, None))
+    _refused("finite", lambda: lib.se12_step_rotate_heads(ctypes.byref(b), Q, 2 * Q, nat.STEP_BF16, 1024, 512, 8, 4, 128, ctypes.byref(r), Q + 16, 4 * Q,
+                                                          nat.STEP_BF16, None))
+    with pytest.raises(ValueError, match="finite"):
+        rotate_heads(_on_cpu()[1], torch.zeros((3, 4, 64)), rotary_scale=scale)
