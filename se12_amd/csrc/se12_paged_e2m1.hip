@@ -107,7 +107,7 @@ __global__ __launch_bounds__(kHeads * kRowThreads) void paged_append4_kernel(App
     // 16 / 8 heads of 256 14 us less one at a time than several, where each lane finds its own. The
     // next rows are on their way while some are worked on (16 tokens of a head of 256 in two turns,
     // both asked for at once: 3 us of 9,001 tokens').
-    constexpr int kTurns = kFew ? 1 : kRows >= 16 ? 1 : 16 / kRows;
+    constexpr int kTurns = kFew ? 1 : 16 / kRows;
     const int lane = tid % kLanes, c0 = 8 * lane, place = tid / kLanes, what_end = kh < a.kvh ? 2 + a.group : 0;
     const int places = n > 1 ? 32 - __builtin_clz(n - 1) : 0;
     auto load = [&](int what, int token) {
@@ -333,14 +333,23 @@ using namespace se12step;
 
 namespace {
 
+// Heads of 64, whose 16 rows are half of those that kRowThreads work on, are few always: 9,001 tokens of
+// 16 / 8 heads 27.3 us, 26.4 a head at a time in pairs of heads, 9 / 3 heads 15.1 and 18.9, 306 tokens of
+// 32 / 8 heads 7.6 and 8.8. (Larger heads in pairs where there are two: 6 / 3 heads of 256 29.4, 26.0 one to a
+// block; 10 / 5 and 14 / 7 alike.)
 template <int DT, int D>
 void launch_append4_of(const Append4Args& a, uint32_t runs, hipStream_t st) {
-    if (2 * (a.b.max_new < 16 ? a.b.max_new : 16) <= kRowThreads / (D / 8))
+    constexpr int kRows = kRowThreads / (D / 8);
+    if (2 * (a.b.max_new < 16 ? a.b.max_new : 16) <= kRows) {
         hipLaunchKernelGGL((paged_append4_kernel<DT, D, true, 1>), dim3(runs * a.kvh), dim3(kRowThreads), 0, st, a);
-    else if (a.kvh == 1)
-        hipLaunchKernelGGL((paged_append4_kernel<DT, D, false, 1>), dim3(runs), dim3(kRowThreads), 0, st, a);
-    else
-        hipLaunchKernelGGL((paged_append4_kernel<DT, D, false, 2>), dim3(runs * ((a.kvh + 1) / 2)), dim3(2 * kRowThreads), 0, st, a);
+        return;
+    }
+    if constexpr (kRows < 2 * 16) {
+        if (a.kvh == 1)
+            hipLaunchKernelGGL((paged_append4_kernel<DT, D, false, 1>), dim3(runs), dim3(kRowThreads), 0, st, a);
+        else
+            hipLaunchKernelGGL((paged_append4_kernel<DT, D, false, 2>), dim3(runs * ((a.kvh + 1) / 2)), dim3(2 * kRowThreads), 0, st, a);
+    }
 }
 
 template <int DT>
