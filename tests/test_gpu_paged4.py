@@ -1128,3 +1128,33 @@ def test_angles_of_any_size(gpu, interleaved):
         ref = pairs(torch.stack([e.turned(x[r], pos[r].item(), inv, interleaved) for r in range(40)]))
         off = (a - ref).abs() <= step * ref.abs() + 2.0 ** -20 * size[..., None]
         assert off.transpose(1, 2).flatten(2)[small].all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_prompts_beyond_32_bit_offsets(gpu, d):
+    """More than 64 columns to a KV head, of one unit alone and of keys in parts: pages beyond 4 GiB of codes as near ones, and
+    queries 2^30 values apart as side by side."""
+    from se12_amd.paged import PagedKvCache
+
+    page, kvh, heads, new = 128, 8, 24, [40, 23, 30]
+    g = _gen(91)
+    columns = 12
+    pages = (9 << 29) // (kvh * page * d // 2)      # 4.5 GiB of codes
+    q, k, v = (torch.randn((1593, h, d), generator=g).to(BF16).to(gpu) for h in (heads, kvh, kvh))
+    got = []
+    for count in (pages, 3 * columns):
+        c = PagedKvCache(count, page, kvh, d, dtype=FP4, device=gpu)
+        table = [[count - 1 - columns * s - j for j in range(columns)] for s in range(3)]
+        before, _ = _batch(gpu, table, [0] * 3, [100, 0, 1493])
+        c.append(before, k, v)
+        batch, _ = _batch(gpu, table, [100, 0, 1493], new)
+        turned = c.append(batch, k[:93], v[:93], q=q[:93])
+        got.append(c.attend(batch, turned, d ** -0.5))
+        del c
+    assert torch.equal(*got) and got[0].isfinite().all()
+    c = _cache(gpu, 8, page, 1, d, 92)
+    batch, _ = _batch(gpu, [[4, 1, 3, 0, 2, 5, 7, 6]], [700], [3])
+    near = q[:3].reshape(3, heads * d)
+    far = torch.empty((3, 1 << 30), dtype=BF16, device=gpu)
+    far[:, :heads * d] = near
+    assert torch.equal(c.attend(batch, far[:, :heads * d].view(3, heads, d), d ** -0.5), c.attend(batch, near.view(3, heads, d), d ** -0.5))
