@@ -32,7 +32,10 @@ def rotary_frequencies(rotary: int, base: float = 10000.0, method: str = "none",
     if method == "parts" and not (context > 0 and 0 <= slow < fast):
         raise ValueError("context must be above 0 and slow below fast")
     if method == "base":
-        base *= factor ** (rotary / (rotary - 2))
+        power = rotary / (rotary - 2)
+        if math.log(base) + power * math.log(factor) > 709.0:
+            raise ValueError(f"base times factor^{power:.3g} must be below e^709, got {base}, {factor}")
+        base *= factor ** power
     freq = base ** (-torch.arange(0, rotary, 2, dtype=torch.float64) / rotary)
     scale = 1.0
     if method == "linear":

@@ -379,3 +379,11 @@ def test_a_factor_that_fp32_does_not_hold_is_refused(scale):
                                                           nat.STEP_BF16, None))
     with pytest.raises(ValueError, match="finite"):
         rotate_heads(_on_cpu()[1], torch.zeros((3, 4, 64)), rotary_scale=scale)
+
+
+@pytest.mark.parametrize("base,factor", [(1e4, 1e308), (1e300, 1e30), (1e308, 2.0)])
+def test_a_base_that_64_bits_do_not_hold_is_refused(base, factor):
+    from se12_amd.rotary import rotary_frequencies
+
+    with pytest.raises(ValueError, match="base"):
+        rotary_frequencies(8, base, "base", factor)
