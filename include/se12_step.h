@@ -215,8 +215,8 @@ typedef struct se12_step_rotation {
 /* se12_step_paged_append for a cache of SE12_STEP_E2M1, with norms and any rotation.
  * Of 32 columns of a token the scale is the one nearest to a sixth of the largest
  * value (ties to the even byte; at most 10240, so values beyond 61440 are held as
- * that, and where the largest is below 2^-16 all are zero); a value the nearest code, ties to
- * even. 32 columns with a NaN or an infinity are held as NaN. A token's codes and
+ * that, and where the largest is 1.5 * 2^-16 or less all are zero); a value the nearest code,
+ * ties to even. 32 columns with a NaN or an infinity are held as NaN. A token's codes and
  * scales depend on that token alone. One launch. */
 int se12_step_paged_append_rotated(const se12_step_pages* pages, const se12_step_batch* batch, const void* q, const void* k,
                                    const void* v, int32_t dtype, int64_t q_stride, int64_t k_stride, int64_t v_stride,
@@ -233,7 +233,8 @@ int se12_step_paged_read(const se12_step_pages* pages, const se12_step_batch* ba
  * where kv_heads is 0) normed and rotated, into q_out and k_out (out_dtype BF16 or
  * FP32, contiguous, 16-byte aligned; each may be its input where that has the same
  * type and rows, else all apart). The batch's page table is not read. head_dim a multiple of
- * 8 up to 256; strides multiples of 4, rows aligned to 4 values. One launch. */
+ * 8 up to 256; strides multiples of 4, rows aligned to 4 values. An append's q may differ
+ * in FP32's last bit (its angles are sums from the first of 16). One launch. */
 int se12_step_rotate_heads(const se12_step_batch* batch, const void* q, const void* k, int32_t dtype, int64_t q_stride,
                            int64_t k_stride, int32_t heads, int32_t kv_heads, int32_t head_dim,
                            const se12_step_rotation* rotation, void* q_out, void* k_out, int32_t out_dtype, void* stream);
@@ -250,7 +251,7 @@ int se12_step_rotate_heads(const se12_step_batch* batch, const void* q, const vo
  * gives zeros. Any finite values of BF16 pages give finite results, those of E4M3
  * pages where none is above 2^112 / keys. SE12_STEP_E2M1 pages: the products' operands
  * are FP16, which holds keys and values exactly, a query to 2^-38 of its largest value, and a
- * weight to 2^-12 of itself or 2^-32 of the row's largest; scores beyond FP32's range
+ * weight to 2^-11 of itself or 2^-32 of the row's largest; scores beyond FP32's range
  * keep their order.
  *
  * `workspace`: se12_step_paged_attention_workspace() bytes for the shape (or for

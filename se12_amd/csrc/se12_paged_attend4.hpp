@@ -3,7 +3,7 @@
 // its own:
 //
 // Operands are FP16. A code times its scale has 6 significant bits, so keys and values
-// are exact (a conversion and a packed product to two of them); a weight is off by 2^-12
+// are exact (a conversion and a packed product to two of them); a weight is off by 2^-11
 // of itself. FP16 spans 40 powers of two, so a query is taken times a power of two that
 // brings its largest value to 2^14 (its scores are taken back by their factor), and a
 // weight times 2^7, with maxima that a score may pass by 2^8: from 2^15 down to 2^-31 of
@@ -14,9 +14,12 @@
 // The scales of 16 tokens and 32 columns are 16 bytes: of each 16 lanes (which share the
 // tokens) lane g takes those of group g, and they go from there to the others by DPP.
 //
-// Bound by the bytes of the pages: 32 sequences to 8,191 keys, 16 / 8 heads of 256, 328 MB in 66 us and
-// 5 of the join (5.0 TB/s, a copy's rate); 3 to 130,000, 28 / 4 heads of 128, 159 MB in 32 + 6. 1,024
-// waves as for the other types: with 2,048 the calls took 75 and 44 for 68 and 40, in 256 registers 91.
+// Bound by the bytes of the pages: 32 sequences to 8,191 keys, 16 / 8 heads of 256, 328 MB in 64 to 67 us
+// and 5 of the join (4.9 to 5.1 TB/s, a copy's rate); 3 to 130,000, 28 / 4 heads of 128, 159 MB in 33 to 34
+// (4.7 to 4.8) and 6.5. 1,024 waves as for the other types: with 2,048 the calls took 75 and 44 for 68 and
+// 40, in 256 registers 91; where a wave has four tiles, 31 tokens of 12 sequences to 5,000 under a window of
+// 4,096, heads of 64, 128 and 256 17.7, 21.0 and 32.3 for 16.9, 19.3 and 25.4. (8 to 2,000, 16 / 8 heads of
+// 128, two tiles to a wave: 12.2 for 13.6.)
 #pragma once
 
 #include "se12_paged_device.hpp"

@@ -10,12 +10,14 @@
 // query heads that read it, so a value column's 8 bytes (16 tokens) have one writer and
 // the angles serve all its rows. Values meet in LDS, where a column's tokens lie apart.
 //
-// Append: 9,001 tokens of 7 prompts, 16 / 8 heads of 256 normed and rotated, BF16 in: 241 MB in 57 to
-// 60 us (4.1 TB/s; a copy 5.0, so 48), the vector units busy for most of it (with the angles in
-// every thread, 1,470 instructions to a wave of 16 rows, 89% of 66 us). One token 4.6 us, 57 of 40 sequences 6.5: starts, lengths, table
-// entry and rows, one after the other.
+// Append: 9,001 tokens of 7 prompts, 16 / 8 heads normed and rotated, BF16 in. Heads of 256: 241 MB in 55
+// to 60 us (4.0 to 4.4 TB/s; a copy 5.0, so 48), bound by the issue of vector instructions: 26.3 of 26.3
+// million quarter cycles, 1,390 of them to a wave; LDS is busy for 54%. Heads of 128: 33 us (24 by
+// bytes), vector instructions 85% of the cycles; of 64: 25 to 26 (12), 88%. One token 4.6 us, 57 of 40
+// sequences 6.4: starts, lengths, table entry and rows, one after the other.
 // Read: bound by bytes. 47,604 tokens of 8 heads of 256 from pages of 4 bits: 494 MB in 104 us (4.75
-// TB/s; a copy 5.0). Values turn in LDS, so that rows are written whole.
+// TB/s; a copy 5.0), of E4M3 585 MB in 130 (4.5), of BF16 780 in 165 (4.7). Values turn in LDS, so that
+// rows are written whole.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -11,13 +11,14 @@
 // Head dim 256: a wave's sums and queries for 32 columns leave room for one wave to a SIMD, which
 // waits for each of its own instructions; eight waves of 16 columns (v_mfma_f32_16x16x32_f16)
 // read each operand twice as often from LDS, but two share a SIMD. (6,194 tokens of 5 prompts
-// behind up to 1,500 keys, 84.7 GFLOP: heads of 256 134 us the call, 0.63 PFLOP/s, 173 the other
-// way; heads of 128 139, 173 the other way.)
+// behind up to 1,500 keys, 84.7 GFLOP, calls: 8 / 4 heads of 256, capped, 135 us, 0.63 PFLOP/s, 173 the
+// other way; 16 / 8 heads of 128 139, 173 the other way, capped 149; 32 / 16 of 64 173, capped 215.)
 //
-// Bound by the vector instructions between the products and the waits of waves for each
-// other's: at 256, of 257,000 cycles 145,000 issue vector instructions (48 of 309 to 64 keys of 16
-// columns exponentials and inverses, at half the rate), the matrix unit is busy for 88,000 and LDS
-// for 116,000.
+// Nothing is full: a SIMD's two waves overlap vector instructions and products in part, and wait for
+// each other's at a tile's barrier. Capped, as above, vector instructions / the matrix unit / LDS: at 256, of
+// 257,000 cycles 56 / 34 / 45% (48 of 309 vector instructions to 64 keys of 16 columns are exponentials
+// and inverses, at half the rate), at 128 of 281,000 72 / 31 / 26%, at 64, with four times the
+// exponentials to a product, of 464,000 78 / 19 / 19%.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

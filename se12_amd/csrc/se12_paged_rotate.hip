@@ -138,7 +138,10 @@ extern "C" int se12_step_rotate_heads(const se12_step_batch* batch, const void* 
     if (kv_heads > 0 && overlap(out[0].p, out[0].bytes, out[1].p, out[1].bytes)) return step_fail(fn, "an output overlaps the other");
     const Batch b{nullptr, 0, batch->lengths, batch->starts, 0, batch->sequences, batch->tokens,
                   batch->max_new < batch->tokens ? batch->max_new : batch->tokens};
-    // tokens of a block: four share the start, where there are enough blocks all the same
+    // tokens of a block: four share the start, where there are blocks enough all the same (us with one and
+    // with four, BF16. 2,048 tokens: 32 / 8 heads of 128 12.5 and 15.9, 16 / 8 of 256 15.0 and 19.3, 8 / 2 of 128 5.7
+    // and 6.1, 2 / 1 of 64 4.2 and 3.8. 4,096: 21.1 and 20.7, 25.9 and 26.7, 11.1 and 9.1, 6.7 and 4.0. 8,192: 41 and
+    // 38, 52 and 48, 18 and 13, 10.2 and 5.2)
     RotateArgs a{q, k, q_stride, k_stride, q_out, k_out, b, device_rotation(rotation), heads, kv_heads, head_dim, batch->tokens >= 4096 ? 4 : 1, 1.0 / head_dim};
     const int64_t blocks = ((int64_t)b.tokens + a.tokens - 1) / a.tokens;
     if (!grid_fits(blocks, kRotateThreads) || (int64_t)a.tokens * (heads + kv_heads) > INT32_MAX)

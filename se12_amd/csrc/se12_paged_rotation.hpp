@@ -7,8 +7,10 @@
 // A row (token and head) is 8 columns to a lane. Sums of squares and angles in 64 bits,
 // each rounded to FP32 once (the mean's root, sine and cosine times scale); all else in
 // single FP32 operations, no product kept longer than the next rounding. So keys are the
-// same bits whatever the launch, and those of the formula in FP32: a digit of a quantised
-// key does not depend on how the work was cut.
+// same bits whatever append wrote them, and those of the formula in FP32: a digit of a
+// quantised key does not depend on how the work was cut. (An append sums a position's angle
+// from its run's first, the rotation by itself works each out: theirs may differ in FP32's
+// last bit, and one BF16 value in 2^16 by a step.)
 #pragma once
 
 #include <hip/hip_runtime.h>

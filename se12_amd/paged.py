@@ -268,8 +268,9 @@ class PagedKvCache:
         value, 10240 at most (so values up to 61440), each value as the nearest code; 32 columns with a NaN or an infinity
         as NaN. What a token is held as depends on that token alone.
 
-        (Norms, interleaved pairs and a scale for a cache of BF16 or E4M3 take a launch more for each of q and k, and
-        memory for k and v in FP32.) An E4M3 page and head's scale is the least power of two (2^-100 or more) that holds its new values; with older
+        (Norms, interleaved pairs and a scale for a cache of BF16 or E4M3 take a launch more for each of q and k, one that
+        widens BF16 v, memory for k and v in FP32, and a copy of `out` there and back where it is not 16-byte aligned.)
+        An E4M3 page and head's scale is the least power of two (2^-100 or more) that holds its new values; with older
         tokens in the page at least what it was, and if it grows the older ones are rounded again. NaN and infinities
         are held as NaN. A page that two entries of the table name must not be written by a call."""
         self._check(batch)
@@ -414,7 +415,7 @@ def rotate_heads(batch: PagedBatch, q: torch.Tensor, k: torch.Tensor | None = No
                  dtype: torch.dtype = torch.bfloat16, out: tuple | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
     """The batch's q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] (BF16 or FP32, both of one type; rows
     may be strided) normed and rotated to their positions as `PagedKvCache.append` does, in `dtype` (bfloat16 or float32):
-    (q, k), k None without k. Into `out` = (q, k) if given; each may be its own input, and is apart from the rest
+    (q, k), k None without k (in BF16 one value in 2^16 may be a step from `append`'s). Into `out` = (q, k) if given; each may be its own input, and is apart from the rest
     otherwise. head_dim a multiple of 8 up to 256. The batch's page table is not read; rows of no sequence are
     not written. No gradients."""
     if not isinstance(batch, PagedBatch):
